@@ -21,6 +21,9 @@ SYMBOLS = (
     "evoattn_peer_data_bytes", "evoattn_peer_flag_bytes", "evoattn_peer_buffer_create", "evoattn_peer_buffer_open",
     "evoattn_peer_buffer_close", "evoattn_peer_buffer_destroy", "evoattn_peer_allreduce_f32",
     "evoattn_bias_to_heads_first", "evoattn_bias_to_heads_first_ld", "evoattn_dbias_to_heads_last", "evoattn_bias_pad_rows",
+    "evoattn_layer_norm_fwd", "evoattn_layer_norm_bwd_workspace_bytes", "evoattn_layer_norm_bwd",
+    "evoattn_relative_bias_fwd", "evoattn_relative_bias_bwd_workspace_bytes", "evoattn_relative_bias_bwd",
+    "evoattn_pair_projection_fwd", "evoattn_pair_projection_bwd_workspace_bytes", "evoattn_pair_projection_bwd",
 )
 STATIC_SCRATCH_BYTES = 64 << 20
 
@@ -68,6 +71,42 @@ class BwdParams(C.Structure):
         ("exchange", C.POINTER(PeerAllReduceParams)),
         ("dbias_cast", C.c_void_p),
         ("dbias_cast_dtype", C.c_int32), ("dbias_cast_heads_last", C.c_int32),
+    ]
+
+
+class LayerNormParams(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int32), ("weight_dtype", C.c_int32), ("bias_dtype", C.c_int32), ("eps", C.c_float),
+        ("n", C.c_int64 * 3), ("C", C.c_int32), ("reserved", C.c_int32),
+        ("x", C.c_void_p), ("x_stride", C.c_int64 * 3), ("weight", C.c_void_p), ("bias", C.c_void_p),
+        ("y", C.c_void_p), ("stats", C.c_void_p),
+        ("d_y", C.c_void_p), ("d_y_stride", C.c_int64 * 3), ("dx", C.c_void_p), ("dweight", C.c_void_p), ("dbias", C.c_void_p),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+    ]
+
+
+class RelativeBiasParams(C.Structure):
+    _fields_ = [
+        ("table_dtype", C.c_int32), ("dtype", C.c_int32), ("base_dtype", C.c_int32),
+        ("B", C.c_int32), ("H", C.c_int32), ("Rq", C.c_int32), ("Rk", C.c_int32),
+        ("buckets", C.c_int32), ("scheme", C.c_int32), ("exact", C.c_int32), ("n_edges", C.c_int32), ("positions64", C.c_int32),
+        ("edges", C.POINTER(C.c_int32)),
+        ("table", C.c_void_p), ("q_pos", C.c_void_p), ("k_pos", C.c_void_p), ("q_pos_stride", C.c_int64), ("k_pos_stride", C.c_int64),
+        ("base", C.c_void_p), ("base_stride", C.c_int64 * 3), ("out", C.c_void_p), ("out_stride", C.c_int64 * 3),
+        ("d_out", C.c_void_p), ("d_out_stride", C.c_int64 * 3), ("dtable", C.c_void_p),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+    ]
+
+
+class PairProjectionParams(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int32), ("weight_dtype", C.c_int32), ("norm_weight_dtype", C.c_int32), ("norm_bias_dtype", C.c_int32),
+        ("eps", C.c_float), ("B", C.c_int32), ("Ri", C.c_int32), ("Rj", C.c_int32), ("C", C.c_int32), ("H", C.c_int32),
+        ("pair", C.c_void_p), ("pair_stride", C.c_int64 * 3),
+        ("weight", C.c_void_p), ("norm_weight", C.c_void_p), ("norm_bias", C.c_void_p),
+        ("out", C.c_void_p), ("out_stride", C.c_int64 * 3), ("d_out", C.c_void_p), ("d_out_stride", C.c_int64 * 3),
+        ("dpair", C.c_void_p), ("dweight", C.c_void_p), ("dnorm_weight", C.c_void_p), ("dnorm_bias", C.c_void_p),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
     ]
 
 
@@ -122,6 +161,11 @@ def load() -> C.CDLL:
         lib.evoattn_bias_pad_rows.argtypes = [C.c_void_p, C.POINTER(C.c_int64), C.c_void_p] + [C.c_int] * 5 + [C.c_void_p]
         lib.evoattn_peer_allreduce_f32.restype = C.c_int
         lib.evoattn_peer_allreduce_f32.argtypes = [C.POINTER(PeerAllReduceParams), C.c_void_p]
+        for name, params in (("layer_norm", LayerNormParams), ("relative_bias", RelativeBiasParams), ("pair_projection", PairProjectionParams)):
+            for part, result in (("fwd", C.c_int), ("bwd", C.c_int), ("bwd_workspace_bytes", C.c_size_t)):
+                fn = getattr(lib, f"evoattn_{name}_{part}")
+                fn.restype = result
+                fn.argtypes = [C.POINTER(params)] + ([] if result is C.c_size_t else [C.c_void_p])
         if lib.evoattn_abi_version() != ABI_VERSION:
             raise RuntimeError("libevoattn.so ABI version mismatch; rebuild it")
         _lib = lib

@@ -16,7 +16,9 @@ CSRC = os.path.join(PKG, "csrc")
 OBJ = os.path.join(PKG, "build")
 LIB = os.path.join(PKG, "libevoattn.so")
 HOST = os.path.join(PKG, "_evohost.so")
-SOURCES = ["api.cu", "generic_kernels.cu", "tmap.cu", "fwd_sm100.cu", "bwd_sm100.cu", "peer_reduce.cu", "extras.cu"]
+SOURCES = ["api.cu", "generic_kernels.cu", "tmap.cu", "fwd_sm100.cu", "bwd_sm100.cu", "peer_reduce.cu", "extras.cu",
+           "norm.cu", "relative_bias.cu", "pair_projection.cu"]
+HOST_SOURCES = ["host.cpp", "host_inputs.cpp"]
 NVCC_FLAGS = [
     "-O3", "-std=c++17", "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo",
     "-Xcompiler", "-fPIC", "-Xptxas", "-v", "--expt-relaxed-constexpr",
@@ -62,16 +64,16 @@ def build(force: bool = False, verbose: bool = False) -> str:
         if force or _stale(o, [s] + headers):
             jobs.append((s, o))
 
-    host_src = os.path.join(CSRC, "host.cpp")
-    host_obj = os.path.join(OBJ, "host.o")
-    host_job = force or _stale(host_obj, [host_src, headers[-1]])
+    host_headers = [headers[-1], os.path.join(CSRC, "host_common.h")]
+    host_objs = [os.path.join(OBJ, f.replace(".cpp", ".o")) for f in HOST_SOURCES]
+    host_jobs = [(os.path.join(CSRC, f), o) for f, o in zip(HOST_SOURCES, host_objs)
+                 if force or _stale(o, [os.path.join(CSRC, f)] + host_headers)]
     cxx, ld = _host_flags()
-    if host_job:
-        jobs.append((host_src, host_obj))
+    jobs += host_jobs
 
     def compile_one(job):
         s, o = job
-        cmd = ["g++", *cxx, "-c", s, "-o", o] if s == host_src else [_nvcc(), *NVCC_FLAGS, "-c", s, "-o", o]
+        cmd = ["g++", *cxx, "-c", s, "-o", o] if s.endswith(".cpp") else [_nvcc(), *NVCC_FLAGS, "-c", s, "-o", o]
         r = subprocess.run(cmd, capture_output=True, text=True)
         with open(o + ".log", "w") as f:
             f.write(r.stdout + r.stderr)
@@ -84,13 +86,13 @@ def build(force: bool = False, verbose: bool = False) -> str:
             if r.returncode != 0:
                 raise RuntimeError(f"compiling {s} failed:\n{r.stderr[-8000:]}")
     objs = [os.path.join(OBJ, s.replace(".cu", ".o")) for s in SOURCES]
-    if force or any(s != host_src for s, _ in jobs) or _stale(LIB, objs):
+    if force or len(jobs) > len(host_jobs) or _stale(LIB, objs):
         r = subprocess.run([_nvcc(), "-shared", "-o", LIB, *objs, "-gencode", "arch=compute_100a,code=sm_100a"],
                            capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError("link failed:\n" + r.stderr[-4000:])
-    if host_job or _stale(HOST, [host_obj]):
-        r = subprocess.run(["g++", "-shared", "-o", HOST, host_obj, "-L", PKG, "-l:libevoattn.so", "-Wl,-rpath,$ORIGIN", *ld], capture_output=True, text=True)
+    if host_jobs or _stale(HOST, host_objs):
+        r = subprocess.run(["g++", "-shared", "-o", HOST, *host_objs, "-L", PKG, "-l:libevoattn.so", "-Wl,-rpath,$ORIGIN", *ld], capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError("link failed:\n" + r.stderr[-4000:])
     return LIB

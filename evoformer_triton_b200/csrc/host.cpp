@@ -15,16 +15,13 @@
 #include <torch/extension.h>
 
 #include <atomic>
-#include <cmath>
 #include <mutex>
-#include <string>
-#include <vector>
 
-#include "evoattn.h"
+#include "host_common.h"
 
 namespace {
 
-using at::Tensor;
+using namespace evohost;
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
@@ -52,13 +49,6 @@ Tensor status_word(int64_t index) {
   status_ptr(c10::Device(c10::kCUDA, static_cast<c10::DeviceIndex>(index)));
   return *g_status[index];
 }
-
-void check(int rc, const char* what) {
-  if (rc != EVOATTN_OK) throw std::runtime_error(std::string(what) + " failed: " + evoattn_strerror(rc) + " (status " + std::to_string(rc) + ")");
-}
-
-int dtype_code(at::ScalarType t) { return t == at::kBFloat16 ? EVOATTN_BF16 : t == at::kHalf ? EVOATTN_FP16 : EVOATTN_FP32; }
-bool known(at::ScalarType t) { return t == at::kBFloat16 || t == at::kHalf || t == at::kFloat; }
 
 struct Dims {
   int64_t B, S, R, H, D;
@@ -149,13 +139,6 @@ Tensor kernel_bias(const Tensor& pb, const Dims& d, at::ScalarType qt, bool head
   check(evoattn_bias_pad_rows(b.data_ptr(), s, r.data_ptr(), dtype_code(b.scalar_type()), (int)d.B, (int)d.H, (int)d.R, (int)ld,
                               st), "evoattn_bias_pad_rows");
   return r;
-}
-
-using Maybe = c10::optional<Tensor>;
-
-[[noreturn]] void raise(PyObject* type, const char* text) {
-  PyErr_SetString(type, text);
-  throw py::error_already_set();
 }
 
 // Everything a kernel is given an address of is checked here: on Q's device, of a size that its strides
@@ -321,4 +304,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("note_fwd", [](int launches, int path) { g_fwd_launches = launches; g_fwd_path = path; });
   m.def("note_bwd", [](int launches, int path) { g_bwd_launches = launches; g_bwd_path = path; });
   m.def("abi_version", [] { return evoattn_abi_version(); });
+  evohost::register_inputs(m);
 }

@@ -246,6 +246,113 @@ int evoattn_dbias_to_heads_last(const float* src_bhrr, void* dst_brrh, int dtype
 int evoattn_bias_pad_rows(const void* src, const int64_t* stride, void* dst, int dtype, int B, int H, int R, int ld,
                           void* cuda_stream);
 
+/* ---- What the attention's inputs are made with.
+ *
+ * Three operators that stand before the attention in a block: layer norm, a learned relative position bias
+ * and the projection of the pair representation to a pair bias.  The reference has none of them.  The types
+ * are EVOATTN_BF16 / FP16 / FP32, sums are taken in fp32 in a fixed order (the same bits in every run), and
+ * every call may be captured in a CUDA graph.  The calls with a workspace need it 16-byte aligned.
+ *
+ * Layer norm over the last axis: y = (x - mean) / sqrt(var + eps) * weight + bias, var the mean squared
+ * deviation.  Rows are indexed by three axes (n[0], n[1], n[2]) with element strides; the C values of a row
+ * are contiguous. */
+typedef struct evoattn_layer_norm_params {
+  int32_t dtype;          /* of x, y, d_y, dx */
+  int32_t weight_dtype;   /* of weight and dweight */
+  int32_t bias_dtype;     /* of bias and dbias */
+  float eps;
+  int64_t n[3];
+  int32_t C;
+  int32_t reserved;
+  const void* x;
+  int64_t x_stride[3];
+  const void* weight;     /* [C] or null (1) */
+  const void* bias;       /* [C] or null (0) */
+  void* y;                /* forward: out, dense */
+  float* stats;           /* [rows][2]: mean and 1 / sqrt(var + eps).  Forward: out, or null; backward: in */
+  const void* d_y;        /* backward */
+  int64_t d_y_stride[3];
+  void* dx;               /* out, dense; null: not wanted */
+  void* dweight;          /* out [C]; null: not wanted */
+  void* dbias;            /* out [C]; null: not wanted */
+  void* workspace;        /* device scratch of at least evoattn_layer_norm_bwd_workspace_bytes() */
+  size_t workspace_bytes;
+} evoattn_layer_norm_params;
+
+int evoattn_layer_norm_fwd(const evoattn_layer_norm_params* p, void* cuda_stream);
+size_t evoattn_layer_norm_bwd_workspace_bytes(const evoattn_layer_norm_params* p);
+int evoattn_layer_norm_bwd(const evoattn_layer_norm_params* p, void* cuda_stream);
+
+/* Relative position bias: out[b,h,i,j] = table[row(k_j - q_i), h] (+ base[b,h,i,j]).  With a = |k_j - q_i|
+ * and f(a) = a below `exact`, else exact + the number of edges[] that are <= a:
+ *   CLIP        row = exact - f where the key follows the query, exact + f elsewhere; no edges (table rows: 2 exact + 1)
+ *   LOG         row = f, plus half of the table's rows where the key follows the query
+ *   LOG_CAUSAL  row = f of the distance back, 0 where the key follows the query
+ * Positions are 32- or 64-bit whole numbers whose differences fit 64 bits. */
+enum { EVOATTN_BUCKETS_CLIP = 0, EVOATTN_BUCKETS_LOG = 1, EVOATTN_BUCKETS_LOG_CAUSAL = 2 };
+#define EVOATTN_MAX_BUCKETS 1024
+#define EVOATTN_MAX_BUCKET_EDGES 128
+typedef struct evoattn_relative_bias_params {
+  int32_t table_dtype;    /* of table and dtable */
+  int32_t dtype;          /* of out (forward) or d_out (backward) */
+  int32_t base_dtype;
+  int32_t B, H, Rq, Rk;
+  int32_t buckets;        /* rows of the table, at most EVOATTN_MAX_BUCKETS */
+  int32_t scheme;
+  int32_t exact;
+  int32_t n_edges;
+  int32_t positions64;    /* non-zero: positions are int64, else int32 */
+  const int32_t* edges;   /* HOST array, ascending, read during the call; at most EVOATTN_MAX_BUCKET_EDGES */
+  const void* table;      /* [buckets][H], dense */
+  const void* q_pos;      /* [B][Rq], rows contiguous */
+  const void* k_pos;      /* [B][Rk] */
+  int64_t q_pos_stride;   /* element stride of b (0: shared) */
+  int64_t k_pos_stride;
+  const void* base;       /* [B,H,Rq,Rk] or null; last axis contiguous */
+  int64_t base_stride[3]; /* element strides of (b,h,i) */
+  void* out;              /* forward; last axis contiguous */
+  int64_t out_stride[3];
+  const void* d_out;      /* backward; last axis contiguous */
+  int64_t d_out_stride[3];
+  void* dtable;           /* backward: out [buckets][H], dense, written in full */
+  void* workspace;        /* backward: device scratch of at least evoattn_relative_bias_bwd_workspace_bytes() */
+  size_t workspace_bytes;
+} evoattn_relative_bias_params;
+
+int evoattn_relative_bias_fwd(const evoattn_relative_bias_params* p, void* cuda_stream);
+size_t evoattn_relative_bias_bwd_workspace_bytes(const evoattn_relative_bias_params* p);
+int evoattn_relative_bias_bwd(const evoattn_relative_bias_params* p, void* cuda_stream);
+
+/* Pair-bias projection: out[b,h,i,j] = sum_c weight[h,c] * y[b,i,j,c], y the layer norm of pair[b,i,j,:]. */
+#define EVOATTN_PROJECTION_MAX_C 512
+#define EVOATTN_PROJECTION_MAX_H 64
+typedef struct evoattn_pair_projection_params {
+  int32_t dtype;          /* of pair, out, d_out, dpair */
+  int32_t weight_dtype;   /* of weight and dweight */
+  int32_t norm_weight_dtype, norm_bias_dtype;
+  float eps;
+  int32_t B, Ri, Rj, C, H;
+  const void* pair;       /* [B,Ri,Rj,C], C contiguous */
+  int64_t pair_stride[3]; /* element strides of (b,i,j) */
+  const void* weight;     /* [H][C], dense */
+  const void* norm_weight;/* [C] or null (1) */
+  const void* norm_bias;  /* [C] or null (0) */
+  void* out;              /* forward: [B,H,Ri,Rj], last axis contiguous */
+  int64_t out_stride[3];  /* element strides of (b,h,i) */
+  const void* d_out;      /* backward: like out */
+  int64_t d_out_stride[3];
+  void* dpair;            /* out, dense; null: not wanted */
+  void* dweight;          /* out; null: not wanted */
+  void* dnorm_weight;     /* out; null: not wanted */
+  void* dnorm_bias;       /* out; null: not wanted */
+  void* workspace;        /* device scratch of at least evoattn_pair_projection_bwd_workspace_bytes() */
+  size_t workspace_bytes;
+} evoattn_pair_projection_params;
+
+int evoattn_pair_projection_fwd(const evoattn_pair_projection_params* p, void* cuda_stream);
+size_t evoattn_pair_projection_bwd_workspace_bytes(const evoattn_pair_projection_params* p);
+int evoattn_pair_projection_bwd(const evoattn_pair_projection_params* p, void* cuda_stream);
+
 /* EVOATTN_PATH_* of the most recent forward / backward call made by this thread. */
 int evoattn_last_path(void);
 
