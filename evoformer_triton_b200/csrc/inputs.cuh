@@ -31,6 +31,37 @@ __device__ __forceinline__ void store_any(void* p, int dtype, long long i, float
   else static_cast<__half*>(p)[i] = __float2half_rn(v);
 }
 
+// Division of 0 <= n < 2^31 by a number that is the same for a whole launch: n * ceil(2^p / d) >> p with p = 31 + ceil(log2 d);
+// the rounded-up factor is off by less than d <= 2^(p - 31), so n < 2^31 leaves the quotient as it is.
+struct FastDiv {
+  uint32_t d = 1, m = 1u << 31;
+  int p = 31;
+  FastDiv() = default;
+  explicit FastDiv(uint32_t by) : d(by) {
+    while ((1ull << (p - 31)) < by) ++p;
+    m = (uint32_t)(((1ull << p) + by - 1) / by);
+  }
+  __device__ __forceinline__ uint32_t div(uint32_t n) const { return (uint32_t)(((uint64_t)n * m) >> p); }
+};
+
+// Sixteen bytes of T as floats and back.
+template <class T> constexpr int kPer16 = 16 / (int)sizeof(T);
+template <class T>
+__device__ __forceinline__ void unpack16(const uint4& w, float* v) {
+  if constexpr (sizeof(T) == 4) {
+    v[0] = __uint_as_float(w.x); v[1] = __uint_as_float(w.y); v[2] = __uint_as_float(w.z); v[3] = __uint_as_float(w.w);
+  } else {
+    unpack2<T>(w.x, v[0], v[1]); unpack2<T>(w.y, v[2], v[3]); unpack2<T>(w.z, v[4], v[5]); unpack2<T>(w.w, v[6], v[7]);
+  }
+}
+template <class T>
+__device__ __forceinline__ uint4 pack16(const float* v) {
+  if constexpr (sizeof(T) == 4)
+    return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+  else
+    return make_uint4(Pack2<T>::pack(v[0], v[1]), Pack2<T>::pack(v[2], v[3]), Pack2<T>::pack(v[4], v[5]), Pack2<T>::pack(v[6], v[7]));
+}
+
 // The sum over a block of up to 1024 threads, the same for all of them; `sm` holds 32 floats a value.
 template <int N>
 __device__ __forceinline__ void block_sum(float (&v)[N], float* sm) {

@@ -64,24 +64,6 @@ struct Buckets {
   }
 };
 
-// Sixteen bytes of T, or as many single values 32 lanes apart, as floats and back.
-template <class T> constexpr int kPer16 = 16 / (int)sizeof(T);
-template <class T>
-__device__ __forceinline__ void unpack16(const uint4& w, float (&v)[kPer16<T>]) {
-  if constexpr (sizeof(T) == 4) {
-    v[0] = __uint_as_float(w.x); v[1] = __uint_as_float(w.y); v[2] = __uint_as_float(w.z); v[3] = __uint_as_float(w.w);
-  } else {
-    unpack2<T>(w.x, v[0], v[1]); unpack2<T>(w.y, v[2], v[3]); unpack2<T>(w.z, v[4], v[5]); unpack2<T>(w.w, v[6], v[7]);
-  }
-}
-template <class T>
-__device__ __forceinline__ uint4 pack16(const float (&v)[kPer16<T>]) {
-  if constexpr (sizeof(T) == 4)
-    return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
-  else
-    return make_uint4(Pack2<T>::pack(v[0], v[1]), Pack2<T>::pack(v[2], v[3]), Pack2<T>::pack(v[4], v[5]), Pack2<T>::pack(v[6], v[7]));
-}
-
 // Heads that a block of the forward holds the table of.
 constexpr int kHeads = 8;
 // A row of the table in shared memory.  Lanes read rows that lie V = 4 or 8 apart (consecutive keys): one
