@@ -6,6 +6,8 @@
 // walks rows of a strip of keys whose positions stay in registers, so the bucket of a score is worked out
 // once for all heads (forward), or not at all where a whole strip of a row falls into one bucket, as
 // it does away from the diagonal (backward).
+#include <string.h>
+
 #include "inputs.cuh"
 
 namespace evo {
@@ -22,6 +24,7 @@ struct RelArgs {
   const void* k_pos;
   long long sq, sk;
   const void* base;
+  int base_pieces;    // rows of the base are whole pieces too
   Str3 sbase;
   void* out;
   Str3 sout;
@@ -38,138 +41,81 @@ __device__ __forceinline__ long long position(const void* p, bool wide, long lon
   return wide ? static_cast<const long long*>(p)[i] : (long long)static_cast<const int*>(p)[i];
 }
 
-// The table's row for a key `rel` ahead of the query.  edges: shared memory.
+constexpr int kNear = 1024;               // distances whose f is looked up
+constexpr int kFarthest = 1 << 28;        // no edge lies beyond
+
+// The table's row for a key `rel` ahead of the query.  Shared memory: f of the distances below kNear (at most 255: buckets
+// with edges are few), and the edges for the others.  Clipped buckets have no edges and need neither.
 struct Buckets {
   int scheme, exact, n_edges, half;
   const int* edges;
-  __device__ __forceinline__ Buckets(const RelArgs& a, const int* sm_edges)
-      : scheme(a.scheme), exact(a.exact), n_edges(a.n_edges), half(a.buckets >> 1), edges(sm_edges) {}
-  __device__ __forceinline__ int operator()(long long rel) const {
-    const bool ahead = rel > 0;
-    if (scheme == EVOATTN_BUCKETS_LOG_CAUSAL && ahead) return 0;
-    const unsigned long long far = ahead ? (unsigned long long)rel : 0ull - (unsigned long long)rel;
-    const int a = far > 0x3fffffffull ? 0x3fffffff : (int)far;
-    int f = a;
-    if (a >= exact) {
-      int lo = 0, hi = n_edges;  // the number of edges that are <= a
-      while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (edges[mid] <= a) lo = mid + 1;
-        else hi = mid;
-      }
-      f = exact + lo;
+  const uint8_t* near;
+  __device__ __forceinline__ Buckets(const RelArgs& a, const int* sm_edges, const uint8_t* sm_near)
+      : scheme(a.scheme), exact(a.exact), n_edges(a.n_edges), half(a.buckets >> 1), edges(sm_edges), near(sm_near) {}
+  __device__ __forceinline__ int search(int a) const {  // exact + the number of edges that are <= a, for a >= exact
+    int lo = 0, hi = n_edges;
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (edges[mid] <= a) lo = mid + 1;
+      else hi = mid;
     }
-    if (scheme == EVOATTN_BUCKETS_CLIP) return ahead ? exact - f : exact + f;
-    return scheme == EVOATTN_BUCKETS_LOG && ahead ? half + f : f;
+    return exact + lo;
+  }
+  __device__ __forceinline__ int operator()(int rel) const {
+    const bool ahead = rel > 0;
+    const int a = ahead ? rel : -rel;
+    if (scheme == EVOATTN_BUCKETS_CLIP) {
+      const int f = min(a, exact);
+      return ahead ? exact - f : exact + f;
+    }
+    if (scheme == EVOATTN_BUCKETS_LOG_CAUSAL && ahead) return 0;
+    const int f = a < kNear ? near[a] : search(a);
+    return ahead ? half + f : f;
+  }
+  // Positions are 64-bit; differences beyond +-2^30 are all the same to a bucket.
+  static __device__ __forceinline__ int difference(long long key, long long query) {
+    const long long d = key - query;
+    return (int)max(-(1ll << 30), min(1ll << 30, d));
   }
 };
-
-// Heads that a block of the forward holds the table of.
-constexpr int kHeads = 8;
-// A row of the table in shared memory.  Lanes read rows that lie V = 4 or 8 apart (consecutive keys): one
-// float of padding every eight rows keeps them in different banks.
-__host__ __device__ constexpr int slot(int row) { return row + (row >> 3); }
-
-// A block of eight warps takes a strip of 32 V keys and kHeads heads and walks rows, one a warp.  V
-// consecutive keys a lane where rows are 16-byte aligned (WIDE), else keys 32 apart.
-template <class T, bool WIDE>
-__global__ void __launch_bounds__(256) relative_fwd(RelArgs a, int rows_per_block) {
-  ptx::grid_dependency_wait();
-  ptx::grid_launch_dependents();
-  constexpr int V = kPer16<T>;
-  extern __shared__ float sm_table[];  // [kHeads][slot(buckets)]
-  __shared__ int sm_edges[kLogEdges];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int groups = (a.H + kHeads - 1) / kHeads;
-  const int b = blockIdx.z / groups, h0 = (blockIdx.z - b * groups) * kHeads, nh = min(kHeads, a.H - h0);
-  const int pitch = slot(a.buckets) + 1;
-  for (int i = threadIdx.x; i < a.n_edges; i += 256) sm_edges[i] = a.edges[i];
-  for (int i = threadIdx.x; i < a.buckets * nh; i += 256) {
-    const int r = i / nh, h = i - r * nh;
-    sm_table[h * pitch + slot(r)] = load_any(a.table, a.table_dtype, (long long)r * a.H + h0 + h);
-  }
-  const Buckets bucket(a, sm_edges);
-  const int j0 = blockIdx.x * 32 * V;
-  long long key[V];
-  int col[V];
-#pragma unroll
-  for (int u = 0; u < V; ++u) {
-    col[u] = WIDE ? j0 + lane * V + u : j0 + u * 32 + lane;
-    key[u] = col[u] < a.Rk ? position(a.k_pos, a.positions64, b * a.sk + col[u]) : 0;
-  }
-  __syncthreads();
-  const int i_end = (int)min((long long)a.Rq, ((long long)blockIdx.y + 1) * rows_per_block);
-  for (int i = blockIdx.y * rows_per_block + warp; i < i_end; i += 8) {
-    const long long q = position(a.q_pos, a.positions64, b * a.sq + i);
-    int s[V];
-    bool same = true;
-#pragma unroll
-    for (int u = 0; u < V; ++u) {
-      s[u] = slot(bucket(key[u] - q));
-      same = same && s[u] == s[0];
+// Fills the shared memory of Buckets (the caller synchronises).
+__device__ __forceinline__ void prepare_buckets(const RelArgs& a, int* sm_edges, uint8_t* sm_near) {
+  if (a.scheme == EVOATTN_BUCKETS_CLIP) return;
+  for (int i = threadIdx.x; i < a.n_edges; i += blockDim.x) sm_edges[i] = a.edges[i];
+  for (int d = threadIdx.x; d < kNear; d += blockDim.x) {
+    int f = d;
+    if (d >= a.exact) {
+      int lo = 0, hi = a.n_edges;
+      while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (a.edges[mid] <= d) lo = mid + 1;
+        else hi = mid;
+      }
+      f = a.exact + lo;
     }
-    for (int h = 0; h < nh; ++h) {
-      const float* t = sm_table + h * pitch;
-      float v[V];
-      if (same) {
-        v[0] = t[s[0]];
-#pragma unroll
-        for (int u = 1; u < V; ++u) v[u] = v[0];
-      } else {
-#pragma unroll
-        for (int u = 0; u < V; ++u) v[u] = t[s[u]];
-      }
-      if (a.base) {
-        const long long at = b * a.sbase.a + (h0 + h) * a.sbase.b + (long long)i * a.sbase.c;
-#pragma unroll
-        for (int u = 0; u < V; ++u)
-          if (col[u] < a.Rk) v[u] += load_any(a.base, a.base_dtype, at + col[u]);
-      }
-      T* o = static_cast<T*>(a.out) + b * a.sout.a + (h0 + h) * a.sout.b + (long long)i * a.sout.c;
-      if (WIDE && col[V - 1] < a.Rk) {
-        *reinterpret_cast<uint4*>(o + col[0]) = pack16<T>(v);
-      } else {
-#pragma unroll
-        for (int u = 0; u < V; ++u)
-          if (col[u] < a.Rk) o[col[u]] = from_float<T>(v[u]);
-      }
-    }
+    sm_near[d] = (uint8_t)f;
   }
 }
 
-// Backward: a warp takes item_rows rows of a strip of 32 V keys of one (b, h) at a time and adds every value to
-// the sum of its bucket.  Every lane has sums of its own (no two lanes add to one address, and the order
-// of the additions is fixed); a row whose strip is one bucket is added up in a register first.  A block keeps
-// the sums of `window` table rows (blockIdx.z says which); strips that cannot touch them are not read.
-template <class T, bool WIDE>
-__global__ void __launch_bounds__(128) relative_bwd(RelArgs a) {
-  ptx::grid_dependency_wait();
-  ptx::grid_launch_dependents();
-  constexpr int V = kPer16<T>;
-  extern __shared__ float sm_sums[];  // [4 warps][window][32 lanes]
-  __shared__ int sm_edges[kLogEdges];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int h = blockIdx.y, first = blockIdx.z * a.window, count = min(a.window, a.buckets - first);
-  for (int i = threadIdx.x; i < a.n_edges; i += 128) sm_edges[i] = a.edges[i];
-  for (int i = threadIdx.x; i < 4 * a.window * 32; i += 128) sm_sums[i] = 0.f;
-  __syncthreads();
-  const Buckets bucket(a, sm_edges);
-  float* sums = sm_sums + warp * a.window * 32 + lane;
-  const int strips = (a.Rk + 32 * V - 1) / (32 * V), chunks = (a.Rq + a.item_rows - 1) / a.item_rows;
-  const long long items = (long long)a.B * strips * chunks;
-  for (long long item = (long long)blockIdx.x * 4 + warp; item < items; item += (long long)gridDim.x * 4) {
-    const int chunk = (int)(item % chunks);
-    const long long rest = item / chunks;
-    const int strip = (int)(rest % strips), b = (int)(rest / strips);
-    const int j0 = strip * 32 * V, i0 = chunk * a.item_rows, ni = min(a.item_rows, a.Rq - i0);
-    long long key[V], least = 0x7fffffffffffffffll, most = -0x7fffffffffffffffll - 1;
-    int col[V];
+// The keys of a strip that a warp holds, V a lane: consecutive ones (WIDE), or 32 apart.  Positions are kept relative to the
+// least one of the strip, in 32 bits: where they span 2^29 or more, which no sequence does, they are read again
+// for every row.  least - query clamped to +-2^30 plus an offset below 2^29 is on the right side of every edge.
+template <int V, bool WIDE>
+struct Strip {
+  int j0, off[V];
+  long long least, most;
+  bool near_together;
+  __device__ __forceinline__ int col(int u) const { return WIDE ? j0 + (threadIdx.x & 31) * V + u : j0 + u * 32 + (threadIdx.x & 31); }
+  __device__ __forceinline__ void load(const RelArgs& a, int b, int first) {
+    j0 = first;
+    long long key[V];
+    least = 0x7fffffffffffffffll;
+    most = -least - 1;
 #pragma unroll
     for (int u = 0; u < V; ++u) {
-      col[u] = WIDE ? j0 + lane * V + u : j0 + u * 32 + lane;
       key[u] = 0;
-      if (col[u] < a.Rk) {
-        key[u] = position(a.k_pos, a.positions64, b * a.sk + col[u]);
+      if (col(u) < a.Rk) {
+        key[u] = position(a.k_pos, a.positions64, b * a.sk + col(u));
         least = min(least, key[u]);
         most = max(most, key[u]);
       }
@@ -179,41 +125,242 @@ __global__ void __launch_bounds__(128) relative_bwd(RelArgs a) {
       least = min(least, __shfl_xor_sync(0xffffffffu, least, o));
       most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
     }
+    near_together = (unsigned long long)most - (unsigned long long)least < (1ull << 29);
+#pragma unroll
+    for (int u = 0; u < V; ++u) off[u] = col(u) < a.Rk ? (int)(key[u] - least) : 0;  // (wrong where not near_together, and not used)
+  }
+  __device__ __forceinline__ void rows(const RelArgs& a, const Buckets& bucket, int b, long long q, int (&r)[V]) const {
+    if (near_together) {
+      const int from = Buckets::difference(least, q);
+#pragma unroll
+      for (int u = 0; u < V; ++u) r[u] = bucket(from + off[u]);
+    } else {
+#pragma unroll
+      for (int u = 0; u < V; ++u) r[u] = bucket(Buckets::difference(col(u) < a.Rk ? position(a.k_pos, a.positions64, b * a.sk + col(u)) : least, q));
+    }
+  }
+};
+
+// Heads that a block of the forward holds the table of.
+constexpr int kHeads = 8;
+// A row of the table in shared memory.  Lanes read rows that lie V = 4 or 8 apart (consecutive keys): one
+// float of padding every eight rows keeps them in different banks.
+__host__ __device__ constexpr int slot(int row) { return row + (row >> 3); }
+
+// V values of the base at p: in pieces of up to 16 bytes where whole (base_pieces), else one by one.
+template <int V>
+__device__ __forceinline__ void add_base(const RelArgs& a, long long at, float (&v)[V]) {
+  if (a.base_dtype == EVOATTN_FP32) {
+    const float* p = static_cast<const float*>(a.base) + at;
+#pragma unroll
+    for (int k = 0; k < V / 4; ++k) {
+      const float4 w = *reinterpret_cast<const float4*>(p + 4 * k);
+      v[4 * k] += w.x; v[4 * k + 1] += w.y; v[4 * k + 2] += w.z; v[4 * k + 3] += w.w;
+    }
+  } else {
+    const uint16_t* p = static_cast<const uint16_t*>(a.base) + at;
+    uint32_t w[V / 2];
+    if constexpr (V == 8) *reinterpret_cast<uint4*>(w) = *reinterpret_cast<const uint4*>(p);
+    else *reinterpret_cast<uint2*>(w) = *reinterpret_cast<const uint2*>(p);
+#pragma unroll
+    for (int k = 0; k < V / 2; ++k) {
+      float lo, hi;
+      if (a.base_dtype == EVOATTN_BF16) unpack2<__nv_bfloat16>(w[k], lo, hi);
+      else unpack2<__half>(w[k], lo, hi);
+      v[2 * k] += lo;
+      v[2 * k + 1] += hi;
+    }
+  }
+}
+
+// A block of eight warps takes a strip of 32 V keys and kHeads heads and walks rows; with fewer rows than warps, the warps
+// share the heads of a row.  A row whose strip is one bucket, as away from the diagonal, is one value a head.
+template <class T, bool WIDE>
+__global__ void __launch_bounds__(256) relative_fwd(RelArgs a, int rows_per_block, int row_warps) {
+  ptx::grid_dependency_wait();
+  ptx::grid_launch_dependents();
+  constexpr int V = kPer16<T>;
+  extern __shared__ float sm_table[];  // [kHeads][slot(buckets)]
+  __shared__ int sm_edges[kLogEdges];
+  __shared__ uint8_t sm_near[kNear];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int groups = (a.H + kHeads - 1) / kHeads;
+  const int b = blockIdx.z / groups, h0 = (blockIdx.z - b * groups) * kHeads, nh = min(kHeads, a.H - h0);
+  const int pitch = slot(a.buckets) + 1;
+  Strip<V, WIDE> strip;
+  strip.load(a, b, blockIdx.x * 32 * V);
+  // lane l: the warp's l-th row (at most 32 of them)
+  const int i0 = blockIdx.y * rows_per_block + warp % row_warps, i_end = (int)min((long long)a.Rq, ((long long)blockIdx.y + 1) * rows_per_block);
+  const int my_i = i0 + lane * row_warps;
+  const long long my_q = my_i < i_end ? position(a.q_pos, a.positions64, b * a.sq + my_i) : 0;
+  prepare_buckets(a, sm_edges, sm_near);
+  for (int i = threadIdx.x; i < a.buckets * nh; i += 256) {
+    const int r = i / nh, h = i - r * nh;
+    sm_table[h * pitch + slot(r)] = load_any(a.table, a.table_dtype, (long long)r * a.H + h0 + h);
+  }
+  __syncthreads();
+  const Buckets bucket(a, sm_edges, sm_near);
+  const int lo = bucket(Buckets::difference(strip.least, my_q)), hi = bucket(Buckets::difference(strip.most, my_q));
+  const int my_kind = lo == hi ? slot(lo) : -1;  // (rows are in the order of distances on either side, so all between are the same)
+  const int first_head = warp / row_warps, head_step = 8 / row_warps;
+  for (int k = 0, i = i0; i < i_end; ++k, i += row_warps) {
+    const int kind = __shfl_sync(0xffffffffu, my_kind, k);
+    const long long q = __shfl_sync(0xffffffffu, my_q, k);
+    int s[V];
+    if (kind < 0) {
+      strip.rows(a, bucket, b, q, s);
+#pragma unroll
+      for (int u = 0; u < V; ++u) s[u] = slot(s[u]);
+    }
+    T* o = static_cast<T*>(a.out) + b * a.sout.a + (h0 + first_head) * a.sout.b + (long long)i * a.sout.c;
+    long long at = b * a.sbase.a + (h0 + first_head) * a.sbase.b + (long long)i * a.sbase.c;
+    const bool whole = WIDE && strip.col(V - 1) < a.Rk;
+    for (int h = first_head; h < nh; h += head_step, o += head_step * a.sout.b, at += head_step * a.sbase.b) {
+      const float* t = sm_table + h * pitch;
+      float v[V];
+      if (kind >= 0) {
+        v[0] = t[kind];
+#pragma unroll
+        for (int u = 1; u < V; ++u) v[u] = v[0];
+      } else {
+#pragma unroll
+        for (int u = 0; u < V; ++u) v[u] = t[s[u]];
+      }
+      if (whole && (!a.base || a.base_pieces)) {
+        if (a.base) add_base<V>(a, at + strip.col(0), v);
+        *reinterpret_cast<uint4*>(o + strip.col(0)) = pack16<T>(v);
+      } else {
+#pragma unroll
+        for (int u = 0; u < V; ++u) {
+          if (strip.col(u) >= a.Rk) continue;
+          if (a.base) v[u] += load_any(a.base, a.base_dtype, at + strip.col(u));
+          o[strip.col(u)] = from_float<T>(v[u]);
+        }
+      }
+    }
+  }
+}
+
+// Backward: a warp takes item_rows rows of a strip of 32 V keys of one (b, h) at a time and adds every value to
+// the sum of its bucket.  Every lane has sums of its own (no two lanes add to one address, and the order
+// of the additions is fixed); rows whose strip is one bucket are added up in a register first.  A block keeps
+// the sums of `window` table rows (blockIdx.z says which); strips that cannot touch them are not read.
+template <class T, bool WIDE>
+struct RowPiece {  // V values of a row
+  static constexpr int V = kPer16<T>;
+  uint4 w;
+  T e[V];
+  __device__ __forceinline__ void load(const RelArgs& a, const Strip<V, WIDE>& strip, const T* row) {
+    if (WIDE && strip.col(V - 1) < a.Rk) {
+      w = *reinterpret_cast<const uint4*>(row + strip.col(0));
+    } else {
+#pragma unroll
+      for (int u = 0; u < V; ++u) e[u] = strip.col(u) < a.Rk ? row[strip.col(u)] : from_float<T>(0.f);
+      if constexpr (WIDE) memcpy(&w, e, 16);
+    }
+  }
+  __device__ __forceinline__ void floats(float (&v)[V]) const {
+    if constexpr (WIDE) unpack16<T>(w, v);
+    else {
+#pragma unroll
+      for (int u = 0; u < V; ++u) v[u] = to_float<T>(e[u]);
+    }
+  }
+  __device__ __forceinline__ float sum() const {
+    float v[V];
+    floats(v);
+#pragma unroll
+    for (int n = V / 2; n > 0; n /= 2)
+#pragma unroll
+      for (int u = 0; u < n; ++u) v[u] += v[u + n];
+    return v[0];
+  }
+};
+
+template <class T, bool WIDE>
+__global__ void __launch_bounds__(128) relative_bwd(RelArgs a) {
+  ptx::grid_dependency_wait();
+  ptx::grid_launch_dependents();
+  constexpr int V = kPer16<T>, U = 4;  // U: rows on the way at once
+  extern __shared__ float sm_sums[];  // [4 warps][window][32 lanes]
+  __shared__ int sm_edges[kLogEdges];
+  __shared__ uint8_t sm_near[kNear];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int h = blockIdx.y, first = blockIdx.z * a.window, count = min(a.window, a.buckets - first);
+  prepare_buckets(a, sm_edges, sm_near);
+  for (int i = threadIdx.x; i < 4 * a.window * 32; i += 128) sm_sums[i] = 0.f;
+  __syncthreads();
+  const Buckets bucket(a, sm_edges, sm_near);
+  float* sums = sm_sums + warp * a.window * 32 + lane;
+  const int strips = (a.Rk + 32 * V - 1) / (32 * V), chunks = (a.Rq + a.item_rows - 1) / a.item_rows;
+  const long long items = (long long)a.B * strips * chunks;
+  for (long long item = (long long)blockIdx.x * 4 + warp; item < items; item += (long long)gridDim.x * 4) {
+    const int chunk = (int)(item % chunks);
+    const long long rest = item / chunks;
+    const int i0 = chunk * a.item_rows, ni = min(a.item_rows, a.Rq - i0), b = (int)(rest / strips);
+    Strip<V, WIDE> strip;
+    strip.load(a, b, (int)(rest % strips) * 32 * V);
     // lane l: what row i0 + l of the strip is: one bucket (>= 0), several (-1), none of this block's (-2)
     const long long my_q = lane < ni ? position(a.q_pos, a.positions64, b * a.sq + i0 + lane) : 0;
     int my_kind = -2;
     if (lane < ni) {
-      const int lo = bucket(least - my_q), hi = bucket(most - my_q);
-      my_kind = lo == hi ? (lo >= first && lo < first + count ? lo : -2) : -1;
+      const int from = Buckets::difference(strip.least, my_q), to = Buckets::difference(strip.most, my_q);
+      const int lo = bucket(from), hi = bucket(to);
+      // between the two are the buckets of all others, but for LOG, whose upper half begins behind the query
+      const bool ordered = a.scheme != EVOATTN_BUCKETS_LOG || from > 0 || to <= 0;
+      my_kind = ordered && (max(lo, hi) < first || min(lo, hi) >= first + count) ? -2 : lo == hi ? lo : -1;
     }
     const T* d = static_cast<const T*>(a.out) + b * a.sout.a + h * a.sout.b + (long long)i0 * a.sout.c;
+    const int kind0 = __shfl_sync(0xffffffffu, my_kind, 0);
     float acc = 0.f;
-    int acc_row = -1;
-    for (int i = 0; i < ni; ++i) {
-      const int kind = __shfl_sync(0xffffffffu, my_kind, i);
-      const long long q = __shfl_sync(0xffffffffu, my_q, i);
-      if (kind == -2) continue;
-      const T* row = d + i * a.sout.c;
-      float v[V];
-      if (WIDE && col[V - 1] < a.Rk) {
-        unpack16<T>(*reinterpret_cast<const uint4*>(row + col[0]), v);
-      } else {
+    if (kind0 != -1 && __all_sync(0xffffffffu, lane >= ni || my_kind == kind0)) {  // one bucket altogether
+      if (kind0 == -2) continue;
+      int i = 0;
+      for (; i + 2 * U <= ni; i += 2 * U) {
+        RowPiece<T, WIDE> p[2 * U];
 #pragma unroll
-        for (int u = 0; u < V; ++u) v[u] = col[u] < a.Rk ? to_float<T>(row[col[u]]) : 0.f;
+        for (int k = 0; k < 2 * U; ++k) p[k].load(a, strip, d + (i + k) * a.sout.c);
+#pragma unroll
+        for (int k = 0; k < 2 * U; ++k) acc += p[k].sum();
       }
-      if (kind >= 0) {
-        if (kind != acc_row) {
-          if (acc_row >= 0) sums[(acc_row - first) * 32] += acc;
-          acc_row = kind;
-          acc = 0.f;
-        }
+      for (; i < ni; ++i) {
+        RowPiece<T, WIDE> p;
+        p.load(a, strip, d + i * a.sout.c);
+        acc += p.sum();
+      }
+      sums[(kind0 - first) * 32] += acc;
+      continue;
+    }
+    int acc_row = -1;
+    RowPiece<T, WIDE> next[U];
+    const auto fetch = [&](int k, int i) {
+      if (i < ni && __shfl_sync(0xffffffffu, my_kind, i & 31) != -2) next[k].load(a, strip, d + i * a.sout.c);
+    };
 #pragma unroll
-        for (int u = 0; u < V; ++u) acc += v[u];
-      } else {
+    for (int k = 0; k < U; ++k) fetch(k, k);
+    for (int i = 0; i < ni; i += U) {
 #pragma unroll
-        for (int u = 0; u < V; ++u) {
-          const int r = bucket(key[u] - q) - first;
-          if (col[u] < a.Rk && r >= 0 && r < count) sums[r * 32] += v[u];
+      for (int k = 0; k < U; ++k) {
+        if (i + k >= ni) break;
+        const int kind = __shfl_sync(0xffffffffu, my_kind, i + k);
+        const long long q = __shfl_sync(0xffffffffu, my_q, i + k);
+        const RowPiece<T, WIDE> p = next[k];
+        fetch(k, i + k + U);
+        if (kind >= 0) {
+          if (kind != acc_row) {
+            if (acc_row >= 0) sums[(acc_row - first) * 32] += acc;
+            acc_row = kind;
+            acc = 0.f;
+          }
+          acc += p.sum();
+        } else if (kind == -1) {
+          float v[V];
+          int r[V];
+          p.floats(v);
+          strip.rows(a, bucket, b, q, r);
+#pragma unroll
+          for (int u = 0; u < V; ++u)
+            if (strip.col(u) < a.Rk && (unsigned)(r[u] - first) < (unsigned)count) sums[(r[u] - first) * 32] += v[u];
         }
       }
     }
@@ -252,13 +399,14 @@ int validate(const evoattn_relative_bias_params* p) {
   if (!p) return EVOATTN_ERR_NULL;
   if (!known_dtype(p->dtype) || !known_dtype(p->table_dtype) || (p->base && !known_dtype(p->base_dtype))) return EVOATTN_ERR_DTYPE;
   if (p->B < 0 || p->H <= 0 || p->Rq < 0 || p->Rk < 0 || p->B > 65535 || p->H > 4096) return EVOATTN_ERR_SHAPE;
-  if (p->Rq > (1 << 24) || p->Rk > (1 << 24)) return EVOATTN_ERR_SHAPE;
+  if (p->Rq > (1 << 23) || p->Rk > (1 << 23)) return EVOATTN_ERR_SHAPE;
   if ((long long)p->B * ((p->H + kHeads - 1) / kHeads) > 65535) return EVOATTN_ERR_SHAPE;
   if (p->buckets <= 0 || p->buckets > EVOATTN_MAX_BUCKETS || p->n_edges < 0 || p->n_edges > kLogEdges || p->exact < 0) return EVOATTN_ERR_SHAPE;
   if (p->n_edges > 0 && !p->edges) return EVOATTN_ERR_NULL;
   for (int i = 0; i < p->n_edges; ++i)  // a distance finds its bucket by bisection
-    if (p->edges[i] < p->exact || (i && p->edges[i] < p->edges[i - 1])) return EVOATTN_ERR_SHAPE;
+    if (p->edges[i] < p->exact || p->edges[i] > kFarthest || (i && p->edges[i] < p->edges[i - 1])) return EVOATTN_ERR_SHAPE;
   const int most = p->exact + p->n_edges;  // the largest f
+  if (p->scheme != EVOATTN_BUCKETS_CLIP && most > 255) return EVOATTN_ERR_SHAPE;  // (kept in bytes)
   switch (p->scheme) {
     case EVOATTN_BUCKETS_CLIP: return p->n_edges == 0 && p->buckets == 2 * p->exact + 1 ? EVOATTN_OK : EVOATTN_ERR_SHAPE;
     case EVOATTN_BUCKETS_LOG: return p->buckets % 2 == 0 && most < p->buckets / 2 ? EVOATTN_OK : EVOATTN_ERR_SHAPE;
@@ -308,17 +456,25 @@ int evoattn_relative_bias_fwd(const evoattn_relative_bias_params* p, void* cuda_
   a.out = p->out;
   a.sout = Str3{p->out_stride[0], p->out_stride[1], p->out_stride[2]};
   const int es = dtype_bytes(p->dtype);
-  const bool wide = rows_of_16_bytes(p->out, p->out_stride, es);
   const int strips = (a.Rk + 512 / es - 1) / (512 / es), groups = (a.H + kHeads - 1) / kHeads;
   int rows = 64;
   while (rows > 8 && (long long)strips * ((a.Rq + rows - 1) / rows) * a.B * groups < 148 * 4) rows /= 2;
-  if ((a.Rq + rows - 1) / rows > 65535) rows = (a.Rq + 65534) / 65535;
+  while ((a.Rq + rows - 1) / rows > 65535) rows *= 2;
+  int row_warps = 8;
+  while (row_warps > 1 && a.Rq <= row_warps / 2) row_warps /= 2;
   const dim3 grid((unsigned)strips, (unsigned)((a.Rq + rows - 1) / rows), (unsigned)(a.B * groups));
   const size_t smem = (size_t)(a.H < kHeads ? a.H : kHeads) * (slot(a.buckets) + 1) * sizeof(float);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(cuda_stream);
   return with_dtype(p->dtype, [&](auto e) {
     using T = decltype(e);
-    const cudaError_t rc = wide ? launch_dependent(relative_fwd<T, true>, grid, 256, smem, st, a, rows) : launch_dependent(relative_fwd<T, false>, grid, 256, smem, st, a, rows);
+    if (p->base) {  // V values of a lane in whole pieces of the base, too
+      const int piece = (int)(kPer16<T> * dtype_bytes(p->base_dtype) < 16 ? kPer16<T> * dtype_bytes(p->base_dtype) : 16);
+      a.base_pieces = ((uintptr_t)p->base | (uintptr_t)(p->base_stride[0] * dtype_bytes(p->base_dtype)) | (uintptr_t)(p->base_stride[1] * dtype_bytes(p->base_dtype)) |
+                       (uintptr_t)(p->base_stride[2] * dtype_bytes(p->base_dtype))) % piece == 0;
+    }
+    const bool wide = rows_of_16_bytes(p->out, p->out_stride, (int)sizeof(T)) && (!p->base || a.base_pieces);
+    const cudaError_t rc = wide ? launch_dependent(relative_fwd<T, true>, grid, 256, smem, st, a, rows, row_warps)
+                                : launch_dependent(relative_fwd<T, false>, grid, 256, smem, st, a, rows, row_warps);
     return rc == cudaSuccess ? EVOATTN_OK : EVOATTN_ERR_CUDA;
   });
 }
