@@ -104,7 +104,7 @@ template <int V, bool WIDE>
 struct Strip {
   int j0, off[V];
   long long least, most;
-  bool near_together;
+  bool near_together, in_order;  // in_order: every lane's keys ascend, so those of one bucket are next to each other
   __device__ __forceinline__ int col(int u) const { return WIDE ? j0 + (threadIdx.x & 31) * V + u : j0 + u * 32 + (threadIdx.x & 31); }
   __device__ __forceinline__ void load(const RelArgs& a, int b, int first) {
     j0 = first;
@@ -126,8 +126,13 @@ struct Strip {
       most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
     }
     near_together = (unsigned long long)most - (unsigned long long)least < (1ull << 29);
+    bool ascending = near_together;
 #pragma unroll
-    for (int u = 0; u < V; ++u) off[u] = col(u) < a.Rk ? (int)(key[u] - least) : 0;  // (wrong where not near_together, and not used)
+    for (int u = 0; u < V; ++u) {
+      off[u] = (int)((col(u) < a.Rk ? key[u] : most) - least);  // (wrong where not near_together, and not used)
+      ascending = ascending && (u == 0 || off[u] >= off[u ? u - 1 : 0]);
+    }
+    in_order = __all_sync(0xffffffffu, ascending);
   }
   __device__ __forceinline__ void rows(const RelArgs& a, const Buckets& bucket, int b, long long q, int (&r)[V]) const {
     if (near_together) {
@@ -358,9 +363,25 @@ __global__ void __launch_bounds__(128) relative_bwd(RelArgs a) {
           int r[V];
           p.floats(v);
           strip.rows(a, bucket, b, q, r);
+          if (strip.in_order) {  // values of one bucket first, then all sums at once
+            bool last[V];
+            float old[V];
 #pragma unroll
-          for (int u = 0; u < V; ++u)
-            if (strip.col(u) < a.Rk && (unsigned)(r[u] - first) < (unsigned)count) sums[(r[u] - first) * 32] += v[u];
+            for (int u = 0; u < V; ++u) {
+              last[u] = (u == V - 1 || r[u + 1 < V ? u + 1 : u] != r[u]) && (unsigned)(r[u] - first) < (unsigned)count;
+              if (u + 1 < V && r[u + 1 < V ? u + 1 : u] == r[u]) v[u + 1 < V ? u + 1 : u] += v[u];
+              r[u] = (r[u] - first) * 32;
+            }
+#pragma unroll
+            for (int u = 0; u < V; ++u) old[u] = last[u] ? sums[r[u]] : 0.f;
+#pragma unroll
+            for (int u = 0; u < V; ++u)
+              if (last[u]) sums[r[u]] = old[u] + v[u];
+          } else {
+#pragma unroll
+            for (int u = 0; u < V; ++u)
+              if (strip.col(u) < a.Rk && (unsigned)(r[u] - first) < (unsigned)count) sums[(r[u] - first) * 32] += v[u];
+          }
         }
       }
     }
@@ -436,7 +457,7 @@ void plan_bwd(RelArgs* a, int es) {
   a->item_rows = 32;
   const auto items = [&] { return (long long)a->B * strips * ((a->Rq + a->item_rows - 1) / a->item_rows); };
   while (a->item_rows > 4 && items() * a->H < 148 * 16) a->item_rows /= 2;
-  const long long blocks = (items() + 3) / 4, most = (148 * 6 + a->H - 1) / a->H;
+  const long long blocks = (items() + 3) / 4, most = 148 * 5 / a->H > 1 ? 148 * 5 / a->H : 1;
   a->blocks = (int)(blocks < most ? blocks : most);
 }
 
