@@ -41,71 +41,63 @@ __device__ __forceinline__ long long position(const void* p, bool wide, long lon
   return wide ? static_cast<const long long*>(p)[i] : (long long)static_cast<const int*>(p)[i];
 }
 
-constexpr int kNear = 1024;               // distances whose f is looked up
+constexpr int kNear = 1024;               // differences up to here are looked up
 constexpr int kFarthest = 1 << 28;        // no edge lies beyond
 
-// The table's row for a key `rel` ahead of the query.  Shared memory: f of the distances below kNear (at most 255: buckets
-// with edges are few), and the edges for the others.  Clipped buckets have no edges and need neither.
-struct Buckets {
-  int scheme, exact, n_edges, half;
-  const int* edges;
-  const uint8_t* near;
-  __device__ __forceinline__ Buckets(const RelArgs& a, const int* sm_edges, const uint8_t* sm_near)
-      : scheme(a.scheme), exact(a.exact), n_edges(a.n_edges), half(a.buckets >> 1), edges(sm_edges), near(sm_near) {}
-  __device__ __forceinline__ int search(int a) const {  // exact + the number of edges that are <= a, for a >= exact
-    int lo = 0, hi = n_edges;
-    while (lo < hi) {
-      const int mid = (lo + hi) >> 1;
-      if (edges[mid] <= a) lo = mid + 1;
-      else hi = mid;
-    }
-    return exact + lo;
-  }
-  __device__ __forceinline__ int operator()(int rel) const {
-    const bool ahead = rel > 0;
-    const int a = ahead ? rel : -rel;
-    if (scheme == EVOATTN_BUCKETS_CLIP) {
-      const int f = min(a, exact);
-      return ahead ? exact - f : exact + f;
-    }
-    if (scheme == EVOATTN_BUCKETS_LOG_CAUSAL && ahead) return 0;
-    const int f = a < kNear ? near[a] : search(a);
-    return ahead ? half + f : f;
-  }
-  // Positions are 64-bit; differences beyond +-2^30 are all the same to a bucket.
-  static __device__ __forceinline__ int difference(long long key, long long query) {
-    const long long d = key - query;
-    return (int)max(-(1ll << 30), min(1ll << 30, d));
-  }
-};
-// Fills the shared memory of Buckets (the caller synchronises).
-__device__ __forceinline__ void prepare_buckets(const RelArgs& a, int* sm_edges, uint8_t* sm_near) {
-  if (a.scheme == EVOATTN_BUCKETS_CLIP) return;
-  for (int i = threadIdx.x; i < a.n_edges; i += blockDim.x) sm_edges[i] = a.edges[i];
-  for (int d = threadIdx.x; d < kNear; d += blockDim.x) {
-    int f = d;
-    if (d >= a.exact) {
-      int lo = 0, hi = a.n_edges;
-      while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (a.edges[mid] <= d) lo = mid + 1;
-        else hi = mid;
-      }
-      f = a.exact + lo;
-    }
-    sm_near[d] = (uint8_t)f;
-  }
+// Positions are 64-bit; differences beyond +-2^30 are all the same to a bucket.
+__device__ __forceinline__ int difference(long long key, long long query) {
+  const long long d = key - query;
+  return (int)max(-(1ll << 30), min(1ll << 30, d));
 }
 
-// The keys of a strip that a warp holds, V a lane: consecutive ones (WIDE), or 32 apart.  Positions are kept relative to the
+// The table's row for a key `rel` ahead of the query.
+__device__ __forceinline__ int bucket_row(const RelArgs& a, int rel) {
+  const bool ahead = rel > 0;
+  const int d = ahead ? rel : -rel;
+  if (a.scheme == EVOATTN_BUCKETS_CLIP) {
+    const int f = min(d, a.exact);
+    return ahead ? a.exact - f : a.exact + f;
+  }
+  if (a.scheme == EVOATTN_BUCKETS_LOG_CAUSAL && ahead) return 0;
+  int f = d;
+  if (d >= a.exact) {
+    int lo = 0, hi = a.n_edges;  // the number of edges that are <= d
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (a.edges[mid] <= d) lo = mid + 1;
+      else hi = mid;
+    }
+    f = a.exact + lo;
+  }
+  return ahead ? (a.buckets >> 1) + f : f;
+}
+
+// The same looked up, as MAP puts it: differences beyond `far` have the bucket of `far`.  Edges beyond kNear are searched.
+template <class MAP>
+struct Buckets {
+  const RelArgs& a;
+  const uint16_t* near;  // shared memory, [2 far + 1]
+  int far;               // 0: not looked up
+  __device__ __forceinline__ Buckets(const RelArgs& args, uint16_t* sm_near) : a(args), near(sm_near) {
+    const int last = a.scheme == EVOATTN_BUCKETS_CLIP ? a.exact : a.n_edges ? a.edges[a.n_edges - 1] : a.exact;
+    far = last <= kNear ? max(last, 1) : 0;
+    if (far)
+      for (int i = threadIdx.x; i < 2 * far + 1; i += blockDim.x) sm_near[i] = (uint16_t)MAP::of(bucket_row(a, i - far));
+  }  // (the caller synchronises)
+  __device__ __forceinline__ int operator()(int rel) const {
+    return far ? near[min(max(rel, -far), far) + far] : MAP::of(bucket_row(a, rel));
+  }
+};
+
+// The keys of a strip of L V keys that L lanes hold, V each: consecutive ones (WIDE), or L apart.  Positions are kept relative to the
 // least one of the strip, in 32 bits: where they span 2^29 or more, which no sequence does, they are read again
 // for every row.  least - query clamped to +-2^30 plus an offset below 2^29 is on the right side of every edge.
-template <int V, bool WIDE>
+template <int V, int L, bool WIDE>
 struct Strip {
   int j0, off[V];
   long long least, most;
   bool near_together, in_order;  // in_order: every lane's keys ascend, so those of one bucket are next to each other
-  __device__ __forceinline__ int col(int u) const { return WIDE ? j0 + (threadIdx.x & 31) * V + u : j0 + u * 32 + (threadIdx.x & 31); }
+  __device__ __forceinline__ int col(int u) const { return WIDE ? j0 + (threadIdx.x & (L - 1)) * V + u : j0 + u * L + (threadIdx.x & (L - 1)); }
   __device__ __forceinline__ void load(const RelArgs& a, int b, int first) {
     j0 = first;
     long long key[V];
@@ -121,7 +113,7 @@ struct Strip {
       }
     }
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
+    for (int o = L / 2; o > 0; o >>= 1) {
       least = min(least, __shfl_xor_sync(0xffffffffu, least, o));
       most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
     }
@@ -134,14 +126,16 @@ struct Strip {
     }
     in_order = __all_sync(0xffffffffu, ascending);
   }
-  __device__ __forceinline__ void rows(const RelArgs& a, const Buckets& bucket, int b, long long q, int (&r)[V]) const {
-    if (near_together) {
-      const int from = Buckets::difference(least, q);
+  // The rows of the table for the query at q, from = difference(least, q).
+  template <class MAP>
+  __device__ __forceinline__ void rows(const RelArgs& a, const Buckets<MAP>& bucket, int b, long long q, int from, int (&r)[V]) const {
+    if (near_together && bucket.far) {
+      from += bucket.far;
 #pragma unroll
-      for (int u = 0; u < V; ++u) r[u] = bucket(from + off[u]);
+      for (int u = 0; u < V; ++u) r[u] = bucket.near[min(max(from + off[u], 0), 2 * bucket.far)];
     } else {
-#pragma unroll
-      for (int u = 0; u < V; ++u) r[u] = bucket(Buckets::difference(col(u) < a.Rk ? position(a.k_pos, a.positions64, b * a.sk + col(u)) : least, q));
+#pragma unroll 1
+      for (int u = 0; u < V; ++u) r[u] = bucket(difference(col(u) < a.Rk ? position(a.k_pos, a.positions64, b * a.sk + col(u)) : least, q));
     }
   }
 };
@@ -151,6 +145,8 @@ constexpr int kHeads = 8;
 // A row of the table in shared memory.  Lanes read rows that lie V = 4 or 8 apart (consecutive keys): one
 // float of padding every eight rows keeps them in different banks.
 __host__ __device__ constexpr int slot(int row) { return row + (row >> 3); }
+struct Slot { static __device__ __forceinline__ int of(int row) { return slot(row); } };
+struct Same { static __device__ __forceinline__ int of(int row) { return row; } };
 
 // V values of the base at p: in pieces of up to 16 bytes where whole (base_pieces), else one by one.
 template <int V>
@@ -186,36 +182,32 @@ __global__ void __launch_bounds__(256) relative_fwd(RelArgs a, int rows_per_bloc
   ptx::grid_launch_dependents();
   constexpr int V = kPer16<T>;
   extern __shared__ float sm_table[];  // [kHeads][slot(buckets)]
-  __shared__ int sm_edges[kLogEdges];
-  __shared__ uint8_t sm_near[kNear];
+  __shared__ uint16_t sm_near[2 * kNear + 1];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int groups = (a.H + kHeads - 1) / kHeads;
   const int b = blockIdx.z / groups, h0 = (blockIdx.z - b * groups) * kHeads, nh = min(kHeads, a.H - h0);
   const int pitch = slot(a.buckets) + 1;
-  Strip<V, WIDE> strip;
+  Strip<V, 32, WIDE> strip;
   strip.load(a, b, blockIdx.x * 32 * V);
   // lane l: the warp's l-th row (at most 32 of them)
   const int i0 = blockIdx.y * rows_per_block + warp % row_warps, i_end = (int)min((long long)a.Rq, ((long long)blockIdx.y + 1) * rows_per_block);
   const int my_i = i0 + lane * row_warps;
   const long long my_q = my_i < i_end ? position(a.q_pos, a.positions64, b * a.sq + my_i) : 0;
-  prepare_buckets(a, sm_edges, sm_near);
+  const Buckets<Slot> bucket(a, sm_near);
   for (int i = threadIdx.x; i < a.buckets * nh; i += 256) {
     const int r = i / nh, h = i - r * nh;
     sm_table[h * pitch + slot(r)] = load_any(a.table, a.table_dtype, (long long)r * a.H + h0 + h);
   }
   __syncthreads();
-  const Buckets bucket(a, sm_edges, sm_near);
-  const int lo = bucket(Buckets::difference(strip.least, my_q)), hi = bucket(Buckets::difference(strip.most, my_q));
-  const int my_kind = lo == hi ? slot(lo) : -1;  // (rows are in the order of distances on either side, so all between are the same)
+  const int lo = bucket(difference(strip.least, my_q)), hi = bucket(difference(strip.most, my_q));
+  const int my_kind = lo == hi ? lo : -1;  // (rows are in the order of distances on either side, so all between are the same)
   const int first_head = warp / row_warps, head_step = 8 / row_warps;
   for (int k = 0, i = i0; i < i_end; ++k, i += row_warps) {
     const int kind = __shfl_sync(0xffffffffu, my_kind, k);
     const long long q = __shfl_sync(0xffffffffu, my_q, k);
     int s[V];
     if (kind < 0) {
-      strip.rows(a, bucket, b, q, s);
-#pragma unroll
-      for (int u = 0; u < V; ++u) s[u] = slot(s[u]);
+      strip.rows(a, bucket, b, q, difference(strip.least, q), s);
     }
     T* o = static_cast<T*>(a.out) + b * a.sout.a + (h0 + first_head) * a.sout.b + (long long)i * a.sout.c;
     long long at = b * a.sbase.a + (h0 + first_head) * a.sbase.b + (long long)i * a.sbase.c;
@@ -246,16 +238,19 @@ __global__ void __launch_bounds__(256) relative_fwd(RelArgs a, int rows_per_bloc
   }
 }
 
-// Backward: a warp takes item_rows rows of a strip of 32 V keys of one (b, h) at a time and adds every value to
-// the sum of its bucket.  Every lane has sums of its own (no two lanes add to one address, and the order
-// of the additions is fixed); rows whose strip is one bucket are added up in a register first.  A block keeps
-// the sums of `window` table rows (blockIdx.z says which); strips that cannot touch them are not read.
+// Backward: a warp takes item_rows rows of a strip of keys of one (b, h) at a time and adds every value to the sum of its
+// bucket.  Every lane has sums of its own (no two lanes add to one address, and the order of the additions is fixed).  A
+// load is kLanes V keys of kTall rows, 128 bytes of each: as near to a square as whole cache lines go, so that few loads lie across
+// the diagonal; the others are one bucket and are added up in a register.  A block keeps the sums of `window` table rows
+// (blockIdx.z says which); loads that cannot touch them are left out.
+constexpr int kLanes = 8, kTall = 32 / kLanes;
+
 template <class T, bool WIDE>
 struct RowPiece {  // V values of a row
   static constexpr int V = kPer16<T>;
   uint4 w;
   T e[V];
-  __device__ __forceinline__ void load(const RelArgs& a, const Strip<V, WIDE>& strip, const T* row) {
+  __device__ __forceinline__ void load(const RelArgs& a, const Strip<V, kLanes, WIDE>& strip, const T* row) {
     if (WIDE && strip.col(V - 1) < a.Rk) {
       w = *reinterpret_cast<const uint4*>(row + strip.col(0));
     } else {
@@ -263,6 +258,11 @@ struct RowPiece {  // V values of a row
       for (int u = 0; u < V; ++u) e[u] = strip.col(u) < a.Rk ? row[strip.col(u)] : from_float<T>(0.f);
       if constexpr (WIDE) memcpy(&w, e, 16);
     }
+  }
+  __device__ __forceinline__ void clear() {
+    w = make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int u = 0; u < V; ++u) e[u] = from_float<T>(0.f);
   }
   __device__ __forceinline__ void floats(float (&v)[V]) const {
     if constexpr (WIDE) unpack16<T>(w, v);
@@ -283,105 +283,126 @@ struct RowPiece {  // V values of a row
 };
 
 template <class T, bool WIDE>
-__global__ void __launch_bounds__(128) relative_bwd(RelArgs a) {
+__global__ void __launch_bounds__(128, 5) relative_bwd(RelArgs a) {
   ptx::grid_dependency_wait();
   ptx::grid_launch_dependents();
-  constexpr int V = kPer16<T>, U = 4;  // U: rows on the way at once
-  extern __shared__ float sm_sums[];  // [4 warps][window][32 lanes]
-  __shared__ int sm_edges[kLogEdges];
-  __shared__ uint8_t sm_near[kNear];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  constexpr int V = kPer16<T>, U = WIDE ? 8 : 4;  // U: loads on the way at once
+  extern __shared__ float sm_sums[];  // [4 warps][window + 1][32 lanes]
+  __shared__ uint16_t sm_near[2 * kNear + 1];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, my_row = lane / kLanes;
   const int h = blockIdx.y, first = blockIdx.z * a.window, count = min(a.window, a.buckets - first);
-  prepare_buckets(a, sm_edges, sm_near);
-  for (int i = threadIdx.x; i < 4 * a.window * 32; i += 128) sm_sums[i] = 0.f;
+  const Buckets<Same> bucket(a, sm_near);
+  const int per_warp = (a.window + 1) * 32;  // (one more row, for what is not of this block's)
+  for (int i = threadIdx.x; i < 4 * per_warp; i += 128) sm_sums[i] = 0.f;
   __syncthreads();
-  const Buckets bucket(a, sm_edges, sm_near);
-  float* sums = sm_sums + warp * a.window * 32 + lane;
-  const int strips = (a.Rk + 32 * V - 1) / (32 * V), chunks = (a.Rq + a.item_rows - 1) / a.item_rows;
-  const long long items = (long long)a.B * strips * chunks;
-  for (long long item = (long long)blockIdx.x * 4 + warp; item < items; item += (long long)gridDim.x * 4) {
-    const int chunk = (int)(item % chunks);
-    const long long rest = item / chunks;
-    const int i0 = chunk * a.item_rows, ni = min(a.item_rows, a.Rq - i0), b = (int)(rest / strips);
-    Strip<V, WIDE> strip;
-    strip.load(a, b, (int)(rest % strips) * 32 * V);
-    // lane l: what row i0 + l of the strip is: one bucket (>= 0), several (-1), none of this block's (-2)
-    const long long my_q = lane < ni ? position(a.q_pos, a.positions64, b * a.sq + i0 + lane) : 0;
-    int my_kind = -2;
-    if (lane < ni) {
-      const int from = Buckets::difference(strip.least, my_q), to = Buckets::difference(strip.most, my_q);
-      const int lo = bucket(from), hi = bucket(to);
-      // between the two are the buckets of all others, but for LOG, whose upper half begins behind the query
-      const bool ordered = a.scheme != EVOATTN_BUCKETS_LOG || from > 0 || to <= 0;
-      my_kind = ordered && (max(lo, hi) < first || min(lo, hi) >= first + count) ? -2 : lo == hi ? lo : -1;
-    }
-    const T* d = static_cast<const T*>(a.out) + b * a.sout.a + h * a.sout.b + (long long)i0 * a.sout.c;
-    const int kind0 = __shfl_sync(0xffffffffu, my_kind, 0);
-    float acc = 0.f;
-    if (kind0 != -1 && __all_sync(0xffffffffu, lane >= ni || my_kind == kind0)) {  // one bucket altogether
-      if (kind0 == -2) continue;
-      int i = 0;
-      for (; i + 2 * U <= ni; i += 2 * U) {
-        RowPiece<T, WIDE> p[2 * U];
+  float* sums = sm_sums + warp * per_warp + lane;
+  const unsigned strips = (a.Rk + kLanes * V - 1) / (kLanes * V), chunks = (a.Rq + a.item_rows - 1) / a.item_rows;
+  const unsigned items = a.B * strips * chunks;
+  // What all scores of keys least .. most and queries q0 .. q1 have in common: their bucket (>= 0), that none is of this
+  // block's (-2), or nothing (-1).  Between the buckets of the two ends are those of all others, but for LOG, whose
+  // upper half begins behind the query.
+  const auto kind_of = [&](long long least, long long most, long long q0, long long q1) {
+    const int from = difference(least, q1), to = difference(most, q0);
+    const int lo = bucket(from), hi = bucket(to);
+    const bool ordered = a.scheme != EVOATTN_BUCKETS_LOG || from > 0 || to <= 0;
+    return ordered && (max(lo, hi) < first || min(lo, hi) >= first + count) ? -2 : lo == hi ? lo : -1;
+  };
+  for (unsigned item = blockIdx.x * 4 + warp; item < items; item += gridDim.x * 4) {
+    const unsigned rest = item / chunks, b = rest / strips;
+    const int i0 = (int)(item - rest * chunks) * a.item_rows, ni = min(a.item_rows, a.Rq - i0), loads = (ni + kTall - 1) / kTall;
+    Strip<V, kLanes, WIDE> strip;
+    strip.load(a, b, (int)(rest - b * strips) * kLanes * V);
+    const long long q_at = b * a.sq + i0;
+    long long q0 = 0x7fffffffffffffffll, q1 = -q0 - 1;  // over the rows of load `lane`, then over all
 #pragma unroll
-        for (int k = 0; k < 2 * U; ++k) p[k].load(a, strip, d + (i + k) * a.sout.c);
-#pragma unroll
-        for (int k = 0; k < 2 * U; ++k) acc += p[k].sum();
+    for (int k = 0; k < kTall; ++k)
+      if (lane * kTall + k < ni) {
+        const long long q = position(a.q_pos, a.positions64, q_at + lane * kTall + k);
+        q0 = min(q0, q);
+        q1 = max(q1, q);
       }
-      for (; i < ni; ++i) {
+    long long all0 = q0, all1 = q1;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      all0 = min(all0, __shfl_xor_sync(0xffffffffu, all0, o));
+      all1 = max(all1, __shfl_xor_sync(0xffffffffu, all1, o));
+    }
+    const int kind = kind_of(strip.least, strip.most, all0, all1);
+    if (kind == -2) continue;
+    const T* d = static_cast<const T*>(a.out) + b * a.sout.a + h * a.sout.b + (long long)(i0 + my_row) * a.sout.c;
+    const long long down = kTall * a.sout.c;
+    if (kind >= 0) {  // one bucket altogether
+      float acc = 0.f;
+      int l = 0;
+      for (; (l + U) * kTall <= ni; l += U) {
+        RowPiece<T, WIDE> p[U];
+#pragma unroll
+        for (int k = 0; k < U; ++k, d += down) p[k].load(a, strip, d);
+#pragma unroll
+        for (int k = 0; k < U; ++k) acc += p[k].sum();
+      }
+      for (; l * kTall + my_row < ni; ++l, d += down) {
         RowPiece<T, WIDE> p;
-        p.load(a, strip, d + i * a.sout.c);
+        p.load(a, strip, d);
         acc += p.sum();
       }
-      sums[(kind0 - first) * 32] += acc;
+      sums[(kind - first) * 32] += acc;
       continue;
     }
-    int acc_row = -1;
-    RowPiece<T, WIDE> next[U];
-    const auto fetch = [&](int k, int i) {
-      if (i < ni && __shfl_sync(0xffffffffu, my_kind, i & 31) != -2) next[k].load(a, strip, d + i * a.sout.c);
+    // Load by load: the lines are asked for first, since there is room for no more than the next load in registers.
+    const int my_kind = lane < loads ? kind_of(strip.least, strip.most, q0, q1) : -2;
+    for (int l = 0; l < loads; ++l)
+      if (lane % kLanes == 0 && l * kTall + my_row < ni) ptx::prefetch_l2(d + l * down + strip.col(0));
+    RowPiece<T, WIDE> next;
+    long long next_q = 0;
+    const auto fetch = [&](int l) {
+      const int i = l * kTall + my_row;
+      if (i < ni) {
+        next.load(a, strip, d + l * down);
+        next_q = position(a.q_pos, a.positions64, q_at + i);
+      } else {
+        next.clear();
+      }
     };
+    float acc = 0.f;
+    int acc_row = -1;
+    fetch(0);
+#pragma unroll 1
+    for (int l = 0; l < loads; ++l) {
+      const int of_load = __shfl_sync(0xffffffffu, my_kind, l);
+      const RowPiece<T, WIDE> p = next;
+      const long long q = next_q;
+      if (l + 1 < loads) fetch(l + 1);
+      if (of_load >= 0) {
+        if (of_load != acc_row) {
+          if (acc_row >= 0) sums[(acc_row - first) * 32] += acc;
+          acc_row = of_load;
+          acc = 0.f;
+        }
+        acc += p.sum();
+      } else if (of_load == -1) {
+        float v[V];
+        int r[V];
+        p.floats(v);
+        strip.rows(a, bucket, b, q, difference(strip.least, q), r);
 #pragma unroll
-    for (int k = 0; k < U; ++k) fetch(k, k);
-    for (int i = 0; i < ni; i += U) {
+        for (int u = 0; u < V; ++u) r[u] = (int)min((unsigned)(r[u] - first), (unsigned)count) * 32;
+        if (strip.in_order) {  // values of one bucket first, then all sums at once
+          bool last[V];
+          float old[V];
 #pragma unroll
-      for (int k = 0; k < U; ++k) {
-        if (i + k >= ni) break;
-        const int kind = __shfl_sync(0xffffffffu, my_kind, i + k);
-        const long long q = __shfl_sync(0xffffffffu, my_q, i + k);
-        const RowPiece<T, WIDE> p = next[k];
-        fetch(k, i + k + U);
-        if (kind >= 0) {
-          if (kind != acc_row) {
-            if (acc_row >= 0) sums[(acc_row - first) * 32] += acc;
-            acc_row = kind;
-            acc = 0.f;
+          for (int u = 0; u < V; ++u) {
+            last[u] = u == V - 1 || r[u + 1 < V ? u + 1 : u] != r[u];
+            if (!last[u]) v[u + 1 < V ? u + 1 : u] += v[u];
           }
-          acc += p.sum();
-        } else if (kind == -1) {
-          float v[V];
-          int r[V];
-          p.floats(v);
-          strip.rows(a, bucket, b, q, r);
-          if (strip.in_order) {  // values of one bucket first, then all sums at once
-            bool last[V];
-            float old[V];
 #pragma unroll
-            for (int u = 0; u < V; ++u) {
-              last[u] = (u == V - 1 || r[u + 1 < V ? u + 1 : u] != r[u]) && (unsigned)(r[u] - first) < (unsigned)count;
-              if (u + 1 < V && r[u + 1 < V ? u + 1 : u] == r[u]) v[u + 1 < V ? u + 1 : u] += v[u];
-              r[u] = (r[u] - first) * 32;
-            }
+          for (int u = 0; u < V; ++u) old[u] = last[u] ? sums[r[u]] : 0.f;
 #pragma unroll
-            for (int u = 0; u < V; ++u) old[u] = last[u] ? sums[r[u]] : 0.f;
+          for (int u = 0; u < V; ++u)
+            if (last[u]) sums[r[u]] = old[u] + v[u];
+        } else {
 #pragma unroll
-            for (int u = 0; u < V; ++u)
-              if (last[u]) sums[r[u]] = old[u] + v[u];
-          } else {
-#pragma unroll
-            for (int u = 0; u < V; ++u)
-              if (strip.col(u) < a.Rk && (unsigned)(r[u] - first) < (unsigned)count) sums[(r[u] - first) * 32] += v[u];
-          }
+          for (int u = 0; u < V; ++u) sums[r[u]] += v[u];  // (where there is no key: zero)
         }
       }
     }
@@ -391,7 +412,7 @@ __global__ void __launch_bounds__(128) relative_bwd(RelArgs a) {
   for (int r = warp; r < count; r += 4) {
     float s = 0.f;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) s += sm_sums[(w * a.window + r) * 32 + lane];
+    for (int w = 0; w < 4; ++w) s += sm_sums[w * per_warp + r * 32 + lane];
     s = warp_sum(s);
     if (lane == 0) a.partial[((long long)h * a.blocks + blockIdx.x) * a.buckets + first + r] = s;
   }
@@ -422,6 +443,7 @@ int validate(const evoattn_relative_bias_params* p) {
   if (p->B < 0 || p->H <= 0 || p->Rq < 0 || p->Rk < 0 || p->B > 65535 || p->H > 4096) return EVOATTN_ERR_SHAPE;
   if (p->Rq > (1 << 23) || p->Rk > (1 << 23)) return EVOATTN_ERR_SHAPE;
   if ((long long)p->B * ((p->H + kHeads - 1) / kHeads) > 65535) return EVOATTN_ERR_SHAPE;
+  if ((long long)p->B * ((p->Rk + 31) / 32) * ((p->Rq + 15) / 16) > 0x7fffffffLL) return EVOATTN_ERR_SHAPE;
   if (p->buckets <= 0 || p->buckets > EVOATTN_MAX_BUCKETS || p->n_edges < 0 || p->n_edges > kLogEdges || p->exact < 0) return EVOATTN_ERR_SHAPE;
   if (p->n_edges > 0 && !p->edges) return EVOATTN_ERR_NULL;
   for (int i = 0; i < p->n_edges; ++i)  // a distance finds its bucket by bisection
@@ -450,13 +472,13 @@ bool rows_of_16_bytes(const void* p, const int64_t* stride, int es) {
   return ((uintptr_t)p & 15) == 0 && stride[0] * es % 16 == 0 && stride[1] * es % 16 == 0 && stride[2] * es % 16 == 0;
 }
 
-// How the backward is cut: rows a warp takes at a time, blocks of four warps a head, table rows a block sums.
+// How the backward is cut: rows a warp takes at a time (up to 32 loads), blocks of four warps a head, table rows a block sums.
 void plan_bwd(RelArgs* a, int es) {
   a->window = a->buckets < 128 ? a->buckets : 128;
-  const int strips = (a->Rk + 512 / es - 1) / (512 / es);
-  a->item_rows = 32;
+  const int wide = kLanes * 16 / es, strips = (a->Rk + wide - 1) / wide;
+  a->item_rows = 32 * kTall;
   const auto items = [&] { return (long long)a->B * strips * ((a->Rq + a->item_rows - 1) / a->item_rows); };
-  while (a->item_rows > 4 && items() * a->H < 148 * 16) a->item_rows /= 2;
+  while (a->item_rows > 4 * kTall && items() * a->H < 148 * 20 * 2) a->item_rows /= 2;
   const long long blocks = (items() + 3) / 4, most = 148 * 5 / a->H > 1 ? 148 * 5 / a->H : 1;
   a->blocks = (int)(blocks < most ? blocks : most);
 }
@@ -527,7 +549,7 @@ int evoattn_relative_bias_bwd(const evoattn_relative_bias_params* p, void* cuda_
   cudaError_t rc = cudaSuccess;
   if (a.blocks) {
     const dim3 grid((unsigned)a.blocks, (unsigned)a.H, (unsigned)((a.buckets + a.window - 1) / a.window));
-    const int smem = 4 * a.window * 32 * (int)sizeof(float);
+    const int smem = 4 * (a.window + 1) * 32 * (int)sizeof(float);
     const bool wide = rows_of_16_bytes(p->d_out, p->d_out_stride, es);
     const int bad = with_dtype(p->dtype, [&](auto e) {
       using T = decltype(e);
