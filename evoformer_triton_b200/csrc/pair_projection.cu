@@ -8,6 +8,8 @@
 //   dweight[h,c] = g[c] M[h,c] + b[c] s[h],  dg[c] = sum_h weight[h,c] M[h,c],  db[c] = sum_h weight[h,c] s[h]
 //
 // so the gradients of all three weights come from sums that do not depend on them.
+#include <string.h>
+
 #include <type_traits>
 
 #include "inputs.cuh"
@@ -33,35 +35,20 @@ struct ProjArgs {
   float* stats;     // [rows][2]
   float* partial;   // [blocks][H][C + 1]: M and s
   int blocks;
-  FastDiv by_Ri, by_Rj;  // rows below 2^31
+  FastDiv by_Ri, by_Rj;
+  int z_dense;      // rows of z one after another
+  int whole;        // z and dz in pieces of eight channels and 16 bytes
 };
-
-constexpr int kMaxPerLane = EVOATTN_PROJECTION_MAX_C / 32;
 
 __device__ __forceinline__ float gain(const ProjArgs& a, int c) { return a.g ? load_any(a.g, a.g_dtype, c) : 1.f; }
 
-struct Row {
-  int b, i, j;
-  __device__ __forceinline__ Row(const ProjArgs& a, long long n) {
-    j = (int)(n % a.Rj);
-    const long long q = n / a.Rj;
-    i = (int)(q % a.Ri);
-    b = (int)(q / a.Ri);
-  }
-  __device__ __forceinline__ long long at(const Str3& s) const { return b * s.a + i * s.b + j * s.c; }
-  __device__ __forceinline__ long long at(const Str3& s, int h) const { return b * s.a + h * s.b + i * s.c + j; }
-};
-
-// ---------------------------------------------------------------- on tensor cores
-//
 // Few heads make the products thin (N = 8 heads or K = 8 heads), and the kernels are bound by the pair representation's way
 // through memory; warp-level MMAs take their operands from the registers that the rows were loaded into, with no staging.
 //
 // A warp takes 16 rows.  Four lanes share a row: lane t of them loads channels 8 t .. 8 t + 7 of every 32, sixteen bytes in
 // 16-bit types.  What a lane holds is at once the A operand of rows x channels (the channels that the MMA calls 2t, 2t + 1 and
 // 2t + 8, 2t + 9 of a step are 8t + 4s .. 8t + 4s + 3 here; G is laid out to match), the accumulator layout of heads x
-// channels products, and, transposed 8 x 8 at a time by movmatrix, the A operand of channels x rows.  The sums over a
-// row are two exchanges.
+// channels products, and, transposed 8 x 8 at a time by movmatrix, the A operand of channels x rows.
 //
 // Products are of bf16 pieces with fp32 sums: an fp32 factor is the sum of three (24 bits), an fp16 one of two, a bf16 one
 // is one.  z enters as it is: sum_c G z[c] - mean sum_c G, with both sums over the same pieces of G, and M likewise from d r z
@@ -70,6 +57,10 @@ struct Row {
 
 __device__ __forceinline__ void mma_k16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_k16_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ void mma_k8(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t b0) {
@@ -106,14 +97,21 @@ template <> struct Pieces<__nv_bfloat16> { static constexpr int kX = 1, kG = 2, 
 template <> struct Pieces<__half> { static constexpr int kX = 2, kG = 2, kTerms = 3; };
 template <> struct Pieces<float> { static constexpr int kX = 3, kG = 3, kTerms = 3; };
 
-// Eight channels of a row.
+// Eight channels of a row, the first `count` of which are there.
 template <class T>
 struct Eight {
   static constexpr int kWords = sizeof(T) / 2;
   uint4 w[kWords];
-  __device__ __forceinline__ void load(const T* p, bool on) {
+  __device__ __forceinline__ void load(const T* p, int count, bool whole) {
+    if (whole) {  // (the same for a launch: C and all rows in pieces of eight channels and 16 bytes)
 #pragma unroll
-    for (int k = 0; k < kWords; ++k) w[k] = on ? reinterpret_cast<const uint4*>(p)[k] : make_uint4(0, 0, 0, 0);
+      for (int k = 0; k < kWords; ++k) w[k] = count > 0 ? reinterpret_cast<const uint4*>(p)[k] : make_uint4(0, 0, 0, 0);
+    } else {
+      T v[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = e < count ? p[e] : from_float<T>(0.f);
+      memcpy(w, v, sizeof(v));
+    }
   }
   __device__ __forceinline__ void floats(float (&v)[8]) const {
 #pragma unroll
@@ -130,94 +128,51 @@ struct Eight {
       for (int k = 0; k < 4; ++k) split2<Pieces<T>::kX>(v[2 * k], v[2 * k + 1], p[k]);
     }
   }
-  static __device__ __forceinline__ void store(T* p, const float (&v)[8]) {
+  static __device__ __forceinline__ void store(T* p, const float (&v)[8], int count, bool whole) {
+    if (whole) {
 #pragma unroll
-    for (int k = 0; k < kWords; ++k) reinterpret_cast<uint4*>(p)[k] = pack16<T>(v + k * kPer16<T>);
+      for (int k = 0; k < kWords; ++k)
+        if (count > 0) reinterpret_cast<uint4*>(p)[k] = pack16<T>(v + k * kPer16<T>);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (e < count) p[e] = from_float<T>(v[e]);
+    }
   }
 };
 
 __device__ __forceinline__ float g_of(const ProjArgs& a, int h, int c) {
   return h < a.H && c < a.C ? load_any(a.w, a.w_dtype, h * a.C + c) * gain(a, c) : 0.f;
 }
-
-// A lane's two rows of a tile: g and g + 8.
-struct Rows2 {
-  long long z[2], o[2];
-  uint32_t n[2];
-  bool on[2];
-  __device__ __forceinline__ Rows2(const ProjArgs& a, uint32_t n0, uint32_t rows) {
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      n[k] = n0 + (threadIdx.x & 31) / 4 + 8 * k;
-      on[k] = n[k] < rows;
-      const uint32_t m = on[k] ? n[k] : 0, q = a.by_Rj.div(m), j = m - q * a.Rj, b = a.by_Ri.div(q), i = q - b * a.Ri;
-      z[k] = b * a.sz.a + i * a.sz.b + j * a.sz.c;
-      o[k] = b * a.sout.a + i * a.sout.c + j;
-    }
-  }
-};
-
-template <class T, int KC>
-struct Tile {
-  Eight<T> x[2][KC];
-  float mean[2], r[2];
-  __device__ __forceinline__ void load(const ProjArgs& a, const Rows2& row) {
-    const int t = threadIdx.x & 3;
-#pragma unroll
-    for (int k = 0; k < 2; ++k)
-#pragma unroll
-      for (int c = 0; c < KC; ++c) x[k][c].load(static_cast<const T*>(a.z) + row.z[k] + c * 32 + t * 8, row.on[k] && c * 32 + t * 8 < a.C);
-  }
-  // Mean and 1 / deviation, the latter about the mean; a row that is not there has r = 0 and adds nothing.
-  __device__ __forceinline__ void statistics(const ProjArgs& a, const Rows2& row) {
-    const float by_C = 1.f / a.C;
-    const int t = threadIdx.x & 3;
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      float s = 0.f;
-#pragma unroll
-      for (int c = 0; c < KC; ++c) {
-        float v[8];
-        x[k][c].floats(v);
-        s += ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
-      }
-      mean[k] = quad_sum(s) * by_C;
-      s = 0.f;
-#pragma unroll
-      for (int c = 0; c < KC; ++c) {
-        if (c * 32 + t * 8 >= a.C) continue;
-        float v[8];
-        x[k][c].floats(v);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) s = fmaf(v[e] - mean[k], v[e] - mean[k], s);
-      }
-      s = quad_sum(s);  // (all lanes, rows that are not there too)
-      r[k] = row.on[k] ? rsqrtf(s * by_C + a.eps) : 0.f;
-    }
-  }
-};
-
-template <class T, int KC, int NT>
-__global__ void __launch_bounds__(256) projection_fwd_mma(ProjArgs a) {
-  ptx::grid_dependency_wait();
-  ptx::grid_launch_dependents();
-  constexpr int GP = Pieces<T>::kG, XP = Pieces<T>::kX;
-  extern __shared__ __align__(16) uint4 sm_g[];  // [KC][NT][GP][32 lanes]
-  __shared__ float sm_sum[NT * 8], sm_t[NT * 8];  // sum_c of the pieces of G; sum_c weight b
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-  const uint32_t rows = (uint32_t)((long long)a.B * a.Ri * a.Rj), step = gridDim.x * 128;
-  uint32_t n0 = (blockIdx.x * 8 + warp) * 16;
-  Tile<T, KC> x;
-  if (n0 < rows) x.load(a, Rows2(a, n0, rows));
-  for (int i = threadIdx.x; i < KC * NT * 32; i += 256) {
+// G[h, c .. c + 7] and on as B operands of rows x channels products, [KC][NT][pieces][lane].
+template <int GP>
+__device__ __forceinline__ void lay_out_by_rows(const ProjArgs& a, int KC, int NT, uint4* sm) {
+  for (int i = threadIdx.x; i < KC * NT * 32; i += blockDim.x) {
     const int l = i & 31, nt = (i >> 5) % NT, kc = (i >> 5) / NT, h = nt * 8 + l / 4, c = kc * 32 + (l & 3) * 8;
     uint32_t p[4][GP];
 #pragma unroll
     for (int k = 0; k < 4; ++k) split2<GP>(g_of(a, h, c + 2 * k), g_of(a, h, c + 2 * k + 1), p[k]);
 #pragma unroll
-    for (int j = 0; j < GP; ++j) sm_g[((kc * NT + nt) * GP + j) * 32 + l] = make_uint4(p[0][j], p[1][j], p[2][j], p[3][j]);
+    for (int j = 0; j < GP; ++j) sm[((kc * NT + nt) * GP + j) * 32 + l] = make_uint4(p[0][j], p[1][j], p[2][j], p[3][j]);
   }
-  for (int h = warp; h < NT * 8; h += 8) {
+}
+// The same as B operands of heads x channels products: pairs of heads of the four channels of a lane's accumulators.
+template <int GP>
+__device__ __forceinline__ void lay_out_by_heads(const ProjArgs& a, int KC, int NT, uint4* sm) {
+  for (int i = threadIdx.x; i < KC * NT * 32; i += blockDim.x) {
+    const int l = i & 31, nt = (i >> 5) % NT, kc = (i >> 5) / NT, h = nt * 8 + (l & 3) * 2, c = kc * 32 + l / 8 * 8 + (l / 4 & 1);
+    uint32_t p[4][GP];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) split2<GP>(g_of(a, h, c + 2 * q), g_of(a, h + 1, c + 2 * q), p[q]);
+#pragma unroll
+    for (int j = 0; j < GP; ++j) sm[((kc * NT + nt) * GP + j) * 32 + l] = make_uint4(p[0][j], p[1][j], p[2][j], p[3][j]);
+  }
+}
+// sum_c of the pieces of G for every head, and sum_c weight b.  All warps of the block take part.
+template <int GP>
+__device__ __forceinline__ void sum_channels(const ProjArgs& a, int heads, float* sm_sum, float* sm_t) {
+  const int lane = threadIdx.x & 31;
+  for (int h = threadIdx.x >> 5; h < heads; h += blockDim.x >> 5) {
     float s = 0.f, tb = 0.f;
     for (int c = lane; c < a.C; c += 32) {
       uint32_t p[GP];
@@ -230,348 +185,502 @@ __global__ void __launch_bounds__(256) projection_fwd_mma(ProjArgs a) {
         v += lo;
       }
       s += v;
-      if (a.b && h < a.H) tb = fmaf(load_any(a.w, a.w_dtype, h * a.C + c), load_any(a.b, a.b_dtype, c), tb);
+      if (sm_t && a.b && h < a.H) tb = fmaf(load_any(a.w, a.w_dtype, h * a.C + c), load_any(a.b, a.b_dtype, c), tb);
     }
     s = warp_sum(s);
     tb = warp_sum(tb);
-    if (lane == 0) sm_sum[h] = s, sm_t[h] = tb;
-  }
-  __syncthreads();
-  for (; n0 < rows; n0 += step) {
-    const Rows2 row(a, n0, rows);
-    x.statistics(a, row);
-    float acc[NT][4] = {};
-#pragma unroll
-    for (int kc = 0; kc < KC; ++kc) {
-      uint32_t lo[4][XP], hi[4][XP];
-      x.x[0][kc].pieces(lo);
-      x.x[1][kc].pieces(hi);
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int j = 0; j < GP; ++j) {
-          const uint4 gw = sm_g[((kc * NT + nt) * GP + j) * 32 + lane];
-#pragma unroll
-          for (int i = 0; i < XP; ++i) {
-            if (i + j >= Pieces<T>::kTerms) continue;
-            mma_k16(acc[nt], lo[0][i], hi[0][i], lo[1][i], hi[1][i], gw.x, gw.y);
-            mma_k16(acc[nt], lo[2][i], hi[2][i], lo[3][i], hi[3][i], gw.z, gw.w);
-          }
-        }
+    if (lane == 0) {
+      sm_sum[h] = s;
+      if (sm_t) sm_t[h] = tb;
     }
+  }
+}
+
+// A lane's two rows of a tile: g and g + 8.
+struct Rows2 {
+  long long z[2], o[2];
+  uint32_t n0;
+  bool on[2];
+  __device__ __forceinline__ Rows2(const ProjArgs& a, uint32_t first, uint32_t rows) : n0(first) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const uint32_t n = row(k);
+      on[k] = n < rows;
+      const uint32_t m = on[k] ? n : 0, q = a.by_Rj.div(m), j = m - q * a.Rj, b = a.by_Ri.div(q), i = q - b * a.Ri;
+      z[k] = a.z_dense ? m * a.sz.c : b * a.sz.a + i * a.sz.b + j * a.sz.c;
+      o[k] = b * a.sout.a + i * a.sout.c + j;
+    }
+  }
+  __device__ __forceinline__ uint32_t row(int k) const { return n0 + (threadIdx.x & 31) / 4 + 8 * k; }
+};
+
+// 16 rows, 32 KC channels.  KEEP: in registers; else read again (from L1 or L2) by every use.
+template <class T, int KC, bool KEEP>
+struct Tile {
+  static constexpr int kUnroll = KEEP ? KC : 1;
+  Eight<T> x[2][KEEP ? KC : 1];
+  const T* at[2];
+  bool on[2];
+  float mean[2], r[2];
+  __device__ __forceinline__ int count(const ProjArgs& a, int c) const { return a.C - c * 32 - (int)(threadIdx.x & 3) * 8; }
+  __device__ __forceinline__ void load(const ProjArgs& a, const Rows2& row) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      at[k] = static_cast<const T*>(a.z) + row.z[k] + (threadIdx.x & 3) * 8;
+      on[k] = row.on[k];
+      if constexpr (KEEP) {
+#pragma unroll
+        for (int c = 0; c < KC; ++c) x[k][c].load(at[k] + c * 32, on[k] ? count(a, c) : 0, a.whole);
+      }
+    }
+  }
+  __device__ __forceinline__ Eight<T> get(const ProjArgs& a, int k, int c) const {
+    if constexpr (KEEP) return x[k][c];
+    Eight<T> e;
+    e.load(at[k] + c * 32, on[k] ? count(a, c) : 0, a.whole);
+    return e;
+  }
+  // Mean and 1 / deviation, the latter about the mean; a row that is not there has r = 0 and adds nothing.
+  __device__ __forceinline__ void about_the_mean(const ProjArgs& a) {
+    const float by_C = 1.f / a.C;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      float s = 0.f;
+#pragma unroll kUnroll
+      for (int c = 0; c < KC; ++c) {
+        float v[8];
+        get(a, k, c).floats(v);
+        s += ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
+      }
+      mean[k] = quad_sum(s) * by_C;
+      s = 0.f;
+#pragma unroll kUnroll
+      for (int c = 0; c < KC; ++c) {
+        float v[8];
+        get(a, k, c).floats(v);
+        const int there = count(a, c);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float d = e < there ? v[e] - mean[k] : 0.f;
+          s = fmaf(d, d, s);
+        }
+      }
+      s = quad_sum(s);  // (all lanes, rows that are not there too)
+      r[k] = on[k] ? rsqrtf(s * by_C + a.eps) : 0.f;
+    }
+  }
+  // In 16-bit types both sums come from MMAs: with a column of ones, and the diagonal of rows x rows (the registers of the A
+  // operand are those of its transpose as B).  The variance is then a difference, good to 2^-22 where the mean is
+  // at most twice the deviation; other rows are done the other way.
+  __device__ __forceinline__ void statistics(const ProjArgs& a) {
+    if constexpr (sizeof(T) == 4) {
+      about_the_mean(a);
+    } else {
+      constexpr bool bf = std::is_same<T, __nv_bfloat16>::value;
+      constexpr uint32_t ones = bf ? 0x3f803f80u : 0x3c003c00u;
+      const auto mma = [](float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+        if constexpr (bf) mma_k16(d, a0, a1, a2, a3, b0, b1);
+        else mma_k16_f16(d, a0, a1, a2, a3, b0, b1);
+      };
+      float sum[4] = {}, lo[4] = {}, hi[4] = {};
+#pragma unroll kUnroll
+      for (int c = 0; c < KC; ++c) {
+        const uint4 l = get(a, 0, c).w[0], h = get(a, 1, c).w[0];
+        mma(sum, l.x, h.x, l.y, h.y, ones, ones);
+        mma(lo, l.x, h.x, l.y, h.y, l.x, l.y);
+        mma(hi, l.x, h.x, l.y, h.y, h.x, h.y);
+        mma(sum, l.z, h.z, l.w, h.w, ones, ones);
+        mma(lo, l.z, h.z, l.w, h.w, l.z, l.w);
+        mma(hi, l.z, h.z, l.w, h.w, h.z, h.w);
+      }
+      const float by_C = 1.f / a.C;
+      const int lane = threadIdx.x & 31, g = lane >> 2, diagonal = (lane & ~3) | (g >> 1);
+      const float square[2] = {__shfl_sync(0xffffffffu, g & 1 ? lo[1] : lo[0], diagonal), __shfl_sync(0xffffffffu, g & 1 ? hi[3] : hi[2], diagonal)};
+      float quick_mean[2], quick_r[2];
+      bool fine[2];
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        quick_mean[k] = sum[2 * k] * by_C;
+        const float var = fmaf(-quick_mean[k], quick_mean[k], square[k] * by_C);
+        fine[k] = quick_mean[k] * quick_mean[k] <= 4.f * var;
+        quick_r[k] = on[k] ? rsqrtf(var + a.eps) : 0.f;
+      }
+      if (!__all_sync(0xffffffffu, fine[0] && fine[1])) about_the_mean(a);
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+        if (fine[k]) mean[k] = quick_mean[k], r[k] = quick_r[k];  // (what a row gets does not depend on its neighbours)
+    }
+  }
+};
+
+// acc[nt] += rows x channels of the tile with G (laid out by rows).
+template <class T, int KC, int NT, class TileT>
+__device__ __forceinline__ void product_by_rows(const ProjArgs& a, const TileT& x, const uint4* sm_g, float (&acc)[NT][4]) {
+  constexpr int GP = Pieces<T>::kG, XP = Pieces<T>::kX;
+  const int lane = threadIdx.x & 31;
+#pragma unroll TileT::kUnroll
+  for (int kc = 0; kc < KC; ++kc) {
+    uint32_t lo[4][XP], hi[4][XP];
+    x.get(a, 0, kc).pieces(lo);
+    x.get(a, 1, kc).pieces(hi);
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int j = 0; j < GP; ++j) {
+        const uint4 gw = sm_g[((kc * NT + nt) * GP + j) * 32 + lane];
+#pragma unroll
+        for (int i = 0; i < XP; ++i) {
+          if (i + j >= Pieces<T>::kTerms) continue;
+          mma_k16(acc[nt], lo[0][i], hi[0][i], lo[1][i], hi[1][i], gw.x, gw.y);
+          mma_k16(acc[nt], lo[2][i], hi[2][i], lo[3][i], hi[3][i], gw.z, gw.w);
+        }
+      }
+  }
+}
+
+template <class T, int KC, int NT, bool KEEP>
+__global__ void __launch_bounds__(256) projection_fwd(ProjArgs a) {
+  ptx::grid_dependency_wait();
+  ptx::grid_launch_dependents();
+  extern __shared__ __align__(16) uint4 sm_g[];  // [KC][NT][GP][32 lanes]
+  __shared__ float sm_sum[NT * 8], sm_t[NT * 8];
+  const int warp = threadIdx.x >> 5, t = threadIdx.x & 3;
+  const uint32_t rows = (uint32_t)((long long)a.B * a.Ri * a.Rj), step = gridDim.x * 128;
+  Rows2 next(a, (blockIdx.x * 8 + warp) * 16, rows);
+  Tile<T, KC, KEEP> x;
+  x.load(a, next);
+  lay_out_by_rows<Pieces<T>::kG>(a, KC, NT, sm_g);
+  sum_channels<Pieces<T>::kG>(a, NT * 8, sm_sum, sm_t);
+  __syncthreads();
+  while (next.n0 < rows) {
+    const Rows2 row = next;
+    x.statistics(a);
+    float acc[NT][4] = {};
+    product_by_rows<T, KC, NT>(a, x, sm_g, acc);
     const float mean[2] = {x.mean[0], x.mean[1]}, r[2] = {x.r[0], x.r[1]};
-    if (n0 + step < rows) x.load(a, Rows2(a, n0 + step, rows));
+    next = Rows2(a, row.n0 + step, rows);
+    x.load(a, next);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int h = nt * 8 + 2 * t + e;
         if (h >= a.H) continue;
+        const float sum = sm_sum[h], tb = sm_t[h];
+        T* out = static_cast<T*>(a.out) + h * a.sout.b;
 #pragma unroll
         for (int k = 0; k < 2; ++k)
-          if (row.on[k])
-            static_cast<T*>(a.out)[row.o[k] + h * a.sout.b] = from_float<T>(fmaf(acc[nt][2 * k + e] - mean[k] * sm_sum[h], r[k], sm_t[h]));
+          if (row.on[k]) out[row.o[k]] = from_float<T>(fmaf(fmaf(-mean[k], sum, acc[nt][2 * k + e]), r[k], tb));
       }
   }
 }
 
-// Backward in one pass over z: dz, and M and s of the block's rows.
+// d of a lane's two rows and heads 8 nt + 2t, 8 nt + 2t + 1, as pieces.
+template <class T, int NT>
+__device__ __forceinline__ void load_d(const ProjArgs& a, const Rows2& row, int nt0, float (&d)[NT][2][2], uint32_t (&dp)[NT][2][Pieces<T>::kX]) {
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int h = (nt0 + nt) * 8 + 2 * (threadIdx.x & 3) + e;
+      const T* p = static_cast<const T*>(a.out) + h * a.sout.b;
+#pragma unroll
+      for (int k = 0; k < 2; ++k) d[nt][k][e] = row.on[k] && h < a.H ? to_float<T>(p[row.o[k]]) : 0.f;
+    }
+#pragma unroll
+    for (int k = 0; k < 2; ++k) split2<Pieces<T>::kX>(d[nt][k][0], d[nt][k][1], dp[nt][k]);
+  }
+}
+
+// Sums over the rows: M before the mean is taken out (d r z), s (d) and q (d r mean), of 32 KC channels and 8 NT heads.
 template <class T, int KC, int NT>
-__global__ void __launch_bounds__(256) projection_bwd_mma(ProjArgs a) {
+struct RowSums {
+  static constexpr int XP = Pieces<T>::kX, AP = 3;
+  float m[KC][2][NT][4] = {}, s[NT] = {}, q[NT] = {};
+  template <class TileT>
+  __device__ __forceinline__ void add(const ProjArgs& a, const TileT& x, const uint32_t (&dp)[NT][2][XP]) {
+    const int t = threadIdx.x & 3;
+    // r and mean of rows 2t, 2t + 1, 2t + 8, 2t + 9, which the lanes 4 (2t) and 4 (2t + 1) hold
+    float r[2][2], mean[2][2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        r[k][e] = __shfl_sync(0xffffffffu, x.r[k], 8 * t + 4 * e);
+        mean[k][e] = __shfl_sync(0xffffffffu, x.mean[k], 8 * t + 4 * e);
+      }
+    uint32_t ap[NT][2][AP];  // pieces of d r, [rows x heads] transposed
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        float d0 = 0.f, d1 = 0.f;
+#pragma unroll
+        for (int i = XP - 1; i >= 0; --i) {
+          float lo, hi;
+          unpack2<__nv_bfloat16>(transposed(dp[nt][k][i]), lo, hi);
+          d0 += lo;
+          d1 += hi;
+        }
+        s[nt] += d0 + d1;
+        d0 *= r[k][0];
+        d1 *= r[k][1];
+        q[nt] = fmaf(d0, mean[k][0], fmaf(d1, mean[k][1], q[nt]));
+        split2<AP>(d0, d1, ap[nt][k]);
+      }
+#pragma unroll
+    for (int kc = 0; kc < KC; ++kc) {
+      uint32_t lo[4][XP], hi[4][XP];
+      x.get(a, 0, kc).pieces(lo);
+      x.get(a, 1, kc).pieces(hi);
+#pragma unroll
+      for (int p = 0; p < 2; ++p)
+#pragma unroll
+        for (int i = 0; i < XP; ++i) {
+          const uint32_t a0 = transposed(lo[2 * p][i]), a1 = transposed(lo[2 * p + 1][i]), a2 = transposed(hi[2 * p][i]), a3 = transposed(hi[2 * p + 1][i]);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int j = 0; j + i < AP; ++j) mma_k16(m[kc][p][nt], a0, a1, a2, a3, ap[nt][0][j], ap[nt][1][j]);
+        }
+    }
+  }
+  // The block's sums in shared memory, [8 NT heads][32 KC + 1]: its warps add theirs in turn.  q is the same for all channels.
+  __device__ __forceinline__ void leave(float* sums) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3, pitch = 32 * KC + 1;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      s[nt] = quad_sum(s[nt]);
+      q[nt] = quad_sum(q[nt]);
+    }
+    for (int w = 0; w < (int)(blockDim.x >> 5); ++w) {
+      __syncthreads();
+      if (warp != w) continue;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        // head 8 nt + g is what the lane's s and q are of; its part of M is heads 2t, 2t + 1
+        const float q0 = __shfl_sync(0xffffffffu, q[nt], 8 * t), q1 = __shfl_sync(0xffffffffu, q[nt], 8 * t + 4);
+#pragma unroll
+        for (int kc = 0; kc < KC; ++kc)
+#pragma unroll
+          for (int p = 0; p < 2; ++p)
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                float& to = sums[(nt * 8 + 2 * t + e) * pitch + kc * 32 + g / 2 * 8 + 2 * (2 * p + k) + (g & 1)];
+                const float v = m[kc][p][nt][2 * k + e] - (e ? q1 : q0);
+                to = w ? to + v : v;
+              }
+        float& to = sums[(nt * 8 + g) * pitch + 32 * KC];
+        if (t == 0) to = w ? to + s[nt] : s[nt];
+      }
+    }
+    __syncthreads();
+  }
+};
+// From there to the block's partial sums [H][C + 1]: heads h0 .. and channels c0 .. of them, s by the first channels' block.
+template <int KC, int NT>
+__device__ __forceinline__ void write_partial(const ProjArgs& a, const float* sums, int block, int h0, int c0) {
+  constexpr int pitch = 32 * KC + 1;
+  float* out = a.partial + (long long)block * a.H * (a.C + 1);
+  for (int i = threadIdx.x; i < 8 * NT * pitch; i += blockDim.x) {
+    const int h = h0 + i / pitch, k = i % pitch, c = c0 + k;
+    if (h >= a.H) break;
+    if (k == 32 * KC) {
+      if (c0 == 0) out[h * (a.C + 1) + a.C] = sums[i];
+    } else if (c < a.C) {
+      out[h * (a.C + 1) + c] = sums[i];
+    }
+  }
+}
+
+// u[c] = sum_h d[h] G[h,c] of chunk kc in the layout of the lane's eight channels.  With d in one piece, its products with both
+// pieces of G are one MMA: K = 8 heads with the first and the same 8 heads with the second.
+template <class T, int NT>
+__device__ __forceinline__ void product_by_heads(const uint4* sm_u, int kc, const uint32_t (&dp)[NT][2][Pieces<T>::kX], float (&u)[2][8]) {
+  constexpr int GP = Pieces<T>::kG, XP = Pieces<T>::kX;
+  const int lane = threadIdx.x & 31;
+  float acc[4][4] = {};
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    uint32_t gw[GP][4];
+#pragma unroll
+    for (int j = 0; j < GP; ++j) *reinterpret_cast<uint4*>(gw[j]) = sm_u[((kc * NT + nt) * GP + j) * 32 + lane];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      if constexpr (XP == 1) {
+        mma_k16(acc[q], dp[nt][0][0], dp[nt][1][0], dp[nt][0][0], dp[nt][1][0], gw[0][q], gw[1][q]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < GP; ++j)
+#pragma unroll
+          for (int i = 0; i < XP; ++i)
+            if (i + j < Pieces<T>::kTerms) mma_k8(acc[q], dp[nt][0][i], dp[nt][1][i], gw[j][q]);
+      }
+    }
+  }
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    u[0][2 * q] = acc[q][0]; u[0][2 * q + 1] = acc[q][1]; u[1][2 * q] = acc[q][2]; u[1][2 * q + 1] = acc[q][3];
+  }
+}
+
+// dz = r u - c0 - (z - mean) c1 with c0 = r mean(u), c1 = r^3 mean(u (z - mean)).
+template <class T, int KC, int NT, class TileT>
+__device__ __forceinline__ void write_dz(const ProjArgs& a, const TileT& x, const Rows2& row, const uint4* sm_u, const uint32_t (&dp)[NT][2][Pieces<T>::kX],
+                                         const float (&c0)[2], const float (&c1)[2]) {
+#pragma unroll TileT::kUnroll
+  for (int kc = 0; kc < KC; ++kc) {
+    float u[2][8];
+    product_by_heads<T, NT>(sm_u, kc, dp, u);
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      float v[8];
+      x.get(a, k, kc).floats(v);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = fmaf(x.r[k], u[k][e], -fmaf(v[e] - x.mean[k], c1[k], c0[k]));
+      if (row.on[k])
+        Eight<T>::store(static_cast<T*>(a.dz) + (long long)row.row(k) * a.C + kc * 32 + (threadIdx.x & 3) * 8, v, x.count(a, kc), a.whole);
+    }
+  }
+}
+
+// Backward in one pass over z: dz, and M and s of the block's rows.  mean(u) and mean(u (z - mean)) are sums over heads,
+//   sum_c u = sum_h d[h] sum_c G[h,c],   sum_c u (z - mean) = sum_h d[h] (sum_c G[h,c] z[c] - mean sum_c G[h,c]),
+// the latter with the product that the forward takes.
+template <class T, int KC, int NT>
+__global__ void __launch_bounds__(256) projection_bwd(ProjArgs a) {
   ptx::grid_dependency_wait();
   ptx::grid_launch_dependents();
-  constexpr int GP = Pieces<T>::kG, XP = Pieces<T>::kX, AP = 3;
-  extern __shared__ __align__(16) uint4 sm_g[];  // [KC][NT][GP][32 lanes]; behind the rows, [H][C + 1] sums
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+  constexpr int kG = KC * NT * Pieces<T>::kG * 32;
+  extern __shared__ __align__(16) uint4 sm_g[];  // G by rows, G by heads; behind the rows' loop, the sums
+  __shared__ float sm_sum[NT * 8];
+  const int warp = threadIdx.x >> 5, t = threadIdx.x & 3;
   const uint32_t rows = (uint32_t)((long long)a.B * a.Ri * a.Rj), step = gridDim.x * 128;
   if (a.dz) {
-    for (int i = threadIdx.x; i < KC * NT * 32; i += 256) {
-      const int l = i & 31, nt = (i >> 5) % NT, kc = (i >> 5) / NT, h = nt * 8 + (l & 3) * 2, c = kc * 32 + l / 8 * 8 + (l / 4 & 1);
-      uint32_t p[4][GP];
-#pragma unroll
-      for (int q = 0; q < 4; ++q) split2<GP>(g_of(a, h, c + 2 * q), g_of(a, h + 1, c + 2 * q), p[q]);
-#pragma unroll
-      for (int j = 0; j < GP; ++j) sm_g[((kc * NT + nt) * GP + j) * 32 + l] = make_uint4(p[0][j], p[1][j], p[2][j], p[3][j]);
-    }
+    lay_out_by_rows<Pieces<T>::kG>(a, KC, NT, sm_g);
+    lay_out_by_heads<Pieces<T>::kG>(a, KC, NT, sm_g + kG);
+    sum_channels<Pieces<T>::kG>(a, NT * 8, sm_sum, nullptr);
   }
   __syncthreads();
   const float by_C = 1.f / a.C;
-  float m_acc[KC][2][NT][4] = {}, s_acc[NT] = {}, q_acc[NT] = {};  // sums of d r z, of d, of d r mean
+  RowSums<T, KC, NT> sums;
   for (uint32_t n0 = (blockIdx.x * 8 + warp) * 16; n0 < rows; n0 += step) {
     const Rows2 row(a, n0, rows);
-    Tile<T, KC> x;
+    Tile<T, KC, true> x;
     x.load(a, row);
-    float d[NT][2][2];  // [row g, g + 8][head 2t, 2t + 1]
+    float d[NT][2][2];
+    uint32_t dp[NT][2][Pieces<T>::kX];
+    load_d<T, NT>(a, row, 0, d, dp);
+    x.statistics(a);
+    if (a.partial) sums.add(a, x, dp);
+    if (!a.dz) continue;
+    float acc[NT][4] = {}, c0[2] = {}, c1[2] = {};
+    product_by_rows<T, KC, NT>(a, x, sm_g, acc);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int k = 0; k < 2; ++k)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int h = nt * 8 + 2 * t + e;
-          d[nt][k][e] = row.on[k] && h < a.H ? to_float<T>(static_cast<const T*>(a.out)[row.o[k] + h * a.sout.b]) : 0.f;
-        }
-    uint32_t dp[NT][2][XP];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int k = 0; k < 2; ++k) split2<XP>(d[nt][k][0], d[nt][k][1], dp[nt][k]);
-    x.statistics(a, row);
-
-    if (a.partial) {
-      // r and mean of rows 2t, 2t + 1, 2t + 8, 2t + 9, which the lanes 4 (2t) and 4 (2t + 1) hold
-      float r[2][2], mean[2][2];
-#pragma unroll
-      for (int k = 0; k < 2; ++k)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          r[k][e] = __shfl_sync(0xffffffffu, x.r[k], 8 * t + 4 * e);
-          mean[k][e] = __shfl_sync(0xffffffffu, x.mean[k], 8 * t + 4 * e);
-        }
-      uint32_t ap[NT][2][AP];  // pieces of d r, [rows x heads] transposed
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+      for (int e = 0; e < 2; ++e) {
+        const float sum = sm_sum[nt * 8 + 2 * t + e];
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-          float d0 = 0.f, d1 = 0.f;
-#pragma unroll
-          for (int i = XP - 1; i >= 0; --i) {
-            float lo, hi;
-            unpack2<__nv_bfloat16>(transposed(dp[nt][k][i]), lo, hi);
-            d0 += lo;
-            d1 += hi;
-          }
-          s_acc[nt] += d0 + d1;
-          d0 *= r[k][0];
-          d1 *= r[k][1];
-          q_acc[nt] = fmaf(d0, mean[k][0], fmaf(d1, mean[k][1], q_acc[nt]));
-          split2<AP>(d0, d1, ap[nt][k]);
-        }
-#pragma unroll
-      for (int kc = 0; kc < KC; ++kc) {
-        uint32_t lo[4][XP], hi[4][XP];
-        x.x[0][kc].pieces(lo);
-        x.x[1][kc].pieces(hi);
-#pragma unroll
-        for (int p = 0; p < 2; ++p)
-#pragma unroll
-          for (int i = 0; i < XP; ++i) {
-            const uint32_t a0 = transposed(lo[2 * p][i]), a1 = transposed(lo[2 * p + 1][i]), a2 = transposed(hi[2 * p][i]), a3 = transposed(hi[2 * p + 1][i]);
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-              for (int j = 0; j + i < AP; ++j) mma_k16(m_acc[kc][p][nt], a0, a1, a2, a3, ap[nt][0][j], ap[nt][1][j]);
-          }
-      }
-    }
-    if (!a.dz) continue;
-    const auto u_of = [&](int kc, float (&u)[2][8]) {
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        float acc[4] = {};
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int j = 0; j < GP; ++j) {
-            const uint32_t gw = reinterpret_cast<const uint32_t*>(sm_g + ((kc * NT + nt) * GP + j) * 32 + lane)[q];
-#pragma unroll
-            for (int i = 0; i < XP; ++i)
-              if (i + j < Pieces<T>::kTerms) mma_k8(acc, dp[nt][0][i], dp[nt][1][i], gw);
-          }
-        u[0][2 * q] = acc[0]; u[0][2 * q + 1] = acc[1]; u[1][2 * q] = acc[2]; u[1][2 * q + 1] = acc[3];
-      }
-    };
-    constexpr bool kKeep = KC <= 4 && sizeof(T) == 2;  // u stays in registers, else it is worked out twice
-    float u_all[kKeep ? KC : 1][2][8], m1[2] = {}, m2[2] = {};
-#pragma unroll
-    for (int kc = 0; kc < KC; ++kc) {
-      float(&u)[2][8] = u_all[kKeep ? kc : 0];
-      u_of(kc, u);
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        float v[8];
-        x.x[k][kc].floats(v);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          m1[k] += u[k][e];
-          m2[k] = fmaf(u[k][e], v[e] - x.mean[k], m2[k]);  // (channels that are not there have u = 0)
+          c0[k] = fmaf(d[nt][k][e], sum, c0[k]);
+          c1[k] = fmaf(d[nt][k][e], fmaf(-x.mean[k], sum, acc[nt][2 * k + e]), c1[k]);
         }
       }
-    }
-    // dz = r u - r m1 - (z - mean) r^2 mean(u (z - mean) r)
-    float c0[2], c1[2];
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-      c0[k] = x.r[k] * quad_sum(m1[k]) * by_C;
-      c1[k] = x.r[k] * x.r[k] * x.r[k] * quad_sum(m2[k]) * by_C;
+      c0[k] = x.r[k] * quad_sum(c0[k]) * by_C;
+      c1[k] = x.r[k] * x.r[k] * x.r[k] * quad_sum(c1[k]) * by_C;
     }
-#pragma unroll
-    for (int kc = 0; kc < KC; ++kc) {
-      float(&u)[2][8] = u_all[kKeep ? kc : 0];
-      if (!kKeep) u_of(kc, u);
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        if (!row.on[k] || kc * 32 + t * 8 >= a.C) continue;
-        float v[8];
-        x.x[k][kc].floats(v);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = fmaf(x.r[k], u[k][e], -fmaf(v[e] - x.mean[k], c1[k], c0[k]));
-        Eight<T>::store(static_cast<T*>(a.dz) + (long long)row.n[k] * a.C + kc * 32 + t * 8, v);
-      }
-    }
+    write_dz<T, KC, NT>(a, x, row, sm_g + kG, dp, c0, c1);
   }
   if (!a.partial) return;
-  // The warps add their sums in turn; q is the same for all channels.
-  float* sums = reinterpret_cast<float*>(sm_g);
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    s_acc[nt] = quad_sum(s_acc[nt]);
-    q_acc[nt] = quad_sum(q_acc[nt]);
-  }
-  for (int w = 0; w < 8; ++w) {
-    __syncthreads();
-    if (warp != w) continue;
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      // head 8 nt + g is what the lane's s and q are of; its part of M is heads 2t, 2t + 1
-      const float q0 = __shfl_sync(0xffffffffu, q_acc[nt], 8 * t), q1 = __shfl_sync(0xffffffffu, q_acc[nt], 8 * t + 4);
-#pragma unroll
-      for (int kc = 0; kc < KC; ++kc)
-#pragma unroll
-        for (int p = 0; p < 2; ++p)
-#pragma unroll
-          for (int k = 0; k < 2; ++k)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const int h = nt * 8 + 2 * t + e, c = kc * 32 + g / 2 * 8 + 2 * (2 * p + k) + (g & 1);
-              if (h >= a.H || c >= a.C) continue;
-              float& to = sums[h * (a.C + 1) + c];
-              const float v = m_acc[kc][p][nt][2 * k + e] - (e ? q1 : q0);
-              to = w ? to + v : v;
-            }
-      const int h = nt * 8 + g;
-      if (t == 0 && h < a.H) {
-        float& to = sums[h * (a.C + 1) + a.C];
-        to = w ? to + s_acc[nt] : s_acc[nt];
-      }
-    }
-  }
-  __syncthreads();
-  const int size = a.H * (a.C + 1);
-  for (int i = threadIdx.x; i < size; i += 256) a.partial[(long long)blockIdx.x * size + i] = sums[i];
+  sums.leave(reinterpret_cast<float*>(sm_g));
+  write_partial<KC, NT>(a, reinterpret_cast<const float*>(sm_g), blockIdx.x, 0, 0);
 }
 
-// ---------------------------------------------------------------- any call
-
-// A warp a row, lane l the channels l, l + 32, ...
-template <class T>
-__device__ __forceinline__ void normalise(const ProjArgs& a, const Row& row, float (&x)[kMaxPerLane], float& mean, float& r) {
-  const T* z = static_cast<const T*>(a.z) + row.at(a.sz);
-  const int lane = threadIdx.x & 31;
-  float s = 0.f;
-#pragma unroll
-  for (int k = 0; k < kMaxPerLane; ++k) {
-    x[k] = lane + 32 * k < a.C ? to_float<T>(z[lane + 32 * k]) : 0.f;
-    s += x[k];
-  }
-  mean = warp_sum(s) / a.C;
-  s = 0.f;
-#pragma unroll
-  for (int k = 0; k < kMaxPerLane; ++k) {
-    x[k] = lane + 32 * k < a.C ? x[k] - mean : 0.f;
-    s = fmaf(x[k], x[k], s);
-  }
-  r = rsqrtf(warp_sum(s) / a.C + a.eps);
-#pragma unroll
-  for (int k = 0; k < kMaxPerLane; ++k) x[k] *= r;
-}
-
-template <class T>
-__global__ void __launch_bounds__(256) projection_fwd(ProjArgs a) {
-  ptx::grid_dependency_wait();
-  ptx::grid_launch_dependents();
-  extern __shared__ float sm[];  // [H][C] and [H]
-  float* sm_t = sm + a.H * a.C;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  for (int i = threadIdx.x; i < a.H * a.C; i += 256) sm[i] = load_any(a.w, a.w_dtype, i) * gain(a, i % a.C);
-  for (int h = warp; h < a.H; h += 8) {
-    float t = 0.f;
-    if (a.b)
-      for (int c = lane; c < a.C; c += 32) t = fmaf(load_any(a.w, a.w_dtype, h * a.C + c), load_any(a.b, a.b_dtype, c), t);
-    t = warp_sum(t);
-    if (lane == 0) sm_t[h] = t;
-  }
-  __syncthreads();
-  const long long rows = (long long)a.B * a.Ri * a.Rj;
-  for (long long n = (long long)blockIdx.x * 8 + warp; n < rows; n += (long long)gridDim.x * 8) {
-    const Row row(a, n);
-    float x[kMaxPerLane], mean, r;
-    normalise<T>(a, row, x, mean, r);
-    for (int h = 0; h < a.H; ++h) {
-      float s = 0.f;
-#pragma unroll
-      for (int k = 0; k < kMaxPerLane; ++k)
-        if (lane + 32 * k < a.C) s = fmaf(x[k], sm[h * a.C + lane + 32 * k], s);
-      s = warp_sum(s);
-      if (lane == 0) static_cast<T*>(a.out)[row.at(a.sout, h)] = from_float<T>(s + sm_t[h]);
-    }
-  }
-}
-
-template <class T>
+// More channels and heads than one block can hold the sums of: dz and the rows' statistics in one kernel ...
+template <class T, int KC, int NT, bool KEEP>
 __global__ void __launch_bounds__(256) projection_dz(ProjArgs a) {
   ptx::grid_dependency_wait();
   ptx::grid_launch_dependents();
-  extern __shared__ float sm[];  // [H][C]
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  for (int i = threadIdx.x; i < a.H * a.C; i += 256) sm[i] = load_any(a.w, a.w_dtype, i) * gain(a, i % a.C);
+  extern __shared__ __align__(16) uint4 sm_g[];  // G by heads
+  const int warp = threadIdx.x >> 5;
+  const uint32_t rows = (uint32_t)((long long)a.B * a.Ri * a.Rj), step = gridDim.x * 128;
+  if (a.dz) lay_out_by_heads<Pieces<T>::kG>(a, KC, NT, sm_g);
   __syncthreads();
-  const long long rows = (long long)a.B * a.Ri * a.Rj;
-  for (long long n = (long long)blockIdx.x * 8 + warp; n < rows; n += (long long)gridDim.x * 8) {
-    const Row row(a, n);
-    float x[kMaxPerLane], mean, r;
-    normalise<T>(a, row, x, mean, r);
-    if (a.stats && lane == 0) reinterpret_cast<float2*>(a.stats)[n] = make_float2(mean, r);
+  const float by_C = 1.f / a.C;
+  for (uint32_t n0 = (blockIdx.x * 8 + warp) * 16; n0 < rows; n0 += step) {
+    const Rows2 row(a, n0, rows);
+    Tile<T, KC, KEEP> x;
+    x.load(a, row);
+    x.statistics(a);
+    if (a.stats && (threadIdx.x & 3) == 0) {
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+        if (row.on[k]) reinterpret_cast<float2*>(a.stats)[row.row(k)] = make_float2(x.mean[k], x.r[k]);
+    }
     if (!a.dz) continue;
-    float u[kMaxPerLane] = {};
-    for (int h = 0; h < a.H; ++h) {
-      const float d = to_float<T>(static_cast<const T*>(a.out)[row.at(a.sout, h)]);
+    float d[NT][2][2], c0[2] = {}, c1[2] = {};
+    uint32_t dp[NT][2][Pieces<T>::kX];
+    load_d<T, NT>(a, row, 0, d, dp);
+#pragma unroll KEEP ? KC : 1
+    for (int kc = 0; kc < KC; ++kc) {
+      float u[2][8];
+      product_by_heads<T, NT>(sm_g, kc, dp, u);
 #pragma unroll
-      for (int k = 0; k < kMaxPerLane; ++k)
-        if (lane + 32 * k < a.C) u[k] = fmaf(d, sm[h * a.C + lane + 32 * k], u[k]);
+      for (int k = 0; k < 2; ++k) {
+        float v[8];
+        x.get(a, k, kc).floats(v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          c0[k] += u[k][e];
+          c1[k] = fmaf(u[k][e], v[e] - x.mean[k], c1[k]);  // (channels that are not there have u = 0)
+        }
+      }
     }
-    float m1 = 0.f, m2 = 0.f;
 #pragma unroll
-    for (int k = 0; k < kMaxPerLane; ++k) {
-      m1 += u[k];
-      m2 = fmaf(u[k], x[k], m2);
+    for (int k = 0; k < 2; ++k) {
+      c0[k] = x.r[k] * quad_sum(c0[k]) * by_C;
+      c1[k] = x.r[k] * x.r[k] * x.r[k] * quad_sum(c1[k]) * by_C;
     }
-    m1 = warp_sum(m1) / a.C;
-    m2 = warp_sum(m2) / a.C;
-#pragma unroll
-    for (int k = 0; k < kMaxPerLane; ++k)
-      if (lane + 32 * k < a.C) static_cast<T*>(a.dz)[n * a.C + lane + 32 * k] = from_float<T>(r * (u[k] - m1 - x[k] * m2));
+    write_dz<T, KC, NT>(a, x, row, sm_g, dp, c0, c1);
   }
 }
 
-// M and s of a share of the rows: a thread a channel (the one behind the last: s), eight heads a block.
+// ... and M and s of 128 channels and 16 heads a block in another, with those statistics.
+constexpr int kSumChannels = 128, kSumHeads = 16;
 template <class T>
-__global__ void __launch_bounds__(128) projection_sums(ProjArgs a) {
+__global__ void __launch_bounds__(256) projection_sums(ProjArgs a) {
   ptx::grid_dependency_wait();
   ptx::grid_launch_dependents();
-  const int c = blockIdx.y * 128 + threadIdx.x, h0 = blockIdx.z * 8, nh = min(8, a.H - h0);
-  if (c > a.C) return;
-  float m[8] = {};
-  const long long rows = (long long)a.B * a.Ri * a.Rj;
-  for (long long n = blockIdx.x; n < rows; n += gridDim.x) {
-    const Row row(a, n);
-    const float2 st = reinterpret_cast<const float2*>(a.stats)[n];
-    const float x = c < a.C ? (to_float<T>(static_cast<const T*>(a.z)[row.at(a.sz) + c]) - st.x) * st.y : 1.f;
+  constexpr int KC = kSumChannels / 32, NT = kSumHeads / 8;
+  __shared__ float sm[kSumHeads * (kSumChannels + 1)];
+  const int warp = threadIdx.x >> 5, c0 = blockIdx.y * kSumChannels, h0 = blockIdx.z * kSumHeads;
+  const uint32_t rows = (uint32_t)((long long)a.B * a.Ri * a.Rj), step = gridDim.x * 128;
+  ProjArgs part = a;  // these channels of z
+  part.z = static_cast<const T*>(a.z) + c0;
+  part.C = a.C - c0;
+  RowSums<T, KC, NT> sums;
+  for (uint32_t n0 = (blockIdx.x * 8 + warp) * 16; n0 < rows; n0 += step) {
+    const Rows2 row(a, n0, rows);
+    Tile<T, KC, true> x;
+    x.load(part, row);
+    float d[NT][2][2];
+    uint32_t dp[NT][2][Pieces<T>::kX];
+    load_d<T, NT>(a, row, h0 / 8, d, dp);
 #pragma unroll
-    for (int h = 0; h < 8; ++h)
-      if (h < nh) m[h] = fmaf(to_float<T>(static_cast<const T*>(a.out)[row.at(a.sout, h0 + h)]), x, m[h]);
+    for (int k = 0; k < 2; ++k) {
+      const float2 st = row.on[k] ? reinterpret_cast<const float2*>(a.stats)[row.row(k)] : make_float2(0.f, 0.f);
+      x.mean[k] = st.x;
+      x.r[k] = st.y;
+    }
+    sums.add(part, x, dp);
   }
-  for (int h = 0; h < nh; ++h) a.partial[((long long)blockIdx.x * a.H + h0 + h) * (a.C + 1) + c] = m[h];
+  sums.leave(sm);
+  write_partial<KC, NT>(a, sm, blockIdx.x, h0, c0);
 }
 
 // The blocks' sums, added in order, and the gradients of the weights from them.  A block has eight channels: 128 shares of
@@ -629,7 +738,7 @@ int validate(const evoattn_pair_projection_params* p) {
   if (p->B < 0 || p->Ri < 0 || p->Rj < 0 || p->C <= 0 || p->H <= 0 || !(p->eps >= 0.f)) return EVOATTN_ERR_SHAPE;
   if (p->C > EVOATTN_PROJECTION_MAX_C || p->H > EVOATTN_PROJECTION_MAX_H) return EVOATTN_ERR_UNSUPPORTED;
   if (p->Ri > (1 << 20) || p->Rj > (1 << 20) || p->B > (1 << 20)) return EVOATTN_ERR_SHAPE;
-  if ((long long)p->B * p->Ri > (1LL << 48) / (p->Rj > 0 ? p->Rj : 1) / p->C) return EVOATTN_ERR_SHAPE;
+  if ((long long)p->B * p->Ri > 0x7fffffffLL / (p->Rj > 0 ? p->Rj : 1)) return EVOATTN_ERR_SHAPE;  // rows are counted in 32 bits
   return EVOATTN_OK;
 }
 
@@ -648,48 +757,53 @@ ProjArgs args_of(const evoattn_pair_projection_params* p) {
 }
 long long rows_of(const ProjArgs& a) { return (long long)a.B * a.Ri * a.Rj; }
 size_t stats_bytes(const ProjArgs& a) { return (size_t)((rows_of(a) * 8 + 15) / 16 * 16); }
-int weights_smem(const ProjArgs& a) { return a.H * (a.C + 1) * (int)sizeof(float); }
+void look_at_rows(ProjArgs* a, int es) {
+  a->z_dense = a->sz.b == a->Rj * a->sz.c && a->sz.a == a->Ri * a->sz.b;
+  a->whole = a->C % 8 == 0 && (((uintptr_t)a->z | (uintptr_t)a->dz) & 15) == 0 && a->sz.a * es % 16 == 0 && a->sz.b * es % 16 == 0 && a->sz.c * es % 16 == 0;
+}
 
-// Whether the tensor-core kernels take a call: rows in pieces of eight channels and 16 bytes.  The backward holds M of all
-// channels and heads in registers, which bounds their product.
-bool rows_in_pieces(const ProjArgs& a, int es) {
-  return a.C % 8 == 0 && rows_of(a) < (1LL << 31) && ((uintptr_t)a.z & 15) == 0 && a.sz.a * es % 16 == 0 && a.sz.b * es % 16 == 0 && a.sz.c * es % 16 == 0;
-}
-bool mma_fwd(const ProjArgs& a, int es) { return rows_in_pieces(a, es) && a.C <= (es == 2 ? 512 : 256); }
-bool mma_bwd(const ProjArgs& a, int es) {
-  if (!rows_in_pieces(a, es) || ((uintptr_t)a.dz & 15)) return false;
-  if (es == 4) return a.C <= 128 && a.H <= 8;
-  return (a.C <= 256 && a.H <= 8) || (a.C <= 128 && a.H <= 16);
-}
-template <int KC_, int NT_> struct Shape { static constexpr int KC = KC_, NT = NT_; };
+template <int KC_, int NT_, bool KEEP_> struct Shape { static constexpr int KC = KC_, NT = NT_; static constexpr bool KEEP = KEEP_; };
+// 32 KC channels and 8 NT heads for a call; rows stay in registers while they take up to 64 a lane.
 template <class T, class F>
-void with_fwd_shape(const ProjArgs& a, F&& f) {
+void with_shape(const ProjArgs& a, F&& f) {
   const auto heads = [&](auto kc) {
     constexpr int KC = decltype(kc)::value;
-    if (a.H <= 8) f(Shape<KC, 1>());
-    else if (a.H <= 16) f(Shape<KC, 2>());
-    else if (a.H <= 32) f(Shape<KC, 4>());
-    else f(Shape<KC, 8>());
+    constexpr bool keep = KC * (int)sizeof(T) <= 16;
+    if (a.H <= 8) f(Shape<KC, 1, keep>());
+    else if (a.H <= 16) f(Shape<KC, 2, keep>());
+    else f(Shape<KC, 8, KC * (int)sizeof(T) <= 8>());
   };
   if (a.C <= 64) heads(std::integral_constant<int, 2>());
   else if (a.C <= 128) heads(std::integral_constant<int, 4>());
   else if (a.C <= 256) heads(std::integral_constant<int, 8>());
-  else if constexpr (sizeof(T) == 2) heads(std::integral_constant<int, 16>());
+  else heads(std::integral_constant<int, 16>());
 }
+// Whether the backward is one kernel, which holds M of all channels and heads in registers beside the rows.
+bool one_pass(const ProjArgs& a, int es) { return es == 4 ? a.C <= 128 && a.H <= 8 : (a.C <= 256 && a.H <= 8) || (a.C <= 128 && a.H <= 16); }
 template <class T, class F>
-void with_bwd_shape(const ProjArgs& a, F&& f) {
+void with_one_pass_shape(const ProjArgs& a, F&& f) {
   if (a.H <= 8) {
-    if (a.C <= 64) f(Shape<2, 1>());
-    else if (a.C <= 128) f(Shape<4, 1>());
-    else if constexpr (sizeof(T) == 2) f(Shape<8, 1>());
+    if (a.C <= 64) f(Shape<2, 1, true>());
+    else if (a.C <= 128) f(Shape<4, 1, true>());
+    else if constexpr (sizeof(T) == 2) f(Shape<8, 1, true>());
   } else if constexpr (sizeof(T) == 2) {
-    if (a.C <= 64) f(Shape<2, 2>());
-    else f(Shape<4, 2>());
+    if (a.C <= 64) f(Shape<2, 2, true>());
+    else f(Shape<4, 2, true>());
   }
 }
-// Blocks of the backward, each of which leaves sums of H (C + 1) floats.
-int bwd_blocks(const ProjArgs& a, bool mma) {
-  const long long rows = rows_of(a), want = mma ? (rows + 127) / 128 : rows, most = mma ? 148 : 592;
+// Blocks of 128 rows that run at once.
+template <class K>
+bool blocks_of(K kern, long long rows, int smem, unsigned* blocks) {
+  int regs = 0;
+  if (!kernel_ready(reinterpret_cast<const void*>(kern), smem, &regs)) return false;
+  const int by_regs = 65536 / ((regs + 7) / 8 * 8 * 256), by_smem = 220 * 1024 / (smem + 2048);
+  const long long want = (rows + 127) / 128, most = 148LL * (by_regs < by_smem ? by_regs : by_smem);
+  *blocks = (unsigned)(want < most ? want : most);
+  return true;
+}
+// Blocks that leave partial sums of H (C + 1) floats: as many as run at once.
+int sum_blocks(const ProjArgs& a, int es) {
+  const long long want = (rows_of(a) + 127) / 128, most = es == 2 && a.C <= 128 && a.H <= 8 ? 296 : 148;
   return (int)(want < most ? want : most);
 }
 
@@ -707,36 +821,29 @@ int evoattn_pair_projection_fwd(const evoattn_pair_projection_params* p, void* c
   if (!a.z || !a.w || !p->out) return EVOATTN_ERR_NULL;
   a.out = p->out;
   a.sout = Str3{p->out_stride[0], p->out_stride[1], p->out_stride[2]};
+  a.dz = nullptr;
+  look_at_rows(&a, dtype_bytes(p->dtype));
   cudaStream_t st = reinterpret_cast<cudaStream_t>(cuda_stream);
-  return with_dtype(p->dtype, [&](auto e) {
+  cudaError_t rc = cudaErrorUnknown;
+  with_dtype(p->dtype, [&](auto e) {
     using T = decltype(e);
-    cudaError_t rc = cudaErrorUnknown;
-    if (mma_fwd(a, (int)sizeof(T))) {
-      with_fwd_shape<T>(a, [&](auto sh) {
-        using Sh = decltype(sh);
-        const auto kern = projection_fwd_mma<T, Sh::KC, Sh::NT>;
-        const int smem = Sh::KC * Sh::NT * Pieces<T>::kG * 512;
-        int regs = 0;
-        if (!kernel_ready(reinterpret_cast<const void*>(kern), smem, &regs)) return;
-        const int by_regs = 65536 / ((regs + 7) / 8 * 8 * 256), by_smem = 220 * 1024 / (smem + 2048);
-        const long long blocks = (rows + 127) / 128, most = 148LL * (by_regs < by_smem ? by_regs : by_smem);
-        rc = launch_dependent(kern, dim3((unsigned)(blocks < most ? blocks : most)), 256, (size_t)smem, st, a);
-      });
-    } else {
-      const auto kern = projection_fwd<T>;
-      if (!kernel_ready(reinterpret_cast<const void*>(kern), weights_smem(a), nullptr)) return (int)EVOATTN_ERR_CUDA;
-      rc = launch_dependent(kern, dim3((unsigned)((rows + 7) / 8 < 148 * 4 ? (rows + 7) / 8 : 148 * 4)), 256, (size_t)weights_smem(a), st, a);
-    }
-    return (int)(rc == cudaSuccess ? EVOATTN_OK : EVOATTN_ERR_CUDA);
+    with_shape<T>(a, [&](auto sh) {
+      using Sh = decltype(sh);
+      const auto kern = projection_fwd<T, Sh::KC, Sh::NT, Sh::KEEP>;
+      const int smem = Sh::KC * Sh::NT * Pieces<T>::kG * 512;
+      unsigned blocks;
+      if (blocks_of(kern, rows, smem, &blocks)) rc = launch_dependent(kern, dim3(blocks), 256, (size_t)smem, st, a);
+    });
+    return 0;
   });
+  return rc == cudaSuccess ? EVOATTN_OK : EVOATTN_ERR_CUDA;
 }
 
 size_t evoattn_pair_projection_bwd_workspace_bytes(const evoattn_pair_projection_params* p) {
   using namespace evo;
   if (validate(p) || !(p->dweight || p->dnorm_weight || p->dnorm_bias)) return 0;
   const ProjArgs a = args_of(p);
-  const bool mma = mma_bwd(a, dtype_bytes(p->dtype));
-  return (mma ? 0 : stats_bytes(a)) + (size_t)bwd_blocks(a, mma) * a.H * (a.C + 1) * sizeof(float);
+  return (one_pass(a, dtype_bytes(p->dtype)) ? 0 : stats_bytes(a)) + (size_t)sum_blocks(a, dtype_bytes(p->dtype)) * a.H * (a.C + 1) * sizeof(float);
 }
 
 int evoattn_pair_projection_bwd(const evoattn_pair_projection_params* p, void* cuda_stream) {
@@ -750,12 +857,13 @@ int evoattn_pair_projection_bwd(const evoattn_pair_projection_params* p, void* c
   if ((uintptr_t)p->workspace & 15) return EVOATTN_ERR_ALIGN;
   a.out = const_cast<void*>(p->d_out);
   a.sout = Str3{p->d_out_stride[0], p->d_out_stride[1], p->d_out_stride[2]};
-  const bool sums = a.dw || a.dg || a.db, mma = mma_bwd(a, dtype_bytes(p->dtype));
-  a.blocks = bwd_blocks(a, mma);
+  look_at_rows(&a, dtype_bytes(p->dtype));
+  const bool sums = a.dw || a.dg || a.db, one = one_pass(a, dtype_bytes(p->dtype));
+  a.blocks = sum_blocks(a, dtype_bytes(p->dtype));
   if (sums) {
     unsigned char* ws = static_cast<unsigned char*>(p->workspace);
-    if (!mma) a.stats = reinterpret_cast<float*>(ws);
-    a.partial = reinterpret_cast<float*>(ws + (mma ? 0 : stats_bytes(a)));
+    if (!one) a.stats = reinterpret_cast<float*>(ws);
+    a.partial = reinterpret_cast<float*>(ws + (one ? 0 : stats_bytes(a)));
   }
   cudaStream_t st = reinterpret_cast<cudaStream_t>(cuda_stream);
   cudaError_t rc = cudaSuccess;
@@ -763,21 +871,26 @@ int evoattn_pair_projection_bwd(const evoattn_pair_projection_params* p, void* c
     with_dtype(p->dtype, [&](auto e) {
       using T = decltype(e);
       rc = cudaErrorUnknown;
-      if (mma) {
-        with_bwd_shape<T>(a, [&](auto sh) {
+      if (one) {
+        with_one_pass_shape<T>(a, [&](auto sh) {
           using Sh = decltype(sh);
-          const auto kern = projection_bwd_mma<T, Sh::KC, Sh::NT>;
-          const int pieces = Sh::KC * Sh::NT * Pieces<T>::kG * 512, smem = pieces > weights_smem(a) ? pieces : weights_smem(a);
-          if (!kernel_ready(reinterpret_cast<const void*>(kern), smem, nullptr)) return;
-          rc = launch_dependent(kern, dim3((unsigned)a.blocks), 256, (size_t)smem, st, a);
+          const auto kern = projection_bwd<T, Sh::KC, Sh::NT>;
+          const int pieces = 2 * Sh::KC * Sh::NT * Pieces<T>::kG * 512, left = 8 * Sh::NT * (32 * Sh::KC + 1) * (int)sizeof(float), smem = pieces > left ? pieces : left;
+          if (kernel_ready(reinterpret_cast<const void*>(kern), smem, nullptr)) rc = launch_dependent(kern, dim3((unsigned)a.blocks), 256, (size_t)smem, st, a);
         });
         return 0;
       }
-      const auto kern = projection_dz<T>;
-      if (!kernel_ready(reinterpret_cast<const void*>(kern), weights_smem(a), nullptr)) return 0;
-      rc = launch_dependent(kern, dim3((unsigned)((rows + 7) / 8 < 148 * 4 ? (rows + 7) / 8 : 148 * 4)), 256, (size_t)weights_smem(a), st, a);
-      if (rc == cudaSuccess && sums)
-        rc = launch_dependent(projection_sums<T>, dim3((unsigned)a.blocks, (unsigned)((a.C + 128) / 128), (unsigned)((a.H + 7) / 8)), 128, 0, st, a);
+      with_shape<T>(a, [&](auto sh) {
+        using Sh = decltype(sh);
+        const auto kern = projection_dz<T, Sh::KC, Sh::NT, Sh::KEEP>;
+        const int smem = Sh::KC * Sh::NT * Pieces<T>::kG * 512;
+        unsigned blocks;
+        if (blocks_of(kern, rows, smem, &blocks)) rc = launch_dependent(kern, dim3(blocks), 256, (size_t)smem, st, a);
+      });
+      if (rc == cudaSuccess && sums) {
+        const dim3 grid((unsigned)a.blocks, (unsigned)((a.C + kSumChannels - 1) / kSumChannels), (unsigned)((a.H + kSumHeads - 1) / kSumHeads));
+        rc = launch_dependent(projection_sums<T>, grid, 256, 0, st, a);
+      }
       return 0;
     });
   if (rc == cudaSuccess && sums) rc = launch_dependent(projection_weights, dim3((unsigned)((a.C + 7) / 8)), 1024, 0, st, a);

@@ -324,7 +324,8 @@ int evoattn_relative_bias_fwd(const evoattn_relative_bias_params* p, void* cuda_
 size_t evoattn_relative_bias_bwd_workspace_bytes(const evoattn_relative_bias_params* p);
 int evoattn_relative_bias_bwd(const evoattn_relative_bias_params* p, void* cuda_stream);
 
-/* Pair-bias projection: out[b,h,i,j] = sum_c weight[h,c] * y[b,i,j,c], y the layer norm of pair[b,i,j,:]. */
+/* Pair-bias projection: out[b,h,i,j] = sum_c weight[h,c] * y[b,i,j,c], y the layer norm of pair[b,i,j,:].
+ * Up to 2^31 - 1 rows (b, i, j), and 2^20 along each axis. */
 #define EVOATTN_PROJECTION_MAX_C 512
 #define EVOATTN_PROJECTION_MAX_H 64
 typedef struct evoattn_pair_projection_params {
