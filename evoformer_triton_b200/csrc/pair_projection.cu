@@ -37,7 +37,7 @@ struct ProjArgs {
   int blocks;
   FastDiv by_Ri, by_Rj;
   int z_dense;      // rows of z one after another
-  int whole;        // z and dz in pieces of eight channels and 16 bytes
+  int small;        // offsets of rows fit 32 bits
 };
 
 __device__ __forceinline__ float gain(const ProjArgs& a, int c) { return a.g ? load_any(a.g, a.g_dtype, c) : 1.f; }
@@ -102,8 +102,10 @@ template <class T>
 struct Eight {
   static constexpr int kWords = sizeof(T) / 2;
   uint4 w[kWords];
-  __device__ __forceinline__ void load(const T* p, int count, bool whole) {
-    if (whole) {  // (the same for a launch: C and all rows in pieces of eight channels and 16 bytes)
+  // WHOLE: C and all rows are in pieces of eight channels and 16 bytes.
+  template <bool WHOLE>
+  __device__ __forceinline__ void load(const T* p, int count) {
+    if constexpr (WHOLE) {
 #pragma unroll
       for (int k = 0; k < kWords; ++k) w[k] = count > 0 ? reinterpret_cast<const uint4*>(p)[k] : make_uint4(0, 0, 0, 0);
     } else {
@@ -128,8 +130,9 @@ struct Eight {
       for (int k = 0; k < 4; ++k) split2<Pieces<T>::kX>(v[2 * k], v[2 * k + 1], p[k]);
     }
   }
-  static __device__ __forceinline__ void store(T* p, const float (&v)[8], int count, bool whole) {
-    if (whole) {
+  template <bool WHOLE>
+  static __device__ __forceinline__ void store(T* p, const float (&v)[8], int count) {
+    if constexpr (WHOLE) {
 #pragma unroll
       for (int k = 0; k < kWords; ++k)
         if (count > 0) reinterpret_cast<uint4*>(p)[k] = pack16<T>(v + k * kPer16<T>);
@@ -202,21 +205,32 @@ struct Rows2 {
   uint32_t n0;
   bool on[2];
   __device__ __forceinline__ Rows2(const ProjArgs& a, uint32_t first, uint32_t rows) : n0(first) {
+    const uint32_t q0 = a.by_Rj.div(first), j0 = first - q0 * a.Rj, b0 = a.by_Ri.div(q0), i0 = q0 - b0 * a.Ri;
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       const uint32_t n = row(k);
+      uint32_t j = j0 + (n - first), i = i0, b = b0;
       on[k] = n < rows;
-      const uint32_t m = on[k] ? n : 0, q = a.by_Rj.div(m), j = m - q * a.Rj, b = a.by_Ri.div(q), i = q - b * a.Ri;
-      z[k] = a.z_dense ? m * a.sz.c : b * a.sz.a + i * a.sz.b + j * a.sz.c;
-      o[k] = b * a.sout.a + i * a.sout.c + j;
+      while (j >= (uint32_t)a.Rj) {
+        j -= a.Rj;
+        if (++i == (uint32_t)a.Ri) i = 0, ++b;
+      }
+      if (a.small) {
+        z[k] = (int)(a.z_dense ? n * (int)a.sz.c : b * (int)a.sz.a + i * (int)a.sz.b + j * (int)a.sz.c);
+        o[k] = (int)(b * (int)a.sout.a + i * (int)a.sout.c + j);
+      } else {
+        z[k] = b * a.sz.a + i * a.sz.b + j * a.sz.c;
+        o[k] = b * a.sout.a + i * a.sout.c + j;
+      }
     }
   }
   __device__ __forceinline__ uint32_t row(int k) const { return n0 + (threadIdx.x & 31) / 4 + 8 * k; }
 };
 
 // 16 rows, 32 KC channels.  KEEP: in registers; else read again (from L1 or L2) by every use.
-template <class T, int KC, bool KEEP>
+template <class T, int KC, bool KEEP, bool WHOLE_>
 struct Tile {
+  static constexpr bool WHOLE = WHOLE_;
   static constexpr int kUnroll = KEEP ? KC : 1;
   Eight<T> x[2][KEEP ? KC : 1];
   const T* at[2];
@@ -230,14 +244,14 @@ struct Tile {
       on[k] = row.on[k];
       if constexpr (KEEP) {
 #pragma unroll
-        for (int c = 0; c < KC; ++c) x[k][c].load(at[k] + c * 32, on[k] ? count(a, c) : 0, a.whole);
+        for (int c = 0; c < KC; ++c) x[k][c].template load<WHOLE>(at[k] + c * 32, on[k] ? count(a, c) : 0);
       }
     }
   }
   __device__ __forceinline__ Eight<T> get(const ProjArgs& a, int k, int c) const {
     if constexpr (KEEP) return x[k][c];
     Eight<T> e;
-    e.load(at[k] + c * 32, on[k] ? count(a, c) : 0, a.whole);
+    e.template load<WHOLE>(at[k] + c * 32, on[k] ? count(a, c) : 0);
     return e;
   }
   // Mean and 1 / deviation, the latter about the mean; a row that is not there has r = 0 and adds nothing.
@@ -338,7 +352,7 @@ __device__ __forceinline__ void product_by_rows(const ProjArgs& a, const TileT& 
   }
 }
 
-template <class T, int KC, int NT, bool KEEP>
+template <class T, int KC, int NT, bool KEEP, bool WHOLE>
 __global__ void __launch_bounds__(256) projection_fwd(ProjArgs a) {
   ptx::grid_dependency_wait();
   ptx::grid_launch_dependents();
@@ -347,7 +361,7 @@ __global__ void __launch_bounds__(256) projection_fwd(ProjArgs a) {
   const int warp = threadIdx.x >> 5, t = threadIdx.x & 3;
   const uint32_t rows = (uint32_t)((long long)a.B * a.Ri * a.Rj), step = gridDim.x * 128;
   Rows2 next(a, (blockIdx.x * 8 + warp) * 16, rows);
-  Tile<T, KC, KEEP> x;
+  Tile<T, KC, KEEP, WHOLE> x;
   x.load(a, next);
   lay_out_by_rows<Pieces<T>::kG>(a, KC, NT, sm_g);
   sum_channels<Pieces<T>::kG>(a, NT * 8, sm_sum, sm_t);
@@ -526,10 +540,18 @@ __device__ __forceinline__ void product_by_heads(const uint4* sm_u, int kc, cons
   }
 }
 
-// dz = r u - c0 - (z - mean) c1 with c0 = r mean(u), c1 = r^3 mean(u (z - mean)).
+// dz = r u - c0 - (z - mean) c1 with c0 = r mean(u), c1 = r^3 mean(u (z - mean)), two channels an instruction.
 template <class T, int KC, int NT, class TileT>
 __device__ __forceinline__ void write_dz(const ProjArgs& a, const TileT& x, const Rows2& row, const uint4* sm_u, const uint32_t (&dp)[NT][2][Pieces<T>::kX],
                                          const float (&c0)[2], const float (&c1)[2]) {
+  ptx::F2 by_u[2], by_z[2], rest[2];
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const float more = fmaf(x.mean[k], c1[k], -c0[k]);
+    by_u[k] = ptx::f2_make(x.r[k], x.r[k]);
+    by_z[k] = ptx::f2_make(-c1[k], -c1[k]);
+    rest[k] = ptx::f2_make(more, more);
+  }
 #pragma unroll TileT::kUnroll
   for (int kc = 0; kc < KC; ++kc) {
     float u[2][8];
@@ -539,9 +561,12 @@ __device__ __forceinline__ void write_dz(const ProjArgs& a, const TileT& x, cons
       float v[8];
       x.get(a, k, kc).floats(v);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = fmaf(x.r[k], u[k][e], -fmaf(v[e] - x.mean[k], c1[k], c0[k]));
+      for (int e = 0; e < 8; e += 2) {
+        const ptx::F2 z = ptx::f2_fma(ptx::f2_make(v[e], v[e + 1]), by_z[k], rest[k]);
+        ptx::f2_get(ptx::f2_fma(ptx::f2_make(u[k][e], u[k][e + 1]), by_u[k], z), v[e], v[e + 1]);
+      }
       if (row.on[k])
-        Eight<T>::store(static_cast<T*>(a.dz) + (long long)row.row(k) * a.C + kc * 32 + (threadIdx.x & 3) * 8, v, x.count(a, kc), a.whole);
+        Eight<T>::template store<TileT::WHOLE>(static_cast<T*>(a.dz) + (long long)row.row(k) * a.C + kc * 32 + (threadIdx.x & 3) * 8, v, x.count(a, kc));
     }
   }
 }
@@ -550,7 +575,7 @@ __device__ __forceinline__ void write_dz(const ProjArgs& a, const TileT& x, cons
 //   sum_c u = sum_h d[h] sum_c G[h,c],   sum_c u (z - mean) = sum_h d[h] (sum_c G[h,c] z[c] - mean sum_c G[h,c]),
 // the latter with the product that the forward takes.
 template <class T, int KC, int NT>
-__global__ void __launch_bounds__(256) projection_bwd(ProjArgs a) {
+__global__ void __launch_bounds__(256, sizeof(T) == 2 && KC <= 4 && NT == 1 ? 2 : 1) projection_bwd(ProjArgs a) {
   ptx::grid_dependency_wait();
   ptx::grid_launch_dependents();
   constexpr int kG = KC * NT * Pieces<T>::kG * 32;
@@ -568,7 +593,7 @@ __global__ void __launch_bounds__(256) projection_bwd(ProjArgs a) {
   RowSums<T, KC, NT> sums;
   for (uint32_t n0 = (blockIdx.x * 8 + warp) * 16; n0 < rows; n0 += step) {
     const Rows2 row(a, n0, rows);
-    Tile<T, KC, true> x;
+    Tile<T, KC, true, true> x;
     x.load(a, row);
     float d[NT][2][2];
     uint32_t dp[NT][2][Pieces<T>::kX];
@@ -602,7 +627,7 @@ __global__ void __launch_bounds__(256) projection_bwd(ProjArgs a) {
 }
 
 // More channels and heads than one block can hold the sums of: dz and the rows' statistics in one kernel ...
-template <class T, int KC, int NT, bool KEEP>
+template <class T, int KC, int NT, bool KEEP, bool WHOLE>
 __global__ void __launch_bounds__(256) projection_dz(ProjArgs a) {
   ptx::grid_dependency_wait();
   ptx::grid_launch_dependents();
@@ -614,7 +639,7 @@ __global__ void __launch_bounds__(256) projection_dz(ProjArgs a) {
   const float by_C = 1.f / a.C;
   for (uint32_t n0 = (blockIdx.x * 8 + warp) * 16; n0 < rows; n0 += step) {
     const Rows2 row(a, n0, rows);
-    Tile<T, KC, KEEP> x;
+    Tile<T, KC, KEEP, WHOLE> x;
     x.load(a, row);
     x.statistics(a);
     if (a.stats && (threadIdx.x & 3) == 0) {
@@ -652,7 +677,7 @@ __global__ void __launch_bounds__(256) projection_dz(ProjArgs a) {
 
 // ... and M and s of 128 channels and 16 heads a block in another, with those statistics.
 constexpr int kSumChannels = 128, kSumHeads = 16;
-template <class T>
+template <class T, bool WHOLE>
 __global__ void __launch_bounds__(256) projection_sums(ProjArgs a) {
   ptx::grid_dependency_wait();
   ptx::grid_launch_dependents();
@@ -666,7 +691,7 @@ __global__ void __launch_bounds__(256) projection_sums(ProjArgs a) {
   RowSums<T, KC, NT> sums;
   for (uint32_t n0 = (blockIdx.x * 8 + warp) * 16; n0 < rows; n0 += step) {
     const Rows2 row(a, n0, rows);
-    Tile<T, KC, true> x;
+    Tile<T, KC, true, WHOLE> x;
     x.load(part, row);
     float d[NT][2][2];
     uint32_t dp[NT][2][Pieces<T>::kX];
@@ -757,21 +782,36 @@ ProjArgs args_of(const evoattn_pair_projection_params* p) {
 }
 long long rows_of(const ProjArgs& a) { return (long long)a.B * a.Ri * a.Rj; }
 size_t stats_bytes(const ProjArgs& a) { return (size_t)((rows_of(a) * 8 + 15) / 16 * 16); }
-void look_at_rows(ProjArgs* a, int es) {
+// Whether rows of z (and dz) are in pieces of eight channels and 16 bytes.
+bool whole_rows(const ProjArgs& a, int es) {
+  return a.C % 8 == 0 && (((uintptr_t)a.z | (uintptr_t)a.dz) & 15) == 0 && a.sz.a * es % 16 == 0 && a.sz.b * es % 16 == 0 && a.sz.c * es % 16 == 0;
+}
+void look_at_rows(ProjArgs* a) {
+  const auto reach = [](const Str3& s, long long x, long long y, long long z) {
+    const auto size = [](long long v) { return (double)(v < 0 ? -v : v); };
+    return size(s.a) * x + size(s.b) * y + size(s.c) * z;
+  };
   a->z_dense = a->sz.b == a->Rj * a->sz.c && a->sz.a == a->Ri * a->sz.b;
-  a->whole = a->C % 8 == 0 && (((uintptr_t)a->z | (uintptr_t)a->dz) & 15) == 0 && a->sz.a * es % 16 == 0 && a->sz.b * es % 16 == 0 && a->sz.c * es % 16 == 0;
+  // (sout.b is the heads', which are not part of a row's offset; row numbers run up to a tile beyond the last)
+  a->small = reach(a->sz, a->B + 1, a->Ri, a->Rj + 64) < 2147483647.0 && reach(Str3{a->sout.a, a->sout.c, 1}, a->B + 1, a->Ri, a->Rj) < 2147483647.0;
 }
 
-template <int KC_, int NT_, bool KEEP_> struct Shape { static constexpr int KC = KC_, NT = NT_; static constexpr bool KEEP = KEEP_; };
+template <int KC_, int NT_, bool KEEP_, bool WHOLE_> struct Shape { static constexpr int KC = KC_, NT = NT_; static constexpr bool KEEP = KEEP_, WHOLE = WHOLE_; };
 // 32 KC channels and 8 NT heads for a call; rows stay in registers while they take up to 64 a lane.
 template <class T, class F>
 void with_shape(const ProjArgs& a, F&& f) {
+  if (!whole_rows(a, (int)sizeof(T))) {  // fewer shapes
+    if (a.C <= 128 && a.H <= 8) f(Shape<4, 1, (int)sizeof(T) <= 4, false>());
+    else if (a.H <= 16) f(Shape<16, 2, false, false>());
+    else f(Shape<16, 8, false, false>());
+    return;
+  }
   const auto heads = [&](auto kc) {
     constexpr int KC = decltype(kc)::value;
     constexpr bool keep = KC * (int)sizeof(T) <= 16;
-    if (a.H <= 8) f(Shape<KC, 1, keep>());
-    else if (a.H <= 16) f(Shape<KC, 2, keep>());
-    else f(Shape<KC, 8, KC * (int)sizeof(T) <= 8>());
+    if (a.H <= 8) f(Shape<KC, 1, keep, true>());
+    else if (a.H <= 16) f(Shape<KC, 2, keep, true>());
+    else f(Shape<KC, 8, KC * (int)sizeof(T) <= 8, true>());
   };
   if (a.C <= 64) heads(std::integral_constant<int, 2>());
   else if (a.C <= 128) heads(std::integral_constant<int, 4>());
@@ -779,16 +819,19 @@ void with_shape(const ProjArgs& a, F&& f) {
   else heads(std::integral_constant<int, 16>());
 }
 // Whether the backward is one kernel, which holds M of all channels and heads in registers beside the rows.
-bool one_pass(const ProjArgs& a, int es) { return es == 4 ? a.C <= 128 && a.H <= 8 : (a.C <= 256 && a.H <= 8) || (a.C <= 128 && a.H <= 16); }
+bool one_pass(const ProjArgs& a, int es) {
+  if (!whole_rows(a, es)) return false;
+  return es == 4 ? a.C <= 128 && a.H <= 8 : (a.C <= 256 && a.H <= 8) || (a.C <= 128 && a.H <= 16);
+}
 template <class T, class F>
 void with_one_pass_shape(const ProjArgs& a, F&& f) {
   if (a.H <= 8) {
-    if (a.C <= 64) f(Shape<2, 1, true>());
-    else if (a.C <= 128) f(Shape<4, 1, true>());
-    else if constexpr (sizeof(T) == 2) f(Shape<8, 1, true>());
+    if (a.C <= 64) f(Shape<2, 1, true, true>());
+    else if (a.C <= 128) f(Shape<4, 1, true, true>());
+    else if constexpr (sizeof(T) == 2) f(Shape<8, 1, true, true>());
   } else if constexpr (sizeof(T) == 2) {
-    if (a.C <= 64) f(Shape<2, 2, true>());
-    else f(Shape<4, 2, true>());
+    if (a.C <= 64) f(Shape<2, 2, true, true>());
+    else f(Shape<4, 2, true, true>());
   }
 }
 // Blocks of 128 rows that run at once.
@@ -822,14 +865,14 @@ int evoattn_pair_projection_fwd(const evoattn_pair_projection_params* p, void* c
   a.out = p->out;
   a.sout = Str3{p->out_stride[0], p->out_stride[1], p->out_stride[2]};
   a.dz = nullptr;
-  look_at_rows(&a, dtype_bytes(p->dtype));
+  look_at_rows(&a);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(cuda_stream);
   cudaError_t rc = cudaErrorUnknown;
   with_dtype(p->dtype, [&](auto e) {
     using T = decltype(e);
     with_shape<T>(a, [&](auto sh) {
       using Sh = decltype(sh);
-      const auto kern = projection_fwd<T, Sh::KC, Sh::NT, Sh::KEEP>;
+      const auto kern = projection_fwd<T, Sh::KC, Sh::NT, Sh::KEEP, Sh::WHOLE>;
       const int smem = Sh::KC * Sh::NT * Pieces<T>::kG * 512;
       unsigned blocks;
       if (blocks_of(kern, rows, smem, &blocks)) rc = launch_dependent(kern, dim3(blocks), 256, (size_t)smem, st, a);
@@ -857,7 +900,7 @@ int evoattn_pair_projection_bwd(const evoattn_pair_projection_params* p, void* c
   if ((uintptr_t)p->workspace & 15) return EVOATTN_ERR_ALIGN;
   a.out = const_cast<void*>(p->d_out);
   a.sout = Str3{p->d_out_stride[0], p->d_out_stride[1], p->d_out_stride[2]};
-  look_at_rows(&a, dtype_bytes(p->dtype));
+  look_at_rows(&a);
   const bool sums = a.dw || a.dg || a.db, one = one_pass(a, dtype_bytes(p->dtype));
   a.blocks = sum_blocks(a, dtype_bytes(p->dtype));
   if (sums) {
@@ -882,14 +925,14 @@ int evoattn_pair_projection_bwd(const evoattn_pair_projection_params* p, void* c
       }
       with_shape<T>(a, [&](auto sh) {
         using Sh = decltype(sh);
-        const auto kern = projection_dz<T, Sh::KC, Sh::NT, Sh::KEEP>;
+        const auto kern = projection_dz<T, Sh::KC, Sh::NT, Sh::KEEP, Sh::WHOLE>;
         const int smem = Sh::KC * Sh::NT * Pieces<T>::kG * 512;
         unsigned blocks;
         if (blocks_of(kern, rows, smem, &blocks)) rc = launch_dependent(kern, dim3(blocks), 256, (size_t)smem, st, a);
       });
       if (rc == cudaSuccess && sums) {
         const dim3 grid((unsigned)a.blocks, (unsigned)((a.C + kSumChannels - 1) / kSumChannels), (unsigned)((a.H + kSumHeads - 1) / kSumHeads));
-        rc = launch_dependent(projection_sums<T>, grid, 256, 0, st, a);
+        rc = whole_rows(a, (int)sizeof(T)) ? launch_dependent(projection_sums<T, true>, grid, 256, 0, st, a) : launch_dependent(projection_sums<T, false>, grid, 256, 0, st, a);
       }
       return 0;
     });
