@@ -53,7 +53,8 @@ __device__ __forceinline__ float gain(const ProjArgs& a, int c) { return a.g ? l
 // Products are of bf16 pieces with fp32 sums: an fp32 factor is the sum of three (24 bits), an fp16 one of two, a bf16 one
 // is one.  z enters as it is: sum_c G z[c] - mean sum_c G, with both sums over the same pieces of G, and M likewise from d r z
 // and d r mean.  G is two pieces (2^-17 of it is left out) where results are rounded to 16 bits, else three; d r always
-// three, since the weights' gradients may be fp32.
+// three, since the weights' gradients may be fp32.  An MMA cuts its sums off where fp32 additions round: a sum that ends in fp32 is
+// one of few MMAs, the products of low pieces first, and is added to the others in fp32.
 
 __device__ __forceinline__ void mma_k16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -338,22 +339,32 @@ __device__ __forceinline__ void product_by_rows(const ProjArgs& a, const TileT& 
     x.get(a, 0, kc).pieces(lo);
     x.get(a, 1, kc).pieces(hi);
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
+    for (int nt = 0; nt < NT; ++nt) {
+      float chunk[4] = {};
+      float(&sum)[4] = sizeof(T) == 4 ? chunk : acc[nt];
+      uint4 gw[GP];
 #pragma unroll
-      for (int j = 0; j < GP; ++j) {
-        const uint4 gw = sm_g[((kc * NT + nt) * GP + j) * 32 + lane];
+      for (int j = 0; j < GP; ++j) gw[j] = sm_g[((kc * NT + nt) * GP + j) * 32 + lane];
+#pragma unroll
+      for (int order = Pieces<T>::kTerms - 1; order >= 0; --order)
 #pragma unroll
         for (int i = 0; i < XP; ++i) {
-          if (i + j >= Pieces<T>::kTerms) continue;
-          mma_k16(acc[nt], lo[0][i], hi[0][i], lo[1][i], hi[1][i], gw.x, gw.y);
-          mma_k16(acc[nt], lo[2][i], hi[2][i], lo[3][i], hi[3][i], gw.z, gw.w);
+          const int j = order - i;
+          if (j < 0 || j >= GP) continue;
+          mma_k16(sum, lo[0][i], hi[0][i], lo[1][i], hi[1][i], gw[j].x, gw[j].y);
+          mma_k16(sum, lo[2][i], hi[2][i], lo[3][i], hi[3][i], gw[j].z, gw[j].w);
         }
+      if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[nt][e] += chunk[e];
       }
+    }
   }
 }
 
+// Three blocks an SM where the registers allow it: [1,768,768,128] to 8 heads 47 -> 43 us, fp16 56 -> 51.
 template <class T, int KC, int NT, bool KEEP, bool WHOLE>
-__global__ void __launch_bounds__(256) projection_fwd(ProjArgs a) {
+__global__ void __launch_bounds__(256, sizeof(T) == 2 && KC <= 4 && NT <= 2 && WHOLE && KEEP ? 3 : 0) projection_fwd(ProjArgs a) {
   ptx::grid_dependency_wait();
   ptx::grid_launch_dependents();
   extern __shared__ __align__(16) uint4 sm_g[];  // [KC][NT][GP][32 lanes]
@@ -448,15 +459,27 @@ struct RowSums {
       x.get(a, 0, kc).pieces(lo);
       x.get(a, 1, kc).pieces(hi);
 #pragma unroll
-      for (int p = 0; p < 2; ++p)
+      for (int p = 0; p < 2; ++p) {
+        uint32_t at[XP][4];
 #pragma unroll
         for (int i = 0; i < XP; ++i) {
-          const uint32_t a0 = transposed(lo[2 * p][i]), a1 = transposed(lo[2 * p + 1][i]), a2 = transposed(hi[2 * p][i]), a3 = transposed(hi[2 * p + 1][i]);
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int j = 0; j + i < AP; ++j) mma_k16(m[kc][p][nt], a0, a1, a2, a3, ap[nt][0][j], ap[nt][1][j]);
+          at[i][0] = transposed(lo[2 * p][i]);
+          at[i][1] = transposed(lo[2 * p + 1][i]);
+          at[i][2] = transposed(hi[2 * p][i]);
+          at[i][3] = transposed(hi[2 * p + 1][i]);
         }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          float sum[4] = {};
+#pragma unroll
+          for (int order = AP - 1; order >= 0; --order)
+#pragma unroll
+            for (int i = 0; i < XP; ++i)
+              if (order - i >= 0) mma_k16(sum, at[i][0], at[i][1], at[i][2], at[i][3], ap[nt][0][order - i], ap[nt][1][order - i]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) m[kc][p][nt][e] += sum[e];
+        }
+      }
     }
   }
   // The block's sums in shared memory, [8 NT heads][32 KC + 1]: its warps add theirs in turn.  q is the same for all channels.
@@ -527,10 +550,12 @@ __device__ __forceinline__ void product_by_heads(const uint4* sm_u, int kc, cons
         mma_k16(acc[q], dp[nt][0][0], dp[nt][1][0], dp[nt][0][0], dp[nt][1][0], gw[0][q], gw[1][q]);
       } else {
 #pragma unroll
-        for (int j = 0; j < GP; ++j)
+        for (int order = Pieces<T>::kTerms - 1; order >= 0; --order)
 #pragma unroll
-          for (int i = 0; i < XP; ++i)
-            if (i + j < Pieces<T>::kTerms) mma_k8(acc[q], dp[nt][0][i], dp[nt][1][i], gw[j][q]);
+          for (int i = 0; i < XP; ++i) {
+            const int j = order - i;
+            if (j >= 0 && j < GP) mma_k8(acc[q], dp[nt][0][i], dp[nt][1][i], gw[j][q]);
+          }
       }
     }
   }
@@ -574,8 +599,9 @@ __device__ __forceinline__ void write_dz(const ProjArgs& a, const TileT& x, cons
 // Backward in one pass over z: dz, and M and s of the block's rows.  mean(u) and mean(u (z - mean)) are sums over heads,
 //   sum_c u = sum_h d[h] sum_c G[h,c],   sum_c u (z - mean) = sum_h d[h] (sum_c G[h,c] z[c] - mean sum_c G[h,c]),
 // the latter with the product that the forward takes.
-template <class T, int KC, int NT>
-__global__ void __launch_bounds__(256, sizeof(T) == 2 && KC <= 4 && NT == 1 ? 2 : 1) projection_bwd(ProjArgs a) {
+// Two blocks an SM where the registers allow it (bf16, 128 channels, 8 heads: one block of 148 registers 116 us, two of 128 95 us).
+template <class T, int KC, int NT, bool WHOLE>
+__global__ void __launch_bounds__(256, sizeof(T) == 2 && KC <= 4 && NT == 1 && WHOLE ? 2 : 1) projection_bwd(ProjArgs a) {
   ptx::grid_dependency_wait();
   ptx::grid_launch_dependents();
   constexpr int kG = KC * NT * Pieces<T>::kG * 32;
@@ -593,7 +619,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 && KC <= 4 && NT == 1 ? 2 
   RowSums<T, KC, NT> sums;
   for (uint32_t n0 = (blockIdx.x * 8 + warp) * 16; n0 < rows; n0 += step) {
     const Rows2 row(a, n0, rows);
-    Tile<T, KC, true, true> x;
+    Tile<T, KC, true, WHOLE> x;
     x.load(a, row);
     float d[NT][2][2];
     uint32_t dp[NT][2][Pieces<T>::kX];
@@ -801,7 +827,7 @@ template <int KC_, int NT_, bool KEEP_, bool WHOLE_> struct Shape { static const
 template <class T, class F>
 void with_shape(const ProjArgs& a, F&& f) {
   if (!whole_rows(a, (int)sizeof(T))) {  // fewer shapes
-    if (a.C <= 128 && a.H <= 8) f(Shape<4, 1, (int)sizeof(T) <= 4, false>());
+    if (a.C <= 128 && a.H <= 8) f(Shape<4, 1, true, false>());
     else if (a.H <= 16) f(Shape<16, 2, false, false>());
     else f(Shape<16, 8, false, false>());
     return;
@@ -820,12 +846,14 @@ void with_shape(const ProjArgs& a, F&& f) {
 }
 // Whether the backward is one kernel, which holds M of all channels and heads in registers beside the rows.
 bool one_pass(const ProjArgs& a, int es) {
-  if (!whole_rows(a, es)) return false;
-  return es == 4 ? a.C <= 128 && a.H <= 8 : (a.C <= 256 && a.H <= 8) || (a.C <= 128 && a.H <= 16);
+  if (es == 4 || !whole_rows(a, es)) return a.C <= 128 && a.H <= 8;
+  return (a.C <= 256 && a.H <= 8) || (a.C <= 128 && a.H <= 16);
 }
 template <class T, class F>
 void with_one_pass_shape(const ProjArgs& a, F&& f) {
-  if (a.H <= 8) {
+  if (!whole_rows(a, (int)sizeof(T))) {
+    f(Shape<4, 1, true, false>());
+  } else if (a.H <= 8) {
     if (a.C <= 64) f(Shape<2, 1, true, true>());
     else if (a.C <= 128) f(Shape<4, 1, true, true>());
     else if constexpr (sizeof(T) == 2) f(Shape<8, 1, true, true>());
@@ -846,7 +874,7 @@ bool blocks_of(K kern, long long rows, int smem, unsigned* blocks) {
 }
 // Blocks that leave partial sums of H (C + 1) floats: as many as run at once.
 int sum_blocks(const ProjArgs& a, int es) {
-  const long long want = (rows_of(a) + 127) / 128, most = es == 2 && a.C <= 128 && a.H <= 8 ? 296 : 148;
+  const long long want = (rows_of(a) + 127) / 128, most = es == 2 && a.C <= 128 && a.H <= 8 && whole_rows(a, es) ? 296 : 148;
   return (int)(want < most ? want : most);
 }
 
@@ -917,7 +945,7 @@ int evoattn_pair_projection_bwd(const evoattn_pair_projection_params* p, void* c
       if (one) {
         with_one_pass_shape<T>(a, [&](auto sh) {
           using Sh = decltype(sh);
-          const auto kern = projection_bwd<T, Sh::KC, Sh::NT>;
+          const auto kern = projection_bwd<T, Sh::KC, Sh::NT, Sh::WHOLE>;
           const int pieces = 2 * Sh::KC * Sh::NT * Pieces<T>::kG * 512, left = 8 * Sh::NT * (32 * Sh::KC + 1) * (int)sizeof(float), smem = pieces > left ? pieces : left;
           if (kernel_ready(reinterpret_cast<const void*>(kern), smem, nullptr)) rc = launch_dependent(kern, dim3((unsigned)a.blocks), 256, (size_t)smem, st, a);
         });
