@@ -89,39 +89,35 @@ struct Buckets {
   }
 };
 
-// The keys of a strip of L V keys that L lanes hold, V each: consecutive ones (WIDE), or L apart.  Positions are kept relative to the
-// least one of the strip, in 32 bits: where they span 2^29 or more, which no sequence does, they are read again
-// for every row.  least - query clamped to +-2^30 plus an offset below 2^29 is on the right side of every edge.
+// The keys of a strip of L V keys that L lanes hold, V each: consecutive ones (WIDE), or L apart; other lanes of the warp
+// hold the same.  Positions are kept relative to the least one of the strip, in 32 bits: where they span 2^29 or more, which
+// no sequence does, they are read again for every row.  least - query clamped to +-2^30 plus an offset below 2^29 is on
+// the right side of every edge.
 template <int V, int L, bool WIDE>
 struct Strip {
   int j0, off[V];
-  long long least, most;
+  long long least, most;         // where near_together
   bool near_together, in_order;  // in_order: every lane's keys ascend, so those of one bucket are next to each other
   __device__ __forceinline__ int col(int u) const { return WIDE ? j0 + (threadIdx.x & (L - 1)) * V + u : j0 + u * L + (threadIdx.x & (L - 1)); }
   __device__ __forceinline__ void load(const RelArgs& a, int b, int first) {
     j0 = first;
-    long long key[V];
-    least = 0x7fffffffffffffffll;
-    most = -least - 1;
+    const long long at = b * a.sk, origin = position(a.k_pos, a.positions64, at + first);
+    int lo = 0, hi = 0;
 #pragma unroll
     for (int u = 0; u < V; ++u) {
-      key[u] = 0;
-      if (col(u) < a.Rk) {
-        key[u] = position(a.k_pos, a.positions64, b * a.sk + col(u));
-        least = min(least, key[u]);
-        most = max(most, key[u]);
-      }
+      off[u] = col(u) < a.Rk ? difference(position(a.k_pos, a.positions64, at + col(u)), origin) : 0x7fffffff;
+      lo = min(lo, off[u]);
+      if (off[u] != 0x7fffffff) hi = max(hi, off[u]);
     }
-#pragma unroll
-    for (int o = L / 2; o > 0; o >>= 1) {
-      least = min(least, __shfl_xor_sync(0xffffffffu, least, o));
-      most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
-    }
-    near_together = (unsigned long long)most - (unsigned long long)least < (1ull << 29);
+    lo = __reduce_min_sync(0xffffffffu, lo);
+    hi = __reduce_max_sync(0xffffffffu, hi);
+    near_together = (long long)hi - lo < 1 << 29;  // (one that was clamped is too far from the origin, which is at 0)
+    least = origin + lo;
+    most = origin + hi;
     bool ascending = near_together;
 #pragma unroll
     for (int u = 0; u < V; ++u) {
-      off[u] = (int)((col(u) < a.Rk ? key[u] : most) - least);  // (wrong where not near_together, and not used)
+      off[u] = (off[u] == 0x7fffffff ? hi : off[u]) - lo;
       ascending = ascending && (u == 0 || off[u] >= off[u ? u - 1 : 0]);
     }
     in_order = __all_sync(0xffffffffu, ascending);
@@ -134,8 +130,13 @@ struct Strip {
 #pragma unroll
       for (int u = 0; u < V; ++u) r[u] = bucket.near[min(max(from + off[u], 0), 2 * bucket.far)];
     } else {
-#pragma unroll 1
-      for (int u = 0; u < V; ++u) r[u] = bucket(difference(col(u) < a.Rk ? position(a.k_pos, a.positions64, b * a.sk + col(u)) : least, q));
+      for (int u = 0; u < V; ++u) {
+        const int c = WIDE ? j0 + (int)(threadIdx.x & (L - 1)) * V + u : j0 + u * L + (int)(threadIdx.x & (L - 1));
+        const int row = bucket(difference(position(a.k_pos, a.positions64, b * a.sk + min(c, a.Rk - 1)), q));
+#pragma unroll
+        for (int k = 0; k < V; ++k)
+          if (k == u) r[k] = row;
+      }
     }
   }
 };
@@ -177,7 +178,7 @@ __device__ __forceinline__ void add_base(const RelArgs& a, long long at, float (
 // A block of eight warps takes a strip of 32 V keys and kHeads heads and walks rows; with fewer rows than warps, the warps
 // share the heads of a row.  A row whose strip is one bucket, as away from the diagonal, is one value a head.
 template <class T, bool WIDE>
-__global__ void __launch_bounds__(256) relative_fwd(RelArgs a, int rows_per_block, int row_warps) {
+__global__ void __launch_bounds__(256, 4) relative_fwd(RelArgs a, int rows_per_block, int row_warps) {
   ptx::grid_dependency_wait();
   ptx::grid_launch_dependents();
   constexpr int V = kPer16<T>;
@@ -200,7 +201,7 @@ __global__ void __launch_bounds__(256) relative_fwd(RelArgs a, int rows_per_bloc
   }
   __syncthreads();
   const int lo = bucket(difference(strip.least, my_q)), hi = bucket(difference(strip.most, my_q));
-  const int my_kind = lo == hi ? lo : -1;  // (rows are in the order of distances on either side, so all between are the same)
+  const int my_kind = strip.near_together && lo == hi ? lo : -1;  // (rows are in the order of distances on either side, so all between are the same)
   const int first_head = warp / row_warps, head_step = 8 / row_warps;
   for (int k = 0, i = i0; i < i_end; ++k, i += row_warps) {
     const int kind = __shfl_sync(0xffffffffu, my_kind, k);
@@ -227,11 +228,23 @@ __global__ void __launch_bounds__(256) relative_fwd(RelArgs a, int rows_per_bloc
         if (a.base) add_base<V>(a, at + strip.col(0), v);
         *reinterpret_cast<uint4*>(o + strip.col(0)) = pack16<T>(v);
       } else {
+        if (a.base) {
+          uint32_t w[V];
+          if (a.base_dtype == EVOATTN_FP32) {
+#pragma unroll
+            for (int u = 0; u < V; ++u) w[u] = strip.col(u) < a.Rk ? static_cast<const uint32_t*>(a.base)[at + strip.col(u)] : 0;
+          } else {
+#pragma unroll
+            for (int u = 0; u < V; ++u) w[u] = strip.col(u) < a.Rk ? static_cast<const uint16_t*>(a.base)[at + strip.col(u)] : 0;
+          }
+#pragma unroll
+          for (int u = 0; u < V; ++u)
+            v[u] += a.base_dtype == EVOATTN_FP32 ? __uint_as_float(w[u])
+                    : a.base_dtype == EVOATTN_BF16 ? __uint_as_float(w[u] << 16) : __half2float(__ushort_as_half((unsigned short)w[u]));
+        }
 #pragma unroll
         for (int u = 0; u < V; ++u) {
-          if (strip.col(u) >= a.Rk) continue;
-          if (a.base) v[u] += load_any(a.base, a.base_dtype, at + strip.col(u));
-          o[strip.col(u)] = from_float<T>(v[u]);
+          if (strip.col(u) < a.Rk) o[strip.col(u)] = from_float<T>(v[u]);
         }
       }
     }
@@ -240,17 +253,19 @@ __global__ void __launch_bounds__(256) relative_fwd(RelArgs a, int rows_per_bloc
 
 // Backward: a warp takes item_rows rows of a strip of keys of one (b, h) at a time and adds every value to the sum of its
 // bucket.  Every lane has sums of its own (no two lanes add to one address, and the order of the additions is fixed).  A
-// load is kLanes V keys of kTall rows, 128 bytes of each: as near to a square as whole cache lines go, so that few loads lie across
-// the diagonal; the others are one bucket and are added up in a register.  A block keeps the sums of `window` table rows
+// load is 64 keys of 4 rows (fp32: 2), whole cache lines of each: as near to a square as those go, so that few loads lie across the
+// diagonal; the others are one bucket and are added up in a register.  A block keeps the sums of `window` table rows
 // (blockIdx.z says which); loads that cannot touch them are left out.
-constexpr int kLanes = 8, kTall = 32 / kLanes;
+template <class T> constexpr int kLanes = 64 / kPer16<T>;
+template <class T> constexpr int kTall = 32 / kLanes<T>;
+constexpr int kLoads = 16;  // of an item, at most
 
 template <class T, bool WIDE>
 struct RowPiece {  // V values of a row
   static constexpr int V = kPer16<T>;
   uint4 w;
   T e[V];
-  __device__ __forceinline__ void load(const RelArgs& a, const Strip<V, kLanes, WIDE>& strip, const T* row) {
+  __device__ __forceinline__ void load(const RelArgs& a, const Strip<V, kLanes<T>, WIDE>& strip, const T* row) {
     if (WIDE && strip.col(V - 1) < a.Rk) {
       w = *reinterpret_cast<const uint4*>(row + strip.col(0));
     } else {
@@ -286,17 +301,17 @@ template <class T, bool WIDE>
 __global__ void __launch_bounds__(128, 5) relative_bwd(RelArgs a) {
   ptx::grid_dependency_wait();
   ptx::grid_launch_dependents();
-  constexpr int V = kPer16<T>, U = WIDE ? 8 : 4;  // U: loads on the way at once
+  constexpr int V = kPer16<T>, L = kLanes<T>, TALL = kTall<T>, U = WIDE ? 8 : 4;  // U: loads on the way at once
   extern __shared__ float sm_sums[];  // [4 warps][window + 1][32 lanes]
   __shared__ uint16_t sm_near[2 * kNear + 1];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, my_row = lane / kLanes;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, my_row = lane / L;
   const int h = blockIdx.y, first = blockIdx.z * a.window, count = min(a.window, a.buckets - first);
   const Buckets<Same> bucket(a, sm_near);
   const int per_warp = (a.window + 1) * 32;  // (one more row, for what is not of this block's)
   for (int i = threadIdx.x; i < 4 * per_warp; i += 128) sm_sums[i] = 0.f;
   __syncthreads();
   float* sums = sm_sums + warp * per_warp + lane;
-  const unsigned strips = (a.Rk + kLanes * V - 1) / (kLanes * V), chunks = (a.Rq + a.item_rows - 1) / a.item_rows;
+  const unsigned strips = (a.Rk + L * V - 1) / (L * V), chunks = (a.Rq + a.item_rows - 1) / a.item_rows;
   const unsigned items = a.B * strips * chunks;
   // What all scores of keys least .. most and queries q0 .. q1 have in common: their bucket (>= 0), that none is of this
   // block's (-2), or nothing (-1).  Between the buckets of the two ends are those of all others, but for LOG, whose
@@ -309,39 +324,35 @@ __global__ void __launch_bounds__(128, 5) relative_bwd(RelArgs a) {
   };
   for (unsigned item = blockIdx.x * 4 + warp; item < items; item += gridDim.x * 4) {
     const unsigned rest = item / chunks, b = rest / strips;
-    const int i0 = (int)(item - rest * chunks) * a.item_rows, ni = min(a.item_rows, a.Rq - i0), loads = (ni + kTall - 1) / kTall;
-    Strip<V, kLanes, WIDE> strip;
-    strip.load(a, b, (int)(rest - b * strips) * kLanes * V);
-    const long long q_at = b * a.sq + i0;
-    long long q0 = 0x7fffffffffffffffll, q1 = -q0 - 1;  // over the rows of load `lane`, then over all
+    const int i0 = (int)(item - rest * chunks) * a.item_rows, ni = min(a.item_rows, a.Rq - i0), loads = (ni + TALL - 1) / TALL;
+    Strip<V, L, WIDE> strip;
+    strip.load(a, b, (int)(rest - b * strips) * L * V);
+    const long long q_at = b * a.sq + i0, q_origin = position(a.q_pos, a.positions64, q_at);
+    int q0 = 0x7fffffff, q1 = -q0;  // relative to q_origin, over the rows of load `lane`
 #pragma unroll
-    for (int k = 0; k < kTall; ++k)
-      if (lane * kTall + k < ni) {
-        const long long q = position(a.q_pos, a.positions64, q_at + lane * kTall + k);
-        q0 = min(q0, q);
-        q1 = max(q1, q);
-      }
-    long long all0 = q0, all1 = q1;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      all0 = min(all0, __shfl_xor_sync(0xffffffffu, all0, o));
-      all1 = max(all1, __shfl_xor_sync(0xffffffffu, all1, o));
+    for (int k = 0; k < TALL; ++k) {  // (rows behind the last: the last one, which changes no least or greatest)
+      const int q = difference(position(a.q_pos, a.positions64, q_at + min(lane * TALL + k, ni - 1)), q_origin);
+      q0 = min(q0, q);
+      q1 = max(q1, q);
     }
-    const int kind = kind_of(strip.least, strip.most, all0, all1);
-    if (kind == -2) continue;
     const T* d = static_cast<const T*>(a.out) + b * a.sout.a + h * a.sout.b + (long long)(i0 + my_row) * a.sout.c;
-    const long long down = kTall * a.sout.c;
+    const long long down = TALL * a.sout.c;
+    const int all0 = __reduce_min_sync(0xffffffffu, q0), all1 = __reduce_max_sync(0xffffffffu, q1);
+    // (positions that span 2^29 or more are looked at one by one)
+    const bool can_tell = strip.near_together && (long long)all1 - all0 < 1 << 29;
+    const int kind = can_tell ? kind_of(strip.least, strip.most, q_origin + all0, q_origin + all1) : -1;
+    if (kind == -2) continue;
     if (kind >= 0) {  // one bucket altogether
       float acc = 0.f;
       int l = 0;
-      for (; (l + U) * kTall <= ni; l += U) {
+      for (; (l + U) * TALL <= ni; l += U) {
         RowPiece<T, WIDE> p[U];
 #pragma unroll
         for (int k = 0; k < U; ++k, d += down) p[k].load(a, strip, d);
 #pragma unroll
         for (int k = 0; k < U; ++k) acc += p[k].sum();
       }
-      for (; l * kTall + my_row < ni; ++l, d += down) {
+      for (; l * TALL + my_row < ni; ++l, d += down) {
         RowPiece<T, WIDE> p;
         p.load(a, strip, d);
         acc += p.sum();
@@ -350,13 +361,13 @@ __global__ void __launch_bounds__(128, 5) relative_bwd(RelArgs a) {
       continue;
     }
     // Load by load: the lines are asked for first, since there is room for no more than the next load in registers.
-    const int my_kind = lane < loads ? kind_of(strip.least, strip.most, q0, q1) : -2;
+    const int my_kind = lane >= loads ? -2 : can_tell ? kind_of(strip.least, strip.most, q_origin + q0, q_origin + q1) : -1;
     for (int l = 0; l < loads; ++l)
-      if (lane % kLanes == 0 && l * kTall + my_row < ni) ptx::prefetch_l2(d + l * down + strip.col(0));
+      if (lane % L == 0 && l * TALL + my_row < ni) ptx::prefetch_l2(d + l * down + strip.col(0));
     RowPiece<T, WIDE> next;
     long long next_q = 0;
     const auto fetch = [&](int l) {
-      const int i = l * kTall + my_row;
+      const int i = l * TALL + my_row;
       if (i < ni) {
         next.load(a, strip, d + l * down);
         next_q = position(a.q_pos, a.positions64, q_at + i);
@@ -370,7 +381,7 @@ __global__ void __launch_bounds__(128, 5) relative_bwd(RelArgs a) {
 #pragma unroll 1
     for (int l = 0; l < loads; ++l) {
       const int of_load = __shfl_sync(0xffffffffu, my_kind, l);
-      const RowPiece<T, WIDE> p = next;
+      const RowPiece<T, WIDE> now = next;
       const long long q = next_q;
       if (l + 1 < loads) fetch(l + 1);
       if (of_load >= 0) {
@@ -379,11 +390,11 @@ __global__ void __launch_bounds__(128, 5) relative_bwd(RelArgs a) {
           acc_row = of_load;
           acc = 0.f;
         }
-        acc += p.sum();
+        acc += now.sum();
       } else if (of_load == -1) {
         float v[V];
         int r[V];
-        p.floats(v);
+        now.floats(v);
         strip.rows(a, bucket, b, q, difference(strip.least, q), r);
 #pragma unroll
         for (int u = 0; u < V; ++u) r[u] = (int)min((unsigned)(r[u] - first), (unsigned)count) * 32;
@@ -443,7 +454,7 @@ int validate(const evoattn_relative_bias_params* p) {
   if (p->B < 0 || p->H <= 0 || p->Rq < 0 || p->Rk < 0 || p->B > 65535 || p->H > 4096) return EVOATTN_ERR_SHAPE;
   if (p->Rq > (1 << 23) || p->Rk > (1 << 23)) return EVOATTN_ERR_SHAPE;
   if ((long long)p->B * ((p->H + kHeads - 1) / kHeads) > 65535) return EVOATTN_ERR_SHAPE;
-  if ((long long)p->B * ((p->Rk + 31) / 32) * ((p->Rq + 15) / 16) > 0x7fffffffLL) return EVOATTN_ERR_SHAPE;
+  if ((long long)p->B * ((p->Rk + 63) / 64) * ((p->Rq + 7) / 8) > 0x7fffffffLL) return EVOATTN_ERR_SHAPE;
   if (p->buckets <= 0 || p->buckets > EVOATTN_MAX_BUCKETS || p->n_edges < 0 || p->n_edges > kLogEdges || p->exact < 0) return EVOATTN_ERR_SHAPE;
   if (p->n_edges > 0 && !p->edges) return EVOATTN_ERR_NULL;
   for (int i = 0; i < p->n_edges; ++i)  // a distance finds its bucket by bisection
@@ -472,13 +483,13 @@ bool rows_of_16_bytes(const void* p, const int64_t* stride, int es) {
   return ((uintptr_t)p & 15) == 0 && stride[0] * es % 16 == 0 && stride[1] * es % 16 == 0 && stride[2] * es % 16 == 0;
 }
 
-// How the backward is cut: rows a warp takes at a time (up to 32 loads), blocks of four warps a head, table rows a block sums.
+// How the backward is cut: rows a warp takes at a time, blocks of four warps a head, table rows a block sums.
 void plan_bwd(RelArgs* a, int es) {
   a->window = a->buckets < 128 ? a->buckets : 128;
-  const int wide = kLanes * 16 / es, strips = (a->Rk + wide - 1) / wide;
-  a->item_rows = 32 * kTall;
+  const int tall = es == 4 ? kTall<float> : kTall<__half>, strips = (a->Rk + 63) / 64;
+  a->item_rows = kLoads * tall;
   const auto items = [&] { return (long long)a->B * strips * ((a->Rq + a->item_rows - 1) / a->item_rows); };
-  while (a->item_rows > 4 * kTall && items() * a->H < 148 * 20 * 2) a->item_rows /= 2;
+  while (a->item_rows > 4 * tall && items() * a->H < 148 * 20 * 2) a->item_rows /= 2;
   const long long blocks = (items() + 3) / 4, most = 148 * 5 / a->H > 1 ? 148 * 5 / a->H : 1;
   a->blocks = (int)(blocks < most ? blocks : most);
 }
