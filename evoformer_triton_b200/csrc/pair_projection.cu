@@ -103,10 +103,19 @@ template <class T>
 struct Eight {
   static constexpr int kWords = sizeof(T) / 2;
   uint4 w[kWords];
-  // WHOLE: C and all rows are in pieces of eight channels and 16 bytes.
-  template <bool WHOLE>
+  // VEC: C and all rows are in pieces of as many channels (8: 16 bytes; 4: 8 bytes, fp32 16; else 1).
+  template <int VEC>
   __device__ __forceinline__ void load(const T* p, int count) {
-    if constexpr (WHOLE) {
+    if constexpr (VEC == 4) {
+      using Four = typename std::conditional<sizeof(T) == 4, uint4, uint2>::type;
+      Four h[2];
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        h[k] = Four();
+        if (count > 4 * k) h[k] = reinterpret_cast<const Four*>(p)[k];
+      }
+      memcpy(w, h, sizeof(h));
+    } else if constexpr (VEC == 8) {
 #pragma unroll
       for (int k = 0; k < kWords; ++k) w[k] = count > 0 ? reinterpret_cast<const uint4*>(p)[k] : make_uint4(0, 0, 0, 0);
     } else {
@@ -131,9 +140,19 @@ struct Eight {
       for (int k = 0; k < 4; ++k) split2<Pieces<T>::kX>(v[2 * k], v[2 * k + 1], p[k]);
     }
   }
-  template <bool WHOLE>
+  template <int VEC>
   static __device__ __forceinline__ void store(T* p, const float (&v)[8], int count) {
-    if constexpr (WHOLE) {
+    if constexpr (VEC == 4) {
+      using Four = typename std::conditional<sizeof(T) == 4, uint4, uint2>::type;
+      uint4 packed[kWords];
+      Four h[2];
+#pragma unroll
+      for (int k = 0; k < kWords; ++k) packed[k] = pack16<T>(v + k * kPer16<T>);
+      memcpy(h, packed, sizeof(h));
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+        if (count > 4 * k) reinterpret_cast<Four*>(p)[k] = h[k];
+    } else if constexpr (VEC == 8) {
 #pragma unroll
       for (int k = 0; k < kWords; ++k)
         if (count > 0) reinterpret_cast<uint4*>(p)[k] = pack16<T>(v + k * kPer16<T>);
@@ -145,59 +164,82 @@ struct Eight {
   }
 };
 
-__device__ __forceinline__ float g_of(const ProjArgs& a, int h, int c) {
-  return h < a.H && c < a.C ? load_any(a.w, a.w_dtype, h * a.C + c) * gain(a, c) : 0.f;
-}
-// G[h, c .. c + 7] and on as B operands of rows x channels products, [KC][NT][pieces][lane].
-template <int GP>
-__device__ __forceinline__ void lay_out_by_rows(const ProjArgs& a, int KC, int NT, uint4* sm) {
-  for (int i = threadIdx.x; i < KC * NT * 32; i += blockDim.x) {
-    const int l = i & 31, nt = (i >> 5) % NT, kc = (i >> 5) / NT, h = nt * 8 + l / 4, c = kc * 32 + (l & 3) * 8;
-    uint32_t p[4][GP];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) split2<GP>(g_of(a, h, c + 2 * k), g_of(a, h, c + 2 * k + 1), p[k]);
-#pragma unroll
-    for (int j = 0; j < GP; ++j) sm[((kc * NT + nt) * GP + j) * 32 + l] = make_uint4(p[0][j], p[1][j], p[2][j], p[3][j]);
-  }
-}
-// The same as B operands of heads x channels products: pairs of heads of the four channels of a lane's accumulators.
-template <int GP>
-__device__ __forceinline__ void lay_out_by_heads(const ProjArgs& a, int KC, int NT, uint4* sm) {
-  for (int i = threadIdx.x; i < KC * NT * 32; i += blockDim.x) {
-    const int l = i & 31, nt = (i >> 5) % NT, kc = (i >> 5) / NT, h = nt * 8 + (l & 3) * 2, c = kc * 32 + l / 8 * 8 + (l / 4 & 1);
-    uint32_t p[4][GP];
-#pragma unroll
-    for (int q = 0; q < 4; ++q) split2<GP>(g_of(a, h, c + 2 * q), g_of(a, h + 1, c + 2 * q), p[q]);
-#pragma unroll
-    for (int j = 0; j < GP; ++j) sm[((kc * NT + nt) * GP + j) * 32 + l] = make_uint4(p[0][j], p[1][j], p[2][j], p[3][j]);
-  }
-}
-// sum_c of the pieces of G for every head, and sum_c weight b.  All warps of the block take part.
-template <int GP>
-__device__ __forceinline__ void sum_channels(const ProjArgs& a, int heads, float* sm_sum, float* sm_t) {
+// Weights first + lane, first + lane + 32, ... as they lie, and then as floats: a warp's loads all go out before one is used.
+template <int KC>
+__device__ __forceinline__ void load_bits(const void* p, int dtype, long long first, int n, uint32_t (&bits)[KC]) {
   const int lane = threadIdx.x & 31;
-  for (int h = threadIdx.x >> 5; h < heads; h += blockDim.x >> 5) {
+  if (dtype == EVOATTN_FP32) {
+#pragma unroll
+    for (int k = 0; k < KC; ++k) bits[k] = lane + 32 * k < n ? static_cast<const uint32_t*>(p)[first + lane + 32 * k] : 0;
+  } else {
+#pragma unroll
+    for (int k = 0; k < KC; ++k) bits[k] = lane + 32 * k < n ? static_cast<const uint16_t*>(p)[first + lane + 32 * k] : 0;
+  }
+}
+__device__ __forceinline__ float of_bits(int dtype, uint32_t bits) {
+  return dtype == EVOATTN_FP32 ? __uint_as_float(bits) : dtype == EVOATTN_BF16 ? __uint_as_float(bits << 16) : __half2float(__ushort_as_half((unsigned short)bits));
+}
+
+// A kernel's weights: G in pieces as B operands of rows x channels products, and as those of heads x channels products, both
+// [KC][NT][pieces][lane] (null: not wanted); the sum over the channels of the pieces of G and that of weight b for every
+// head.  Eight heads at a time, one a warp.  Ends with a barrier.
+template <int KC, int NT, int GP>
+__device__ __forceinline__ void prepare_weights(const ProjArgs& a, uint4* by_rows, uint4* by_heads, float* sm_sum, float* sm_t) {
+  __shared__ float sm_G[8][32 * KC + 4];  // (4 floats apart: eight heads in different banks)
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  for (int nt = 0; nt < NT; ++nt) {
+    const int h = nt * 8 + warp;
+    const bool biased = a.b && sm_t;
+    uint32_t w[KC], gains[KC], biases[KC];
+    load_bits<KC>(a.w, a.w_dtype, (long long)h * a.C, h < a.H ? a.C : 0, w);
+    if (a.g) load_bits<KC>(a.g, a.g_dtype, 0, a.C, gains);
+    if (biased) load_bits<KC>(a.b, a.b_dtype, 0, a.C, biases);
+    if (nt) __syncthreads();
     float s = 0.f, tb = 0.f;
-    for (int c = lane; c < a.C; c += 32) {
+#pragma unroll
+    for (int k = 0; k < KC; ++k) {
+      const float weight = of_bits(a.w_dtype, w[k]), G = a.g ? weight * of_bits(a.g_dtype, gains[k]) : weight;
+      sm_G[warp][lane + 32 * k] = G;
+      if (biased) tb = fmaf(weight, of_bits(a.b_dtype, biases[k]), tb);
       uint32_t p[GP];
-      split2<GP>(g_of(a, h, c), 0.f, p);
+      split2<GP>(G, 0.f, p);
       float v = 0.f;
 #pragma unroll
-      for (int j = GP - 1; j >= 0; --j) {
-        float lo, hi;
-        unpack2<__nv_bfloat16>(p[j], lo, hi);
-        v += lo;
-      }
+      for (int j = GP - 1; j >= 0; --j) v += __uint_as_float(p[j] << 16);
       s += v;
-      if (sm_t && a.b && h < a.H) tb = fmaf(load_any(a.w, a.w_dtype, h * a.C + c), load_any(a.b, a.b_dtype, c), tb);
     }
-    s = warp_sum(s);
-    tb = warp_sum(tb);
-    if (lane == 0) {
-      sm_sum[h] = s;
-      if (sm_t) sm_t[h] = tb;
+    if (sm_sum) {
+      s = warp_sum(s);
+      if (biased) tb = warp_sum(tb);
+      if (lane == 0) {
+        sm_sum[h] = s;
+        if (sm_t) sm_t[h] = tb;
+      }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < KC * 32; i += blockDim.x) {
+      const int l = i & 31, kc = i >> 5;
+      const auto write = [&](uint4* sm, const float (&v)[8]) {
+        uint32_t p[4][GP];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) split2<GP>(v[2 * k], v[2 * k + 1], p[k]);
+#pragma unroll
+        for (int j = 0; j < GP; ++j) sm[((kc * NT + nt) * GP + j) * 32 + l] = make_uint4(p[0][j], p[1][j], p[2][j], p[3][j]);
+      };
+      float v[8];
+      if (by_rows) {  // eight channels of head l / 4
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = sm_G[l / 4][kc * 32 + (l & 3) * 8 + k];
+        write(by_rows, v);
+      }
+      if (by_heads) {  // pairs of heads of the four channels of a lane's accumulators
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = sm_G[(l & 3) * 2 + (k & 1)][kc * 32 + l / 8 * 8 + (l / 4 & 1) + (k & ~1)];
+        write(by_heads, v);
+      }
     }
   }
+  __syncthreads();
 }
 
 // A lane's two rows of a tile: g and g + 8.
@@ -229,9 +271,9 @@ struct Rows2 {
 };
 
 // 16 rows, 32 KC channels.  KEEP: in registers; else read again (from L1 or L2) by every use.
-template <class T, int KC, bool KEEP, bool WHOLE_>
+template <class T, int KC, bool KEEP, int VEC_>
 struct Tile {
-  static constexpr bool WHOLE = WHOLE_;
+  static constexpr int VEC = VEC_;
   static constexpr int kUnroll = KEEP ? KC : 1;
   Eight<T> x[2][KEEP ? KC : 1];
   const T* at[2];
@@ -245,14 +287,14 @@ struct Tile {
       on[k] = row.on[k];
       if constexpr (KEEP) {
 #pragma unroll
-        for (int c = 0; c < KC; ++c) x[k][c].template load<WHOLE>(at[k] + c * 32, on[k] ? count(a, c) : 0);
+        for (int c = 0; c < KC; ++c) x[k][c].template load<VEC>(at[k] + c * 32, on[k] ? count(a, c) : 0);
       }
     }
   }
   __device__ __forceinline__ Eight<T> get(const ProjArgs& a, int k, int c) const {
     if constexpr (KEEP) return x[k][c];
     Eight<T> e;
-    e.template load<WHOLE>(at[k] + c * 32, on[k] ? count(a, c) : 0);
+    e.template load<VEC>(at[k] + c * 32, on[k] ? count(a, c) : 0);
     return e;
   }
   // Mean and 1 / deviation, the latter about the mean; a row that is not there has r = 0 and adds nothing.
@@ -363,8 +405,8 @@ __device__ __forceinline__ void product_by_rows(const ProjArgs& a, const TileT& 
 }
 
 // Three blocks an SM where the registers allow it: [1,768,768,128] to 8 heads 47 -> 43 us, fp16 56 -> 51.
-template <class T, int KC, int NT, bool KEEP, bool WHOLE>
-__global__ void __launch_bounds__(256, sizeof(T) == 2 && KC <= 4 && NT <= 2 && WHOLE && KEEP ? 3 : 0) projection_fwd(ProjArgs a) {
+template <class T, int KC, int NT, bool KEEP, int VEC>
+__global__ void __launch_bounds__(256, sizeof(T) == 2 && KC <= 4 && NT <= 2 && VEC == 8 && KEEP ? 3 : 0) projection_fwd(ProjArgs a) {
   ptx::grid_dependency_wait();
   ptx::grid_launch_dependents();
   extern __shared__ __align__(16) uint4 sm_g[];  // [KC][NT][GP][32 lanes]
@@ -372,11 +414,9 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 && KC <= 4 && NT <= 2 && W
   const int warp = threadIdx.x >> 5, t = threadIdx.x & 3;
   const uint32_t rows = (uint32_t)((long long)a.B * a.Ri * a.Rj), step = gridDim.x * 128;
   Rows2 next(a, (blockIdx.x * 8 + warp) * 16, rows);
-  Tile<T, KC, KEEP, WHOLE> x;
+  Tile<T, KC, KEEP, VEC> x;
   x.load(a, next);
-  lay_out_by_rows<Pieces<T>::kG>(a, KC, NT, sm_g);
-  sum_channels<Pieces<T>::kG>(a, NT * 8, sm_sum, sm_t);
-  __syncthreads();
+  prepare_weights<KC, NT, Pieces<T>::kG>(a, sm_g, nullptr, sm_sum, sm_t);
   while (next.n0 < rows) {
     const Rows2 row = next;
     x.statistics(a);
@@ -591,7 +631,7 @@ __device__ __forceinline__ void write_dz(const ProjArgs& a, const TileT& x, cons
         ptx::f2_get(ptx::f2_fma(ptx::f2_make(u[k][e], u[k][e + 1]), by_u[k], z), v[e], v[e + 1]);
       }
       if (row.on[k])
-        Eight<T>::template store<TileT::WHOLE>(static_cast<T*>(a.dz) + (long long)row.row(k) * a.C + kc * 32 + (threadIdx.x & 3) * 8, v, x.count(a, kc));
+        Eight<T>::template store<TileT::VEC>(static_cast<T*>(a.dz) + (long long)row.row(k) * a.C + kc * 32 + (threadIdx.x & 3) * 8, v, x.count(a, kc));
     }
   }
 }
@@ -600,8 +640,8 @@ __device__ __forceinline__ void write_dz(const ProjArgs& a, const TileT& x, cons
 //   sum_c u = sum_h d[h] sum_c G[h,c],   sum_c u (z - mean) = sum_h d[h] (sum_c G[h,c] z[c] - mean sum_c G[h,c]),
 // the latter with the product that the forward takes.
 // Two blocks an SM where the registers allow it (bf16, 128 channels, 8 heads: one block of 148 registers 116 us, two of 128 95 us).
-template <class T, int KC, int NT, bool WHOLE>
-__global__ void __launch_bounds__(256, sizeof(T) == 2 && KC <= 4 && NT == 1 && WHOLE ? 2 : 1) projection_bwd(ProjArgs a) {
+template <class T, int KC, int NT, int VEC>
+__global__ void __launch_bounds__(256, sizeof(T) == 2 && KC <= 4 && NT == 1 && VEC == 8 ? 2 : 1) projection_bwd(ProjArgs a) {
   ptx::grid_dependency_wait();
   ptx::grid_launch_dependents();
   constexpr int kG = KC * NT * Pieces<T>::kG * 32;
@@ -609,17 +649,12 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 && KC <= 4 && NT == 1 && W
   __shared__ float sm_sum[NT * 8];
   const int warp = threadIdx.x >> 5, t = threadIdx.x & 3;
   const uint32_t rows = (uint32_t)((long long)a.B * a.Ri * a.Rj), step = gridDim.x * 128;
-  if (a.dz) {
-    lay_out_by_rows<Pieces<T>::kG>(a, KC, NT, sm_g);
-    lay_out_by_heads<Pieces<T>::kG>(a, KC, NT, sm_g + kG);
-    sum_channels<Pieces<T>::kG>(a, NT * 8, sm_sum, nullptr);
-  }
-  __syncthreads();
+  if (a.dz) prepare_weights<KC, NT, Pieces<T>::kG>(a, sm_g, sm_g + kG, sm_sum, nullptr);
   const float by_C = 1.f / a.C;
   RowSums<T, KC, NT> sums;
   for (uint32_t n0 = (blockIdx.x * 8 + warp) * 16; n0 < rows; n0 += step) {
     const Rows2 row(a, n0, rows);
-    Tile<T, KC, true, WHOLE> x;
+    Tile<T, KC, true, VEC> x;
     x.load(a, row);
     float d[NT][2][2];
     uint32_t dp[NT][2][Pieces<T>::kX];
@@ -653,19 +688,18 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 && KC <= 4 && NT == 1 && W
 }
 
 // More channels and heads than one block can hold the sums of: dz and the rows' statistics in one kernel ...
-template <class T, int KC, int NT, bool KEEP, bool WHOLE>
+template <class T, int KC, int NT, bool KEEP, int VEC>
 __global__ void __launch_bounds__(256) projection_dz(ProjArgs a) {
   ptx::grid_dependency_wait();
   ptx::grid_launch_dependents();
   extern __shared__ __align__(16) uint4 sm_g[];  // G by heads
   const int warp = threadIdx.x >> 5;
   const uint32_t rows = (uint32_t)((long long)a.B * a.Ri * a.Rj), step = gridDim.x * 128;
-  if (a.dz) lay_out_by_heads<Pieces<T>::kG>(a, KC, NT, sm_g);
-  __syncthreads();
+  if (a.dz) prepare_weights<KC, NT, Pieces<T>::kG>(a, nullptr, sm_g, nullptr, nullptr);
   const float by_C = 1.f / a.C;
   for (uint32_t n0 = (blockIdx.x * 8 + warp) * 16; n0 < rows; n0 += step) {
     const Rows2 row(a, n0, rows);
-    Tile<T, KC, KEEP, WHOLE> x;
+    Tile<T, KC, KEEP, VEC> x;
     x.load(a, row);
     x.statistics(a);
     if (a.stats && (threadIdx.x & 3) == 0) {
@@ -703,7 +737,7 @@ __global__ void __launch_bounds__(256) projection_dz(ProjArgs a) {
 
 // ... and M and s of 128 channels and 16 heads a block in another, with those statistics.
 constexpr int kSumChannels = 128, kSumHeads = 16;
-template <class T, bool WHOLE>
+template <class T, int VEC>
 __global__ void __launch_bounds__(256) projection_sums(ProjArgs a) {
   ptx::grid_dependency_wait();
   ptx::grid_launch_dependents();
@@ -717,7 +751,7 @@ __global__ void __launch_bounds__(256) projection_sums(ProjArgs a) {
   RowSums<T, KC, NT> sums;
   for (uint32_t n0 = (blockIdx.x * 8 + warp) * 16; n0 < rows; n0 += step) {
     const Rows2 row(a, n0, rows);
-    Tile<T, KC, true, WHOLE> x;
+    Tile<T, KC, true, VEC> x;
     x.load(part, row);
     float d[NT][2][2];
     uint32_t dp[NT][2][Pieces<T>::kX];
@@ -808,9 +842,13 @@ ProjArgs args_of(const evoattn_pair_projection_params* p) {
 }
 long long rows_of(const ProjArgs& a) { return (long long)a.B * a.Ri * a.Rj; }
 size_t stats_bytes(const ProjArgs& a) { return (size_t)((rows_of(a) * 8 + 15) / 16 * 16); }
-// Whether rows of z (and dz) are in pieces of eight channels and 16 bytes.
-bool whole_rows(const ProjArgs& a, int es) {
-  return a.C % 8 == 0 && (((uintptr_t)a.z | (uintptr_t)a.dz) & 15) == 0 && a.sz.a * es % 16 == 0 && a.sz.b * es % 16 == 0 && a.sz.c * es % 16 == 0;
+// The channels of a piece in which rows of z (and dz) can be read and written: 8 (16 bytes, fp32 twice), 4 or 1.
+int vector_of(const ProjArgs& a, int es) {
+  for (int vec = 8; vec >= 4; vec /= 2) {
+    const int bytes = vec * es < 16 ? vec * es : 16;
+    if (a.C % vec == 0 && ((uintptr_t)a.z | (uintptr_t)a.dz | (uintptr_t)(a.sz.a * es) | (uintptr_t)(a.sz.b * es) | (uintptr_t)(a.sz.c * es)) % bytes == 0) return vec;
+  }
+  return 1;
 }
 void look_at_rows(ProjArgs* a) {
   const auto reach = [](const Str3& s, long long x, long long y, long long z) {
@@ -822,22 +860,24 @@ void look_at_rows(ProjArgs* a) {
   a->small = reach(a->sz, a->B + 1, a->Ri, a->Rj + 64) < 2147483647.0 && reach(Str3{a->sout.a, a->sout.c, 1}, a->B + 1, a->Ri, a->Rj) < 2147483647.0;
 }
 
-template <int KC_, int NT_, bool KEEP_, bool WHOLE_> struct Shape { static constexpr int KC = KC_, NT = NT_; static constexpr bool KEEP = KEEP_, WHOLE = WHOLE_; };
+template <int KC_, int NT_, bool KEEP_, int VEC_> struct Shape { static constexpr int KC = KC_, NT = NT_, VEC = VEC_; static constexpr bool KEEP = KEEP_; };
 // 32 KC channels and 8 NT heads for a call; rows stay in registers while they take up to 64 a lane.
 template <class T, class F>
 void with_shape(const ProjArgs& a, F&& f) {
-  if (!whole_rows(a, (int)sizeof(T))) {  // fewer shapes
-    if (a.C <= 128 && a.H <= 8) f(Shape<4, 1, true, false>());
-    else if (a.H <= 16) f(Shape<16, 2, false, false>());
-    else f(Shape<16, 8, false, false>());
+  const int vec = vector_of(a, (int)sizeof(T));
+  if (vec < 8) {  // fewer shapes
+    if (a.C <= 128 && a.H <= 8 && vec == 4) f(Shape<4, 1, true, 4>());
+    else if (a.C <= 128 && a.H <= 8) f(Shape<4, 1, true, 1>());
+    else if (a.H <= 16) f(Shape<16, 2, false, 1>());
+    else f(Shape<16, 8, false, 1>());
     return;
   }
   const auto heads = [&](auto kc) {
     constexpr int KC = decltype(kc)::value;
     constexpr bool keep = KC * (int)sizeof(T) <= 16;
-    if (a.H <= 8) f(Shape<KC, 1, keep, true>());
-    else if (a.H <= 16) f(Shape<KC, 2, keep, true>());
-    else f(Shape<KC, 8, KC * (int)sizeof(T) <= 8, true>());
+    if (a.H <= 8) f(Shape<KC, 1, keep, 8>());
+    else if (a.H <= 16) f(Shape<KC, 2, keep, 8>());
+    else f(Shape<KC, 8, KC * (int)sizeof(T) <= 8, 8>());
   };
   if (a.C <= 64) heads(std::integral_constant<int, 2>());
   else if (a.C <= 128) heads(std::integral_constant<int, 4>());
@@ -846,20 +886,23 @@ void with_shape(const ProjArgs& a, F&& f) {
 }
 // Whether the backward is one kernel, which holds M of all channels and heads in registers beside the rows.
 bool one_pass(const ProjArgs& a, int es) {
-  if (es == 4 || !whole_rows(a, es)) return a.C <= 128 && a.H <= 8;
+  if (es == 4 || vector_of(a, es) < 8) return a.C <= 128 && a.H <= 8;
   return (a.C <= 256 && a.H <= 8) || (a.C <= 128 && a.H <= 16);
 }
 template <class T, class F>
 void with_one_pass_shape(const ProjArgs& a, F&& f) {
-  if (!whole_rows(a, (int)sizeof(T))) {
-    f(Shape<4, 1, true, false>());
+  const int vec = vector_of(a, (int)sizeof(T));
+  if (vec == 4) {
+    f(Shape<4, 1, true, 4>());
+  } else if (vec == 1) {
+    f(Shape<4, 1, true, 1>());
   } else if (a.H <= 8) {
-    if (a.C <= 64) f(Shape<2, 1, true, true>());
-    else if (a.C <= 128) f(Shape<4, 1, true, true>());
-    else if constexpr (sizeof(T) == 2) f(Shape<8, 1, true, true>());
+    if (a.C <= 64) f(Shape<2, 1, true, 8>());
+    else if (a.C <= 128) f(Shape<4, 1, true, 8>());
+    else if constexpr (sizeof(T) == 2) f(Shape<8, 1, true, 8>());
   } else if constexpr (sizeof(T) == 2) {
-    if (a.C <= 64) f(Shape<2, 2, true, true>());
-    else f(Shape<4, 2, true, true>());
+    if (a.C <= 64) f(Shape<2, 2, true, 8>());
+    else f(Shape<4, 2, true, 8>());
   }
 }
 // Blocks of 128 rows that run at once.
@@ -874,7 +917,7 @@ bool blocks_of(K kern, long long rows, int smem, unsigned* blocks) {
 }
 // Blocks that leave partial sums of H (C + 1) floats: as many as run at once.
 int sum_blocks(const ProjArgs& a, int es) {
-  const long long want = (rows_of(a) + 127) / 128, most = es == 2 && a.C <= 128 && a.H <= 8 && whole_rows(a, es) ? 296 : 148;
+  const long long want = (rows_of(a) + 127) / 128, most = es == 2 && a.C <= 128 && a.H <= 8 && vector_of(a, es) == 8 ? 296 : 148;
   return (int)(want < most ? want : most);
 }
 
@@ -900,7 +943,7 @@ int evoattn_pair_projection_fwd(const evoattn_pair_projection_params* p, void* c
     using T = decltype(e);
     with_shape<T>(a, [&](auto sh) {
       using Sh = decltype(sh);
-      const auto kern = projection_fwd<T, Sh::KC, Sh::NT, Sh::KEEP, Sh::WHOLE>;
+      const auto kern = projection_fwd<T, Sh::KC, Sh::NT, Sh::KEEP, Sh::VEC>;
       const int smem = Sh::KC * Sh::NT * Pieces<T>::kG * 512;
       unsigned blocks;
       if (blocks_of(kern, rows, smem, &blocks)) rc = launch_dependent(kern, dim3(blocks), 256, (size_t)smem, st, a);
@@ -945,7 +988,7 @@ int evoattn_pair_projection_bwd(const evoattn_pair_projection_params* p, void* c
       if (one) {
         with_one_pass_shape<T>(a, [&](auto sh) {
           using Sh = decltype(sh);
-          const auto kern = projection_bwd<T, Sh::KC, Sh::NT, Sh::WHOLE>;
+          const auto kern = projection_bwd<T, Sh::KC, Sh::NT, Sh::VEC>;
           const int pieces = 2 * Sh::KC * Sh::NT * Pieces<T>::kG * 512, left = 8 * Sh::NT * (32 * Sh::KC + 1) * (int)sizeof(float), smem = pieces > left ? pieces : left;
           if (kernel_ready(reinterpret_cast<const void*>(kern), smem, nullptr)) rc = launch_dependent(kern, dim3((unsigned)a.blocks), 256, (size_t)smem, st, a);
         });
@@ -953,14 +996,14 @@ int evoattn_pair_projection_bwd(const evoattn_pair_projection_params* p, void* c
       }
       with_shape<T>(a, [&](auto sh) {
         using Sh = decltype(sh);
-        const auto kern = projection_dz<T, Sh::KC, Sh::NT, Sh::KEEP, Sh::WHOLE>;
+        const auto kern = projection_dz<T, Sh::KC, Sh::NT, Sh::KEEP, Sh::VEC>;
         const int smem = Sh::KC * Sh::NT * Pieces<T>::kG * 512;
         unsigned blocks;
         if (blocks_of(kern, rows, smem, &blocks)) rc = launch_dependent(kern, dim3(blocks), 256, (size_t)smem, st, a);
       });
       if (rc == cudaSuccess && sums) {
         const dim3 grid((unsigned)a.blocks, (unsigned)((a.C + kSumChannels - 1) / kSumChannels), (unsigned)((a.H + kSumHeads - 1) / kSumHeads));
-        rc = whole_rows(a, (int)sizeof(T)) ? launch_dependent(projection_sums<T, true>, grid, 256, 0, st, a) : launch_dependent(projection_sums<T, false>, grid, 256, 0, st, a);
+        rc = vector_of(a, (int)sizeof(T)) == 8 ? launch_dependent(projection_sums<T, 8>, grid, 256, 0, st, a) : launch_dependent(projection_sums<T, 1>, grid, 256, 0, st, a);
       }
       return 0;
     });

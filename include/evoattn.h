@@ -251,7 +251,8 @@ int evoattn_bias_pad_rows(const void* src, const int64_t* stride, void* dst, int
  * Three operators that stand before the attention in a block: layer norm, a learned relative position bias
  * and the projection of the pair representation to a pair bias.  The reference has none of them.  The types
  * are EVOATTN_BF16 / FP16 / FP32, sums are taken in fp32 in a fixed order (the same bits in every run), and
- * every call may be captured in a CUDA graph.  The calls with a workspace need it 16-byte aligned.
+ * every call may be captured in a CUDA graph.  A workspace is 16-byte aligned; its size is asked for with the
+ * parameters of the call, addresses included (other alignments take other kernels).
  *
  * Layer norm over the last axis: y = (x - mean) / sqrt(var + eps) * weight + bias, var the mean squared
  * deviation.  Rows are indexed by three axes (n[0], n[1], n[2]) with element strides; the C values of a row

@@ -80,9 +80,12 @@ def bucket(rel, scheme, n, max_distance):
 
 
 def bucket_rows(q, k, scheme, n, max_distance):
-    """[B, Rq, Rk] rows of the table; positions as Python whole numbers, so nothing overflows."""
+    """[B, Rq, Rk] rows of the table; differences that 64 bits might not hold are taken in Python's whole numbers."""
     M = max_distance + 1
     of = torch.tensor([bucket(r, scheme, n, max_distance) for r in range(-M, M + 1)])
+    if max((abs(v) for row in q + k for v in row), default=0) < 2 ** 61:
+        rel = torch.tensor(k).unsqueeze(1) - torch.tensor(q).unsqueeze(2)
+        return of[rel.clamp(-M, M) + M]
     rel = [[[min(max(kj - qi, -M), M) + M for kj in ks] for qi in qs] for qs, ks in zip(q, k)]
     return of[torch.tensor(rel, dtype=torch.long).reshape(len(q), len(q[0]), len(k[0]))]
 
