@@ -382,7 +382,7 @@ __global__ void __launch_bounds__(1024) norm_sum_partials(NormArgs a) {
   const int lane = threadIdx.x & 31, part = threadIdx.x >> 5, c = blockIdx.x * 32 + lane, which = blockIdx.y;
   float s = 0.f;
   if (c < a.C) {
-#pragma unroll 4
+#pragma unroll 10
     for (int k = part; k < a.blocks; k += 32) s += a.partial[((long long)k * 2 + which) * a.C + c];
   }
   sm[part][lane] = s;

@@ -768,48 +768,49 @@ __global__ void __launch_bounds__(256) projection_sums(ProjArgs a) {
   write_partial<KC, NT>(a, sm, blockIdx.x, h0, c0);
 }
 
-// The blocks' sums, added in order, and the gradients of the weights from them.  A block has eight channels: 128 shares of
-// the sums of eight heads at a time, a warp four of them.
+// The blocks' sums, added in order, and the gradients of the weights from them.  A block has two channels and sums eight heads
+// at a time: 24 values (the third of a head: s), each in 42 shares, so that a thread's few loads go out at once.
+constexpr int kWeightChannels = 2, kShares = 42;
 __global__ void __launch_bounds__(1024) projection_weights(ProjArgs a) {
   ptx::grid_dependency_wait();
   ptx::grid_launch_dependents();
-  __shared__ float sm[32][8][9], sm_m[EVOATTN_PROJECTION_MAX_H][9];  // [..][8]: s
+  constexpr int V = kWeightChannels + 1;
+  __shared__ float sm[kShares][8 * V], sm_m[EVOATTN_PROJECTION_MAX_H][V];
   const long long size = (long long)a.H * (a.C + 1);
-  const int c0 = blockIdx.x * 8;
+  const int c0 = blockIdx.x * kWeightChannels, share = threadIdx.x / (8 * V), v = threadIdx.x % (8 * V), hh = v / V, cc = v % V;
   for (int h0 = 0; h0 < a.H; h0 += 8) {
-    // 32 shares of 8 heads x 4 pairs of channels would leave s out: 72 values, each summed by 14 threads
-    for (int i = threadIdx.x; i < 72 * 32; i += 1024) {
-      const int share = i / 72, v = i - share * 72, hh = v / 9, cc = v - hh * 9, h = h0 + hh, c = cc == 8 ? a.C : c0 + cc;
+    const int h = h0 + hh, c = cc == kWeightChannels ? a.C : c0 + cc;
+    if (share < kShares) {
       float s = 0.f;
-      if (h < a.H && c <= a.C && (cc == 8 || c < a.C)) {
+      if (h < a.H && (cc == kWeightChannels || c < a.C)) {
         const float* p = a.partial + h * (a.C + 1) + c;
-#pragma unroll 4
-        for (int k = share; k < a.blocks; k += 32) s += p[k * size];
+#pragma unroll 8
+        for (int k = share; k < a.blocks; k += kShares) s += p[k * size];
       }
-      sm[share][hh][cc] = s;
+      sm[share][v] = s;
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < 72; i += 1024) {
+    if (threadIdx.x < 8 * V && h < a.H) {
       float s = 0.f;
 #pragma unroll
-      for (int k = 0; k < 32; ++k) s += sm[k][i / 9][i % 9];
-      if (h0 + i / 9 < a.H) sm_m[h0 + i / 9][i % 9] = s;
+      for (int k = 0; k < kShares; ++k) s += sm[k][v];
+      sm_m[h][cc] = s;
     }
     __syncthreads();
   }
-  const int c = c0 + (int)threadIdx.x % 8;
+  const int mine = threadIdx.x % kWeightChannels, c = c0 + mine, h = threadIdx.x / kWeightChannels;
   if (c >= a.C) return;
-  if (a.dw && threadIdx.x / 8 < a.H) {
-    const int h = threadIdx.x / 8;
+  if (a.dw && h < a.H) {
     const float b = a.b ? load_any(a.b, a.b_dtype, c) : 0.f;
-    store_any(a.dw, a.w_dtype, h * a.C + c, fmaf(gain(a, c), sm_m[h][threadIdx.x % 8], b * sm_m[h][8]));
+    store_any(a.dw, a.w_dtype, h * a.C + c, fmaf(gain(a, c), sm_m[h][mine], b * sm_m[h][kWeightChannels]));
   }
-  if (threadIdx.x >= 8) return;
+  if (threadIdx.x >= kWeightChannels) return;
   float dg = 0.f, db = 0.f;
-  for (int h = 0; h < a.H; ++h) {
-    const float w = load_any(a.w, a.w_dtype, h * a.C + c);
-    dg = fmaf(w, sm_m[h][threadIdx.x], dg);
-    db = fmaf(w, sm_m[h][8], db);
+#pragma unroll 8
+  for (int k = 0; k < a.H; ++k) {
+    const float w = load_any(a.w, a.w_dtype, k * a.C + c);
+    dg = fmaf(w, sm_m[k][mine], dg);
+    db = fmaf(w, sm_m[k][kWeightChannels], db);
   }
   if (a.dg) store_any(a.dg, a.g_dtype, c, dg);
   if (a.db) store_any(a.db, a.b_dtype, c, db);
@@ -1007,7 +1008,7 @@ int evoattn_pair_projection_bwd(const evoattn_pair_projection_params* p, void* c
       }
       return 0;
     });
-  if (rc == cudaSuccess && sums) rc = launch_dependent(projection_weights, dim3((unsigned)((a.C + 7) / 8)), 1024, 0, st, a);
+  if (rc == cudaSuccess && sums) rc = launch_dependent(projection_weights, dim3((unsigned)((a.C + kWeightChannels - 1) / kWeightChannels)), 1024, 0, st, a);
   return rc == cudaSuccess ? EVOATTN_OK : EVOATTN_ERR_CUDA;
 }
 

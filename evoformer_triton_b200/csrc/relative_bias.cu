@@ -24,7 +24,6 @@ struct RelArgs {
   const void* k_pos;
   long long sq, sk;
   const void* base;
-  int base_pieces;    // rows of the base are whole pieces too
   Str3 sbase;
   void* out;
   Str3 sout;
@@ -149,7 +148,7 @@ __host__ __device__ constexpr int slot(int row) { return row + (row >> 3); }
 struct Slot { static __device__ __forceinline__ int of(int row) { return slot(row); } };
 struct Same { static __device__ __forceinline__ int of(int row) { return row; } };
 
-// V values of the base at p: in pieces of up to 16 bytes where whole (base_pieces), else one by one.
+// V values of the base, in pieces of up to 16 bytes.
 template <int V>
 __device__ __forceinline__ void add_base(const RelArgs& a, long long at, float (&v)[V]) {
   if (a.base_dtype == EVOATTN_FP32) {
@@ -175,9 +174,14 @@ __device__ __forceinline__ void add_base(const RelArgs& a, long long at, float (
   }
 }
 
+template <class T> __device__ __forceinline__ uint32_t same2(float v) {  // a 16-bit value twice
+  if constexpr (sizeof(T) == 2) return Pack2<T>::pack(v, v);
+  return 0;
+}
+
 // A block of eight warps takes a strip of 32 V keys and kHeads heads and walks rows; with fewer rows than warps, the warps
 // share the heads of a row.  A row whose strip is one bucket, as away from the diagonal, is one value a head.
-template <class T, bool WIDE>
+template <class T, bool WIDE, bool BASE>
 __global__ void __launch_bounds__(256, 4) relative_fwd(RelArgs a, int rows_per_block, int row_warps) {
   ptx::grid_dependency_wait();
   ptx::grid_launch_dependents();
@@ -211,10 +215,32 @@ __global__ void __launch_bounds__(256, 4) relative_fwd(RelArgs a, int rows_per_b
       strip.rows(a, bucket, b, q, difference(strip.least, q), s);
     }
     T* o = static_cast<T*>(a.out) + b * a.sout.a + (h0 + first_head) * a.sout.b + (long long)i * a.sout.c;
-    long long at = b * a.sbase.a + (h0 + first_head) * a.sbase.b + (long long)i * a.sbase.c;
+    const long long down = head_step * a.sout.b;
+    const float* t = sm_table + first_head * pitch;
+    const int down_t = head_step * pitch;
     const bool whole = WIDE && strip.col(V - 1) < a.Rk;
-    for (int h = first_head; h < nh; h += head_step, o += head_step * a.sout.b, at += head_step * a.sbase.b) {
-      const float* t = sm_table + h * pitch;
+    if constexpr (!BASE) {
+      if (whole) {  // the common cases: a row is one value a head, or V of them
+        o += strip.col(0);
+        if (kind >= 0) {
+          t += kind;
+          for (int h = first_head; h < nh; h += head_step, o += down, t += down_t) {
+            const uint32_t w = sizeof(T) == 4 ? __float_as_uint(*t) : same2<T>(*t);
+            *reinterpret_cast<uint4*>(o) = make_uint4(w, w, w, w);
+          }
+        } else {
+          for (int h = first_head; h < nh; h += head_step, o += down, t += down_t) {
+            float v[V];
+#pragma unroll
+            for (int u = 0; u < V; ++u) v[u] = t[s[u]];
+            *reinterpret_cast<uint4*>(o) = pack16<T>(v);
+          }
+        }
+        continue;
+      }
+    }
+    long long at = b * a.sbase.a + (h0 + first_head) * a.sbase.b + (long long)i * a.sbase.c;
+    for (int h = first_head; h < nh; h += head_step, o += down, t += down_t, at += head_step * a.sbase.b) {
       float v[V];
       if (kind >= 0) {
         v[0] = t[kind];
@@ -224,29 +250,28 @@ __global__ void __launch_bounds__(256, 4) relative_fwd(RelArgs a, int rows_per_b
 #pragma unroll
         for (int u = 0; u < V; ++u) v[u] = t[s[u]];
       }
-      if (whole && (!a.base || a.base_pieces)) {
-        if (a.base) add_base<V>(a, at + strip.col(0), v);
+      if (BASE && whole) {  // (WIDE: the base's rows are whole pieces too)
+        add_base<V>(a, at + strip.col(0), v);
         *reinterpret_cast<uint4*>(o + strip.col(0)) = pack16<T>(v);
-      } else {
-        if (a.base) {
-          uint32_t w[V];
-          if (a.base_dtype == EVOATTN_FP32) {
-#pragma unroll
-            for (int u = 0; u < V; ++u) w[u] = strip.col(u) < a.Rk ? static_cast<const uint32_t*>(a.base)[at + strip.col(u)] : 0;
-          } else {
-#pragma unroll
-            for (int u = 0; u < V; ++u) w[u] = strip.col(u) < a.Rk ? static_cast<const uint16_t*>(a.base)[at + strip.col(u)] : 0;
-          }
-#pragma unroll
-          for (int u = 0; u < V; ++u)
-            v[u] += a.base_dtype == EVOATTN_FP32 ? __uint_as_float(w[u])
-                    : a.base_dtype == EVOATTN_BF16 ? __uint_as_float(w[u] << 16) : __half2float(__ushort_as_half((unsigned short)w[u]));
-        }
-#pragma unroll
-        for (int u = 0; u < V; ++u) {
-          if (strip.col(u) < a.Rk) o[strip.col(u)] = from_float<T>(v[u]);
-        }
+        continue;
       }
+      if constexpr (BASE) {
+        uint32_t w[V];
+        if (a.base_dtype == EVOATTN_FP32) {
+#pragma unroll
+          for (int u = 0; u < V; ++u) w[u] = strip.col(u) < a.Rk ? static_cast<const uint32_t*>(a.base)[at + strip.col(u)] : 0;
+        } else {
+#pragma unroll
+          for (int u = 0; u < V; ++u) w[u] = strip.col(u) < a.Rk ? static_cast<const uint16_t*>(a.base)[at + strip.col(u)] : 0;
+        }
+#pragma unroll
+        for (int u = 0; u < V; ++u)
+          v[u] += a.base_dtype == EVOATTN_FP32 ? __uint_as_float(w[u])
+                  : a.base_dtype == EVOATTN_BF16 ? __uint_as_float(w[u] << 16) : __half2float(__ushort_as_half((unsigned short)w[u]));
+      }
+#pragma unroll
+      for (int u = 0; u < V; ++u)
+        if (strip.col(u) < a.Rk) o[strip.col(u)] = from_float<T>(v[u]);
     }
   }
 }
@@ -429,23 +454,22 @@ __global__ void __launch_bounds__(128, 5) relative_bwd(RelArgs a) {
   }
 }
 
-// The blocks' sums of a head, added in order: a warp for 32 table rows, eight shares of the blocks.
-__global__ void __launch_bounds__(256) relative_sum_partials(RelArgs a) {
+// The blocks' sums of a head, added in order: 32 table rows a block, 32 shares of the sums.
+__global__ void __launch_bounds__(1024) relative_sum_partials(RelArgs a) {
   ptx::grid_dependency_wait();
   ptx::grid_launch_dependents();
-  __shared__ float sm[8][32];
+  __shared__ float sm[32][33];
   const int lane = threadIdx.x & 31, part = threadIdx.x >> 5, r = blockIdx.x * 32 + lane, h = blockIdx.y;
   float s = 0.f;
-  if (r < a.buckets)
-    for (int k = part; k < a.blocks; k += 8) s += a.partial[((long long)h * a.blocks + k) * a.buckets + r];
+  if (r < a.buckets) {
+#pragma unroll 8
+    for (int k = part; k < a.blocks; k += 32) s += a.partial[((long long)h * a.blocks + k) * a.buckets + r];
+  }
   sm[part][lane] = s;
   __syncthreads();
-  if (part == 0 && r < a.buckets) {
-    s = 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) s += sm[i][lane];
-    store_any(a.dtable, a.table_dtype, (long long)r * a.H + h, s);
-  }
+  s = warp_sum(sm[lane][part]);  // (a warp a table row)
+  const int out = blockIdx.x * 32 + part;
+  if (lane == 0 && out < a.buckets) store_any(a.dtable, a.table_dtype, (long long)out * a.H + h, s);
 }
 
 int validate(const evoattn_relative_bias_params* p) {
@@ -521,14 +545,15 @@ int evoattn_relative_bias_fwd(const evoattn_relative_bias_params* p, void* cuda_
   cudaStream_t st = reinterpret_cast<cudaStream_t>(cuda_stream);
   return with_dtype(p->dtype, [&](auto e) {
     using T = decltype(e);
+    bool base_pieces = false;
     if (p->base) {  // V values of a lane in whole pieces of the base, too
       const int piece = (int)(kPer16<T> * dtype_bytes(p->base_dtype) < 16 ? kPer16<T> * dtype_bytes(p->base_dtype) : 16);
-      a.base_pieces = ((uintptr_t)p->base | (uintptr_t)(p->base_stride[0] * dtype_bytes(p->base_dtype)) | (uintptr_t)(p->base_stride[1] * dtype_bytes(p->base_dtype)) |
+      base_pieces = ((uintptr_t)p->base | (uintptr_t)(p->base_stride[0] * dtype_bytes(p->base_dtype)) | (uintptr_t)(p->base_stride[1] * dtype_bytes(p->base_dtype)) |
                        (uintptr_t)(p->base_stride[2] * dtype_bytes(p->base_dtype))) % piece == 0;
     }
-    const bool wide = rows_of_16_bytes(p->out, p->out_stride, (int)sizeof(T)) && (!p->base || a.base_pieces);
-    const cudaError_t rc = wide ? launch_dependent(relative_fwd<T, true>, grid, 256, smem, st, a, rows, row_warps)
-                                : launch_dependent(relative_fwd<T, false>, grid, 256, smem, st, a, rows, row_warps);
+    const bool wide = rows_of_16_bytes(p->out, p->out_stride, (int)sizeof(T)) && (!p->base || base_pieces);
+    const auto kern = p->base ? (wide ? relative_fwd<T, true, true> : relative_fwd<T, false, true>) : wide ? relative_fwd<T, true, false> : relative_fwd<T, false, false>;
+    const cudaError_t rc = launch_dependent(kern, grid, 256, smem, st, a, rows, row_warps);
     return rc == cudaSuccess ? EVOATTN_OK : EVOATTN_ERR_CUDA;
   });
 }
@@ -571,7 +596,7 @@ int evoattn_relative_bias_bwd(const evoattn_relative_bias_params* p, void* cuda_
     });
     if (bad) return EVOATTN_ERR_CUDA;
   }
-  if (rc == cudaSuccess) rc = launch_dependent(relative_sum_partials, dim3((unsigned)((a.buckets + 31) / 32), (unsigned)a.H), 256, 0, st, a);
+  if (rc == cudaSuccess) rc = launch_dependent(relative_sum_partials, dim3((unsigned)((a.buckets + 31) / 32), (unsigned)a.H), 1024, 0, st, a);
   return rc == cudaSuccess ? EVOATTN_OK : EVOATTN_ERR_CUDA;
 }
 
