@@ -40,11 +40,15 @@ def _log_buckets(n: int, max_distance: int, causal: bool):
     side = n if causal else n // 2  # buckets of one direction
     exact = side // 2
     m = side - exact
-    edges, d = [], exact
+    edges = []
     for k in range(1, m):
-        while d ** m * exact ** k < max_distance ** k * exact ** m:
+        reached = lambda d: d ** m * exact ** k >= max_distance ** k * exact ** m  # noqa: B023, E731
+        d = int(exact * (max_distance / exact) ** (k / m))  # (floating point says where to look)
+        while not reached(d):
             d += 1
-        edges.append(d)
+        while d > exact and reached(d - 1):
+            d -= 1
+        edges.append(max(d, exact))
     return exact, edges
 
 
