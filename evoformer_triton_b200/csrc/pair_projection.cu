@@ -54,7 +54,9 @@ __device__ __forceinline__ float gain(const ProjArgs& a, int c) { return a.g ? l
 // Products are of bf16 pieces with fp32 sums: an fp32 factor is the sum of three (24 bits), an fp16 one of two, a bf16 one
 // is one.  z enters as it is: sum_c G z[c] - mean sum_c G, with both sums over the same pieces of G, and M likewise from d r z
 // and d r mean.  G is two pieces (2^-17 of it is left out) where results are rounded to 16 bits, else three; d r always
-// three, since the weights' gradients may be fp32.  An MMA cuts its sums off where fp32 additions round: a sum that ends in fp32 is
+// three, since the weights' gradients may be fp32.  The rows x channels product of fp16 rows takes them as they are, with G in
+// two fp16 pieces, each head's times a power of two that brings its largest to 8 .. 16, so that no piece is too small for
+// the type.  An MMA cuts its sums off where fp32 additions round: a sum that ends in fp32 is
 // one of few MMAs, the products of low pieces first, and is added to the others in fp32.
 
 __device__ __forceinline__ void mma_k16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -79,15 +81,15 @@ __device__ __forceinline__ float quad_sum(float v) {
   return v + __shfl_xor_sync(0xffffffffu, v, 2);
 }
 
-// Two floats as N bf16 pieces each, packed by piece.
-template <int N>
+// Two floats as N pieces of 16 bits each, packed by piece.
+template <int N, class P = __nv_bfloat16>
 __device__ __forceinline__ void split2(float lo, float hi, uint32_t (&w)[N]) {
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    w[i] = Pack2<__nv_bfloat16>::pack(lo, hi);
+    w[i] = Pack2<P>::pack(lo, hi);
     if (i + 1 < N) {
       float a, b;
-      unpack2<__nv_bfloat16>(w[i], a, b);
+      unpack2<P>(w[i], a, b);
       lo -= a;
       hi -= b;
     }
@@ -98,6 +100,7 @@ template <class T> struct Pieces;  // pieces of a value of type T, and of G besi
 template <> struct Pieces<__nv_bfloat16> { static constexpr int kX = 1, kG = 2, kTerms = 2; };
 template <> struct Pieces<__half> { static constexpr int kX = 2, kG = 2, kTerms = 3; };
 template <> struct Pieces<float> { static constexpr int kX = 3, kG = 3, kTerms = 3; };
+template <class T> constexpr bool kNativeRows = std::is_same<T, __half>::value;
 
 // Eight channels of a row, the first `count` of which are there.
 template <class T>
@@ -184,9 +187,13 @@ __device__ __forceinline__ float of_bits(int dtype, uint32_t bits) {
 // A kernel's weights: G in pieces as B operands of rows x channels products, and as those of heads x channels products, both
 // [KC][NT][pieces][lane] (null: not wanted); the sum over the channels of the pieces of G and that of weight b for every
 // head.  Eight heads at a time, one a warp.  Ends with a barrier.
-template <int KC, int NT, int GP>
-__device__ __forceinline__ void prepare_weights(const ProjArgs& a, uint4* by_rows, uint4* by_heads, float* sm_sum, float* sm_t) {
+// sm_scale: what products by rows are to be multiplied by (null: 1).
+template <class T, int KC, int NT>
+__device__ __forceinline__ void prepare_weights(const ProjArgs& a, uint4* by_rows, uint4* by_heads, float* sm_sum, float* sm_t, float* sm_scale) {
+  constexpr int GP = Pieces<T>::kG;
+  using P = typename std::conditional<kNativeRows<T>, __half, __nv_bfloat16>::type;  // pieces of products by rows
   __shared__ float sm_G[8][32 * KC + 4];  // (4 floats apart: eight heads in different banks)
+  __shared__ float sm_up[8];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   for (int nt = 0; nt < NT; ++nt) {
     const int h = nt * 8 + warp;
@@ -196,47 +203,65 @@ __device__ __forceinline__ void prepare_weights(const ProjArgs& a, uint4* by_row
     if (a.g) load_bits<KC>(a.g, a.g_dtype, 0, a.C, gains);
     if (biased) load_bits<KC>(a.b, a.b_dtype, 0, a.C, biases);
     if (nt) __syncthreads();
-    float s = 0.f, tb = 0.f;
+    float s = 0.f, tb = 0.f, G[KC], most = 0.f;
 #pragma unroll
     for (int k = 0; k < KC; ++k) {
-      const float weight = of_bits(a.w_dtype, w[k]), G = a.g ? weight * of_bits(a.g_dtype, gains[k]) : weight;
-      sm_G[warp][lane + 32 * k] = G;
+      const float weight = of_bits(a.w_dtype, w[k]);
+      G[k] = a.g ? weight * of_bits(a.g_dtype, gains[k]) : weight;
       if (biased) tb = fmaf(weight, of_bits(a.b_dtype, biases[k]), tb);
+      sm_G[warp][lane + 32 * k] = G[k];
+      most = fmaxf(most, fabsf(G[k]));
+    }
+    if constexpr (kNativeRows<T>) {
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+      int up = most > 0.f && most < INFINITY ? 3 - ilogbf(most) : 0;
+      up = min(max(up, -100), 100);
+      if (lane == 0) sm_up[warp] = scalbnf(1.f, up);
+      if (sm_scale && lane == 0) sm_scale[h] = scalbnf(1.f, -up);
+      __syncwarp();
+    }
+#pragma unroll
+    for (int k = 0; k < KC; ++k) {
       uint32_t p[GP];
-      split2<GP>(G, 0.f, p);
+      split2<GP, P>(kNativeRows<T> ? G[k] * sm_up[warp] : G[k], 0.f, p);
       float v = 0.f;
 #pragma unroll
-      for (int j = GP - 1; j >= 0; --j) v += __uint_as_float(p[j] << 16);
+      for (int j = GP - 1; j >= 0; --j) {
+        float lo, hi;
+        unpack2<P>(p[j], lo, hi);
+        v += lo;
+      }
       s += v;
     }
     if (sm_sum) {
       s = warp_sum(s);
       if (biased) tb = warp_sum(tb);
       if (lane == 0) {
-        sm_sum[h] = s;
+        sm_sum[h] = kNativeRows<T> && sm_scale ? s * sm_scale[h] : s;
         if (sm_t) sm_t[h] = tb;
       }
     }
     __syncthreads();
     for (int i = threadIdx.x; i < KC * 32; i += blockDim.x) {
       const int l = i & 31, kc = i >> 5;
-      const auto write = [&](uint4* sm, const float (&v)[8]) {
+      const auto write = [&](uint4* sm, const float (&v)[8], auto piece) {
         uint32_t p[4][GP];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) split2<GP>(v[2 * k], v[2 * k + 1], p[k]);
+        for (int k = 0; k < 4; ++k) split2<GP, decltype(piece)>(v[2 * k], v[2 * k + 1], p[k]);
 #pragma unroll
         for (int j = 0; j < GP; ++j) sm[((kc * NT + nt) * GP + j) * 32 + l] = make_uint4(p[0][j], p[1][j], p[2][j], p[3][j]);
       };
       float v[8];
       if (by_rows) {  // eight channels of head l / 4
 #pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] = sm_G[l / 4][kc * 32 + (l & 3) * 8 + k];
-        write(by_rows, v);
+        for (int k = 0; k < 8; ++k) v[k] = sm_G[l / 4][kc * 32 + (l & 3) * 8 + k] * (kNativeRows<T> ? sm_up[l / 4] : 1.f);
+        write(by_rows, v, P());
       }
       if (by_heads) {  // pairs of heads of the four channels of a lane's accumulators
 #pragma unroll
         for (int k = 0; k < 8; ++k) v[k] = sm_G[(l & 3) * 2 + (k & 1)][kc * 32 + l / 8 * 8 + (l / 4 & 1) + (k & ~1)];
-        write(by_heads, v);
+        write(by_heads, v, __nv_bfloat16());
       }
     }
   }
@@ -378,6 +403,18 @@ __device__ __forceinline__ void product_by_rows(const ProjArgs& a, const TileT& 
   const int lane = threadIdx.x & 31;
 #pragma unroll TileT::kUnroll
   for (int kc = 0; kc < KC; ++kc) {
+    if constexpr (kNativeRows<T>) {
+      const uint4 l = x.get(a, 0, kc).w[0], h = x.get(a, 1, kc).w[0];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int j = GP - 1; j >= 0; --j) {
+          const uint4 gw = sm_g[((kc * NT + nt) * GP + j) * 32 + lane];
+          mma_k16_f16(acc[nt], l.x, h.x, l.y, h.y, gw.x, gw.y);
+          mma_k16_f16(acc[nt], l.z, h.z, l.w, h.w, gw.z, gw.w);
+        }
+      continue;
+    }
     uint32_t lo[4][XP], hi[4][XP];
     x.get(a, 0, kc).pieces(lo);
     x.get(a, 1, kc).pieces(hi);
@@ -411,13 +448,13 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 && KC <= 4 && NT <= 2 && V
   ptx::grid_dependency_wait();
   ptx::grid_launch_dependents();
   extern __shared__ __align__(16) uint4 sm_g[];  // [KC][NT][GP][32 lanes]
-  __shared__ float sm_sum[NT * 8], sm_t[NT * 8];
+  __shared__ float sm_sum[NT * 8], sm_t[NT * 8], sm_scale[NT * 8];
   const int warp = threadIdx.x >> 5, t = threadIdx.x & 3;
   const uint32_t rows = (uint32_t)((long long)a.B * a.Ri * a.Rj), step = gridDim.x * 128;
   Rows2 next(a, (blockIdx.x * 8 + warp) * 16, rows);
   Tile<T, KC, KEEP, VEC> x;
   x.load(a, next);
-  prepare_weights<KC, NT, Pieces<T>::kG>(a, sm_g, nullptr, sm_sum, sm_t);
+  prepare_weights<T, KC, NT>(a, sm_g, nullptr, sm_sum, sm_t, sm_scale);
   while (next.n0 < rows) {
     const Rows2 row = next;
     x.statistics(a);
@@ -432,11 +469,11 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 && KC <= 4 && NT <= 2 && V
       for (int e = 0; e < 2; ++e) {
         const int h = nt * 8 + 2 * t + e;
         if (h >= a.H) continue;
-        const float sum = sm_sum[h], tb = sm_t[h];
+        const float sum = sm_sum[h], tb = sm_t[h], scale = kNativeRows<T> ? sm_scale[h] : 1.f;
         T* out = static_cast<T*>(a.out) + h * a.sout.b;
 #pragma unroll
         for (int k = 0; k < 2; ++k)
-          if (row.on[k]) out[row.o[k]] = from_float<T>(fmaf(fmaf(-mean[k], sum, acc[nt][2 * k + e]), r[k], tb));
+          if (row.on[k]) out[row.o[k]] = from_float<T>(fmaf(fmaf(-mean[k], sum, acc[nt][2 * k + e] * scale), r[k], tb));
       }
   }
 }
@@ -647,10 +684,10 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 && KC <= 4 && NT == 1 && V
   ptx::grid_launch_dependents();
   constexpr int kG = KC * NT * Pieces<T>::kG * 32;
   extern __shared__ __align__(16) uint4 sm_g[];  // G by rows, G by heads; behind the rows' loop, the sums
-  __shared__ float sm_sum[NT * 8];
+  __shared__ float sm_sum[NT * 8], sm_scale[NT * 8];
   const int warp = threadIdx.x >> 5, t = threadIdx.x & 3;
   const uint32_t rows = (uint32_t)((long long)a.B * a.Ri * a.Rj), step = gridDim.x * 128;
-  if (a.dz) prepare_weights<KC, NT, Pieces<T>::kG>(a, sm_g, sm_g + kG, sm_sum, nullptr);
+  if (a.dz) prepare_weights<T, KC, NT>(a, sm_g, sm_g + kG, sm_sum, nullptr, sm_scale);
   const float by_C = 1.f / a.C;
   RowSums<T, KC, NT> sums;
   for (uint32_t n0 = (blockIdx.x * 8 + warp) * 16; n0 < rows; n0 += step) {
@@ -669,11 +706,11 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 && KC <= 4 && NT == 1 && V
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const float sum = sm_sum[nt * 8 + 2 * t + e];
+        const float sum = sm_sum[nt * 8 + 2 * t + e], scale = kNativeRows<T> ? sm_scale[nt * 8 + 2 * t + e] : 1.f;
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
           c0[k] = fmaf(d[nt][k][e], sum, c0[k]);
-          c1[k] = fmaf(d[nt][k][e], fmaf(-x.mean[k], sum, acc[nt][2 * k + e]), c1[k]);
+          c1[k] = fmaf(d[nt][k][e], fmaf(-x.mean[k], sum, acc[nt][2 * k + e] * scale), c1[k]);
         }
       }
 #pragma unroll
@@ -696,7 +733,7 @@ __global__ void __launch_bounds__(256) projection_dz(ProjArgs a) {
   extern __shared__ __align__(16) uint4 sm_g[];  // G by heads
   const int warp = threadIdx.x >> 5;
   const uint32_t rows = (uint32_t)((long long)a.B * a.Ri * a.Rj), step = gridDim.x * 128;
-  if (a.dz) prepare_weights<KC, NT, Pieces<T>::kG>(a, nullptr, sm_g, nullptr, nullptr);
+  if (a.dz) prepare_weights<T, KC, NT>(a, nullptr, sm_g, nullptr, nullptr, nullptr);
   const float by_C = 1.f / a.C;
   for (uint32_t n0 = (blockIdx.x * 8 + warp) * 16; n0 < rows; n0 += step) {
     const Rows2 row(a, n0, rows);

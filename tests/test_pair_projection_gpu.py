@@ -53,6 +53,15 @@ def test_weights_of_other_types_or_none(weights):
     _against_oracle(_draw((1, 33, 40, 128), BF, 1), W, None if weights in ("none", "bias") else g, None if weights in ("none", "gain") else b)
 
 
+@pytest.mark.parametrize("dtype", [BF, HF, F32], ids=["bf16", "fp16", "fp32"])
+def test_weights_of_any_size(dtype):
+    """Heads whose weights differ by twelve orders of magnitude, zero among them, and gains that differ by four."""
+    W, g, b = _weights(8, 128)
+    W = W * torch.tensor([1e-9, 1e-6, 1e-3, 1.0, 30.0, 1e3, 0.0, -1.0], device=DEV)[:, None]
+    g = g * torch.logspace(-2, 2, 128, device=DEV)
+    _against_oracle(_draw((1, 20, 33, 128), dtype, 1), W, g, b, d=_draw((1, 1, 8, 20, 33), dtype, 5) * 0.01)
+
+
 @pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "fp32"])
 @pytest.mark.parametrize("C", [64, 50])
 def test_pair_is_read_where_it_lies(C, dtype):
