@@ -205,6 +205,25 @@ def test_together_with_the_attention(R):
         assert a.shape == b.shape and torch.isfinite(a).all() and evo_oracle.rel_err(a.float(), b.float()) < 3e-2, n
 
 
+@pytest.mark.parametrize("R", [64, 77])
+def test_one_bias_for_a_batch(R):
+    """A bias of positions that the batch shares, expanded: the attention reads it in place, and its gradient is summed over the
+    batch.  As with the bias copied out, to the roundings of d(bias) and of sums in no fixed order."""
+    import evoformer_triton_b200 as evo
+    B, S, H, D = 3, 4, 4, 32
+    q, k, v, d = (_draw((B, S, R, H, D), BF, i) for i in range(4))
+    table = _draw((65, H), F32, 5).requires_grad_()
+    pos = torch.arange(R, device=DEV)
+    res = []
+    for copied in (False, True):
+        bias = evo.relative_position_bias(table, pos, max_distance=32, dtype=BF).expand(B, 1, H, R, R)
+        bias = bias.clone(memory_format=torch.contiguous_format) if copied else bias
+        out = evo.evoformer_attention(q, k, v, [None, bias])
+        res.append((out.detach(), torch.autograd.grad(out, table, d)[0]))
+    assert torch.equal(res[0][0], res[1][0])
+    assert evo_oracle.rel_err(res[0][1], res[1][1]) < 4e-3
+
+
 def test_together_in_a_cuda_graph():
     """A block's forward and backward captured once and replayed on other values, beside a second captured block."""
     B, S, R, H, D, C, Cz = 1, 3, 77, 4, 32, 64, 128
