@@ -674,9 +674,29 @@ __device__ __forceinline__ void write_dz(const ProjArgs& a, const TileT& x, cons
   }
 }
 
-// Backward in one pass over z: dz, and M and s of the block's rows.  mean(u) and mean(u (z - mean)) are sums over heads,
+// c0 = sum_c u and c1 = sum_c u (z - mean) of a lane's two rows, as far as the lane's heads go:
 //   sum_c u = sum_h d[h] sum_c G[h,c],   sum_c u (z - mean) = sum_h d[h] (sum_c G[h,c] z[c] - mean sum_c G[h,c]),
 // the latter with the product that the forward takes.
+template <class T, int KC, int NT, class TileT>
+__device__ __forceinline__ void sums_over_heads(const ProjArgs& a, const TileT& x, const uint4* by_rows, const float* sm_sum, const float* sm_scale, const float (&d)[NT][2][2],
+                                                float (&c0)[2], float (&c1)[2]) {
+  float acc[NT][4] = {};
+  product_by_rows<T, KC, NT>(a, x, by_rows, acc);
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int h = nt * 8 + 2 * (threadIdx.x & 3) + e;
+      const float sum = sm_sum[h], scale = kNativeRows<T> ? sm_scale[h] : 1.f;
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        c0[k] = fmaf(d[nt][k][e], sum, c0[k]);
+        c1[k] = fmaf(d[nt][k][e], fmaf(-x.mean[k], sum, acc[nt][2 * k + e] * scale), c1[k]);
+      }
+    }
+}
+
+// Backward in one pass over z: dz, and M and s of the block's rows.
 // Two blocks an SM where the registers allow it (bf16, 128 channels, 8 heads: one block of 148 registers 116 us, two of 128 95 us).
 template <class T, int KC, int NT, int VEC>
 __global__ void __launch_bounds__(256, sizeof(T) == 2 && KC <= 4 && NT == 1 && VEC == 8 ? 2 : 1) projection_bwd(ProjArgs a) {
@@ -685,7 +705,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 && KC <= 4 && NT == 1 && V
   constexpr int kG = KC * NT * Pieces<T>::kG * 32;
   extern __shared__ __align__(16) uint4 sm_g[];  // G by rows, G by heads; behind the rows' loop, the sums
   __shared__ float sm_sum[NT * 8], sm_scale[NT * 8];
-  const int warp = threadIdx.x >> 5, t = threadIdx.x & 3;
+  const int warp = threadIdx.x >> 5;
   const uint32_t rows = (uint32_t)((long long)a.B * a.Ri * a.Rj), step = gridDim.x * 128;
   if (a.dz) prepare_weights<T, KC, NT>(a, sm_g, sm_g + kG, sm_sum, nullptr, sm_scale);
   const float by_C = 1.f / a.C;
@@ -700,19 +720,8 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 && KC <= 4 && NT == 1 && V
     x.statistics(a);
     if (a.partial) sums.add(a, x, dp);
     if (!a.dz) continue;
-    float acc[NT][4] = {}, c0[2] = {}, c1[2] = {};
-    product_by_rows<T, KC, NT>(a, x, sm_g, acc);
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const float sum = sm_sum[nt * 8 + 2 * t + e], scale = kNativeRows<T> ? sm_scale[nt * 8 + 2 * t + e] : 1.f;
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          c0[k] = fmaf(d[nt][k][e], sum, c0[k]);
-          c1[k] = fmaf(d[nt][k][e], fmaf(-x.mean[k], sum, acc[nt][2 * k + e] * scale), c1[k]);
-        }
-      }
+    float c0[2] = {}, c1[2] = {};
+    sums_over_heads<T, KC, NT>(a, x, sm_g, sm_sum, sm_scale, d, c0, c1);
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       c0[k] = x.r[k] * quad_sum(c0[k]) * by_C;
@@ -725,15 +734,23 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 && KC <= 4 && NT == 1 && V
   write_partial<KC, NT>(a, reinterpret_cast<const float*>(sm_g), blockIdx.x, 0, 0);
 }
 
+// Whether the sums over heads are taken (with G in both layouts) where rows are kept: [1,512,512,256] to 16 heads, bf16, backward 198 ->
+// 169 us.  Rows that are read again for every use are better off with u worked out twice ([1,768,768,384] to 8 531, not 596).
+template <class T>
+__host__ __device__ constexpr bool both_layouts(int KC, int NT, bool keep) { return keep && KC * NT * Pieces<T>::kG <= 192; }
+
 // More channels and heads than one block can hold the sums of: dz and the rows' statistics in one kernel ...
 template <class T, int KC, int NT, bool KEEP, int VEC>
 __global__ void __launch_bounds__(256) projection_dz(ProjArgs a) {
   ptx::grid_dependency_wait();
   ptx::grid_launch_dependents();
-  extern __shared__ __align__(16) uint4 sm_g[];  // G by heads
+  constexpr bool kBoth = both_layouts<T>(KC, NT, KEEP);
+  constexpr int kG = KC * NT * Pieces<T>::kG * 32;
+  extern __shared__ __align__(16) uint4 sm_g[];  // G by heads, and by rows if kBoth
+  __shared__ float sm_sum[NT * 8], sm_scale[NT * 8];
   const int warp = threadIdx.x >> 5;
   const uint32_t rows = (uint32_t)((long long)a.B * a.Ri * a.Rj), step = gridDim.x * 128;
-  if (a.dz) prepare_weights<T, KC, NT>(a, nullptr, sm_g, nullptr, nullptr, nullptr);
+  if (a.dz) prepare_weights<T, KC, NT>(a, kBoth ? sm_g + kG : nullptr, sm_g, sm_sum, nullptr, sm_scale);
   const float by_C = 1.f / a.C;
   for (uint32_t n0 = (blockIdx.x * 8 + warp) * 16; n0 < rows; n0 += step) {
     const Rows2 row(a, n0, rows);
@@ -749,18 +766,22 @@ __global__ void __launch_bounds__(256) projection_dz(ProjArgs a) {
     float d[NT][2][2], c0[2] = {}, c1[2] = {};
     uint32_t dp[NT][2][Pieces<T>::kX];
     load_d<T, NT>(a, row, 0, d, dp);
+    if constexpr (kBoth) {
+      sums_over_heads<T, KC, NT>(a, x, sm_g + kG, sm_sum, sm_scale, d, c0, c1);
+    } else {
 #pragma unroll KEEP ? KC : 1
-    for (int kc = 0; kc < KC; ++kc) {
-      float u[2][8];
-      product_by_heads<T, NT>(sm_g, kc, dp, u);
+      for (int kc = 0; kc < KC; ++kc) {
+        float u[2][8];
+        product_by_heads<T, NT>(sm_g, kc, dp, u);
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        float v[8];
-        x.get(a, k, kc).floats(v);
+        for (int k = 0; k < 2; ++k) {
+          float v[8];
+          x.get(a, k, kc).floats(v);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          c0[k] += u[k][e];
-          c1[k] = fmaf(u[k][e], v[e] - x.mean[k], c1[k]);  // (channels that are not there have u = 0)
+          for (int e = 0; e < 8; ++e) {
+            c0[k] += u[k][e];
+            c1[k] = fmaf(u[k][e], v[e] - x.mean[k], c1[k]);  // (channels that are not there have u = 0)
+          }
         }
       }
     }
@@ -1036,7 +1057,7 @@ int evoattn_pair_projection_bwd(const evoattn_pair_projection_params* p, void* c
       with_shape<T>(a, [&](auto sh) {
         using Sh = decltype(sh);
         const auto kern = projection_dz<T, Sh::KC, Sh::NT, Sh::KEEP, Sh::VEC>;
-        const int smem = Sh::KC * Sh::NT * Pieces<T>::kG * 512;
+        const int smem = (both_layouts<T>(Sh::KC, Sh::NT, Sh::KEEP) ? 2 : 1) * Sh::KC * Sh::NT * Pieces<T>::kG * 512;
         unsigned blocks;
         if (blocks_of(kern, rows, smem, &blocks)) rc = launch_dependent(kern, dim3(blocks), 256, (size_t)smem, st, a);
       });
