@@ -928,6 +928,8 @@ void with_shape(const ProjArgs& a, F&& f) {
   if (vec < 8) {  // fewer shapes
     if (a.C <= 128 && a.H <= 8 && vec == 4) f(Shape<4, 1, true, 4>());
     else if (a.C <= 128 && a.H <= 8) f(Shape<4, 1, true, 1>());
+    else if (a.C <= 128 && a.H <= 16 && vec == 4) f(Shape<4, 2, true, 4>());
+    else if (a.C <= 128 && a.H <= 16) f(Shape<4, 2, true, 1>());
     else if (a.H <= 16) f(Shape<16, 2, false, 1>());
     else f(Shape<16, 8, false, 1>());
     return;
@@ -1063,7 +1065,8 @@ int evoattn_pair_projection_bwd(const evoattn_pair_projection_params* p, void* c
       });
       if (rc == cudaSuccess && sums) {
         const dim3 grid((unsigned)a.blocks, (unsigned)((a.C + kSumChannels - 1) / kSumChannels), (unsigned)((a.H + kSumHeads - 1) / kSumHeads));
-        rc = vector_of(a, (int)sizeof(T)) == 8 ? launch_dependent(projection_sums<T, 8>, grid, 256, 0, st, a) : launch_dependent(projection_sums<T, 1>, grid, 256, 0, st, a);
+        const int vec = vector_of(a, (int)sizeof(T));
+        rc = launch_dependent(vec == 8 ? projection_sums<T, 8> : vec == 4 ? projection_sums<T, 4> : projection_sums<T, 1>, grid, 256, 0, st, a);
       }
       return 0;
     });

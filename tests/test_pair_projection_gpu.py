@@ -42,7 +42,8 @@ def _weights(H, C, dtype=F32, affine=True):
 @pytest.mark.parametrize("dtype", [BF, HF, F32], ids=["bf16", "fp16", "fp32"])
 @pytest.mark.parametrize("B,I,J,C,H", [(1, 1, 1, 1, 1), (1, 1, 1, 128, 8), (1, 3, 5, 7, 3), (2, 9, 9, 32, 4), (1, 17, 17, 64, 1), (1, 31, 33, 128, 4), (2, 40, 40, 128, 8),
                                        (1, 20, 50, 100, 5), (1, 24, 24, 256, 8), (1, 16, 16, 192, 16), (1, 12, 12, 384, 12), (1, 10, 14, 512, 64), (1, 7, 200, 130, 9),
-                                       (1, 64, 64, 48, 32), (1, 101, 101, 128, 4), (1, 300, 260, 32, 2)], ids=str)
+                                       (1, 64, 64, 48, 32), (1, 101, 101, 128, 4), (1, 300, 260, 32, 2), (1, 30, 41, 100, 12), (1, 30, 41, 99, 16),
+                                       (1, 9, 30, 300, 10), (1, 9, 30, 301, 40)], ids=str)
 def test_sizes(B, I, J, C, H, dtype):
     _against_oracle(_draw((B, I, J, C), dtype, 1, 2.0, 0.3), *_weights(H, C))
 
