@@ -921,7 +921,8 @@ void look_at_rows(ProjArgs* a) {
 }
 
 template <int KC_, int NT_, bool KEEP_, int VEC_> struct Shape { static constexpr int KC = KC_, NT = NT_, VEC = VEC_; static constexpr bool KEEP = KEEP_; };
-// 32 KC channels and 8 NT heads for a call; rows stay in registers while they take up to 64 a lane.
+// 32 KC channels and 8 NT heads for a call; rows stay in registers up to 256 channels (fp32, 256 to 8 heads, [1,512,512,256]: forward 73
+// us, read again for every use 126), with more than 16 heads up to 8 words a lane and row.
 template <class T, class F>
 void with_shape(const ProjArgs& a, F&& f) {
   const int vec = vector_of(a, (int)sizeof(T));
@@ -936,7 +937,7 @@ void with_shape(const ProjArgs& a, F&& f) {
   }
   const auto heads = [&](auto kc) {
     constexpr int KC = decltype(kc)::value;
-    constexpr bool keep = KC * (int)sizeof(T) <= 16;
+    constexpr bool keep = KC <= 8;
     if (a.H <= 8) f(Shape<KC, 1, keep, 8>());
     else if (a.H <= 16) f(Shape<KC, 2, keep, 8>());
     else f(Shape<KC, 8, KC * (int)sizeof(T) <= 8, 8>());
