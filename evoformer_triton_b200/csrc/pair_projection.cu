@@ -968,6 +968,11 @@ void with_one_pass_shape(const ProjArgs& a, F&& f) {
     else f(Shape<4, 2, true, 8>());
   }
 }
+// The same of the shapes that with_shape() gives: those whose backward is one kernel need none of the two.
+template <class T>
+constexpr bool one_pass_shape(int KC, int NT, int VEC) {
+  return sizeof(T) == 4 || VEC < 8 ? KC <= 4 && NT == 1 : (KC <= 8 && NT == 1) || (KC <= 4 && NT <= 2);
+}
 // Blocks of 128 rows that run at once.
 template <class K>
 bool blocks_of(K kern, long long rows, int smem, unsigned* blocks) {
@@ -1059,10 +1064,12 @@ int evoattn_pair_projection_bwd(const evoattn_pair_projection_params* p, void* c
       }
       with_shape<T>(a, [&](auto sh) {
         using Sh = decltype(sh);
-        const auto kern = projection_dz<T, Sh::KC, Sh::NT, Sh::KEEP, Sh::VEC>;
-        const int smem = (both_layouts<T>(Sh::KC, Sh::NT, Sh::KEEP) ? 2 : 1) * Sh::KC * Sh::NT * Pieces<T>::kG * 512;
-        unsigned blocks;
-        if (blocks_of(kern, rows, smem, &blocks)) rc = launch_dependent(kern, dim3(blocks), 256, (size_t)smem, st, a);
+        if constexpr (!one_pass_shape<T>(Sh::KC, Sh::NT, Sh::VEC)) {
+          const auto kern = projection_dz<T, Sh::KC, Sh::NT, Sh::KEEP, Sh::VEC>;
+          const int smem = (both_layouts<T>(Sh::KC, Sh::NT, Sh::KEEP) ? 2 : 1) * Sh::KC * Sh::NT * Pieces<T>::kG * 512;
+          unsigned blocks;
+          if (blocks_of(kern, rows, smem, &blocks)) rc = launch_dependent(kern, dim3(blocks), 256, (size_t)smem, st, a);
+        }
       });
       if (rc == cudaSuccess && sums) {
         const dim3 grid((unsigned)a.blocks, (unsigned)((a.C + kSumChannels - 1) / kSumChannels), (unsigned)((a.H + kSumHeads - 1) / kSumHeads));
