@@ -130,9 +130,11 @@ struct Strip {
 #pragma unroll
       for (int u = 0; u < V; ++u) r[u] = bucket.near[min(max(from + off[u], 0), 2 * bucket.far)];
     } else {
+      // A place without a key has the row of the lane's key before it: equal rows of keys in order stay next to each other.
+      int row = 0;
       for (int u = 0; u < V; ++u) {
         const int c = WIDE ? j0 + (int)(threadIdx.x & (L - 1)) * V + u : j0 + u * L + (int)(threadIdx.x & (L - 1));
-        const int row = bucket(difference(position(a.k_pos, a.positions64, b * a.sk + min(c, a.Rk - 1)), q));
+        if (c < a.Rk) row = bucket(difference(position(a.k_pos, a.positions64, b * a.sk + c), q));
 #pragma unroll
         for (int k = 0; k < V; ++k)
           if (k == u) r[k] = row;

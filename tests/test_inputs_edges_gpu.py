@@ -1,0 +1,43 @@
+"""GPU: the operators before the attention at the edges of what they take."""
+import pytest
+import torch
+
+from oracle import inputs_oracle as oc
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+BF, HF, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+def _draw(shape, dtype, seed, std=1.0, mean=0.0):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    return (torch.randn(shape, generator=g, device=DEV) * std + mean).to(dtype)
+
+
+# ---------------------------------------------------------------- relative position bias
+
+def _keys_that_jump_back(n, apart):
+    """Two chains far from each other in pieces of `apart` keys, the last of which may be cut short: a piece is one chain up to the
+    length of the short one, and the other one, but for the first of every 64 keys, behind that."""
+    i = torch.arange(n)
+    return torch.where((i % apart < n % apart) | (i % 64 < apart), 5, 2000)
+
+
+@pytest.mark.parametrize("kind", [("log_causal", 32, 4096), ("log", 64, 5000), ("log_causal", 32, 128)], ids=str)
+@pytest.mark.parametrize("dtype", [BF, HF, F32], ids=["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("Rk", [3, 18, 34, 77, 437])
+def test_relative_gradient_of_keys_in_no_order(Rk, dtype, kind):
+    """The gradient of ones counts the keys of a bucket, exactly (whole numbers below 2^24): rows on 16 bytes and off them, a last strip
+    that ends anywhere, borders beyond those that are looked up and within."""
+    import evoformer_triton_b200 as evo
+    scheme, n, M = kind
+    H, q = 2, torch.tensor([3000, 2000, 5, 0, 1999])
+    for keys in (_keys_that_jump_back(Rk, 8), _keys_that_jump_back(Rk, 16), torch.arange(Rk).flip(0) * 7, (torch.arange(Rk) * 37) % 3001):
+        rows = oc.bucket_rows([q.tolist()], [keys.tolist()], scheme, n, M).reshape(-1)
+        want = torch.bincount(rows, minlength=n).to(F32).unsqueeze(1).expand(n, H)
+        table = _draw((n, H), F32, 1).requires_grad_()
+        out = evo.relative_position_bias(table, q.to(DEV), keys.to(DEV), max_distance=M, buckets=scheme, dtype=dtype)
+        for pitch in (out.stride(3), Rk + 1 - Rk % 2):
+            d = torch.ones((1, 1, H, len(q), pitch), dtype=dtype, device=DEV)[..., :Rk]
+            g, = torch.autograd.grad(out, table, d, retain_graph=True)
+            assert torch.equal(g.cpu(), want), (pitch, (g.cpu() - want)[:, 0].nonzero().flatten().tolist())
