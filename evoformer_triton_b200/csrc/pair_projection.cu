@@ -643,15 +643,17 @@ __device__ __forceinline__ void product_by_heads(const uint4* sm_u, int kc, cons
   }
 }
 
-// dz = r u - c0 - (z - mean) c1 with c0 = r mean(u), c1 = r^3 mean(u (z - mean)), two channels an instruction.
+// dz = r (u - c0 - (z - mean) c1) with c0 = mean(u), c1 = r^2 mean(u (z - mean)), two channels an instruction.  Powers of r are never
+// formed by themselves, and r comes last: each factor is of the size of a result then, where r^3 alone, or r c1, leaves
+// fp32's range in rows that deviate by 10^14 or by 10^-14.  (One multiplication more: backward of [2,768,768,128] to 8 heads, bf16, 141 -> 143 us.)
 template <class T, int KC, int NT, class TileT>
 __device__ __forceinline__ void write_dz(const ProjArgs& a, const TileT& x, const Rows2& row, const uint4* sm_u, const uint32_t (&dp)[NT][2][Pieces<T>::kX],
                                          const float (&c0)[2], const float (&c1)[2]) {
-  ptx::F2 by_u[2], by_z[2], rest[2];
+  ptx::F2 by_r[2], by_z[2], rest[2];
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
     const float more = fmaf(x.mean[k], c1[k], -c0[k]);
-    by_u[k] = ptx::f2_make(x.r[k], x.r[k]);
+    by_r[k] = ptx::f2_make(x.r[k], x.r[k]);
     by_z[k] = ptx::f2_make(-c1[k], -c1[k]);
     rest[k] = ptx::f2_make(more, more);
   }
@@ -666,7 +668,7 @@ __device__ __forceinline__ void write_dz(const ProjArgs& a, const TileT& x, cons
 #pragma unroll
       for (int e = 0; e < 8; e += 2) {
         const ptx::F2 z = ptx::f2_fma(ptx::f2_make(v[e], v[e + 1]), by_z[k], rest[k]);
-        ptx::f2_get(ptx::f2_fma(ptx::f2_make(u[k][e], u[k][e + 1]), by_u[k], z), v[e], v[e + 1]);
+        ptx::f2_get(ptx::f2_mul(ptx::f2_add(ptx::f2_make(u[k][e], u[k][e + 1]), z), by_r[k]), v[e], v[e + 1]);
       }
       if (row.on[k])
         Eight<T>::template store<TileT::VEC>(static_cast<T*>(a.dz) + (long long)row.row(k) * a.C + kc * 32 + (threadIdx.x & 3) * 8, v, x.count(a, kc));
@@ -724,8 +726,8 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 && KC <= 4 && NT == 1 && V
     sums_over_heads<T, KC, NT>(a, x, sm_g, sm_sum, sm_scale, d, c0, c1);
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-      c0[k] = x.r[k] * quad_sum(c0[k]) * by_C;
-      c1[k] = x.r[k] * x.r[k] * x.r[k] * quad_sum(c1[k]) * by_C;
+      c0[k] = quad_sum(c0[k]) * by_C;
+      c1[k] = x.r[k] * (x.r[k] * (quad_sum(c1[k]) * by_C));
     }
     write_dz<T, KC, NT>(a, x, row, sm_g + kG, dp, c0, c1);
   }
@@ -787,8 +789,8 @@ __global__ void __launch_bounds__(256) projection_dz(ProjArgs a) {
     }
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-      c0[k] = x.r[k] * quad_sum(c0[k]) * by_C;
-      c1[k] = x.r[k] * x.r[k] * x.r[k] * quad_sum(c1[k]) * by_C;
+      c0[k] = quad_sum(c0[k]) * by_C;
+      c1[k] = x.r[k] * (x.r[k] * (quad_sum(c1[k]) * by_C));
     }
     write_dz<T, KC, NT>(a, x, row, sm_g, dp, c0, c1);
   }

@@ -41,3 +41,23 @@ def test_relative_gradient_of_keys_in_no_order(Rk, dtype, kind):
             d = torch.ones((1, 1, H, len(q), pitch), dtype=dtype, device=DEV)[..., :Rk]
             g, = torch.autograd.grad(out, table, d, retain_graph=True)
             assert torch.equal(g.cpu(), want), (pitch, (g.cpu() - want)[:, 0].nonzero().flatten().tolist())
+
+
+# ---------------------------------------------------------------- pair-bias projection
+
+@pytest.mark.parametrize("dtype", [BF, HF, F32], ids=["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("C_,H", [(128, 8), (64, 16), (256, 16), (384, 4), (100, 5), (130, 20)], ids=str)
+def test_projection_of_rows_of_any_scale(C_, H, dtype):
+    """Rows that deviate by 10^-17 to 10^17 (fp16: as far as it goes), with no eps that would hide the small ones, and gradients
+    of any size: rows scaled by s have the result of s = 1 and dpair / s."""
+    import evoformer_triton_b200 as evo
+    exps = torch.arange(-17, 18, device=DEV).double() if dtype != HF else torch.linspace(-2, 4, 35, device=DEV).double()
+    z = (_draw((1, 35, 6, C_), F32, 1).double() * (10.0 ** exps)[None, :, None, None]).to(dtype).requires_grad_()
+    W, g, b = _draw((H, C_), F32, 2, C_ ** -0.5), _draw((C_,), F32, 3, 0.2, 1.0), _draw((C_,), F32, 4, 0.2)
+    for size in (1.0, 1e-3) if dtype == HF else (1.0, 1e-10, 1e10):
+        d = (_draw((1, 1, H, 35, 6), F32, 5) * size).to(dtype)
+        out = evo.pair_bias_projection(z, W, g, b, eps=0.0)
+        dz, = torch.autograd.grad(out, z, d)
+        want = oc.pair_projection(z.detach(), W, g, b, 0.0, d)
+        oc.check("out", out, want[0])
+        oc.check("dpair", dz, want[1])
