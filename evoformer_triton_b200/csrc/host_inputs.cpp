@@ -39,7 +39,16 @@ float checked_eps(double eps) {
   if (!(eps >= 0.0) || std::isinf(eps)) value_error("eps must be a finite number that is not negative");
   return (float)eps;
 }
-void once(const char* op) {
+// Derivatives in forward mode (dual tensors) are not worked out.  A dual tensor need not require a gradient, so a call that
+// took it as an ordinary one would return a result whose derivative is zero; the same goes for a dual gradient.
+bool is_dual(const Tensor& t) { return t.defined() && t._fw_grad(/*level=*/0).defined(); }
+std::string no_forward_mode(const char* op) { return std::string(op) + " has no derivative in forward mode"; }
+void no_duals(const char* op, std::initializer_list<const Maybe*> inputs) {
+  for (const Maybe* t : inputs)
+    if (*t && is_dual(**t)) runtime_error(no_forward_mode(op));
+}
+void once(const char* op, const Tensor& grad) {
+  if (is_dual(grad)) throw std::runtime_error(no_forward_mode(op));
   if (at::GradMode::is_enabled()) throw std::runtime_error(std::string(op) + " can be differentiated once; its gradient has no graph (create_graph)");
 }
 bool wants_grad(std::initializer_list<const Maybe*> inputs) {
@@ -119,7 +128,7 @@ struct LayerNorm : public torch::autograd::Function<LayerNorm> {
     return c.y;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    once("layer_norm");
+    once("layer_norm", grads[0]);
     const variable_list s = ctx->get_saved_variables();
     const c10::cuda::CUDAGuard guard(s[0].device());
     NormCall c(s[0], s[1].defined() ? Maybe(s[1]) : Maybe(), s[2].defined() ? Maybe(s[2]) : Maybe(), (float)ctx->saved_data["eps"].toDouble());
@@ -165,6 +174,8 @@ struct LayerNorm : public torch::autograd::Function<LayerNorm> {
 };
 
 Tensor layer_norm(const Tensor& x, const Maybe& weight, const Maybe& bias, double eps) {
+  const Maybe xm(x);
+  no_duals("layer_norm", {&xm, &weight, &bias});
   check_main(x, "layer_norm", "x");
   if (x.dim() < 1 || x.size(-1) < 1) value_error("x must have a last axis of at least one value");
   const int64_t C = x.size(-1);
@@ -172,7 +183,6 @@ Tensor layer_norm(const Tensor& x, const Maybe& weight, const Maybe& bias, doubl
   if (weight) check_weight(*weight, x, "weight", {C});
   if (bias) check_weight(*bias, x, "bias", {C});
   const float e = checked_eps(eps);
-  const Maybe xm(x);
   if (wants_grad({&xm, &weight, &bias})) return LayerNorm::apply(x, weight, bias, eps);
   const c10::cuda::CUDAGuard guard(x.device());
   NormCall c(x, weight, bias, e);
@@ -247,7 +257,7 @@ struct RelativeBias : public torch::autograd::Function<RelativeBias> {
     return out;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    once("relative_position_bias");
+    once("relative_position_bias", grads[0]);
     const variable_list s = ctx->get_saved_variables();
     auto& sd = ctx->saved_data;
     const Tensor& d_in = grads[0];
@@ -285,6 +295,8 @@ void check_positions(const Tensor& t, const Tensor& table, const char* name) {
 
 Tensor relative_position_bias(const Tensor& table, const Tensor& q, const Maybe& keys, const Maybe& base, c10::optional<at::ScalarType> dtype,
                               int64_t scheme, int64_t exact, std::vector<int32_t> edges) {
+  const Maybe tm(table);
+  no_duals("relative_position_bias", {&tm, &base});
   check_main(table, "relative_position_bias", "table");
   if (table.dim() != 2 || table.size(0) < 1 || table.size(1) < 1) value_error("table must have the shape [buckets, H]");
   const Tensor k = keys.value_or(q);
@@ -306,7 +318,6 @@ Tensor relative_position_bias(const Tensor& table, const Tensor& q, const Maybe&
   const at::ScalarType type = dtype ? *dtype : base ? base->scalar_type() : table.scalar_type();
   if (!known(type)) type_error("dtype must be bfloat16, float16 or float32");
   const RelativePlan plan{scheme, exact, table.size(0), std::move(edges)};
-  const Maybe tm(table);
   if (wants_grad({&tm, &base})) return RelativeBias::apply(table, base, q, k, plan, B, (int64_t)type);
   const c10::cuda::CUDAGuard guard(table.device());
   RelativeCall c(table, q, k, plan, B);
@@ -352,7 +363,7 @@ struct PairProjection : public torch::autograd::Function<PairProjection> {
     return out;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    once("pair_bias_projection");
+    once("pair_bias_projection", grads[0]);
     const variable_list s = ctx->get_saved_variables();
     const c10::cuda::CUDAGuard guard(s[0].device());
     ProjectionCall c(s[0], s[1], s[2].defined() ? Maybe(s[2]) : Maybe(), s[3].defined() ? Maybe(s[3]) : Maybe(), (float)ctx->saved_data["eps"].toDouble());
@@ -376,6 +387,8 @@ struct PairProjection : public torch::autograd::Function<PairProjection> {
 };
 
 Tensor pair_bias_projection(const Tensor& pair, const Tensor& weight, const Maybe& norm_weight, const Maybe& norm_bias, double eps) {
+  const Maybe zm(pair), wm(weight);
+  no_duals("pair_bias_projection", {&zm, &wm, &norm_weight, &norm_bias});
   check_main(pair, "pair_bias_projection", "pair");
   if (pair.dim() != 4 || pair.size(3) < 1) value_error("pair must have the shape [B, N_res, N_res, C]");
   const int64_t C = pair.size(3);
@@ -386,7 +399,6 @@ Tensor pair_bias_projection(const Tensor& pair, const Tensor& weight, const Mayb
   if (norm_weight) check_weight(*norm_weight, pair, "norm_weight", {C});
   if (norm_bias) check_weight(*norm_bias, pair, "norm_bias", {C});
   const float e = checked_eps(eps);
-  const Maybe zm(pair), wm(weight);
   if (wants_grad({&zm, &wm, &norm_weight, &norm_bias})) return PairProjection::apply(pair, weight, norm_weight, norm_bias, eps);
   const c10::cuda::CUDAGuard guard(pair.device());
   ProjectionCall c(pair, weight, norm_weight, norm_bias, e);

@@ -4,7 +4,7 @@ projection of the pair representation to a pair bias.
 The reference's op begins at Q, K, V and a finished pair bias; these are the steps of a block before it.  All
 three run on CUDA tensors (bfloat16, float16, float32) in kernels of this package, forward and backward, with
 sums in fp32 taken in a fixed order: the same bits in every run.  They can be captured in a CUDA graph,
-and can be differentiated once.
+and can be differentiated once, in reverse mode.
 """
 from __future__ import annotations
 

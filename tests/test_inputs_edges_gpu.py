@@ -61,3 +61,31 @@ def test_projection_of_rows_of_any_scale(C_, H, dtype):
         want = oc.pair_projection(z.detach(), W, g, b, 0.0, d)
         oc.check("out", out, want[0])
         oc.check("dpair", dz, want[1])
+
+
+# ---------------------------------------------------------------- derivatives that are not there
+
+def test_forward_derivatives_are_refused():
+    import evoformer_triton_b200 as evo
+    from torch.autograd import forward_ad
+    z, W, table, pos = _draw((1, 4, 4, 64), F32, 1), _draw((4, 64), F32, 2), _draw((65, 4), F32, 3), torch.arange(4, device=DEV)
+    base = _draw((1, 1, 4, 4, 4), F32, 4)
+    calls = ((evo.layer_norm, [z, z[0, 0, 0], z[0, 0, 1]], {}), (evo.pair_bias_projection, [z, W, z[0, 0, 0], z[0, 0, 1]], {}),
+             (lambda t, p: evo.relative_position_bias(t, pos, max_distance=32, pair_bias=p), [table, base], {}))
+    for fn, args, kw in calls:
+        for i in range(len(args)):
+            for grads in (False, True):
+                with forward_ad.dual_level(), torch.set_grad_enabled(grads):
+                    a = list(args)
+                    a[i] = forward_ad.make_dual(a[i], torch.ones_like(a[i]))
+                    with pytest.raises(RuntimeError, match="forward mode"):
+                        fn(*a, **kw)
+        fn(*args, **kw)
+        # the gradient of a result, asked for with a gradient that has a derivative itself
+        leaf = args[0].clone().requires_grad_()
+        out = fn(leaf, *args[1:], **kw)
+        with forward_ad.dual_level():
+            d = forward_ad.make_dual(torch.ones_like(out), torch.ones_like(out))
+            with pytest.raises(RuntimeError, match="forward mode"):
+                torch.autograd.grad(out, leaf, d, retain_graph=True)
+        torch.autograd.grad(out, leaf, torch.ones_like(out))
