@@ -301,6 +301,7 @@ template <class T, int KC, bool KEEP, int VEC_>
 struct Tile {
   static constexpr int VEC = VEC_;
   static constexpr int kUnroll = KEEP ? KC : 1;
+  static_assert(KC % 2 == 0, "statistics() takes two times 32 channels at once");
   Eight<T> x[2][KEEP ? KC : 1];
   const T* at[2];
   bool on[2];
@@ -353,8 +354,11 @@ struct Tile {
     }
   }
   // In 16-bit types both sums come from MMAs: with a column of ones, and the diagonal of rows x rows (the registers of the A
-  // operand are those of its transpose as B).  The variance is then a difference, good to 2^-22 where the mean is
-  // at most twice the deviation; other rows are done the other way.
+  // operand are those of its transpose as B).  The variance is then a difference: where the mean is at most twice the deviation, five
+  // times as far off, relative to it, as the mean square is; other rows are done the other way.  What MMAs cut off always makes a
+  // sum of squares smaller, so a sum is of four (64 channels), 2.5 * 2^-23 of it at most, and these are added in fp32.  One sum over all
+  // channels had r up to 3.8e-6 too large (512 channels, fp16), these 2.6e-7; 32 channels a sum cost registers: forward of
+  // [2,768,768,128] to 8 heads, bf16, 72 -> 78 us, backward 144 -> 154.
   __device__ __forceinline__ void statistics(const ProjArgs& a) {
     if constexpr (sizeof(T) == 4) {
       about_the_mean(a);
@@ -365,25 +369,34 @@ struct Tile {
         if constexpr (bf) mma_k16(d, a0, a1, a2, a3, b0, b1);
         else mma_k16_f16(d, a0, a1, a2, a3, b0, b1);
       };
-      float sum[4] = {}, lo[4] = {}, hi[4] = {};
-#pragma unroll kUnroll
-      for (int c = 0; c < KC; ++c) {
-        const uint4 l = get(a, 0, c).w[0], h = get(a, 1, c).w[0];
-        mma(sum, l.x, h.x, l.y, h.y, ones, ones);
-        mma(lo, l.x, h.x, l.y, h.y, l.x, l.y);
-        mma(hi, l.x, h.x, l.y, h.y, h.x, h.y);
-        mma(sum, l.z, h.z, l.w, h.w, ones, ones);
-        mma(lo, l.z, h.z, l.w, h.w, l.z, l.w);
-        mma(hi, l.z, h.z, l.w, h.w, h.z, h.w);
-      }
       const float by_C = 1.f / a.C;
       const int lane = threadIdx.x & 31, g = lane >> 2, diagonal = (lane & ~3) | (g >> 1);
-      const float square[2] = {__shfl_sync(0xffffffffu, g & 1 ? lo[1] : lo[0], diagonal), __shfl_sync(0xffffffffu, g & 1 ? hi[3] : hi[2], diagonal)};
+      float total[2] = {}, square[2] = {};
+#pragma unroll kUnroll
+      for (int c0 = 0; c0 < KC; c0 += 2) {
+        float sum[4] = {}, lo[4] = {}, hi[4] = {};
+#pragma unroll
+        for (int c = c0; c < c0 + 2; ++c) {
+          const uint4 l = get(a, 0, c).w[0], h = get(a, 1, c).w[0];
+          mma(sum, l.x, h.x, l.y, h.y, ones, ones);
+          mma(lo, l.x, h.x, l.y, h.y, l.x, l.y);
+          mma(hi, l.x, h.x, l.y, h.y, h.x, h.y);
+          mma(sum, l.z, h.z, l.w, h.w, ones, ones);
+          mma(lo, l.z, h.z, l.w, h.w, l.z, l.w);
+          mma(hi, l.z, h.z, l.w, h.w, h.z, h.w);
+        }
+        total[0] += sum[0];
+        total[1] += sum[2];
+        square[0] += g & 1 ? lo[1] : lo[0];  // (on the diagonal in one of the row's four lanes)
+        square[1] += g & 1 ? hi[3] : hi[2];
+      }
+#pragma unroll
+      for (int k = 0; k < 2; ++k) square[k] = __shfl_sync(0xffffffffu, square[k], diagonal);
       float quick_mean[2], quick_r[2];
       bool fine[2];
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
-        quick_mean[k] = sum[2 * k] * by_C;
+        quick_mean[k] = total[k] * by_C;
         const float var = fmaf(-quick_mean[k], quick_mean[k], square[k] * by_C);
         fine[k] = quick_mean[k] * quick_mean[k] <= 4.f * var;
         quick_r[k] = on[k] ? rsqrtf(var + a.eps) : 0.f;
@@ -742,8 +755,10 @@ template <class T>
 __host__ __device__ constexpr bool both_layouts(int KC, int NT, bool keep) { return keep && KC * NT * Pieces<T>::kG <= 192; }
 
 // More channels and heads than one block can hold the sums of: dz and the rows' statistics in one kernel ...
+// Up to 16 heads of 512 channels the compiler would otherwise spill for a fourth block an SM: backward of [1,768,768,512] to 16, bf16, 739 us
+// with three, 830 with four.
 template <class T, int KC, int NT, bool KEEP, int VEC>
-__global__ void __launch_bounds__(256) projection_dz(ProjArgs a) {
+__global__ void __launch_bounds__(256, sizeof(T) == 2 && KC == 16 && NT == 2 && VEC == 8 ? 3 : 0) projection_dz(ProjArgs a) {
   ptx::grid_dependency_wait();
   ptx::grid_launch_dependents();
   constexpr bool kBoth = both_layouts<T>(KC, NT, KEEP);

@@ -89,3 +89,23 @@ def test_forward_derivatives_are_refused():
             with pytest.raises(RuntimeError, match="forward mode"):
                 torch.autograd.grad(out, leaf, d, retain_graph=True)
         torch.autograd.grad(out, leaf, torch.ones_like(out))
+
+
+@pytest.mark.parametrize("dtype", [BF, HF], ids=["bf16", "fp16"])
+@pytest.mark.parametrize("C_,H", [(128, 8), (256, 8), (256, 16), (512, 8), (500, 16)], ids=str)
+def test_spread_of_rows_off_zero_does_not_lean(C_, H, dtype):
+    """Rows whose mean is 1.9 deviations, and the sum of an fp32 gain's gradient, all of whose terms (a row's d . out) are positive. A
+    rounding goes either way and averages out over 2 304 rows and C channels; what is cut off does not.  An MMA cuts off less
+    than a unit of its sum, half of one on average; of 64 channels, four MMAs at 1/4, 2/4, 3/4 and the whole of the sum of squares cut
+    off 2.5 * 2^-24 of it.  The variance is 1 / 4.61 of the mean square, r half as far off as it: 2.5 * 2^-24 * 4.61 / 2 = 3.5e-7.
+    The MMA of the sums over rows cuts off less than a unit again, 1.2e-7.  (One chain over 512 channels: 3.8e-6.)"""
+    import evoformer_triton_b200 as evo
+    R = 48
+    z = _draw((1, R, R, C_), dtype, 1, 1.0, 1.9)
+    W = _draw((H, C_), F32, 2, C_ ** -0.5).requires_grad_()
+    g = torch.ones(C_, device=DEV, requires_grad=True)
+    out = evo.pair_bias_projection(z, W, g)
+    d = out.detach()
+    dg, = torch.autograd.grad(out, g, d)
+    want = oc.pair_projection(z, W.detach(), g.detach(), None, 1e-5, d)[3][0]
+    assert abs(float(dg.double().sum() / want.sum()) - 1) < 5.4e-7
