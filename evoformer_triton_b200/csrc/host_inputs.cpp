@@ -35,6 +35,11 @@ void check_weight(const Tensor& w, const Tensor& t, const char* name, at::IntArr
     value_error(s + "]");
   }
 }
+// Sizes are 32-bit in the C ABI: a view of many times the same values may have more along an axis.
+void check_sizes(at::IntArrayRef sizes, int64_t most, const char* text) {
+  for (const int64_t n : sizes)
+    if (n > most) value_error(text);
+}
 float checked_eps(double eps) {
   if (!(eps >= 0.0) || std::isinf(eps)) value_error("eps must be a finite number that is not negative");
   return (float)eps;
@@ -315,6 +320,7 @@ Tensor relative_position_bias(const Tensor& table, const Tensor& q, const Maybe&
       value_error("pair_bias must have the shape [B, 1, H, N, N_keys] of the positions and the table");
     B = t.size(0);
   }
+  check_sizes({B, H, Rq, Rk}, 1 << 23, "relative_position_bias takes up to 2^23 entries along an axis");
   const at::ScalarType type = dtype ? *dtype : base ? base->scalar_type() : table.scalar_type();
   if (!known(type)) type_error("dtype must be bfloat16, float16 or float32");
   const RelativePlan plan{scheme, exact, table.size(0), std::move(edges)};
@@ -396,6 +402,7 @@ Tensor pair_bias_projection(const Tensor& pair, const Tensor& weight, const Mayb
   check_weight(weight, pair, "weight", {weight.size(0), C});
   if (C > EVOATTN_PROJECTION_MAX_C || weight.size(0) > EVOATTN_PROJECTION_MAX_H)
     value_error("pair_bias_projection takes up to " + std::to_string(EVOATTN_PROJECTION_MAX_C) + " channels and " + std::to_string(EVOATTN_PROJECTION_MAX_H) + " heads");
+  check_sizes(pair.sizes(), 1 << 20, "pair may have up to 2^20 entries along an axis");
   if (norm_weight) check_weight(*norm_weight, pair, "norm_weight", {C});
   if (norm_bias) check_weight(*norm_bias, pair, "norm_bias", {C});
   const float e = checked_eps(eps);

@@ -109,3 +109,22 @@ def test_spread_of_rows_off_zero_does_not_lean(C_, H, dtype):
     dg, = torch.autograd.grad(out, g, d)
     want = oc.pair_projection(z, W.detach(), g.detach(), None, 1e-5, d)[3][0]
     assert abs(float(dg.double().sum() / want.sum()) - 1) < 5.4e-7
+
+
+# ---------------------------------------------------------------- sizes that no counter holds
+
+def test_sizes_beyond_the_counters_are_refused():
+    """Views of one value: 2^32 + 1 of them along an axis are not one."""
+    import evoformer_triton_b200 as evo
+    far = 2 ** 32 + 1
+    pos, W, table = torch.zeros(1, dtype=torch.int64, device=DEV), _draw((2, 8), F32, 1), _draw((65, 2), F32, 2)
+    for bad in (lambda: evo.pair_bias_projection(torch.zeros(1, 1, 1, 8, device=DEV).expand(far, 1, 1, 8), W),
+                lambda: evo.pair_bias_projection(torch.zeros(1, 1, 1, 8, device=DEV).expand(1, far, 1, 8), W),
+                lambda: evo.pair_bias_projection(torch.zeros(1, 1, 1, 8, device=DEV).expand(1, 1, far, 8), W),
+                lambda: evo.relative_position_bias(table, pos.expand(far), pos, max_distance=32),
+                lambda: evo.relative_position_bias(table, pos, pos.expand(far), max_distance=32),
+                lambda: evo.relative_position_bias(table, pos[None].expand(far, 1), pos, max_distance=32),
+                lambda: evo.relative_position_bias(table[:, :1].expand(65, far), pos, max_distance=32),
+                lambda: evo.relative_position_bias(table, pos, max_distance=32, pair_bias=torch.zeros(1, 1, 2, 1, 1, device=DEV).expand(far, 1, 2, 1, 1))):
+        with pytest.raises(ValueError):
+            bad()
