@@ -488,7 +488,6 @@ int validate(const evoattn_relative_bias_params* p) {
   for (int i = 0; i < p->n_edges; ++i)  // a distance finds its bucket by bisection
     if (p->edges[i] < p->exact || p->edges[i] > kFarthest || (i && p->edges[i] < p->edges[i - 1])) return EVOATTN_ERR_SHAPE;
   const int most = p->exact + p->n_edges;  // the largest f
-  if (p->scheme != EVOATTN_BUCKETS_CLIP && most > 255) return EVOATTN_ERR_SHAPE;  // (kept in bytes)
   switch (p->scheme) {
     case EVOATTN_BUCKETS_CLIP: return p->n_edges == 0 && p->buckets == 2 * p->exact + 1 ? EVOATTN_OK : EVOATTN_ERR_SHAPE;
     case EVOATTN_BUCKETS_LOG: return p->buckets % 2 == 0 && most < p->buckets / 2 ? EVOATTN_OK : EVOATTN_ERR_SHAPE;

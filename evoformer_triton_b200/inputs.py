@@ -17,7 +17,7 @@ from . import _lib
 
 _SCHEMES = {"clip": 0, "log": 1, "log_causal": 2}
 MAX_BUCKETS = 1024
-MAX_LOG_BUCKETS = 256
+MAX_LOG_BUCKETS = 256  # (causal ones have 127 borders, which are handed over with every launch)
 
 
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,

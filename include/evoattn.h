@@ -289,8 +289,8 @@ int evoattn_layer_norm_bwd(const evoattn_layer_norm_params* p, void* cuda_stream
  *   CLIP        row = exact - f where the key follows the query, exact + f elsewhere; no edges (table rows: 2 exact + 1)
  *   LOG         row = f, plus half of the table's rows where the key follows the query
  *   LOG_CAUSAL  row = f of the distance back, 0 where the key follows the query
- * exact + n_edges is at most 255 for the last two, and no edge lies beyond 2^28.  Positions are 32- or 64-bit whole
- * numbers whose differences fit 64 bits.  Rq and Rk up to 2^23. */
+ * f has to be a row of the table (LOG: of half of it) for every distance; no edge lies below `exact` or beyond
+ * 2^28.  Positions are 32- or 64-bit whole numbers whose differences fit 64 bits.  Rq and Rk up to 2^23. */
 enum { EVOATTN_BUCKETS_CLIP = 0, EVOATTN_BUCKETS_LOG = 1, EVOATTN_BUCKETS_LOG_CAUSAL = 2 };
 #define EVOATTN_MAX_BUCKETS 1024
 #define EVOATTN_MAX_BUCKET_EDGES 128

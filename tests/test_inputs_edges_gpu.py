@@ -1,4 +1,6 @@
 """GPU: the operators before the attention at the edges of what they take."""
+import ctypes as C
+
 import pytest
 import torch
 
@@ -128,3 +130,34 @@ def test_sizes_beyond_the_counters_are_refused():
                 lambda: evo.relative_position_bias(table, pos, max_distance=32, pair_bias=torch.zeros(1, 1, 2, 1, 1, device=DEV).expand(far, 1, 2, 1, 1))):
         with pytest.raises(ValueError):
             bad()
+
+
+@pytest.mark.parametrize("scheme,exact,edges,buckets", [(2, 300, list(range(310, 1010, 50)), 400), (1, 260, [270, 700, 3000], 900), (2, 1000, [], 1024)], ids=str)
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "fp32"])
+def test_many_distances_with_a_bucket_of_their_own(scheme, exact, edges, buckets, dtype):
+    """More than a byte counts, through the C ABI: the forward to the bit, the gradient of ones exactly."""
+    from evoformer_triton_b200 import _lib
+    lib = _lib.load()
+    Rq, Rk = 7, 1201
+    q, k = torch.tensor([0, 1, 900, 1800, 2400, 2399, 1200], device=DEV), torch.arange(0, 2 * Rk, 2, device=DEV)
+    rel = k[None] - q[:, None]
+    a = rel.abs()
+    f = torch.where(a < exact, a, exact + torch.bucketize(a, torch.tensor(edges, dtype=torch.int64, device=DEV), right=True))
+    rows = torch.where(rel > 0, 0 * f, f) if scheme == 2 else f + (rel > 0) * (buckets // 2)
+    table = _draw((buckets, 1), F32, 1)
+    out = torch.empty((1, 1, Rq, Rk), dtype=dtype, device=DEV)
+    strides = (C.c_int64 * 3)(Rq * Rk, Rq * Rk, Rk)
+    code = 0 if dtype == BF else 2
+    p = _lib.RelativeBiasParams(table_dtype=2, dtype=code, B=1, H=1, Rq=Rq, Rk=Rk, buckets=buckets, scheme=scheme, exact=exact, n_edges=len(edges), positions64=1,
+                                edges=(C.c_int32 * max(1, len(edges)))(*edges), table=table.data_ptr(), q_pos=q.data_ptr(), k_pos=k.data_ptr(),
+                                out=out.data_ptr(), out_stride=strides)
+    stream = C.c_void_p(torch.cuda.current_stream().cuda_stream)
+    assert lib.evoattn_relative_bias_fwd(C.byref(p), stream) == 0
+    assert torch.equal(out[0, 0], table[rows, 0].to(dtype))
+    d, dtable = torch.ones_like(out), torch.empty_like(table)
+    p.d_out, p.d_out_stride, p.dtable = d.data_ptr(), strides, dtable.data_ptr()
+    need = lib.evoattn_relative_bias_bwd_workspace_bytes(C.byref(p))
+    ws = torch.empty(need, dtype=torch.uint8, device=DEV)
+    p.workspace, p.workspace_bytes = ws.data_ptr(), need
+    assert lib.evoattn_relative_bias_bwd(C.byref(p), stream) == 0
+    assert torch.equal(dtable[:, 0], torch.bincount(rows.reshape(-1), minlength=buckets).to(F32))
