@@ -161,3 +161,28 @@ def test_many_distances_with_a_bucket_of_their_own(scheme, exact, edges, buckets
     p.workspace, p.workspace_bytes = ws.data_ptr(), need
     assert lib.evoattn_relative_bias_bwd(C.byref(p), stream) == 0
     assert torch.equal(dtable[:, 0], torch.bincount(rows.reshape(-1), minlength=buckets).to(F32))
+
+
+def test_layer_norm_leaves_what_is_not_wanted():
+    """Through the C ABI: with no place for a gradient given, the others are written and nothing beside them."""
+    from evoformer_triton_b200 import _lib
+    lib = _lib.load()
+    N, C_ = 70, 96
+    x, dy, w = _draw((N, C_), BF, 1), _draw((N, C_), BF, 2), _draw((C_,), F32, 3)
+    h, r = oc.normalise(x.double(), 1e-5)
+    stats = torch.stack([x.double().mean(-1), r[:, 0]], 1).float()
+    want = oc.layer_norm(x, w, w, 1e-5, dy)
+    for names in (("dx",), ("dweight",), ("dbias",), ("dx", "dbias"), ("dweight", "dbias")):
+        got = {"dx": torch.full((N + 2, C_), 7.0, dtype=BF, device=DEV), "dweight": torch.full((3, C_), 7.0, device=DEV), "dbias": torch.full((3, C_), 7.0, device=DEV)}
+        p = _lib.LayerNormParams(dtype=0, weight_dtype=2, bias_dtype=2, eps=1e-5, n=(1, 1, N), C=C_, x=x.data_ptr(), x_stride=(0, 0, C_), weight=w.data_ptr(), bias=w.data_ptr(),
+                                 stats=stats.data_ptr(), d_y=dy.data_ptr(), d_y_stride=(0, 0, C_), **{n: got[n][1].data_ptr() for n in names})
+        need = lib.evoattn_layer_norm_bwd_workspace_bytes(C.byref(p))
+        ws = torch.empty(max(need, 1), dtype=torch.uint8, device=DEV)
+        p.workspace, p.workspace_bytes = ws.data_ptr(), need
+        assert lib.evoattn_layer_norm_bwd(C.byref(p), C.c_void_p(torch.cuda.current_stream().cuda_stream)) == 0
+        for k, (n, t) in enumerate(got.items()):
+            if n not in names:
+                assert (t == 7.0).all(), n
+                continue
+            assert (t[0] == 7.0).all() and (t[-1] == 7.0).all()
+            oc.check(n, t[1:-1] if n == "dx" else t[1], want[1 + k])
