@@ -7,8 +7,10 @@
 //   dz = r (u - mean(u) - xh mean(u xh))
 //   dweight[h,c] = g[c] M[h,c] + b[c] s[h],  dg[c] = sum_h weight[h,c] M[h,c],  db[c] = sum_h weight[h,c] s[h]
 //
-// so the gradients of all three weights come from sums that do not depend on them.  Bound by memory forward, by issue slots
-// and registers backward: [2,768,768,128] to 8 heads, bf16, 67 us (4.8 TB/s) and 137 (4.5 TB/s) on a card whose copies run at 6.5.
+// so the gradients of all three weights come from sums that do not depend on them.  [2,768,768,128] to 8 heads, bf16: 67 us (4.8 TB/s)
+// and 144 (4.3 TB/s) on a card whose copies run at 6.5.  What is short is warps that cover the latency of loads and of one
+// MMA after another, for want of registers: 22 of 64 warps an SM forward, with 58 % of DRAM and 59 % of the issue slots busy, and 16 of 64
+// backward, with 49 and 55 %.
 #include <string.h>
 
 #include <type_traits>

@@ -5,8 +5,10 @@
 // Memory bound both ways: one write (and one read of the base) of B H Rq Rk values, one read of them.  A warp
 // walks rows of a strip of keys whose positions stay in registers, so the bucket of a score is worked out
 // once for all heads (forward), or not at all where a whole strip falls into one bucket, as it does away from
-// the diagonal.  [2,16,2048,2048] bf16, 32 logarithmic buckets: forward 48 us (5.5 TB/s), backward 76 (3.5 TB/s; its items
-// without their data are 21 of them: positions to read, buckets to find).
+// the diagonal.  [2,16,2048,2048] bf16, 32 logarithmic buckets: forward 47 us (5.7 TB/s), backward 82 (3.3 TB/s; its items
+// without their data are 27 of them: positions to read, buckets to find).  Far from memory's time: tables of more than 128 rows in the
+// backward (a pass per 128: [1,16,2048,2048] bf16, 601 rows, 193 us for 20), rows of the gradient off 16 bytes
+// ([1,8,2047,2047] bf16 43 us for 10) and an added bias forward ([1,8,2048,2048] bf16 39 us for 20).
 #include <string.h>
 
 #include "inputs.cuh"

@@ -58,7 +58,8 @@ def relative_position_bias(table: torch.Tensor, positions: torch.Tensor, key_pos
     """A pair bias ``[B, 1, H, N, N_keys]`` looked up in ``table`` (``[n, H]``) by the distance of two residues.
 
     ``positions`` are the residue numbers (int64 or int32) ``[N]``, or ``[B, N]`` where they differ over the batch;
-    ``key_positions`` those of the keys where they are not the same, as for a single new query.  With ``[N]`` the
+    ``key_positions`` those of the keys where they are not the same, for an attention that has them (the one of this
+    package has the queries' residues as keys).  With ``[N]`` the
     result has B = 1: ``expand`` it, the attention reads it in place.  ``buckets``:
 
     * ``"clip"``: ``clamp(position - key_position, -max_distance, max_distance) + max_distance``; n = 2 max_distance + 1.
@@ -96,5 +97,8 @@ def pair_bias_projection(pair: torch.Tensor, weight: torch.Tensor, norm_weight: 
 
     ``weight`` is ``[H, C]`` as a linear layer holds it; all weights may be of another type than ``pair``.  ``pair`` may be
     strided with its C values contiguous (``pair.transpose(1, 2)`` around ending nodes).  C up to 512, H up to 64.
+    Where ``pair`` has 16 bits, ``weight * norm_weight`` enters the products with 16 bits (bfloat16; 22 in the forward of
+    float16), fp32 weights too: a result is off by up to 2 ** -16 of the sum of its terms' magnitudes beside its rounding.
+    The gradients of the weights are fp32 sums of fp32 factors.
     Rows of the result begin on 16-byte boundaries, so the attention takes it as it is for any N_res."""
     return _lib.host().pair_bias_projection(pair, weight, norm_weight, norm_bias, eps)
