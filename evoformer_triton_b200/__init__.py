@@ -9,11 +9,15 @@ Public surface:
     layer_norm                    layer norm with its backward, rows read where they lie
     relative_position_bias        a learned pair bias by buckets of residue distance
     pair_bias_projection          the pair representation, normalised and projected to a pair bias in one pass
+    rotary_embedding              q and k turned by their positions; rotary_frequencies: of what, scaled for long contexts
+    packed_attention              attention over packed sequences with grouped heads, causal or both ways
 """
 from .attention import (EvoformerAttention, EvoformerAttentionTrueLayout, GatedEvoformerAttention,
                         check_device_status, evoformer_attention, force_generic)
 from .inputs import layer_norm, pair_bias_projection, relative_position_bias
+from .sequences import packed_attention, rotary_embedding, rotary_frequencies
 
 __all__ = ["EvoformerAttention", "EvoformerAttentionTrueLayout", "GatedEvoformerAttention",
            "evoformer_attention", "check_device_status", "force_generic",
-           "layer_norm", "relative_position_bias", "pair_bias_projection"]
+           "layer_norm", "relative_position_bias", "pair_bias_projection",
+           "rotary_embedding", "rotary_frequencies", "packed_attention"]

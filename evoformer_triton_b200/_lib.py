@@ -24,6 +24,7 @@ SYMBOLS = (
     "evoattn_layer_norm_fwd", "evoattn_layer_norm_bwd_workspace_bytes", "evoattn_layer_norm_bwd",
     "evoattn_relative_bias_fwd", "evoattn_relative_bias_bwd_workspace_bytes", "evoattn_relative_bias_bwd",
     "evoattn_pair_projection_fwd", "evoattn_pair_projection_bwd_workspace_bytes", "evoattn_pair_projection_bwd",
+    "evoattn_rotary", "evoattn_packed_fwd_workspace_bytes", "evoattn_packed_fwd", "evoattn_packed_bwd_workspace_bytes", "evoattn_packed_bwd",
 )
 STATIC_SCRATCH_BYTES = 64 << 20
 
@@ -110,6 +111,30 @@ class PairProjectionParams(C.Structure):
     ]
 
 
+class RotaryParams(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int32), ("layout", C.c_int32), ("inverse", C.c_int32), ("positions64", C.c_int32), ("frequencies64", C.c_int32),
+        ("amplitude", C.c_float), ("n", C.c_int64 * 3),
+        ("H", C.c_int32), ("Hk", C.c_int32), ("D", C.c_int32), ("rotary", C.c_int32),
+        ("q", C.c_void_p), ("q_stride", C.c_int64 * 4), ("k", C.c_void_p), ("k_stride", C.c_int64 * 4),
+        ("q_out", C.c_void_p), ("k_out", C.c_void_p),
+        ("positions", C.c_void_p), ("position_stride", C.c_int64 * 3), ("frequencies", C.c_void_p),
+    ]
+
+
+class PackedParams(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int32), ("B", C.c_int32), ("H", C.c_int32), ("Hk", C.c_int32), ("D", C.c_int32),
+        ("causal", C.c_int32), ("offsets64", C.c_int32), ("key_form", C.c_int32), ("flags", C.c_uint32), ("scale", C.c_float),
+        ("Tq", C.c_int64), ("Tk", C.c_int64),
+        ("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p),
+        ("q_stride", C.c_int64 * 2), ("k_stride", C.c_int64 * 2), ("v_stride", C.c_int64 * 2),
+        ("offsets", C.c_void_p), ("key_offsets", C.c_void_p), ("o", C.c_void_p), ("lse", C.c_void_p), ("status", C.c_void_p),
+        ("d_o", C.c_void_p), ("do_stride", C.c_int64 * 2), ("dq", C.c_void_p), ("dk", C.c_void_p), ("dv", C.c_void_p),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+    ]
+
+
 _lib = None
 _lock = threading.Lock()
 
@@ -166,6 +191,15 @@ def load() -> C.CDLL:
                 fn = getattr(lib, f"evoattn_{name}_{part}")
                 fn.restype = result
                 fn.argtypes = [C.POINTER(params)] + ([] if result is C.c_size_t else [C.c_void_p])
+        lib.evoattn_rotary.restype = C.c_int
+        lib.evoattn_rotary.argtypes = [C.POINTER(RotaryParams), C.c_void_p]
+        for part in ("fwd", "bwd"):
+            fn = getattr(lib, f"evoattn_packed_{part}")
+            fn.restype = C.c_int
+            fn.argtypes = [C.POINTER(PackedParams), C.c_void_p]
+            fn = getattr(lib, f"evoattn_packed_{part}_workspace_bytes")
+            fn.restype = C.c_size_t
+            fn.argtypes = [C.POINTER(PackedParams)]
         if lib.evoattn_abi_version() != ABI_VERSION:
             raise RuntimeError("libevoattn.so ABI version mismatch; rebuild it")
         _lib = lib

@@ -12,10 +12,17 @@ thread_local int g_last_path = EVOATTN_PATH_NONE;
 thread_local int g_last_launches = 0;
 thread_local int g_ctx_bound_device = -1;
 
+}  // namespace
+
+void evo::note_call(int path, int launches) {
+  g_last_path = path;
+  g_last_launches = launches;
+}
+
 // Tensor maps are encoded through the driver API, which needs the device's primary context
 // to be current on the calling thread.  A thread that has made no runtime call yet (PyTorch's
 // autograd worker on its first backward) gets it bound here, once per thread and device.
-void bind_context_once() {
+void evo::bind_context_once() {
   int dev = -1;
   if (cudaGetDevice(&dev) != cudaSuccess) return;
   if (g_ctx_bound_device != dev) {
@@ -23,6 +30,10 @@ void bind_context_once() {
     g_ctx_bound_device = dev;
   }
 }
+
+namespace {
+
+using evo::bind_context_once;
 
 bool stride_ok16(const int64_t* s, int esize) {
   for (int i = 0; i < 4; ++i)

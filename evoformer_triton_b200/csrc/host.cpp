@@ -9,11 +9,6 @@
 // head layout or the true one, None for mask and bias, additive or boolean masks, gating, both bias
 // layouts.  The N_seq-sharded op, which exchanges d(pair_bias) in its backward, and a call that is being
 // traced stay in Python and take their checks and the preparation of their inputs from here.
-#include <ATen/cuda/CUDAContext.h>
-#include <c10/cuda/CUDAGuard.h>
-#include <torch/csrc/jit/frontend/tracer.h>
-#include <torch/extension.h>
-
 #include <atomic>
 #include <mutex>
 
@@ -34,7 +29,9 @@ std::mutex g_status_mutex;
 std::atomic<int32_t*> g_status_ptr[kMaxDevices];
 Tensor* g_status[kMaxDevices] = {};  // (never destroyed: the CUDA context may be gone before they would be)
 
-int32_t* status_ptr(c10::Device dev) {
+}  // namespace
+
+int32_t* evohost::status_ptr(c10::Device dev) {
   const int i = dev.index();
   TORCH_CHECK(i >= 0 && i < kMaxDevices, "device index out of range");
   if (int32_t* p = g_status_ptr[i].load(std::memory_order_acquire)) return p;
@@ -45,6 +42,14 @@ int32_t* status_ptr(c10::Device dev) {
   }
   return g_status_ptr[i].load(std::memory_order_acquire);
 }
+bool evohost::generic_forced() { return g_force_generic.load(std::memory_order_relaxed) != 0; }
+void evohost::note_call(bool bwd) {
+  (bwd ? g_bwd_launches : g_fwd_launches) = evoattn_last_launch_count();
+  (bwd ? g_bwd_path : g_fwd_path) = evoattn_last_path();
+}
+
+namespace {
+
 Tensor status_word(int64_t index) {
   status_ptr(c10::Device(c10::kCUDA, static_cast<c10::DeviceIndex>(index)));
   return *g_status[index];
@@ -305,4 +310,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("note_bwd", [](int launches, int path) { g_bwd_launches = launches; g_bwd_path = path; });
   m.def("abi_version", [] { return evoattn_abi_version(); });
   evohost::register_inputs(m);
+  evohost::register_sequences(m);
 }

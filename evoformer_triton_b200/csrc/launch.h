@@ -93,6 +93,11 @@ bool exchange_lane(cudaStream_t* side, cudaEvent_t* fork, cudaEvent_t* join);
 // d(pair_bias) from the fp32 buffer it was summed in to a.dbias_out, in its type and layout (extras.cu).
 int launch_dbias_out(const Args& a, cudaStream_t st, int* launches);
 
+// Records what evoattn_last_path() and evoattn_last_launch_count() report on this thread; binds the device's primary
+// context to a thread that has none (api.cu).
+void note_call(int path, int launches);
+void bind_context_once();
+
 // From here on `a` reads the effective dO of a gated output (contiguous, in scratch).
 inline void use_effective_d_o(Args* a) {
   a->d_o = a->d_o_eff;

@@ -1,0 +1,83 @@
+// Attention over packed sequences: what a request has to hold, and which kernels serve it.
+#include "packed.cuh"
+
+namespace evo {
+namespace {
+
+constexpr long long kMaxRows = 1LL << 30;
+
+int validate(const evoattn_packed_params* p, bool bwd) {
+  if (!p || !p->q || !p->k || !p->v || !p->offsets || !p->o) return EVOATTN_ERR_NULL;
+  if (!known_dtype(p->dtype)) return EVOATTN_ERR_DTYPE;
+  if (p->B < 1 || p->H < 1 || p->Hk < 1 || p->H % p->Hk || p->H > 65535 || p->D < 1) return EVOATTN_ERR_SHAPE;
+  if (p->Tq < 1 || p->Tk < 1 || p->Tq > kMaxRows || p->Tk > kMaxRows || p->B > kMaxRows || p->Tq * p->H > 8 * kMaxRows) return EVOATTN_ERR_SHAPE;
+  if (p->D > EVOATTN_PACKED_MAX_D) return EVOATTN_ERR_UNSUPPORTED;
+  if (p->key_form != EVOATTN_PACKED_KEY_OFFSETS && p->key_form != EVOATTN_PACKED_KEY_RANGES) return EVOATTN_ERR_DTYPE;
+  if (p->key_form == EVOATTN_PACKED_KEY_RANGES && !p->key_offsets) return EVOATTN_ERR_NULL;
+  if (!(p->scale - p->scale == 0.f)) return EVOATTN_ERR_SHAPE;  // (NaN or infinite)
+  if (!bwd) return EVOATTN_OK;
+  if (!p->lse || !p->d_o || !p->dk != !p->dv) return EVOATTN_ERR_NULL;
+  if (p->dk && p->key_form != EVOATTN_PACKED_KEY_OFFSETS) return EVOATTN_ERR_UNSUPPORTED;
+  return EVOATTN_OK;
+}
+
+PackedArgs arguments(const evoattn_packed_params* p) {
+  PackedArgs a{};
+  a.q = p->q; a.k = p->k; a.v = p->v; a.o = p->o; a.lse = p->lse;
+  a.d_o = p->d_o; a.dq = p->dq; a.dk = p->dk; a.dv = p->dv;
+  for (int i = 0; i < 2; ++i) a.sq[i] = p->q_stride[i], a.sk[i] = p->k_stride[i], a.sv[i] = p->v_stride[i], a.sdo[i] = p->do_stride[i];
+  a.offsets = p->offsets;
+  a.key_offsets = p->key_offsets ? p->key_offsets : p->offsets;
+  a.B = p->B; a.H = p->H; a.Hk = p->Hk; a.D = p->D; a.G = p->H / p->Hk;
+  a.causal = p->causal != 0; a.wide = p->offsets64 != 0; a.ranges = p->key_form == EVOATTN_PACKED_KEY_RANGES;
+  a.Tq = (int)p->Tq; a.Tk = (int)p->Tk; a.lse_ld = (int)p->Tq;
+  a.scale = p->scale;
+  a.status = p->status;
+  return a;
+}
+
+}  // namespace
+}  // namespace evo
+
+extern "C" {
+
+using namespace evo;
+
+size_t evoattn_packed_fwd_workspace_bytes(const evoattn_packed_params* p) {
+  return 0;
+}
+
+int evoattn_packed_fwd(const evoattn_packed_params* p, void* cuda_stream) {
+  const int rc = validate(p, false);
+  if (rc) return rc;
+  const PackedArgs a = arguments(p);
+  bind_context_once();
+  int launches = 0;
+  const int rl = launch_packed_generic_fwd(p->dtype, a, reinterpret_cast<cudaStream_t>(cuda_stream), &launches);
+  note_call(EVOATTN_PATH_GENERIC, launches);
+  return rl;
+}
+
+size_t evoattn_packed_bwd_workspace_bytes(const evoattn_packed_params* p) {
+  if (validate(p, true)) return 0;
+  return (size_t)p->H * p->Tq * sizeof(float);
+}
+
+int evoattn_packed_bwd(const evoattn_packed_params* p, void* cuda_stream) {
+  const int rc = validate(p, true);
+  if (rc) return rc;
+  const size_t need = evoattn_packed_bwd_workspace_bytes(p);
+  if (!p->workspace || p->workspace_bytes < need) return EVOATTN_ERR_WORKSPACE;
+  if ((uintptr_t)p->workspace & 255) return EVOATTN_ERR_ALIGN;
+  PackedArgs a = arguments(p);
+  a.delta = static_cast<float*>(p->workspace);
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(cuda_stream);
+  int launches = 0;
+  bind_context_once();
+  int rl = launch_packed_delta(p->dtype, a, st, &launches);
+  if (!rl) rl = launch_packed_generic_bwd(p->dtype, a, st, &launches);
+  note_call(EVOATTN_PATH_GENERIC, launches);
+  return rl;
+}
+
+}  // extern "C"

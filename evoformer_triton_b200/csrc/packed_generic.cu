@@ -1,0 +1,374 @@
+// Attention over packed sequences on CUDA cores, forward and backward: fp32, head dimensions that are not in eights or
+// above 128, and tensors off 16 bytes.  Everything in fp32.
+//
+//   o_i = sum_j p_ij v_j,  p_ij = exp(scale q_i k_j - lse_i) over the keys j of i's sequence (causal: j <= i + nk - nq)
+//   dv_j = sum_i p_ij do_i,  ds_ij = p_ij (do_i v_j - delta_i),  delta_i = do_i o_i,  dq_i = scale sum_j ds_ij k_j,
+//   dk_j = scale sum_i ds_ij q_i
+//
+// Tiles of TILE queries by TILE keys, 256 threads as 16 x 16, each with TILE / 16 rows and as many columns of the scores
+// and as many rows of every product.  Keys and queries of a thread are 16 apart, so that its rows of DP + 4 floats lie in
+// other banks than its neighbours'.  The backward is two kernels, one that walks the queries of a key tile (all heads of
+// the group in turn) and one that walks the keys of a query tile: the scores are formed twice, and no sum depends on the
+// order in which blocks run.
+#include <math.h>
+
+#include "packed.cuh"
+
+namespace evo {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr float kLog2e = 1.4426950408889634f;
+
+template <int DP>
+struct GenericCfg {
+  static constexpr int TILE = DP > 128 ? 32 : 64;  // (four tiles of 64 x 256 floats would not fit)
+  static constexpr int NR = TILE / 16, NC = DP / 64, LD = DP + 4, LP = TILE + 4;
+  static constexpr size_t bytes(int tiles, int scores) { return sizeof(float) * ((size_t)tiles * TILE * LD + (size_t)scores * TILE * LP + 2 * TILE); }
+};
+
+// Rows [0, n) of a tile into shared memory as floats, zeros beyond n and D.
+template <class T, int DP>
+__device__ __forceinline__ void load_rows(float* dst, const void* src, long long stride, int n, int D) {
+  constexpr int TILE = GenericCfg<DP>::TILE, LD = GenericCfg<DP>::LD;
+  const T* p = static_cast<const T*>(src);
+  for (int i = threadIdx.x; i < TILE * DP; i += kThreads) {
+    const int r = i / DP, d = i % DP;
+    dst[r * LD + d] = r < n && d < D ? to_float(p[r * stride + d]) : 0.f;
+  }
+}
+__device__ __forceinline__ float4 ld4(const float* p) { return *reinterpret_cast<const float4*>(p); }
+__device__ __forceinline__ float dot4(float4 a, float4 b, float s) { return fmaf(a.x, b.x, fmaf(a.y, b.y, fmaf(a.z, b.z, fmaf(a.w, b.w, s)))); }
+
+// s[r][c] = row (ty + 16 r) of x times row (tx + 16 c) of y.
+template <int DP>
+__device__ __forceinline__ void products(const float* x, const float* y, int ty, int tx, float (&s)[GenericCfg<DP>::NR][GenericCfg<DP>::NR]) {
+  constexpr int NR = GenericCfg<DP>::NR, LD = GenericCfg<DP>::LD;
+#pragma unroll
+  for (int r = 0; r < NR; ++r)
+#pragma unroll
+    for (int c = 0; c < NR; ++c) s[r][c] = 0.f;
+#pragma unroll 4
+  for (int d = 0; d < DP; d += 4) {
+    float4 u[NR], w[NR];
+#pragma unroll
+    for (int r = 0; r < NR; ++r) u[r] = ld4(x + (ty + 16 * r) * LD + d);
+#pragma unroll
+    for (int c = 0; c < NR; ++c) w[c] = ld4(y + (tx + 16 * c) * LD + d);
+#pragma unroll
+    for (int r = 0; r < NR; ++r)
+#pragma unroll
+      for (int c = 0; c < NR; ++c) s[r][c] = dot4(u[r], w[c], s[r][c]);
+  }
+}
+// acc[r][.] += sum_j p(row ty + 16 r, j) * y[j][4 tx + 64 c ..]; p as [row][j] (ROWS) or [j][row].
+template <int DP, bool ROWS>
+__device__ __forceinline__ void accumulate(const float* p, const float* y, int ty, int tx, float4 (&acc)[GenericCfg<DP>::NR][GenericCfg<DP>::NC]) {
+  using C = GenericCfg<DP>;
+#pragma unroll 4
+  for (int j = 0; j < C::TILE; ++j) {
+    float w[C::NR];
+#pragma unroll
+    for (int r = 0; r < C::NR; ++r) w[r] = ROWS ? p[(ty + 16 * r) * C::LP + j] : p[j * C::LP + ty + 16 * r];
+#pragma unroll
+    for (int c = 0; c < C::NC; ++c) {
+      const float4 v = ld4(y + j * C::LD + 4 * tx + 64 * c);
+#pragma unroll
+      for (int r = 0; r < C::NR; ++r) {
+        acc[r][c].x = fmaf(w[r], v.x, acc[r][c].x); acc[r][c].y = fmaf(w[r], v.y, acc[r][c].y);
+        acc[r][c].z = fmaf(w[r], v.z, acc[r][c].z); acc[r][c].w = fmaf(w[r], v.w, acc[r][c].w);
+      }
+    }
+  }
+}
+template <class T>
+__device__ __forceinline__ void store_row(T* row, int tx, int c, float4 v, float by, int D) {
+  const float f[4] = {v.x * by, v.y * by, v.z * by, v.w * by};
+#pragma unroll
+  for (int u = 0; u < 4; ++u)
+    if (4 * tx + 64 * c + u < D) row[4 * tx + 64 * c + u] = from_float<T>(f[u]);
+}
+__device__ __forceinline__ float max16(float v) {
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+__device__ __forceinline__ float sum16(float v) {
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+template <class T, int DP>
+__global__ void __launch_bounds__(kThreads) packed_generic_fwd_kernel(const PackedArgs a) {
+  using C = GenericCfg<DP>;
+  constexpr int TILE = C::TILE, NR = C::NR, NC = C::NC;
+  extern __shared__ __align__(16) float sm[];
+  float *sQ = sm, *sK = sQ + TILE * C::LD, *sV = sK + TILE * C::LD, *sP = sV + TILE * C::LD;
+  __shared__ int place[34];
+  const int h = blockIdx.y, tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  T* o = static_cast<T*>(a.o);
+  if (h == 0) zero_outside(a.offsets, a.wide, a.B, a.Tq, a.o, (long long)a.H * a.D * sizeof(T), blockIdx.x, gridDim.x);
+  const Place at = locate(a.B, blockIdx.x, TILE, place, [&](int b) { return query_span(a, b).n; });
+  if (at.seq < 0) return;
+  const Span qs = query_span(a, at.seq), ks = key_span(a, at.seq);
+  const int i0 = at.tile * TILE, rows = min(TILE, qs.n - i0), shift = ks.n - qs.n, hk = h / a.G;
+  const int seen = keys_seen(a, qs.n, ks.n, i0, TILE);
+  load_rows<T, DP>(sQ, static_cast<const T*>(a.q) + (long long)(qs.begin + i0) * a.sq[0] + (long long)h * a.sq[1], a.sq[0], rows, a.D);
+  const float c = a.scale * kLog2e;
+  float m[NR], l[NR];
+  float4 acc[NR][NC];
+#pragma unroll
+  for (int r = 0; r < NR; ++r) {
+    m[r] = -INFINITY;
+    l[r] = 0.f;
+#pragma unroll
+    for (int k = 0; k < NC; ++k) acc[r][k] = make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+  for (int j0 = 0; j0 < seen; j0 += TILE) {
+    __syncthreads();
+    const long long row = ks.begin + j0;
+    load_rows<T, DP>(sK, static_cast<const T*>(a.k) + row * a.sk[0] + (long long)hk * a.sk[1], a.sk[0], ks.n - j0, a.D);
+    load_rows<T, DP>(sV, static_cast<const T*>(a.v) + row * a.sv[0] + (long long)hk * a.sv[1], a.sv[0], ks.n - j0, a.D);
+    __syncthreads();
+    float s[NR][NR];
+    products<DP>(sQ, sK, ty, tx, s);
+#pragma unroll
+    for (int r = 0; r < NR; ++r) {
+      const int last = a.causal ? min(ks.n - 1, i0 + ty + 16 * r + shift) : ks.n - 1;  // the last key of this row
+      float mx = -INFINITY;
+#pragma unroll
+      for (int k = 0; k < NR; ++k) {
+        s[r][k] = j0 + tx + 16 * k <= last ? s[r][k] * c : -INFINITY;
+        mx = fmaxf(mx, s[r][k]);
+      }
+      const float up = fmaxf(m[r], max16(mx));
+      const float from = up == -INFINITY ? 0.f : up;  // (a row that has seen no key: all exponentials are 0)
+      const float alpha = exp2f(m[r] - from);
+      m[r] = up;
+      float sum = 0.f;
+#pragma unroll
+      for (int k = 0; k < NR; ++k) {
+        const float p = exp2f(s[r][k] - from);
+        sum += p;
+        sP[(ty + 16 * r) * C::LP + tx + 16 * k] = p;
+      }
+      l[r] = l[r] * alpha + sum16(sum);
+#pragma unroll
+      for (int k = 0; k < NC; ++k) { acc[r][k].x *= alpha; acc[r][k].y *= alpha; acc[r][k].z *= alpha; acc[r][k].w *= alpha; }
+    }
+    __syncthreads();
+    accumulate<DP, true>(sP, sV, ty, tx, acc);
+  }
+#pragma unroll
+  for (int r = 0; r < NR; ++r) {
+    const int i = ty + 16 * r;
+    if (i >= rows) continue;
+    const float inv = l[r] > 0.f ? 1.f / l[r] : 0.f;
+    T* out = o + ((long long)(qs.begin + i0 + i) * a.H + h) * a.D;
+#pragma unroll
+    for (int k = 0; k < NC; ++k) store_row(out, tx, k, acc[r][k], m[r] == -INFINITY ? 0.f : inv, a.D);
+    if (tx == 0 && a.lse) a.lse[(long long)h * a.lse_ld + qs.begin + i0 + i] = m[r] == -INFINITY ? -INFINITY : m[r] + log2f(l[r]);
+  }
+}
+
+// p and ds of a tile, in place of the scores and of dO V^T.
+template <int NR>
+__device__ __forceinline__ void p_and_ds(const PackedArgs& a, float (&s)[NR][NR], float (&dp)[NR][NR], const float* lse, const float* delta, int i0, int j0, int nq, int nk, int ty, int tx) {
+  const float c = a.scale * kLog2e;
+#pragma unroll
+  for (int r = 0; r < NR; ++r) {
+    const int i = ty + 16 * r;
+    const int last = i0 + i >= nq ? -1 : a.causal ? min(nk - 1, i0 + i + nk - nq) : nk - 1;
+#pragma unroll
+    for (int k = 0; k < NR; ++k) {
+      const bool seen = j0 + tx + 16 * k <= last;
+      s[r][k] = seen ? exp2f(s[r][k] * c - lse[i]) : 0.f;
+      dp[r][k] = seen ? s[r][k] * (dp[r][k] - delta[i]) : 0.f;
+    }
+  }
+}
+template <int DP>
+__device__ __forceinline__ void load_statistics(const PackedArgs& a, float* lse, float* delta, int h, int row, int rows) {
+  for (int i = threadIdx.x; i < GenericCfg<DP>::TILE; i += kThreads) {
+    lse[i] = i < rows ? a.lse[(long long)h * a.lse_ld + row + i] : 0.f;
+    delta[i] = i < rows ? a.delta[(long long)h * a.lse_ld + row + i] : 0.f;
+  }
+}
+
+template <class T, int DP>
+__global__ void __launch_bounds__(kThreads) packed_generic_dq_kernel(const PackedArgs a) {
+  using C = GenericCfg<DP>;
+  constexpr int TILE = C::TILE, NR = C::NR, NC = C::NC;
+  extern __shared__ __align__(16) float sm[];
+  float *sQ = sm, *sO = sQ + TILE * C::LD, *sK = sO + TILE * C::LD, *sV = sK + TILE * C::LD, *sS = sV + TILE * C::LD;
+  float *lse = sS + TILE * C::LP, *delta = lse + TILE;
+  __shared__ int place[34];
+  const int h = blockIdx.y, tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  if (h == 0) zero_outside(a.offsets, a.wide, a.B, a.Tq, a.dq, (long long)a.H * a.D * sizeof(T), blockIdx.x, gridDim.x);
+  const Place at = locate(a.B, blockIdx.x, TILE, place, [&](int b) { return query_span(a, b).n; });
+  if (at.seq < 0) return;
+  const Span qs = query_span(a, at.seq), ks = key_span(a, at.seq);
+  const int i0 = at.tile * TILE, rows = min(TILE, qs.n - i0), hk = h / a.G, seen = keys_seen(a, qs.n, ks.n, i0, TILE);
+  const long long row = qs.begin + i0;
+  load_rows<T, DP>(sQ, static_cast<const T*>(a.q) + row * a.sq[0] + (long long)h * a.sq[1], a.sq[0], rows, a.D);
+  load_rows<T, DP>(sO, static_cast<const T*>(a.d_o) + row * a.sdo[0] + (long long)h * a.sdo[1], a.sdo[0], rows, a.D);
+  load_statistics<DP>(a, lse, delta, h, (int)row, rows);
+  float4 acc[NR][NC];
+#pragma unroll
+  for (int r = 0; r < NR; ++r)
+#pragma unroll
+    for (int k = 0; k < NC; ++k) acc[r][k] = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int j0 = 0; j0 < seen; j0 += TILE) {
+    __syncthreads();
+    const long long key = ks.begin + j0;
+    load_rows<T, DP>(sK, static_cast<const T*>(a.k) + key * a.sk[0] + (long long)hk * a.sk[1], a.sk[0], ks.n - j0, a.D);
+    load_rows<T, DP>(sV, static_cast<const T*>(a.v) + key * a.sv[0] + (long long)hk * a.sv[1], a.sv[0], ks.n - j0, a.D);
+    __syncthreads();
+    float s[NR][NR], dp[NR][NR];
+    products<DP>(sQ, sK, ty, tx, s);
+    products<DP>(sO, sV, ty, tx, dp);
+    p_and_ds(a, s, dp, lse, delta, i0, j0, qs.n, ks.n, ty, tx);
+#pragma unroll
+    for (int r = 0; r < NR; ++r)
+#pragma unroll
+      for (int k = 0; k < NR; ++k) sS[(ty + 16 * r) * C::LP + tx + 16 * k] = dp[r][k];
+    __syncthreads();
+    accumulate<DP, true>(sS, sK, ty, tx, acc);
+  }
+#pragma unroll
+  for (int r = 0; r < NR; ++r) {
+    if (ty + 16 * r >= rows) continue;
+    T* out = static_cast<T*>(a.dq) + ((row + ty + 16 * r) * a.H + h) * a.D;
+#pragma unroll
+    for (int k = 0; k < NC; ++k) store_row(out, tx, k, acc[r][k], a.scale, a.D);
+  }
+}
+
+template <class T, int DP>
+__global__ void __launch_bounds__(kThreads) packed_generic_dkv_kernel(const PackedArgs a) {
+  using C = GenericCfg<DP>;
+  constexpr int TILE = C::TILE, NR = C::NR, NC = C::NC;
+  extern __shared__ __align__(16) float sm[];
+  float *sQ = sm, *sO = sQ + TILE * C::LD, *sK = sO + TILE * C::LD, *sV = sK + TILE * C::LD, *sP = sV + TILE * C::LD, *sS = sP + TILE * C::LP;
+  float *lse = sS + TILE * C::LP, *delta = lse + TILE;
+  __shared__ int place[34];
+  const int hk = blockIdx.y, tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  const long long row_bytes = (long long)a.Hk * a.D * sizeof(T);
+  if (hk == 0) {
+    zero_outside(a.key_offsets, a.wide, a.B, a.Tk, a.dk, row_bytes, blockIdx.x, gridDim.x);
+    zero_outside(a.key_offsets, a.wide, a.B, a.Tk, a.dv, row_bytes, blockIdx.x, gridDim.x);
+  }
+  const Place at = locate(a.B, blockIdx.x, TILE, place, [&](int b) { return key_span(a, b).n; });
+  if (at.seq < 0) return;
+  const Span qs = query_span(a, at.seq), ks = key_span(a, at.seq);
+  const int j0 = at.tile * TILE, keys = min(TILE, ks.n - j0);
+  const long long key = ks.begin + j0;
+  load_rows<T, DP>(sK, static_cast<const T*>(a.k) + key * a.sk[0] + (long long)hk * a.sk[1], a.sk[0], keys, a.D);
+  load_rows<T, DP>(sV, static_cast<const T*>(a.v) + key * a.sv[0] + (long long)hk * a.sv[1], a.sv[0], keys, a.D);
+  float4 dk[NR][NC], dv[NR][NC];
+#pragma unroll
+  for (int r = 0; r < NR; ++r)
+#pragma unroll
+    for (int k = 0; k < NC; ++k) dk[r][k] = dv[r][k] = make_float4(0.f, 0.f, 0.f, 0.f);
+  // the first query that sees a key of this tile
+  const int first = a.causal ? max(0, j0 - (ks.n - qs.n)) : 0;
+  for (int g = 0; g < a.G; ++g) {
+    const int h = hk * a.G + g;
+    for (int i0 = first / TILE * TILE; i0 < qs.n; i0 += TILE) {
+      __syncthreads();
+      const long long row = qs.begin + i0;
+      const int rows = min(TILE, qs.n - i0);
+      load_rows<T, DP>(sQ, static_cast<const T*>(a.q) + row * a.sq[0] + (long long)h * a.sq[1], a.sq[0], rows, a.D);
+      load_rows<T, DP>(sO, static_cast<const T*>(a.d_o) + row * a.sdo[0] + (long long)h * a.sdo[1], a.sdo[0], rows, a.D);
+      load_statistics<DP>(a, lse, delta, h, (int)row, rows);
+      __syncthreads();
+      float s[NR][NR], dp[NR][NR];
+      products<DP>(sQ, sK, ty, tx, s);
+      products<DP>(sO, sV, ty, tx, dp);
+      p_and_ds(a, s, dp, lse, delta, i0, j0, qs.n, ks.n, ty, tx);
+#pragma unroll
+      for (int r = 0; r < NR; ++r)
+#pragma unroll
+        for (int k = 0; k < NR; ++k) {
+          sP[(ty + 16 * r) * C::LP + tx + 16 * k] = s[r][k];
+          sS[(ty + 16 * r) * C::LP + tx + 16 * k] = dp[r][k];
+        }
+      __syncthreads();
+      accumulate<DP, false>(sP, sO, ty, tx, dv);
+      accumulate<DP, false>(sS, sQ, ty, tx, dk);
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < NR; ++r) {
+    if (ty + 16 * r >= keys) continue;
+    const long long at_row = ((key + ty + 16 * r) * a.Hk + hk) * a.D;
+#pragma unroll
+    for (int k = 0; k < NC; ++k) {
+      store_row(static_cast<T*>(a.dk) + at_row, tx, k, dk[r][k], a.scale, a.D);
+      store_row(static_cast<T*>(a.dv) + at_row, tx, k, dv[r][k], 1.f, a.D);
+    }
+  }
+}
+
+// delta: a warp per row and head.
+template <class T>
+__global__ void __launch_bounds__(256) packed_delta_kernel(const PackedArgs a) {
+  const long long item = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  if (item >= (long long)a.Tq * a.H) return;
+  const long long t = item / a.H;
+  const int h = (int)(item % a.H);
+  const T* o = static_cast<const T*>(a.o) + item * a.D;
+  const T* d = static_cast<const T*>(a.d_o) + t * a.sdo[0] + (long long)h * a.sdo[1];
+  float s = 0.f;
+  for (int x = lane; x < a.D; x += 32) s = fmaf(to_float(o[x]), to_float(d[x]), s);
+  s = warp_sum(s);
+  if (lane == 0) a.delta[(long long)h * a.lse_ld + t] = s;
+}
+
+template <class K>
+int run(K kern, const PackedArgs& a, long long rows, int tile, int heads, size_t smem, cudaStream_t st, int* launches) {
+  if (!kernel_ready(reinterpret_cast<const void*>(kern), (int)smem, nullptr)) return EVOATTN_ERR_CUDA;
+  kern<<<dim3((unsigned)(rows / tile + a.B), (unsigned)heads), kThreads, smem, st>>>(a);
+  *launches += 1;
+  return cudaGetLastError() == cudaSuccess ? EVOATTN_OK : EVOATTN_ERR_CUDA;
+}
+template <class T, int DP>
+int fwd(const PackedArgs& a, cudaStream_t st, int* launches) {
+  using C = GenericCfg<DP>;
+  return run(packed_generic_fwd_kernel<T, DP>, a, a.Tq, C::TILE, a.H, C::bytes(3, 1), st, launches);
+}
+template <class T, int DP>
+int bwd(const PackedArgs& a, cudaStream_t st, int* launches) {
+  using C = GenericCfg<DP>;
+  if (a.dk) {
+    const int rc = run(packed_generic_dkv_kernel<T, DP>, a, a.Tk, C::TILE, a.Hk, C::bytes(4, 2), st, launches);
+    if (rc) return rc;
+  }
+  return a.dq ? run(packed_generic_dq_kernel<T, DP>, a, a.Tq, C::TILE, a.H, C::bytes(4, 1), st, launches) : EVOATTN_OK;
+}
+
+}  // namespace
+
+int launch_packed_generic_fwd(int dtype, const PackedArgs& a, cudaStream_t st, int* launches) {
+  return with_dtype(dtype, [&](auto t) {
+    using T = decltype(t);
+    return a.D <= 64 ? fwd<T, 64>(a, st, launches) : a.D <= 128 ? fwd<T, 128>(a, st, launches) : fwd<T, 256>(a, st, launches);
+  });
+}
+int launch_packed_generic_bwd(int dtype, const PackedArgs& a, cudaStream_t st, int* launches) {
+  return with_dtype(dtype, [&](auto t) {
+    using T = decltype(t);
+    return a.D <= 64 ? bwd<T, 64>(a, st, launches) : a.D <= 128 ? bwd<T, 128>(a, st, launches) : bwd<T, 256>(a, st, launches);
+  });
+}
+int launch_packed_delta(int dtype, const PackedArgs& a, cudaStream_t st, int* launches) {
+  return with_dtype(dtype, [&](auto t) {
+    packed_delta_kernel<decltype(t)><<<(unsigned)(((long long)a.Tq * a.H + 7) / 8), 256, 0, st>>>(a);
+    *launches += 1;
+    return cudaGetLastError() == cudaSuccess ? EVOATTN_OK : EVOATTN_ERR_CUDA;
+  });
+}
+
+}  // namespace evo

@@ -356,6 +356,84 @@ int evoattn_pair_projection_fwd(const evoattn_pair_projection_params* p, void* c
 size_t evoattn_pair_projection_bwd_workspace_bytes(const evoattn_pair_projection_params* p);
 int evoattn_pair_projection_bwd(const evoattn_pair_projection_params* p, void* cuda_stream);
 
+/* ---- Sequences of different lengths, packed one behind another.
+ *
+ * Rotary positions and attention over packed sequences with grouped heads.  The reference has neither.  The
+ * types are EVOATTN_BF16 / FP16 / FP32; every call may be captured in a CUDA graph, and gives the same bits in
+ * every run (no sum depends on the order in which blocks run).
+ *
+ * Rotary positions: pairs of the first `rotary` values of every head turned by position * frequency,
+ * (a, b) -> amplitude (a cos - b sin, a sin + b cos); the values behind them are copied.  Tokens are indexed by three
+ * axes (n[0], n[1], n[2]) with element strides; a head's D values are contiguous.  q or k may be null.  The
+ * gradient is the call on the gradients with `inverse` set. */
+enum { EVOATTN_ROTARY_HALF = 0, EVOATTN_ROTARY_INTERLEAVED = 1 }; /* pairs (i, i + rotary / 2), or (2 i, 2 i + 1) */
+#define EVOATTN_ROTARY_MAX_D 1024
+typedef struct evoattn_rotary_params {
+  int32_t dtype;
+  int32_t layout;
+  int32_t inverse;        /* non-zero: turned back */
+  int32_t positions64;    /* non-zero: positions are int64, else int32 */
+  int32_t frequencies64;  /* non-zero: frequencies are double, else float */
+  float amplitude;
+  int64_t n[3];           /* at most 2^31 - 1 tokens */
+  int32_t H, Hk, D, rotary;
+  const void* q;          /* [n][H][D] or null */
+  int64_t q_stride[4];    /* element strides of the three token axes and the head */
+  const void* k;          /* [n][Hk][D] or null */
+  int64_t k_stride[4];
+  void* q_out;            /* dense */
+  void* k_out;
+  const void* positions;  /* [n] */
+  int64_t position_stride[3];
+  const void* frequencies;/* [rotary / 2], dense: radians a position */
+} evoattn_rotary_params;
+
+int evoattn_rotary(const evoattn_rotary_params* p, void* cuda_stream);
+
+/* Attention over packed sequences: o_i = sum_j softmax_j(scale q_i k_j) v_j over the keys j of i's sequence, and with
+ * `causal` those with j <= i + (keys - queries): the last query sees every key.  Query head h reads the keys of head
+ * h / (H / Hk).  A query that sees no key gets 0; so does every row of o, dq, dk and dv that belongs to no sequence.
+ *
+ * offsets (on the device) are read by the kernels: the queries of sequence b are rows offsets[b] to offsets[b+1].  Whatever
+ * they hold, no row outside the tensors is touched; they have to ascend for the rows to be right.  A key range [B][2] (begin,
+ * end) lets the keys of a sequence lie anywhere, as in the slots of a cache; it has no backward. */
+enum { EVOATTN_PACKED_KEY_OFFSETS = 0, EVOATTN_PACKED_KEY_RANGES = 1 };
+#define EVOATTN_PACKED_MAX_D 256
+typedef struct evoattn_packed_params {
+  int32_t dtype;          /* of q, k, v, o, d_o, dq, dk, dv */
+  int32_t B, H, Hk, D;    /* sequences, query heads, key heads (a divisor of H), head dimension */
+  int32_t causal;
+  int32_t offsets64;      /* non-zero: both offsets are int64, else int32 */
+  int32_t key_form;       /* EVOATTN_PACKED_KEY_* */
+  uint32_t flags;         /* EVOATTN_FLAG_FORCE_GENERIC */
+  float scale;
+  int64_t Tq, Tk;         /* rows of q and of k and v, at most 2^30 */
+  const void* q;          /* [Tq][H][D], D contiguous */
+  const void* k;          /* [Tk][Hk][D] */
+  const void* v;
+  int64_t q_stride[2];    /* element strides of (row, head) */
+  int64_t k_stride[2];
+  int64_t v_stride[2];
+  const void* offsets;    /* [B+1] */
+  const void* key_offsets;/* [B+1] or [B][2]; null: offsets */
+  void* o;                /* [Tq][H][D], dense.  Forward: out; backward: in */
+  float* lse;             /* [H][Tq]: log2 of the sum of exp2(scale log2(e) q k), -inf for a row without a key.  Forward: out,
+                             or null; backward: in */
+  int32_t* status;        /* optional device word, as in evoattn_fwd_params */
+  const void* d_o;        /* backward */
+  int64_t do_stride[2];
+  void* dq;               /* out, dense; null: not wanted */
+  void* dk;               /* out, dense; dk and dv are both wanted or both null */
+  void* dv;
+  void* workspace;        /* device scratch of at least evoattn_packed_{fwd,bwd}_workspace_bytes(), 256-byte aligned */
+  size_t workspace_bytes;
+} evoattn_packed_params;
+
+size_t evoattn_packed_fwd_workspace_bytes(const evoattn_packed_params* p);
+int evoattn_packed_fwd(const evoattn_packed_params* p, void* cuda_stream);
+size_t evoattn_packed_bwd_workspace_bytes(const evoattn_packed_params* p);
+int evoattn_packed_bwd(const evoattn_packed_params* p, void* cuda_stream);
+
 /* EVOATTN_PATH_* of the most recent forward / backward call made by this thread. */
 int evoattn_last_path(void);
 
