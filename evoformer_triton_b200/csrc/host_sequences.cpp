@@ -132,6 +132,15 @@ py::object rotary_embedding(const Tensor& q, const Maybe& k, const Tensor& posit
 
 // ---------------------------------------------------------------- attention over packed sequences
 
+// Where the tensor-core kernels could take a call (16 bits, head dimensions in eights up to 128), an operand that a tensor
+// map cannot read (rows off 16 bytes, steps of zero or backwards) is copied; elsewhere it is read as it lies.
+Tensor mapped(const Tensor& t) {
+  const Tensor r = last_axis_dense(t);
+  if (r.scalar_type() == at::kFloat || r.size(2) % 8 || r.size(2) > 128 || r.numel() == 0) return r;
+  const auto step = [](int64_t n, int64_t st) { return n == 1 || (st > 0 && st % 8 == 0); };
+  return !((uintptr_t)r.data_ptr() & 15) && step(r.size(0), r.stride(0)) && step(r.size(1), r.stride(1)) ? r : r.clone(at::MemoryFormat::Contiguous);
+}
+
 struct PackedPlan {
   bool causal;
   double scale;
@@ -140,7 +149,7 @@ struct PackedCall {
   Tensor q, k, v, offsets, keys, o, lse;
   evoattn_packed_params p{};
   PackedCall(const Tensor& q_in, const Tensor& k_in, const Tensor& v_in, const Tensor& off, const Tensor& key_off, const PackedPlan& plan)
-      : q(last_axis_dense(q_in)), k(last_axis_dense(k_in)), v(last_axis_dense(v_in)), offsets(off), keys(key_off) {
+      : q(mapped(q_in)), k(mapped(k_in)), v(mapped(v_in)), offsets(off), keys(key_off) {
     p.dtype = dtype_code(q.scalar_type());
     p.B = (int32_t)(offsets.size(0) - 1); p.H = (int32_t)q.size(1); p.Hk = (int32_t)k.size(1); p.D = (int32_t)q.size(2);
     p.causal = plan.causal;
@@ -203,7 +212,7 @@ struct Packed : public torch::autograd::Function<Packed> {
     if (ctx->needs_input_grad(0)) dq = make(c.q), p.dq = address(dq) ? dq.data_ptr() : nullptr;
     if (keys) dk = make(c.k), dv = make(c.v), p.dk = dk.data_ptr(), p.dv = dv.data_ptr();
     if (!c.empty()) {
-      const Tensor d = last_axis_dense(grads[0].scalar_type() == c.q.scalar_type() ? grads[0] : grads[0].to(c.q.scalar_type()));
+      const Tensor d = mapped(grads[0].scalar_type() == c.q.scalar_type() ? grads[0] : grads[0].to(c.q.scalar_type()));
       p.o = s[5].data_ptr();
       p.lse = s[6].data_ptr<float>();
       p.d_o = d.data_ptr();

@@ -1,5 +1,5 @@
 // Attention over packed sequences: what a request has to hold, and which kernels serve it.
-#include "packed.cuh"
+#include "packed_sm100.cuh"
 
 namespace evo {
 namespace {
@@ -36,6 +36,15 @@ PackedArgs arguments(const evoattn_packed_params* p) {
   return a;
 }
 
+bool tensor_cores(const evoattn_packed_params* p, const PackedArgs& a, bool bwd) {
+  return !(p->flags & EVOATTN_FLAG_FORCE_GENERIC) && sm100_packed_supported(p->dtype, a, bwd);
+}
+int check_workspace(const evoattn_packed_params* p, size_t need) {
+  if (!need) return EVOATTN_OK;
+  if (!p->workspace || p->workspace_bytes < need) return EVOATTN_ERR_WORKSPACE;
+  return (uintptr_t)p->workspace & 255 ? EVOATTN_ERR_ALIGN : EVOATTN_OK;
+}
+
 }  // namespace
 }  // namespace evo
 
@@ -44,18 +53,24 @@ extern "C" {
 using namespace evo;
 
 size_t evoattn_packed_fwd_workspace_bytes(const evoattn_packed_params* p) {
-  return 0;
+  if (validate(p, false)) return 0;
+  const PackedArgs a = arguments(p);
+  return tensor_cores(p, a, false) ? sm100_packed_fwd_workspace_bytes(a) : 0;
 }
 
 int evoattn_packed_fwd(const evoattn_packed_params* p, void* cuda_stream) {
-  const int rc = validate(p, false);
+  int rc = validate(p, false);
+  if (rc) return rc;
+  rc = check_workspace(p, evoattn_packed_fwd_workspace_bytes(p));
   if (rc) return rc;
   const PackedArgs a = arguments(p);
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(cuda_stream);
   bind_context_once();
   int launches = 0;
-  const int rl = launch_packed_generic_fwd(p->dtype, a, reinterpret_cast<cudaStream_t>(cuda_stream), &launches);
-  note_call(EVOATTN_PATH_GENERIC, launches);
-  return rl;
+  const bool fast = tensor_cores(p, a, false);
+  rc = fast ? launch_sm100_packed_fwd(p->dtype, a, p->workspace, st, &launches) : launch_packed_generic_fwd(p->dtype, a, st, &launches);
+  note_call(fast ? EVOATTN_PATH_TCGEN05 : EVOATTN_PATH_GENERIC, launches);
+  return rc;
 }
 
 size_t evoattn_packed_bwd_workspace_bytes(const evoattn_packed_params* p) {
@@ -66,9 +81,8 @@ size_t evoattn_packed_bwd_workspace_bytes(const evoattn_packed_params* p) {
 int evoattn_packed_bwd(const evoattn_packed_params* p, void* cuda_stream) {
   const int rc = validate(p, true);
   if (rc) return rc;
-  const size_t need = evoattn_packed_bwd_workspace_bytes(p);
-  if (!p->workspace || p->workspace_bytes < need) return EVOATTN_ERR_WORKSPACE;
-  if ((uintptr_t)p->workspace & 255) return EVOATTN_ERR_ALIGN;
+  const int rw = check_workspace(p, evoattn_packed_bwd_workspace_bytes(p));
+  if (rw) return rw;
   PackedArgs a = arguments(p);
   a.delta = static_cast<float*>(p->workspace);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(cuda_stream);
