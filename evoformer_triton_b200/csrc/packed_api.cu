@@ -37,7 +37,7 @@ PackedArgs arguments(const evoattn_packed_params* p) {
 }
 
 bool tensor_cores(const evoattn_packed_params* p, const PackedArgs& a, bool bwd) {
-  return !(p->flags & EVOATTN_FLAG_FORCE_GENERIC) && sm100_packed_supported(p->dtype, a, bwd);
+  return !(p->flags & EVOATTN_FLAG_FORCE_GENERIC) && (bwd ? sm100_packed_bwd_supported(p->dtype, a) : sm100_packed_supported(p->dtype, a));
 }
 int check_workspace(const evoattn_packed_params* p, size_t need) {
   if (!need) return EVOATTN_OK;
@@ -75,23 +75,29 @@ int evoattn_packed_fwd(const evoattn_packed_params* p, void* cuda_stream) {
 
 size_t evoattn_packed_bwd_workspace_bytes(const evoattn_packed_params* p) {
   if (validate(p, true)) return 0;
-  return (size_t)p->H * p->Tq * sizeof(float);
+  const PackedArgs a = arguments(p);
+  return tensor_cores(p, a, true) ? sm100_packed_bwd_workspace_bytes(a) : (size_t)p->H * p->Tq * sizeof(float);
 }
 
 int evoattn_packed_bwd(const evoattn_packed_params* p, void* cuda_stream) {
-  const int rc = validate(p, true);
+  int rc = validate(p, true);
   if (rc) return rc;
-  const int rw = check_workspace(p, evoattn_packed_bwd_workspace_bytes(p));
-  if (rw) return rw;
+  rc = check_workspace(p, evoattn_packed_bwd_workspace_bytes(p));
+  if (rc) return rc;
   PackedArgs a = arguments(p);
-  a.delta = static_cast<float*>(p->workspace);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(cuda_stream);
-  int launches = 0;
   bind_context_once();
-  int rl = launch_packed_delta(p->dtype, a, st, &launches);
-  if (!rl) rl = launch_packed_generic_bwd(p->dtype, a, st, &launches);
-  note_call(EVOATTN_PATH_GENERIC, launches);
-  return rl;
+  int launches = 0;
+  const bool fast = tensor_cores(p, a, true);
+  if (fast) {
+    rc = launch_sm100_packed_bwd(p->dtype, a, p->workspace, st, &launches);
+  } else {
+    a.delta = static_cast<float*>(p->workspace);
+    rc = launch_packed_delta(p->dtype, a, st, &launches);
+    if (!rc) rc = launch_packed_generic_bwd(p->dtype, a, st, &launches);
+  }
+  note_call(fast ? EVOATTN_PATH_TCGEN05 : EVOATTN_PATH_GENERIC, launches);
+  return rc;
 }
 
 }  // extern "C"

@@ -424,7 +424,7 @@ int launch_d(const PackedArgs& a, void* ws, cudaStream_t st, int* launches) {
 
 }  // namespace
 
-bool sm100_packed_supported(int dtype, const PackedArgs& a, bool bwd) {
+bool sm100_packed_supported(int dtype, const PackedArgs& a) {
   if (dtype == EVOATTN_FP32 || a.D % 8 || a.D > 128 || !(a.scale > 0.f)) return false;
   // (numbers of items fit 31 bits)
   if ((a.Tq / kTileRows + a.B) * (long long)a.H >= 1LL << 31 || (a.Tk / kTileRows + a.B) * (long long)a.Hk >= 1LL << 31) return false;

@@ -52,9 +52,12 @@ inline bool packed_map_ok(const void* base, const long long* stride, int T, int 
   return rows && (heads == 1 || (stride[1] > 0 && stride[1] % 8 == 0 && stride[1] < most));
 }
 
-bool sm100_packed_supported(int dtype, const PackedArgs& a, bool bwd);
+bool sm100_packed_supported(int dtype, const PackedArgs& a);
+bool sm100_packed_bwd_supported(int dtype, const PackedArgs& a);
 size_t sm100_packed_fwd_workspace_bytes(const PackedArgs& a);
 int launch_sm100_packed_fwd(int dtype, const PackedArgs& a, void* workspace, cudaStream_t st, int* launches);
+size_t sm100_packed_bwd_workspace_bytes(const PackedArgs& a);
+int launch_sm100_packed_bwd(int dtype, const PackedArgs& a, void* workspace, cudaStream_t st, int* launches);
 
 __device__ __forceinline__ PackedTile load_tile(const PackedTile* p) {
   const uint4 u = __ldcg(reinterpret_cast<const uint4*>(p)), w = __ldcg(reinterpret_cast<const uint4*>(p) + 1);
