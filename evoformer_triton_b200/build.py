@@ -17,7 +17,7 @@ OBJ = os.path.join(PKG, "build")
 LIB = os.path.join(PKG, "libevoattn.so")
 HOST = os.path.join(PKG, "_evohost.so")
 SOURCES = ["api.cu", "generic_kernels.cu", "tmap.cu", "fwd_sm100.cu", "bwd_sm100.cu", "peer_reduce.cu", "extras.cu",
-           "norm.cu", "relative_bias.cu", "pair_projection.cu", "rotary.cu", "packed_api.cu", "packed_generic.cu", "packed_plan.cu", "packed_fwd.cu", "packed_bwd.cu"]
+           "norm.cu", "relative_bias.cu", "pair_projection.cu", "rotary.cu", "packed_api.cu", "packed_generic.cu", "packed_plan.cu", "packed_fwd.cu", "packed_bwd.cu", "packed_few.cu"]
 HOST_SOURCES = ["host.cpp", "host_inputs.cpp", "host_sequences.cpp"]
 NVCC_FLAGS = [
     "-O3", "-std=c++17", "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo",

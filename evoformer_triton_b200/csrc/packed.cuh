@@ -21,6 +21,7 @@ struct PackedArgs {
   int B, H, Hk, D, G;  // G = H / Hk
   int causal, wide, ranges;  // offsets are int64; key_offsets is [B][2] (begin, end)
   int Tq, Tk, lse_ld;
+  int few_tokens;  // sequences of up to this many queries are left to packed_few.cu; 0: none
   float scale;
   int* status;
 };

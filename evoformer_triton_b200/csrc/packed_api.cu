@@ -39,6 +39,25 @@ PackedArgs arguments(const evoattn_packed_params* p) {
 bool tensor_cores(const evoattn_packed_params* p, const PackedArgs& a, bool bwd) {
   return !(p->flags & EVOATTN_FLAG_FORCE_GENERIC) && (bwd ? sm100_packed_bwd_supported(p->dtype, a) : sm100_packed_supported(p->dtype, a));
 }
+// Which kernels a forward takes, and their scratch.  The host knows how many sequences and queries there are, not how they
+// fall.  Sequences of a few queries against keys of their own go to packed_few.cu, the others to the tiles; calls whose
+// queries are few altogether go there as a whole (the worst is that all queries are one sequence's: 64 units then),
+// which saves the launches for the tiles.
+struct Forward {
+  bool generic;
+  size_t few, tiles;
+  size_t bytes() const { return few + tiles; }
+};
+int few_tokens(const PackedArgs& a) { return a.G > 16 ? 2 : 32 / a.G; }
+Forward forward_plan(const evoattn_packed_params* p, const PackedArgs& a) {
+  Forward f{!tensor_cores(p, a, false), 0, 0};
+  if (f.generic) return f;
+  const bool own_keys = p->key_offsets && !p->lse;
+  const bool all_few = own_keys && a.Tq <= (long long)few_tokens(a) * a.B && (long long)a.Tq * a.G <= 1024;
+  if (own_keys && (a.B > 1 || all_few)) f.few = (packed_few_workspace_bytes(a) + 255) / 256 * 256;
+  if (!all_few) f.tiles = sm100_packed_fwd_workspace_bytes(a);
+  return f;
+}
 int check_workspace(const evoattn_packed_params* p, size_t need) {
   if (!need) return EVOATTN_OK;
   if (!p->workspace || p->workspace_bytes < need) return EVOATTN_ERR_WORKSPACE;
@@ -55,21 +74,29 @@ using namespace evo;
 size_t evoattn_packed_fwd_workspace_bytes(const evoattn_packed_params* p) {
   if (validate(p, false)) return 0;
   const PackedArgs a = arguments(p);
-  return tensor_cores(p, a, false) ? sm100_packed_fwd_workspace_bytes(a) : 0;
+  return forward_plan(p, a).bytes();
 }
 
 int evoattn_packed_fwd(const evoattn_packed_params* p, void* cuda_stream) {
   int rc = validate(p, false);
   if (rc) return rc;
-  rc = check_workspace(p, evoattn_packed_fwd_workspace_bytes(p));
+  PackedArgs a = arguments(p);
+  const Forward f = forward_plan(p, a);
+  rc = check_workspace(p, f.bytes());
   if (rc) return rc;
-  const PackedArgs a = arguments(p);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(cuda_stream);
   bind_context_once();
   int launches = 0;
-  const bool fast = tensor_cores(p, a, false);
-  rc = fast ? launch_sm100_packed_fwd(p->dtype, a, p->workspace, st, &launches) : launch_packed_generic_fwd(p->dtype, a, st, &launches);
-  note_call(fast ? EVOATTN_PATH_TCGEN05 : EVOATTN_PATH_GENERIC, launches);
+  if (f.generic) {
+    rc = launch_packed_generic_fwd(p->dtype, a, st, &launches);
+  } else {
+    if (f.few) {
+      a.few_tokens = f.tiles ? few_tokens(a) : a.Tq;
+      rc = launch_packed_few(p->dtype, a, !f.tiles, p->workspace, st, &launches);
+    }
+    if (!rc && f.tiles) rc = launch_sm100_packed_fwd(p->dtype, a, static_cast<unsigned char*>(p->workspace) + f.few, st, &launches);
+  }
+  note_call(f.generic ? EVOATTN_PATH_GENERIC : EVOATTN_PATH_TCGEN05, launches);
   return rc;
 }
 

@@ -12,7 +12,7 @@ template <class F>
 __device__ __forceinline__ void each_tile(const PackedArgs& a, bool queries, int unit, F&& f) {
   for (int b = threadIdx.x >> 5; b < a.B; b += kThreads / 32) {
     const Span q = query_span(a, b), k = key_span(a, b);
-    const int n = queries ? q.n : k.n;
+    const int n = !queries ? k.n : q.n > a.few_tokens ? q.n : 0;
     for (int x = (threadIdx.x & 31) * unit; x < n; x += 32 * unit) {
       PackedTile t{};
       t.rows = min(unit, n - x);

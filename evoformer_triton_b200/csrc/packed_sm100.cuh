@@ -41,9 +41,9 @@ inline PackedPlan place_plan(const PackedArgs& a, void* ws, bool queries, int un
 // Writes the lists, those with the most work first (packed_plan.cu).
 int launch_packed_plan(const PackedArgs& a, const PackedPlan& plan, bool queries, int unit, bool keys, cudaStream_t st, int* launches);
 
-// [T][heads][D] rows of 16 bits as a 3-D map (D, T, heads) with boxes of 64 values (128 bytes, swizzled) by 128 rows;
+// [T][heads][D] rows of 16 bits as a 3-D map (D, T, heads) with boxes of 64 values (128 bytes, swizzled) by `rows`;
 // values beyond D and rows beyond T read as zero.
-bool make_packed_map(CUtensorMap* out, const void* base, const long long* stride, int T, int heads, int D);
+bool make_packed_map(CUtensorMap* out, const void* base, const long long* stride, int T, int heads, int D, int rows = kTileRows);
 // Whether such a map can be made (strides are in elements of 16 bits).
 inline bool packed_map_ok(const void* base, const long long* stride, int T, int heads) {
   if (reinterpret_cast<uintptr_t>(base) & 15) return false;
@@ -58,6 +58,10 @@ size_t sm100_packed_fwd_workspace_bytes(const PackedArgs& a);
 int launch_sm100_packed_fwd(int dtype, const PackedArgs& a, void* workspace, cudaStream_t st, int* launches);
 size_t sm100_packed_bwd_workspace_bytes(const PackedArgs& a);
 int launch_sm100_packed_bwd(int dtype, const PackedArgs& a, void* workspace, cudaStream_t st, int* launches);
+
+// Few query rows against many keys (packed_few.cu): sequences of up to a.few_tokens queries; `clear`: the rows of no sequence too.
+size_t packed_few_workspace_bytes(const PackedArgs& a);
+int launch_packed_few(int dtype, const PackedArgs& a, bool clear, void* workspace, cudaStream_t st, int* launches);
 
 __device__ __forceinline__ PackedTile load_tile(const PackedTile* p) {
   const uint4 u = __ldcg(reinterpret_cast<const uint4*>(p)), w = __ldcg(reinterpret_cast<const uint4*>(p) + 1);

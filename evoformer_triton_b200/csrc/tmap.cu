@@ -117,13 +117,13 @@ bool make_bias16_map(CUtensorMap* out, const void* base, const Str3& st, int B, 
   return r == CUDA_SUCCESS;
 }
 
-bool make_packed_map(CUtensorMap* out, const void* base, const long long* st, int T, int heads, int D) {
+bool make_packed_map(CUtensorMap* out, const void* base, const long long* st, int T, int heads, int D, int rows) {
   std::call_once(g_once, resolve);
   if (!g_encode) return false;
   const uint64_t row = static_cast<uint64_t>(D) * 2;
   cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)T, (cuuint64_t)heads};
   cuuint64_t strides[2] = {fix_stride(st[0], 2, row, T), fix_stride(st[1], 2, row, heads)};
-  cuuint32_t box[3] = {64, kTileRows, 1};
+  cuuint32_t box[3] = {64, (cuuint32_t)rows, 1};
   cuuint32_t estr[3] = {1, 1, 1};
   CUresult r = g_encode(out, CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, const_cast<void*>(base), dims, strides, box, estr,
                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,

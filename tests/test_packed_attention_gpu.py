@@ -108,6 +108,36 @@ def test_a_few_tokens_each_and_one_long(dtype):
     _check(*_qkv(sum(nq), sum(nk), 8, 2, 128, dtype), nq, nk, train=False)
 
 
+def test_thousands_of_tokens():
+    """More sequences than a launch of the kernel for few rows takes; empty ones, sequences without keys, rows of none."""
+    import evoformer_triton_b200 as evo
+    g = torch.Generator().manual_seed(3)
+    nk = torch.randint(0, 70, (5000,), generator=g).tolist()
+    nq = [int(i % 7 != 3) for i in range(5000)]
+    nq[4990], nk[4990] = 40, 3000
+    _check(*_qkv(sum(nq), sum(nk), 2, 1, 64, BF), nq, nk, train=False)
+    q, k, v = _qkv(sum(nq) + 9, sum(nk), 2, 1, 64, BF)
+    off = torch.tensor(_sums(nq, 4), device=DEV)
+    out = evo.packed_attention(q, k, v, off, torch.tensor(_sums(nk), device=DEV))
+    assert not out[:4].any() and not out[-5:].any() and out[4:-5].any(-1).any()
+
+
+@pytest.mark.parametrize("nq", [[1] * 6 + [64, 1], [3, 2, 1, 200, 4]], ids=["one of many", "mixed"])
+def test_tokens_beside_prompts(nq):
+    """New tokens and prompts in one call, each to its kernel."""
+    nk = [900, 33, 64, 1, 4000, 129, 700, 17][:len(nq)]
+    for H, Hk, D in ((8, 2, 64), (6, 1, 128), (40, 1, 64)):
+        for causal in (True, False):
+            _check(*_qkv(sum(nq), sum(nk), H, Hk, D, BF), nq, nk, causal, train=False)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF], ids=IDS.get)
+@pytest.mark.parametrize("nk", [[100_000], [70_000, 64, 513, 512], [5000] * 40], ids=["one long", "uneven", "even"])
+def test_long_rows_of_keys_are_shared_out(nk, dtype):
+    for H, Hk, D in ((4, 4, 128), (16, 1, 64)):
+        _check(*_qkv(len(nk), sum(nk), H, Hk, D, dtype), [1] * len(nk), nk, train=False)
+
+
 @pytest.mark.parametrize("dtype", [BF, HF, F32], ids=IDS.get)
 @pytest.mark.parametrize("nq", [[1, 1, 1, 1, 1], [100, 1, 140, 37, 3]], ids=["tokens", "pieces"])
 def test_keys_in_slots(nq, dtype):
@@ -252,6 +282,13 @@ def test_cuda_core_kernels_agree(dtype):
         _check(*_qkv(2, 400, 4, 2, 128, dtype), [1, 1], [260, 140], train=False)
     finally:
         evo.force_generic(False)
+
+
+def test_which_kernels_a_call_takes():
+    from evoformer_triton_b200 import _lib, attention
+    for dtype, D, want in ((BF, 64, _lib.PATH_TCGEN05), (HF, 128, _lib.PATH_TCGEN05), (BF, 8, _lib.PATH_TCGEN05), (F32, 64, _lib.PATH_GENERIC), (BF, 136, _lib.PATH_GENERIC), (BF, 20, _lib.PATH_GENERIC)):
+        _check(*_qkv(150, 150, 2, 1, D, dtype), [150])
+        assert attention.last_path["fwd"] == attention.last_path["bwd"] == want
 
 
 def test_gradients_against_differences():
