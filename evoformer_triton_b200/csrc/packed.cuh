@@ -108,7 +108,4 @@ __device__ __forceinline__ void zero_outside(const void* offsets, int wide, int 
 // The forward and backward on CUDA cores (packed_generic.cu).
 int launch_packed_generic_fwd(int dtype, const PackedArgs& a, cudaStream_t st, int* launches);
 int launch_packed_generic_bwd(int dtype, const PackedArgs& a, cudaStream_t st, int* launches);
-// The row sums of dO * O, which both backward forms begin with (packed_generic.cu).
-int launch_packed_delta(int dtype, const PackedArgs& a, cudaStream_t st, int* launches);
-
 }  // namespace evo

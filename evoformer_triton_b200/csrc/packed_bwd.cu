@@ -181,33 +181,37 @@ packed_dkv_sm100_kernel(const PackedArgs a, const PackedPlan plan, const FastDiv
   const bool failed = *abort_flag != 0;
   const int n_items = failed ? 0 : __ldcg(plan.counts + 1) * (int)heads.d;
 
-  // The steps of a CTA, one after another over its items: head g of the group, query tile i.
+  // The steps of a CTA, one after another over its items: head g of the group, query tile i, `left` of the item from here on.
   struct Step {
     PackedTile t;
-    int hk, turn, g, i, end;
-    __device__ __forceinline__ bool first() const { return g == 0 && i == end - t.tiles; }
+    int hk, turn, g, i, end, left;
+    __device__ __forceinline__ bool first() const { return left == t.steps; }
+    __device__ __forceinline__ bool last() const { return left == 1; }
     __device__ __forceinline__ int real() const { return t.n - i * BT; }
+    __device__ __forceinline__ void next() {
+      --left;
+      if (++i == end) { i = end - t.tiles; ++g; }
+    }
   };
   auto item = [&](int idx, Step& s) {
     const int tile = (int)heads.div((uint32_t)idx);
     s.hk = idx - tile * (int)heads.d;
     s.t = load_tile(plan.keys + tile);
-    s.g = 0;
+    s.left = s.t.steps;
     s.end = (s.t.n + BT - 1) / BT;
-    s.i = s.end - s.t.tiles;
+    s.g = s.t.tiles ? s.t.begin / s.t.tiles : 0;
+    s.i = s.end - s.t.tiles + s.t.begin - s.g * s.t.tiles;
   };
   auto begin = [&](Step& s) {  // the first step of the next item that has any, from s.turn on
     for (int idx; (idx = item_of(s.turn)) < n_items; ++s.turn) {
       item(idx, s);
-      if (s.t.tiles > 0) return true;
+      if (s.left > 0) return true;
     }
     return false;
   };
-  auto last = [&](const Step& s) { return s.i + 1 == s.end && s.g + 1 == a.G; };
   auto advance = [&](Step& s) {
-    if (++s.i < s.end) return true;
-    s.i = s.end - s.t.tiles;
-    if (++s.g < a.G) return true;
+    s.next();
+    if (s.left > 0) return true;
     ++s.turn;
     return begin(s);
   };
@@ -268,7 +272,7 @@ packed_dkv_sm100_kernel(const PackedArgs a, const PackedPlan plan, const FastDiv
         const uint32_t el = elect_one();
         issue_product<T, DP>(el, tS, smem_s + C::offK, smem_s + C::offQ + stage * C::kTile);
         mma_commit_if_s(el, s_full);
-        if (last(x)) mma_commit_if_s(el, k_empty);
+        if (x.last()) mma_commit_if_s(el, k_empty);
       };
       auto gradients = [&](const Step& x, uint32_t stage, uint32_t parity) {
         if (x.first()) {
@@ -280,7 +284,7 @@ packed_dkv_sm100_kernel(const PackedArgs a, const PackedPlan plan, const FastDiv
         const uint32_t el = elect_one();
         issue_product<T, DP>(el, tP, smem_s + C::offV, smem_s + C::offD + stage * C::kTile);
         mma_commit_if_s(el, dp_full);
-        if (last(x)) mma_commit_if_s(el, v_empty);
+        if (x.last()) mma_commit_if_s(el, v_empty);
       };
       if (more) {
         scores(s, st, par);
@@ -288,7 +292,7 @@ packed_dkv_sm100_kernel(const PackedArgs a, const PackedPlan plan, const FastDiv
       }
 #pragma unroll 1
       while (more) {
-        const bool first = s.first(), end = last(s);
+        const bool first = s.first(), end = s.last();
         const uint32_t cs = st;
         next();
         more = advance(s);  // (s, st, par: the step after this one)
@@ -365,84 +369,94 @@ packed_dkv_sm100_kernel(const PackedArgs a, const PackedPlan plan, const FastDiv
       Step s;
       item(idx, s);
 #pragma unroll 1
-      for (; s.t.tiles > 0 && s.g < a.G; ++s.g) {
-#pragma unroll 1
-        for (int i = s.end - s.t.tiles; i < s.end; ++i, ++n) {
-          // queries of this half before `lo` do not see the key
-          const int lo = a.causal ? s.t.shift + row - i * BT - 64 * w : 0;
-          const bool cut = __any_sync(0xffffffffu, lo > 0);
-          const uint32_t stats = smem_s + C::offStats + st * (2 * BT * 4) + 64 * w * 4;
-          mbar_wait_s(q_full(st), par, abort_s, DEV_TIMEOUT_SYNC);
-          mbar_wait_s(s_full, n & 1, abort_s, DEV_TIMEOUT_MMA);
-          tc_fence_after();
-          F2 p[32];
-          auto exps = [&](auto with_mask) {
-            uint32_t sr[2][32];
-            tmem_ld32(tS, sr[0]);
+      for (; s.left > 0; s.next(), ++n) {
+        // queries of this half before `lo` do not see the key
+        const int lo = a.causal ? s.t.shift + row - s.i * BT - 64 * w : 0;
+        const bool cut = __any_sync(0xffffffffu, lo > 0);
+        const uint32_t stats = smem_s + C::offStats + st * (2 * BT * 4) + 64 * w * 4;
+        mbar_wait_s(q_full(st), par, abort_s, DEV_TIMEOUT_SYNC);
+        mbar_wait_s(s_full, n & 1, abort_s, DEV_TIMEOUT_MMA);
+        tc_fence_after();
+        F2 p[32];
+        auto exps = [&](auto with_mask) {
+          uint32_t sr[2][32];
+          tmem_ld32(tS, sr[0]);
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-              tmem_wait_ld();
-              if (k == 0) tmem_ld32(tS + 32, sr[1]);
-              uint32_t pk[16];
+          for (int k = 0; k < 2; ++k) {
+            tmem_wait_ld();
+            if (k == 0) tmem_ld32(tS + 32, sr[1]);
+            uint32_t pk[16];
 #pragma unroll
-              for (int e = 0; e < 32; e += 4) {
-                const float4 nl = lds_v4f(stats + (32 * k + e) * 4);
-                const F2 nl2[2] = {f2_make(nl.x, nl.y), f2_make(nl.z, nl.w)};
+            for (int e = 0; e < 32; e += 4) {
+              const float4 nl = lds_v4f(stats + (32 * k + e) * 4);
+              const F2 nl2[2] = {f2_make(nl.x, nl.y), f2_make(nl.z, nl.w)};
 #pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                  float x0, x1;
-                  f2_get(f2_fma(f2_from_bits(sr[k][e + 2 * u], sr[k][e + 2 * u + 1]), c2, nl2[u]), x0, x1);
-                  if constexpr (decltype(with_mask)::value) {
-                    x0 = 32 * k + e + 2 * u >= lo ? x0 : -kInf;
-                    x1 = 32 * k + e + 2 * u + 1 >= lo ? x1 : -kInf;
-                  }
-                  const float p0 = ex2(x0), p1 = ex2(x1);
-                  p[16 * k + e / 2 + u] = f2_make(p0, p1);
-                  pk[e / 2 + u] = Pack2<T>::pack(p0, p1);
+              for (int u = 0; u < 2; ++u) {
+                float x0, x1;
+                f2_get(f2_fma(f2_from_bits(sr[k][e + 2 * u], sr[k][e + 2 * u + 1]), c2, nl2[u]), x0, x1);
+                if constexpr (decltype(with_mask)::value) {
+                  x0 = 32 * k + e + 2 * u >= lo ? x0 : -kInf;
+                  x1 = 32 * k + e + 2 * u + 1 >= lo ? x1 : -kInf;
                 }
+                const float p0 = ex2(x0), p1 = ex2(x1);
+                p[16 * k + e / 2 + u] = f2_make(p0, p1);
+                pk[e / 2 + u] = Pack2<T>::pack(p0, p1);
               }
-              tmem_st16(tS + 16 * k, pk);
             }
-          };
-          if (cut) exps(std::true_type{});
-          else exps(std::false_type{});
-          tmem_wait_st();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive_s(p_full);
-          mbar_wait_s(dp_full, n & 1, abort_s, DEV_TIMEOUT_MMA);
-          tc_fence_after();
-          {
-            uint32_t dr[2][32];
-            tmem_ld32(tP, dr[0]);
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-              tmem_wait_ld();
-              if (k == 0) tmem_ld32(tP + 32, dr[1]);
-              uint32_t dk[16];
-              scores_gradient<T>(dr[k], p + 16 * k, [&](int e) {
-                const float2 nd = lds_v2f(stats + (BT + 32 * k + 2 * e) * 4);
-                return f2_make(nd.x, nd.y);
-              }, dk);
-              tmem_st16(tP + 16 * k, dk);
-            }
+            tmem_st16(tS + 16 * k, pk);
           }
-          tmem_wait_st();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive_s(ds_full);
-          if (++st == NS) { st = 0; par ^= 1; }
+        };
+        if (cut) exps(std::true_type{});
+        else exps(std::false_type{});
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_s(p_full);
+        mbar_wait_s(dp_full, n & 1, abort_s, DEV_TIMEOUT_MMA);
+        tc_fence_after();
+        {
+          uint32_t dr[2][32];
+          tmem_ld32(tP, dr[0]);
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            tmem_wait_ld();
+            if (k == 0) tmem_ld32(tP + 32, dr[1]);
+            uint32_t dk[16];
+            scores_gradient<T>(dr[k], p + 16 * k, [&](int e) {
+              const float2 nd = lds_v2f(stats + (BT + 32 * k + 2 * e) * 4);
+              return f2_make(nd.x, nd.y);
+            }, dk);
+            tmem_st16(tP + 16 * k, dk);
+          }
         }
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_s(ds_full);
+        if (++st == NS) { st = 0; par ^= 1; }
       }
-      const bool any = s.t.tiles > 0;
+      const bool any = s.t.steps > 0;
       if (any) {
         mbar_wait_s(out_full, kv & 1, abort_s, DEV_TIMEOUT_MMA);
         ++kv;
         tc_fence_after();
       }
-      const long long at = ((long long)(s.t.row + row) * a.Hk + s.hk) * a.D;
-      if (w == 0) store_rows<T, DP>(t_lane + C::colDV, static_cast<T*>(a.dv) + at, 0, a.D, 1.f, row < s.t.rows, any);
-      else store_rows<T, DP>(t_lane + C::colDK, static_cast<T*>(a.dk) + at, 0, a.D, a.scale, row < s.t.rows, any);
+      const uint32_t src = t_lane + (w == 0 ? C::colDV : C::colDK);
+      if (s.t.parts == 1) {
+        const long long at = ((long long)(s.t.row + row) * a.Hk + s.hk) * a.D;
+        store_rows<T, DP>(src, static_cast<T*>(w == 0 ? a.dv : a.dk) + at, 0, a.D, w == 0 ? 1.f : a.scale, row < s.t.rows, any);
+      } else {
+        float4* out = reinterpret_cast<float4*>(plan.sums) + (((long long)s.t.slot * a.Hk + s.hk) * 2 + w) * (DP / 4 * BT) + row;
+#pragma unroll
+        for (int d = 0; d < DP; d += 32) {
+          uint32_t r[32];
+          tmem_ld32(src + d, r);
+          tmem_wait_ld();
+#pragma unroll
+          for (int e = 0; e < 32; e += 4)
+            out[(d + e) / 4 * BT] = make_float4(__uint_as_float(r[e]), __uint_as_float(r[e + 1]), __uint_as_float(r[e + 2]), __uint_as_float(r[e + 3]));
+        }
+      }
       tc_fence_before();  // (the next item's first MMAs into them follow a later arrival)
     }
   }
@@ -455,7 +469,7 @@ packed_dkv_sm100_kernel(const PackedArgs a, const PackedPlan plan, const FastDiv
 // so that the exponentials of a step run while the dP of that step is formed.
 template <class T, int DP>
 __global__ void __launch_bounds__(kThreads, 1)
-packed_dq_sm100_kernel(const PackedArgs a, const PackedPlan plan, const FastDiv heads, const __grid_constant__ CUtensorMap tmQ,
+packed_dq_sm100_kernel(const PackedArgs a, const PackedPlan plan, const FastDiv heads, const int follows, const __grid_constant__ CUtensorMap tmQ,
                        const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmD) {
   using C = DqCfg<DP>;
   constexpr int NK = C::kK, NV = C::kV;
@@ -487,7 +501,9 @@ packed_dq_sm100_kernel(const PackedArgs a, const PackedPlan plan, const FastDiv 
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
   }
-  grid_dependency_wait();
+  // Behind the kernel for dK and dV this one begins as its CTAs leave: it reads nothing of theirs before the end, and what it
+  // reads was complete before they began.
+  if (!follows) grid_dependency_wait();
   grid_launch_dependents();
   if (tid == 0) *abort_flag = (a.status && *reinterpret_cast<volatile int*>(a.status) != 0) ? 1 : 0;
   tc_fence_before();
@@ -495,7 +511,7 @@ packed_dq_sm100_kernel(const PackedArgs a, const PackedPlan plan, const FastDiv 
   tc_fence_after();
   const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
   const bool failed = *abort_flag != 0;
-  const int n_items = failed ? 0 : __ldcg(plan.counts) * (int)heads.d;
+  const int n_items = failed || !a.dq ? 0 : __ldcg(plan.counts) * (int)heads.d;
   auto item = [&](int idx, int& h) {
     const int tile = (int)heads.div((uint32_t)idx);
     h = idx - tile * (int)heads.d;
@@ -599,7 +615,7 @@ packed_dq_sm100_kernel(const PackedArgs a, const PackedPlan plan, const FastDiv 
       }
     } else {
       // =============================== K (warp 2) and V (warp 3): what lies behind the end; rows of no sequence ===============================
-      if (warp == 3 && !failed) clear_outside(a.offsets, a.wide, a.B, a.Tq, a.dq, a.H * a.D / 8, lane);
+      if (warp == 3 && !failed && a.dq) clear_outside(a.offsets, a.wide, a.B, a.Tq, a.dq, a.H * a.D / 8, lane);
 #pragma unroll 1
       for (int turn = 0, idx; (idx = item_of(turn)) < n_items; ++turn) {
         int h;
@@ -701,6 +717,34 @@ packed_dq_sm100_kernel(const PackedArgs a, const PackedPlan plan, const FastDiv 
       store_rows<T, DP / 2>(t_lane + C::colDQ + w * (DP / 2), static_cast<T*>(a.dq) + ((long long)(t.row + row) * a.H + h) * a.D, w * (DP / 2), a.D, a.scale, valid, any);
       tc_fence_before();  // (the next item's first dQ follows a later arrival)
     }
+    if (follows) {
+      // The parts of dK and dV, in order: 8 columns of a row a thread, neighbours have neighbouring rows.
+      grid_dependency_wait();
+      const int joins = failed ? 0 : __ldcg(plan.counts + 2);
+      constexpr int kPieces = 2 * DP / 8;  // of (dV, dK)
+      const int at = (warp - 4) * 32 + lane;
+#pragma unroll 1
+      for (int x = blockIdx.x * 2 + at / BT; x < joins * a.Hk * kPieces; x += gridDim.x * 2) {
+        const int piece = x % kPieces, hk = x / kPieces % a.Hk, r = at % BT, d = piece % (DP / 8) * 8;
+        const uint4 j = __ldcg(reinterpret_cast<const uint4*>(plan.joins + x / kPieces / a.Hk));  // row, rows, slot, parts
+        const bool is_dk = piece >= DP / 8;
+        if (r >= (int)j.y || d >= a.D) continue;
+        const float4* in = reinterpret_cast<const float4*>(plan.sums) + (((long long)j.z * a.Hk + hk) * 2 + is_dk) * (DP / 4 * BT) + d / 4 * BT + r;
+        float f[8] = {};
+#pragma unroll 4
+        for (int p = 0; p < (int)j.w; ++p) {
+          const float4 u = __ldcg(in), v = __ldcg(in + BT);
+          f[0] += u.x; f[1] += u.y; f[2] += u.z; f[3] += u.w;
+          f[4] += v.x; f[5] += v.y; f[6] += v.z; f[7] += v.w;
+          in += (long long)a.Hk * 2 * (DP / 4 * BT);
+        }
+        const float by = is_dk ? a.scale : 1.f;
+        uint32_t o[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) o[u] = Pack2<T>::pack(f[2 * u] * by, f[2 * u + 1] * by);
+        *reinterpret_cast<uint4*>(static_cast<T*>(is_dk ? a.dk : a.dv) + ((long long)(j.x + r) * a.Hk + hk) * a.D + d) = make_uint4(o[0], o[1], o[2], o[3]);
+      }
+    }
   }
 
   end_of_cta(abort_flag, a.status);
@@ -727,16 +771,17 @@ int launch(const PackedArgs& a, const PackedPlan& plan, cudaStream_t st, int* la
     auto kern = packed_dkv_sm100_kernel<T, DP>;
     const int rc = prepare(kern, DkvCfg<DP>::bytes);
     if (rc) return rc;
-    const long long most = key_tiles(a) * a.Hk;
+    const long long most = (key_tiles(a) + most_slots(a, sms)) * a.Hk;
     launch_dependent(kern, dim3((unsigned)(most < sms ? most : sms)), kThreads, DkvCfg<DP>::bytes, st, a, plan, FastDiv((uint32_t)a.Hk), tq, tk, tv, td);
     *launches += 1;
   }
-  if (a.dq) {
+  // (also where no dQ is wanted, if there may be parts of dK and dV to join)
+  if (a.dq || most_slots(a, sms) > 0) {
     auto kern = packed_dq_sm100_kernel<T, DP>;
     const int rc = prepare(kern, DqCfg<DP>::bytes);
     if (rc) return rc;
-    const long long most = query_units(a, BT) * a.H;
-    launch_dependent(kern, dim3((unsigned)(most < sms ? most : sms)), kThreads, DqCfg<DP>::bytes, st, a, plan, FastDiv((uint32_t)a.H), tq, tk, tv, td);
+    const long long most = a.dk ? sms : query_units(a, BT) * a.H;
+    launch_dependent(kern, dim3((unsigned)(most < sms ? most : sms)), kThreads, DqCfg<DP>::bytes, st, a, plan, FastDiv((uint32_t)a.H), (int)(a.dk != nullptr), tq, tk, tv, td);
     *launches += 1;
   }
   return cudaGetLastError() == cudaSuccess ? EVOATTN_OK : EVOATTN_ERR_CUDA;
@@ -749,13 +794,12 @@ size_t delta_bytes(const PackedArgs& a) { return ((size_t)a.H * a.Tq * sizeof(fl
 bool sm100_packed_bwd_supported(int dtype, const PackedArgs& a) {
   return sm100_packed_supported(dtype, a) && packed_map_ok(a.d_o, a.sdo, a.Tq, a.H) && ((reinterpret_cast<uintptr_t>(a.dq) | reinterpret_cast<uintptr_t>(a.dk) | reinterpret_cast<uintptr_t>(a.dv)) & 15) == 0;
 }
-size_t sm100_packed_bwd_workspace_bytes(const PackedArgs& a) { return delta_bytes(a) + plan_bytes(a, true, BT, true); }
+size_t sm100_packed_bwd_workspace_bytes(const PackedArgs& a) { return delta_bytes(a) + plan_bytes(a, true, BT, true, sm_count()).all(); }
 int launch_sm100_packed_bwd(int dtype, const PackedArgs& args, void* ws, cudaStream_t st, int* launches) {
   PackedArgs a = args;
   a.delta = static_cast<float*>(ws);
-  const PackedPlan plan = place_plan(a, static_cast<unsigned char*>(ws) + delta_bytes(a), true, BT);
-  int rc = launch_packed_plan(a, plan, true, BT, true, st, launches);
-  if (!rc) rc = launch_packed_delta(dtype, a, st, launches);
+  const PackedPlan plan = place_plan(static_cast<unsigned char*>(ws) + delta_bytes(a), plan_bytes(a, true, BT, true, sm_count()));
+  const int rc = launch_packed_prepare(dtype, a, plan, true, BT, true, true, st, launches);
   if (rc) return rc;
   if (dtype == EVOATTN_BF16) return a.D <= 64 ? launch<__nv_bfloat16, 64>(a, plan, st, launches) : launch<__nv_bfloat16, 128>(a, plan, st, launches);
   return a.D <= 64 ? launch<__half, 64>(a, plan, st, launches) : launch<__half, 128>(a, plan, st, launches);

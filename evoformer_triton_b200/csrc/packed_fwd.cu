@@ -35,6 +35,12 @@ template <class T> struct Lag;
 template <> struct Lag<__half> { static constexpr float kMaxSum = 32768.f, kRise = 8.f; };
 template <> struct Lag<__nv_bfloat16> { static constexpr float kMaxSum = 4294967296.f, kRise = 25.f; };
 
+#ifndef EMU
+#define EMU 4
+#endif
+// Which pairs of 16 go to the FMA pipes.
+__device__ __forceinline__ constexpr bool on_fma(int pair) { return pair * EMU / 16 != (pair + 1) * EMU / 16; }
+
 template <int DP>
 struct FwdCfg {
   static constexpr int kPanels = DP / 64;             // of 64 values: 128 bytes a row, swizzled
@@ -284,13 +290,20 @@ packed_fwd_sm100_kernel(const PackedArgs a, const PackedPlan plan, const FastDiv
                 const uint32_t* s = sr[k & 1];
 #pragma unroll
                 for (int e = 0; e < 32; e += 2) {
-                  float x0, x1;
-                  f2_get(f2_fma(f2_from_bits(s[e], s[e + 1]), c2, nm2), x0, x1);
-                  if constexpr (decltype(with_mask)::value) {
-                    x0 = 32 * k + e <= lim ? x0 : -kInf;
-                    x1 = 32 * k + e + 1 <= lim ? x1 : -kInf;
+                  const F2 x = f2_fma(f2_from_bits(s[e], s[e + 1]), c2, nm2);
+                  float p0, p1;
+                  if (!decltype(with_mask)::value && on_fma(e / 2)) {
+                    exp2_fma<T, true>(x, p0, p1);
+                  } else {
+                    float x0, x1;
+                    f2_get(x, x0, x1);
+                    if constexpr (decltype(with_mask)::value) {
+                      x0 = 32 * k + e <= lim ? x0 : -kInf;
+                      x1 = 32 * k + e + 1 <= lim ? x1 : -kInf;
+                    }
+                    p0 = ex2(x0);
+                    p1 = ex2(x1);
                   }
-                  const float p0 = ex2(x0), p1 = ex2(x1);
                   ls[(e / 2) & 3] = f2_add(ls[(e / 2) & 3], f2_make(p0, p1));
                   pk[16 * k + e / 2] = Pack2<T>::pack(p0, p1);
                 }
@@ -407,8 +420,8 @@ int launch(const PackedArgs& a, void* ws, cudaStream_t st, int* launches) {
   if (!kernel_ready(reinterpret_cast<const void*>(kern), (int)C::bytes, &regs)) return EVOATTN_ERR_CUDA;
   // (setmaxnreg.inc would wait for registers that the launch does not have)
   if (kThreads * regs < 256 * kSoftmaxRegs + 128 * kServiceRegs) return EVOATTN_ERR_UNSUPPORTED;
-  const PackedPlan plan = place_plan(a, ws, true, unit);
-  const int rc = launch_packed_plan(a, plan, true, unit, false, st, launches);
+  const PackedPlan plan = place_plan(ws, plan_bytes(a, true, unit, false, sms));
+  const int rc = launch_packed_prepare(std::is_same<T, __nv_bfloat16>::value ? EVOATTN_BF16 : EVOATTN_FP16, a, plan, true, unit, false, false, st, launches);
   if (rc) return rc;
   const int heads = PAIR ? a.H : a.H / 2;
   const long long most = query_units(a, unit) * heads;
@@ -431,7 +444,7 @@ bool sm100_packed_supported(int dtype, const PackedArgs& a) {
   if (reinterpret_cast<uintptr_t>(a.o) & 15) return false;
   return packed_map_ok(a.q, a.sq, a.Tq, a.H) && packed_map_ok(a.k, a.sk, a.Tk, a.Hk) && packed_map_ok(a.v, a.sv, a.Tk, a.Hk);
 }
-size_t sm100_packed_fwd_workspace_bytes(const PackedArgs& a) { return plan_bytes(a, true, head_pairs(a) ? BM : 2 * BM, false); }
+size_t sm100_packed_fwd_workspace_bytes(const PackedArgs& a) { return plan_bytes(a, true, head_pairs(a) ? BM : 2 * BM, false, sm_count()).all(); }
 int launch_sm100_packed_fwd(int dtype, const PackedArgs& a, void* ws, cudaStream_t st, int* launches) {
   if (dtype == EVOATTN_BF16) return launch_d<__nv_bfloat16>(a, ws, st, launches);
   return launch_d<__half>(a, ws, st, launches);

@@ -311,22 +311,6 @@ __global__ void __launch_bounds__(kThreads) packed_generic_dkv_kernel(const Pack
   }
 }
 
-// delta: a warp per row and head.
-template <class T>
-__global__ void __launch_bounds__(256) packed_delta_kernel(const PackedArgs a) {
-  const long long item = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
-  if (item >= (long long)a.Tq * a.H) return;
-  const long long t = item / a.H;
-  const int h = (int)(item % a.H);
-  const T* o = static_cast<const T*>(a.o) + item * a.D;
-  const T* d = static_cast<const T*>(a.d_o) + t * a.sdo[0] + (long long)h * a.sdo[1];
-  float s = 0.f;
-  for (int x = lane; x < a.D; x += 32) s = fmaf(to_float(o[x]), to_float(d[x]), s);
-  s = warp_sum(s);
-  if (lane == 0) a.delta[(long long)h * a.lse_ld + t] = s;
-}
-
 template <class K>
 int run(K kern, const PackedArgs& a, long long rows, int tile, int heads, size_t smem, cudaStream_t st, int* launches) {
   if (!kernel_ready(reinterpret_cast<const void*>(kern), (int)smem, nullptr)) return EVOATTN_ERR_CUDA;
@@ -363,12 +347,4 @@ int launch_packed_generic_bwd(int dtype, const PackedArgs& a, cudaStream_t st, i
     return a.D <= 64 ? bwd<T, 64>(a, st, launches) : a.D <= 128 ? bwd<T, 128>(a, st, launches) : bwd<T, 256>(a, st, launches);
   });
 }
-int launch_packed_delta(int dtype, const PackedArgs& a, cudaStream_t st, int* launches) {
-  return with_dtype(dtype, [&](auto t) {
-    packed_delta_kernel<decltype(t)><<<(unsigned)(((long long)a.Tq * a.H + 7) / 8), 256, 0, st>>>(a);
-    *launches += 1;
-    return cudaGetLastError() == cudaSuccess ? EVOATTN_OK : EVOATTN_ERR_CUDA;
-  });
-}
-
 }  // namespace evo

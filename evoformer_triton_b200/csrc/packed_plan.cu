@@ -1,91 +1,216 @@
-// The lists of tiles that the tensor-core kernels of attention over packed sequences walk, made on the device, where the
-// offsets are: a counting sort by the work of a tile, most first, so that what a persistent grid ends with is short.
+// What precedes the tensor-core kernels of attention over packed sequences: the lists of tiles that they walk, made on the
+// device, where the offsets are, and the row sums of dO * O for the backward, in one launch.
 #include "packed_sm100.cuh"
 
 namespace evo {
 namespace {
 
-constexpr int kThreads = 1024, kClasses = 2048;  // tiles that meet more than kClasses others are of one class
+constexpr int kThreads = 512;
+constexpr int kClasses = 2048;  // by work; what has more is of one class
 
-// A warp per sequence, its lanes over the tiles.
-template <class F>
-__device__ __forceinline__ void each_tile(const PackedArgs& a, bool queries, int unit, F&& f) {
-  for (int b = threadIdx.x >> 5; b < a.B; b += kThreads / 32) {
-    const Span q = query_span(a, b), k = key_span(a, b);
-    const int n = !queries ? k.n : q.n > a.few_tokens ? q.n : 0;
-    for (int x = (threadIdx.x & 31) * unit; x < n; x += 32 * unit) {
-      PackedTile t{};
-      t.rows = min(unit, n - x);
-      if (queries) {
-        t.row = q.begin + x;
-        t.other = k.begin;
-        t.n = k.n;
-        t.shift = x + k.n - q.n;
-        t.tiles = (keys_seen(a, q.n, k.n, x, unit) + kTileRows - 1) / kTileRows;
-      } else {
-        t.row = k.begin + x;
-        t.other = q.begin;
-        t.n = q.n;
-        t.shift = x + q.n - k.n;
-        const int first = a.causal ? max(0, t.shift) : 0;  // the first query that sees a key of the tile
-        t.tiles = first < q.n ? (q.n + kTileRows - 1) / kTileRows - first / kTileRows : 0;
+struct Sums {
+  int first[kClasses];
+  int warps[kThreads / 32 + 1];
+  long long steps;
+  int slots, joins;
+};
+
+// The tiles of all sequences, a warp per sequence and its lanes over the tiles; called several times, so the spans of the
+// first sequence (with 16 or fewer the only one) stay in registers.
+struct Tiles {
+  Span q, k;
+  __device__ __forceinline__ Tiles(const PackedArgs& a) {
+    const int b = threadIdx.x >> 5;
+    if (b < a.B) { q = query_span(a, b); k = key_span(a, b); }
+  }
+  template <class F>
+  __device__ __forceinline__ void each(const PackedArgs& a, bool queries, int unit, F&& f) const {
+    for (int b = threadIdx.x >> 5; b < a.B; b += kThreads / 32) {
+      const bool mine = b < kThreads / 32;
+      const Span qs = mine ? q : query_span(a, b), ks = mine ? k : key_span(a, b);
+      const int n = !queries ? ks.n : qs.n > a.few_tokens ? qs.n : 0;
+      for (int x = (threadIdx.x & 31) * unit; x < n; x += 32 * unit) {
+        PackedTile t{};
+        t.rows = min(unit, n - x);
+        t.parts = 1;
+        if (queries) {
+          t.row = qs.begin + x;
+          t.other = ks.begin;
+          t.n = ks.n;
+          t.shift = x + ks.n - qs.n;
+          t.tiles = (keys_seen(a, qs.n, ks.n, x, unit) + kTileRows - 1) / kTileRows;
+          t.steps = t.tiles;
+        } else {
+          t.row = ks.begin + x;
+          t.other = qs.begin;
+          t.n = qs.n;
+          t.shift = x + qs.n - ks.n;
+          const int first = a.causal ? max(0, t.shift) : 0;  // the first query that sees a key of the tile
+          t.tiles = first < qs.n ? (qs.n + kTileRows - 1) / kTileRows - first / kTileRows : 0;
+          t.steps = t.tiles * a.G;
+        }
+        f(t);
       }
-      f(t);
+    }
+  }
+};
+
+// A list by a counting sort, most work first, so that what a persistent grid ends with is short.  Key tiles whose steps are
+// more than `share` times those of an SM are cut into parts, which leave fp32 sums to be joined: a group of
+// heads or a long sequence makes single tiles that would outlast everything else.
+__device__ __forceinline__ void make_list(const PackedArgs& a, const PackedPlan& plan, bool queries, int unit, int sms, Sums& s) {
+  const Tiles tiles(a);
+  PackedTile* out = queries ? plan.queries : plan.keys;
+  for (int i = threadIdx.x; i < kClasses; i += kThreads) s.first[i] = 0;
+  if (threadIdx.x == 0) { s.steps = 0; s.slots = 0; s.joins = 0; }
+  __syncthreads();
+  int longest = kLongest;
+  if (!queries) {
+    long long sum = 0;
+    tiles.each(a, false, unit, [&](const PackedTile& t) { sum += t.steps; });
+    if (sum) atomicAdd(reinterpret_cast<unsigned long long*>(&s.steps), (unsigned long long)sum);
+    __syncthreads();
+    longest = part_steps(s.steps * a.Hk, sms);
+  }
+  auto place = [](int steps) { return kClasses - 1 - min(steps, kClasses - 1); };
+  auto cut = [&](const PackedTile& t) { return t.steps > longest ? (t.steps + longest - 1) / longest : 1; };
+  tiles.each(a, queries, unit, [&](const PackedTile& t) {
+    const int parts = cut(t);
+    atomicAdd(&s.first[place((t.steps + parts - 1) / parts)], parts);
+  });
+  __syncthreads();
+  // exclusive sums of the classes, four a thread
+  constexpr int kEach = kClasses / kThreads;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int x[kEach], own = 0;
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) own += x[i] = s.first[kEach * threadIdx.x + i];
+  int sum = own;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int up = __shfl_up_sync(0xffffffffu, sum, o);
+    if (lane >= o) sum += up;
+  }
+  if (lane == 31) s.warps[warp] = sum;
+  __syncthreads();
+  int before = sum - own, all = 0;
+  for (int w = 0; w < kThreads / 32; ++w) {
+    if (w < warp) before += s.warps[w];
+    all += s.warps[w];
+  }
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    s.first[kEach * threadIdx.x + i] = before;
+    before += x[i];
+  }
+  if (threadIdx.x == 0) plan.counts[queries ? 0 : 1] = all;
+  __syncthreads();
+  tiles.each(a, queries, unit, [&](PackedTile t) {
+    const int steps = t.steps, parts = cut(t), each = (steps + parts - 1) / parts;
+    if (parts > 1) {
+      t.slot = atomicAdd(&s.slots, parts);
+      plan.joins[atomicAdd(&s.joins, 1)] = PackedJoin{t.row, t.rows, t.slot, parts};
+    }
+    const int at = atomicAdd(&s.first[place(each)], parts);
+    t.parts = parts;
+    for (int p = 0; p < parts; ++p) {
+      t.begin = p * each;
+      t.steps = min(each, steps - t.begin);
+      out[at + p] = t;
+      ++t.slot;
+    }
+  });
+  __syncthreads();
+  if (threadIdx.x == 0 && !queries) plan.counts[2] = s.joins;
+}
+
+// delta: VEC values of 16 bytes at a time, `lanes` lanes a row (a power of two), four rows of a lane on their way.
+template <class T, bool VEC>
+__device__ __forceinline__ void row_sums(const PackedArgs& a, long long block, long long blocks, int lanes, const FastDiv& heads) {
+  const int team = threadIdx.x / lanes, lane = threadIdx.x % lanes, teams = kThreads / lanes;
+  const long long items = (long long)a.Tq * a.H;
+  const T* o = static_cast<const T*>(a.o);
+  const T* d_o = static_cast<const T*>(a.d_o);
+  constexpr int V = VEC ? kPer16<T> : 1, U = 4;
+  for (long long i0 = block * teams * U + team; i0 < items; i0 += blocks * teams * U) {
+    float s[U] = {};
+    long long to[U];
+    const T* d[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const long long i = i0 + (long long)u * teams;
+      const long long t = i < items ? (items <= 0x7fffffffLL ? (long long)heads.div((uint32_t)i) : i / a.H) : 0;
+      const int h = i < items ? (int)(i - t * a.H) : 0;
+      d[u] = d_o + t * a.sdo[0] + (long long)h * a.sdo[1];
+      to[u] = (long long)h * a.lse_ld + t;
+    }
+    for (int x = lane * V; x < a.D; x += lanes * V) {
+      if constexpr (VEC) {
+        uint4 w[U], z[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const long long i = min(i0 + (long long)u * teams, items - 1);
+          w[u] = *reinterpret_cast<const uint4*>(o + i * a.D + x);
+          z[u] = *reinterpret_cast<const uint4*>(d[u] + x);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          float f[V], g[V];
+          unpack16<T>(w[u], f);
+          unpack16<T>(z[u], g);
+#pragma unroll
+          for (int e = 0; e < V; ++e) s[u] = fmaf(f[e], g[e], s[u]);
+        }
+      } else {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const long long i = min(i0 + (long long)u * teams, items - 1);
+          s[u] = fmaf(to_float(o[i * a.D + x]), to_float(d[u][x]), s[u]);
+        }
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      for (int m = lanes / 2; m > 0; m >>= 1) s[u] += __shfl_xor_sync(0xffffffffu, s[u], m);
+      if (lane == 0 && i0 + (long long)u * teams < items) a.delta[to[u]] = s[u];
     }
   }
 }
 
-__global__ void __launch_bounds__(kThreads) packed_plan_kernel(const PackedArgs a, const PackedPlan plan, const int queries, const int unit, const int keys) {
-  __shared__ int first[kClasses];
-  __shared__ int sums[33];
+// Block 0 makes the list of queries, block 1 (or 0) that of keys, the others the row sums.
+template <class T, bool VEC>
+__global__ void __launch_bounds__(kThreads) packed_prepare_kernel(const PackedArgs a, const PackedPlan plan, const int queries, const int unit, const int keys,
+                                                                  const int sms, const int lanes, const FastDiv heads) {
+  __shared__ Sums s;
   ptx::grid_dependency_wait();
   ptx::grid_launch_dependents();
-  for (int list = 0; list < 2; ++list) {
-    if (!(list == 0 ? queries : keys)) continue;
-    const int u = list == 0 ? unit : kTileRows;
-    PackedTile* out = list == 0 ? plan.queries : plan.keys;
-    __syncthreads();
-    for (int i = threadIdx.x; i < kClasses; i += kThreads) first[i] = 0;
-    __syncthreads();
-    auto place = [](const PackedTile& t) { return kClasses - 1 - min(t.tiles, kClasses - 1); };
-    each_tile(a, list == 0, u, [&](const PackedTile& t) { atomicAdd(&first[place(t)], 1); });
-    __syncthreads();
-    // exclusive sums of the classes: two a thread
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int x0 = first[2 * threadIdx.x], x1 = first[2 * threadIdx.x + 1];
-    int sum = x0 + x1;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int up = __shfl_up_sync(0xffffffffu, sum, o);
-      if (lane >= o) sum += up;
-    }
-    if (lane == 31) sums[warp] = sum;
-    __syncthreads();
-    if (warp == 0) {
-      int s = sums[lane];
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int up = __shfl_up_sync(0xffffffffu, s, o);
-        if (lane >= o) s += up;
-      }
-      sums[lane] = s;
-    }
-    __syncthreads();
-    const int before = sum - x0 - x1 + (warp ? sums[warp - 1] : 0);
-    first[2 * threadIdx.x] = before;
-    first[2 * threadIdx.x + 1] = before + x0;
-    if (threadIdx.x == 0) plan.counts[list] = sums[31];
-    __syncthreads();
-    each_tile(a, list == 0, u, [&](const PackedTile& t) { out[atomicAdd(&first[place(t)], 1)] = t; });
+  const int lists = queries + keys;
+  if ((int)blockIdx.x < lists) {
+    const bool q = queries && blockIdx.x == 0;
+    make_list(a, plan, q, q ? unit : kTileRows, sms, s);
+  } else {
+    row_sums<T, VEC>(a, blockIdx.x - lists, gridDim.x - lists, lanes, heads);
   }
 }
 
 }  // namespace
 
-int launch_packed_plan(const PackedArgs& a, const PackedPlan& plan, bool queries, int unit, bool keys, cudaStream_t st, int* launches) {
-  launch_dependent(packed_plan_kernel, dim3(1), kThreads, 0, st, a, plan, (int)queries, unit, (int)keys);
-  *launches += 1;
-  return cudaGetLastError() == cudaSuccess ? EVOATTN_OK : EVOATTN_ERR_CUDA;
+int launch_packed_prepare(int dtype, const PackedArgs& a, const PackedPlan& plan, bool queries, int unit, bool keys, bool delta, cudaStream_t st, int* launches) {
+  const int sms = sm_count();
+  if (sms <= 0) return EVOATTN_ERR_CUDA;
+  return with_dtype(dtype, [&](auto t) {
+    using T = decltype(t);
+    constexpr int V = kPer16<T>;
+    const bool vec = delta && a.D % V == 0 && ((reinterpret_cast<uintptr_t>(a.o) | reinterpret_cast<uintptr_t>(a.d_o)) & 15) == 0 && a.sdo[0] % V == 0 && a.sdo[1] % V == 0;
+    int lanes = 1;
+    while (lanes < 32 && lanes * (vec ? V : 1) < a.D) lanes *= 2;
+    const long long rows = ((long long)a.Tq * a.H + kThreads / lanes * 4 - 1) / (kThreads / lanes * 4);
+    const int blocks = (queries ? 1 : 0) + (keys ? 1 : 0) + (delta ? (int)(rows < sms * 4LL ? rows : sms * 4LL) : 0);
+    launch_dependent(vec ? packed_prepare_kernel<T, true> : packed_prepare_kernel<T, false>, dim3((unsigned)blocks), kThreads, 0, st, a, plan, (int)queries, unit, (int)keys,
+                     sms, lanes, FastDiv((uint32_t)a.H));
+    *launches += 1;
+    return cudaGetLastError() == cudaSuccess ? EVOATTN_OK : EVOATTN_ERR_CUDA;
+  });
 }
 
 }  // namespace evo

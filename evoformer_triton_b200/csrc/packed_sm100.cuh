@@ -11,35 +11,65 @@ namespace evo {
 constexpr int kTileRows = 128;
 constexpr float kLog2e = 1.4426950408889634f;
 
-// A tile of queries with the keys that it meets, or of keys with the queries.
+// A tile of queries with the keys that it meets, or of keys (or a part of one) with the queries.
 struct PackedTile {
   int row, rows;    // first row of the tile in its tensor, rows of the sequence from there on (at most the tile's)
   int other, n;     // first row of the sequence in the other tensor, its rows there
   int shift;        // position of the tile's first row as the other tensor counts: query i sees the keys up to i + shift,
                     // key j is seen by the queries from j + shift on
-  int tiles;        // tiles of 128 rows of the other tensor that it meets: [0, tiles) of the keys; the last ones of the queries
+  int tiles;        // tiles of 128 rows of the other tensor that it meets: the first ones of the keys; the last ones of the queries
+  int begin, steps; // of the steps of a key tile (the tiles of the group's heads, one after another) this part's
+  int parts, slot;  // parts of the tile, and where this one leaves its sums
   int pad[2];
 };
-static_assert(sizeof(PackedTile) == 32, "two 16-byte loads");
-
-// Where lists lie in a workspace: 256 bytes with their lengths, then the tiles.
-struct PackedPlan {
-  int* counts;               // [0] query units, [1] key tiles
-  PackedTile *queries, *keys;
+static_assert(sizeof(PackedTile) == 48, "three 16-byte loads");
+struct PackedJoin {
+  int row, rows, slot, parts;
 };
+
+// Where lists lie in a workspace: 256 bytes with their lengths, the tiles, the key tiles whose parts are to be joined and the parts.
+struct PackedPlan {
+  int* counts;               // [0] query units, [1] key tiles and parts, [2] joins
+  PackedTile *queries, *keys;
+  PackedJoin* joins;
+  float* sums;               // [slot][Hk][dV, dK][DP / 4][128 rows][4]
+};
+// Steps of a part: half of what an SM has to do, and no fewer than kShortest, which is what a part costs by itself.
+constexpr int kShortest = 4, kLongest = 0x7fffffff;
+__host__ __device__ inline int part_steps(long long steps, int sms) {
+  const long long n = (steps + 2 * sms - 1) / (2 * sms);
+  return n < kShortest ? kShortest : n > kLongest ? kLongest : (int)n;
+}
 inline long long query_units(const PackedArgs& a, int unit) { return a.Tq / unit + a.B; }
 inline long long key_tiles(const PackedArgs& a) { return a.Tk / kTileRows + a.B; }
-inline size_t plan_bytes(const PackedArgs& a, bool queries, int unit, bool keys) {
-  const size_t n = (queries ? query_units(a, unit) : 0) + (keys ? key_tiles(a) : 0);
-  return (256 + n * sizeof(PackedTile) + 255) / 256 * 256;
+// A tile of more than n = part_steps() steps makes fewer than 2 steps / n parts, and all steps are at most 2 sms n: so all
+// heads' slots are fewer than 4 sms, and no more than kShortest allows.  The same bounds what parts add to the list.
+inline long long most_slots(const PackedArgs& a, int sms) {
+  const long long steps = (a.Tq / kTileRows + 1LL) * a.G, each = (steps + kShortest - 1) / kShortest, all = key_tiles(a) * each, most = (4LL * sms + a.Hk - 1) / a.Hk;
+  return each < 2 ? 0 : all < most ? all : most;
 }
-inline PackedPlan place_plan(const PackedArgs& a, void* ws, bool queries, int unit) {
+inline size_t round256(size_t n) { return (n + 255) / 256 * 256; }
+struct PlanBytes {
+  size_t queries, keys, joins, sums;
+  size_t all() const { return 256 + queries + keys + joins + sums; }
+};
+inline PlanBytes plan_bytes(const PackedArgs& a, bool queries, int unit, bool keys, int sms) {
+  const long long slots = keys ? most_slots(a, sms) : 0;
+  const int dp = a.D <= 64 ? 64 : 128;
+  return PlanBytes{queries ? round256(query_units(a, unit) * sizeof(PackedTile)) : 0, keys ? round256((key_tiles(a) + slots) * sizeof(PackedTile)) : 0,
+                   round256(slots * sizeof(PackedJoin)), round256((size_t)slots * a.Hk * 2 * kTileRows * dp * sizeof(float))};
+}
+inline PackedPlan place_plan(void* ws, const PlanBytes& n) {
   unsigned char* p = static_cast<unsigned char*>(ws);
-  PackedTile* q = reinterpret_cast<PackedTile*>(p + 256);
-  return PackedPlan{reinterpret_cast<int*>(p), q, q + (queries ? query_units(a, unit) : 0)};
+  PackedPlan plan{reinterpret_cast<int*>(p), nullptr, nullptr, nullptr, nullptr};
+  plan.queries = reinterpret_cast<PackedTile*>(p += 256);
+  plan.keys = reinterpret_cast<PackedTile*>(p += n.queries);
+  plan.joins = reinterpret_cast<PackedJoin*>(p += n.keys);
+  plan.sums = reinterpret_cast<float*>(p + n.joins);
+  return plan;
 }
-// Writes the lists, those with the most work first (packed_plan.cu).
-int launch_packed_plan(const PackedArgs& a, const PackedPlan& plan, bool queries, int unit, bool keys, cudaStream_t st, int* launches);
+// Writes the lists, those with the most work first, and the row sums of dO * O, in one launch (packed_plan.cu).
+int launch_packed_prepare(int dtype, const PackedArgs& a, const PackedPlan& plan, bool queries, int unit, bool keys, bool delta, cudaStream_t st, int* launches);
 
 // [T][heads][D] rows of 16 bits as a 3-D map (D, T, heads) with boxes of 64 values (128 bytes, swizzled) by `rows`;
 // values beyond D and rows beyond T read as zero.
@@ -63,9 +93,47 @@ int launch_sm100_packed_bwd(int dtype, const PackedArgs& a, void* workspace, cud
 size_t packed_few_workspace_bytes(const PackedArgs& a);
 int launch_packed_few(int dtype, const PackedArgs& a, bool clear, void* workspace, cudaStream_t st, int* launches);
 
+// 2^x of two values on the FMA pipes, for a part of the exponentials of a tile: the special-function units make 16 a cycle
+// and SM, which is as long as the tile's MMAs take (head dimension 128) or twice that (64).  x = n + f with n whole (by
+// adding and taking off 1.5 2^23) and |f| <= 1/2; 2^f by a polynomial whose largest relative error is the smallest there
+// is for its degree (fitted by exchange): 7.5e-5 of degree 3, 2.6e-6 of degree 4, a twenty-fifth and a hundredth of half a step of bf16 and fp16;
+// n is added to the exponent's bits.  Exponents below -126 count as that; with BOTH those above 126 too.
+template <class T, bool BOTH>
+__device__ __forceinline__ void exp2_fma(ptx::F2 x, float& p0, float& p1) {
+  using namespace ptx;
+  float x0, x1;
+  f2_get(x, x0, x1);
+  x0 = fmaxf(x0, -126.f);
+  x1 = fmaxf(x1, -126.f);
+  if constexpr (BOTH) {
+    x0 = fminf(x0, 126.f);
+    x1 = fminf(x1, 126.f);
+  }
+  x = f2_make(x0, x1);
+  const F2 t = f2_add(x, f2_make(12582912.f, 12582912.f));
+  const F2 f = f2_fma(f2_add(t, f2_make(-12582912.f, -12582912.f)), f2_make(-1.f, -1.f), x);
+  F2 p;
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+    p = f2_fma(f, f2_make(0.055171669f, 0.055171669f), f2_make(0.24261112f, 0.24261112f));
+    p = f2_fma(p, f, f2_make(0.69326099f, 0.69326099f));
+    p = f2_fma(p, f, f2_make(0.99992807f, 0.99992807f));
+  } else {
+    p = f2_fma(f, f2_make(0.0095701019f, 0.0095701019f), f2_make(0.05591786f, 0.05591786f));
+    p = f2_fma(p, f, f2_make(0.24024745f, 0.24024745f));
+    p = f2_fma(p, f, f2_make(0.69312181f, 0.69312181f));
+    p = f2_fma(p, f, f2_make(0.99999926f, 0.99999926f));
+  }
+  float t0, t1;
+  f2_get(t, t0, t1);
+  f2_get(p, p0, p1);
+  p0 = __uint_as_float(__float_as_uint(p0) + (__float_as_uint(t0) << 23));
+  p1 = __uint_as_float(__float_as_uint(p1) + (__float_as_uint(t1) << 23));
+}
+
 __device__ __forceinline__ PackedTile load_tile(const PackedTile* p) {
-  const uint4 u = __ldcg(reinterpret_cast<const uint4*>(p)), w = __ldcg(reinterpret_cast<const uint4*>(p) + 1);
-  return PackedTile{(int)u.x, (int)u.y, (int)u.z, (int)u.w, (int)w.x, (int)w.y, {0, 0}};
+  const uint4* x = reinterpret_cast<const uint4*>(p);
+  const uint4 u = __ldcg(x), v = __ldcg(x + 1), w = __ldcg(x + 2);
+  return PackedTile{(int)u.x, (int)u.y, (int)u.z, (int)u.w, (int)v.x, (int)v.y, (int)v.z, (int)v.w, (int)w.x, (int)w.y, {0, 0}};
 }
 // The items of a CTA in turns that go back and forth over the CTAs, so that the last one to get a long item is the first
 // to get a short one.
