@@ -7,8 +7,8 @@
 // (frequency / 2 pi) are formed in fp64 (off by 2^-53 of them), whole turns are taken off there, and sine and cosine are of
 // the fraction, which fp32 holds to 2^-26 of a turn.
 //
-// Bound by memory.  A block takes the tokens of a strip: sines and cosines of each once, into shared memory, then all
-// heads of q and k, 16 bytes at a time.
+// Bound by memory.  A block takes a strip of tokens: their sines and cosines once, into shared memory; then a thread keeps one
+// piece of a head (16 bytes, or two of them that make pairs), with its sines and cosines in registers, and walks heads.
 #include "inputs.cuh"
 
 namespace evo {
@@ -28,24 +28,53 @@ struct RotaryArgs {
   FastDiv inner, middle;      // tokens -> three axes
 };
 
-constexpr int kThreads = 256;
+// Two heads' loads at once a thread and some five heads a thread, four blocks an SM.  16 384 tokens of 40 heads of 128 bf16
+// values take 58 us (5.7 TB/s) so, 61 with one head at once, 63 with four (and two blocks), 61 with ten heads a thread.
+// Before, a thread took whatever pieces came, with the index arithmetic and the sines and cosines read again for each: 64.
+constexpr int kThreads = 256, kAtOnce = 2, kHeads = 5;
+constexpr int kMinBlocks = 6, kMostTokens = 16;  // blocks that every SM gets before they grow, up to this many tokens
 
-// V values are handled at once: V pairs (half) or V / 2 (neighbours).
+// 16 bytes of values, or one.
 template <class T, int V>
-__global__ void __launch_bounds__(kThreads) rotary_kernel(const RotaryArgs a, const int strip) {
-  extern __shared__ float2 turn[];  // [strip][n]: cos and sin, times the amplitude
-  const long long t0 = (long long)blockIdx.x * strip;
-  const int tokens = (int)(a.tokens - t0 < strip ? a.tokens - t0 : strip);
-  auto axes = [&](long long t, uint32_t& i0, uint32_t& i1, uint32_t& i2) {
-    const uint32_t u = a.inner.div((uint32_t)t);
-    i2 = (uint32_t)t - u * a.inner.d;
+struct Piece {
+  using Raw = uint4;
+  static __device__ __forceinline__ void get(const uint4& r, float* f) { unpack16<T>(r, f); }
+  static __device__ __forceinline__ uint4 put(const float* f) { return pack16<T>(f); }
+};
+template <class T>
+struct Piece<T, 1> {
+  using Raw = T;
+  static __device__ __forceinline__ void get(const T& r, float* f) { *f = to_float(r); }
+  static __device__ __forceinline__ T put(const float* f) { return from_float<T>(*f); }
+};
+
+struct Shape {
+  FastDiv head, lanes, pairs;  // pieces of a head; threads that share a token's heads; pairs of a token
+  int per, strip, side;        // pieces of a head that are turned; tokens of a block, and of a pass over its threads
+};
+
+// A piece is V values of the turned ones (half: two of them, n apart) or of the others.
+template <class T, int V, bool HALF>
+__global__ void __launch_bounds__(kThreads, 4) rotary_kernel(const RotaryArgs a, const Shape g) {
+  extern __shared__ __align__(16) float2 turn[];  // [strip][n]: cos and sin, times the amplitude
+  constexpr bool kTwo = HALF || V == 1;  // (one value at a time, neighbours are two pieces that are one apart)
+  constexpr int P = kTwo ? V : V / 2;    // pairs of a piece
+  using Chunk = typename Piece<T, V>::Raw;
+  ptx::grid_dependency_wait();
+  ptx::grid_launch_dependents();
+  const long long t0 = (long long)blockIdx.x * g.strip;
+  const int tokens = (int)(a.tokens - t0 < g.strip ? a.tokens - t0 : g.strip);
+  const int apart = HALF ? a.n : 1;
+  auto axes = [&](int t, uint32_t& i0, uint32_t& i1, uint32_t& i2) {
+    const uint32_t x = (uint32_t)(t0 + t), u = a.inner.div(x);
+    i2 = x - u * a.inner.d;
     i0 = a.middle.div(u);
     i1 = u - i0 * a.middle.d;
   };
   for (int i = threadIdx.x; i < tokens * a.n; i += kThreads) {
-    const int t = i / a.n, p = i - t * a.n;
+    const int t = (int)g.pairs.div((uint32_t)i), p = i - t * a.n;
     uint32_t i0, i1, i2;
-    axes(t0 + t, i0, i1, i2);
+    axes(t, i0, i1, i2);
     const long long at = i0 * a.sp[0] + i1 * a.sp[1] + i2 * a.sp[2];
     const double pos = (double)(a.wide ? static_cast<const long long*>(a.positions)[at] : (long long)static_cast<const int*>(a.positions)[at]);
     const double f = a.f64 ? static_cast<const double*>(a.frequencies)[p] : (double)static_cast<const float*>(a.frequencies)[p];
@@ -55,63 +84,90 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const RotaryArgs a, co
     turn[i] = make_float2(c * a.amplitude, s * a.amplitude * a.sign);
   }
   __syncthreads();
-  const int pairs_at_once = a.half || V == 1 ? V : V / 2;
-  const int per = a.n / pairs_at_once;                        // steps of a head's rotated values
-  const int all = per + (a.D - 2 * a.n) / V;                  // ... and of its others
-  const int heads = a.heads[0] + a.heads[1], per_token = heads * all;
-  for (int i = threadIdx.x; i < tokens * per_token; i += kThreads) {
-    const int t = i / per_token, r = i - t * per_token;
-    int h = r / all;
-    const int step = r - h * all;
-    const int which = h >= a.heads[0];
-    h -= which ? a.heads[0] : 0;
-    uint32_t i0, i1, i2;
-    axes(t0 + t, i0, i1, i2);
-    const T* x = static_cast<const T*>(a.x[which]) + i0 * a.sx[which][0] + i1 * a.sx[which][1] + i2 * a.sx[which][2] + h * a.sx[which][3];
-    T* y = static_cast<T*>(a.y[which]) + ((t0 + t) * a.heads[which] + h) * a.D;
-    struct alignas(sizeof(T) * V) Chunk { T v[V]; };
-    auto load = [&](int d) { return *reinterpret_cast<const Chunk*>(x + d); };
-    auto store = [&](int d, const Chunk& c) { *reinterpret_cast<Chunk*>(y + d) = c; };
-    if (step >= per) {
-      const int d = 2 * a.n + (step - per) * V;
-      store(d, load(d));
-    } else if (a.half || V == 1) {
-      const int d = a.half ? step * V : 2 * step, apart = a.half ? a.n : 1;  // (one pair at a time: neighbours are one apart)
-      Chunk u = load(d), w = load(d + apart);
+  const int heads = a.heads[0] + a.heads[1], lanes = (int)g.lanes.d;
+  // (a head may have more pieces than a block has threads: they take turns)
+  for (int first = 0; first < (int)g.head.d; first += kThreads) {
+    const int wide = min((int)g.head.d - first, kThreads);
+    const int group = first == 0 ? (int)g.head.div(threadIdx.x) : 0, step = first + (int)threadIdx.x - group * (int)g.head.d;
+    const int ti = (int)g.lanes.div((uint32_t)group), hl = group - ti * lanes;
+    if (ti >= g.side || step >= first + wide) continue;
+    const bool turned = step < g.per;
+    const int d = turned ? (kTwo && V == 1 && !HALF ? 2 * step : step * V) : 2 * a.n + (step - g.per) * V;
+    for (int t = ti; t < tokens; t += g.side) {
+      uint32_t i0, i1, i2;
+      axes(t, i0, i1, i2);
+      float2 cs[P];
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
-        const float2 cs = turn[t * a.n + step * V + e];
-        const float p = to_float(u.v[e]), q = to_float(w.v[e]);
-        u.v[e] = from_float<T>(p * cs.x - q * cs.y);
-        w.v[e] = from_float<T>(p * cs.y + q * cs.x);
-      }
-      store(d, u);
-      store(d + apart, w);
-    } else if constexpr (V > 1) {
-      const int d = step * V;
-      Chunk u = load(d);
+      for (int e = 0; e < P; ++e) cs[e] = turned ? turn[t * a.n + step * P + e] : make_float2(1.f, 0.f);
+      const T* x[2];
+      T* y[2];
 #pragma unroll
-      for (int e = 0; e < V; e += 2) {
-        const float2 cs = turn[t * a.n + (d + e) / 2];
-        const float p = to_float(u.v[e]), q = to_float(u.v[e + 1]);
-        u.v[e] = from_float<T>(p * cs.x - q * cs.y);
-        u.v[e + 1] = from_float<T>(p * cs.y + q * cs.x);
+      for (int w = 0; w < 2; ++w) {
+        x[w] = static_cast<const T*>(a.x[w]) + i0 * a.sx[w][0] + i1 * a.sx[w][1] + i2 * a.sx[w][2] + d;
+        y[w] = static_cast<T*>(a.y[w]) + (t0 + t) * a.heads[w] * a.D + d;
       }
-      store(d, u);
+      for (int h0 = hl; h0 < heads; h0 += lanes * kAtOnce) {
+        Chunk u[kAtOnce], w[kAtOnce];
+        T* to[kAtOnce];
+#pragma unroll
+        for (int k = 0; k < kAtOnce; ++k) {
+          int h = h0 + k * lanes;
+          to[k] = nullptr;
+          if (h >= heads) continue;
+          const bool second = h >= a.heads[0];
+          h -= second ? a.heads[0] : 0;
+          const T* from = second ? x[1] + h * a.sx[1][3] : x[0] + h * a.sx[0][3];
+          to[k] = (second ? y[1] : y[0]) + h * a.D;
+          u[k] = *reinterpret_cast<const Chunk*>(from);
+          if (kTwo && turned) w[k] = *reinterpret_cast<const Chunk*>(from + apart);
+        }
+#pragma unroll
+        for (int k = 0; k < kAtOnce; ++k) {
+          if (to[k] == nullptr) continue;
+          if (turned) {
+            float p[V], q[V];
+            Piece<T, V>::get(u[k], p);
+            if (kTwo) Piece<T, V>::get(w[k], q);
+#pragma unroll
+            for (int e = 0; e < P; ++e) {
+              float &lo = p[kTwo ? e : 2 * e], &hi = kTwo ? q[e] : p[V > 1 ? 2 * e + 1 : 0];
+              const float x0 = lo, x1 = hi;
+              lo = x0 * cs[e].x - x1 * cs[e].y;
+              hi = x0 * cs[e].y + x1 * cs[e].x;
+            }
+            u[k] = Piece<T, V>::put(p);
+            if (kTwo) *reinterpret_cast<Chunk*>(to[k] + apart) = Piece<T, V>::put(q);
+          }
+          *reinterpret_cast<Chunk*>(to[k]) = u[k];
+        }
+      }
     }
   }
 }
 
-template <class T, int V>
+template <class T, int V, bool HALF>
 int launch(const RotaryArgs& a, cudaStream_t st) {
   const int sms = sm_count();
   if (sms <= 0) return EVOATTN_ERR_CUDA;
-  long long strip = a.tokens / (sms * 16LL);
-  strip = strip < 1 ? 1 : strip > 8 ? 8 : strip;
-  const size_t smem = (size_t)strip * a.n * sizeof(float2);
-  auto kern = rotary_kernel<T, V>;
+  Shape g;
+  g.per = a.n / (HALF || V == 1 ? V : V / 2);
+  const int head = g.per + (a.D - 2 * a.n) / V, heads = a.heads[0] + a.heads[1];
+  g.head = FastDiv((uint32_t)head);
+  g.pairs = FastDiv((uint32_t)a.n);
+  // a thread has kHeads heads of a token or so, fewer where there are few tokens
+  const int groups = head < kThreads ? kThreads / head : 1;
+  const long long few = a.tokens / (sms * (long long)kMinBlocks);  // tokens of a block that leave every SM some blocks
+  int lanes = (heads + kHeads - 1) / kHeads;
+  if (few * lanes < groups) lanes = (int)(groups / (few > 0 ? few : 1));
+  lanes = lanes > groups ? groups : lanes > heads ? heads : lanes;
+  g.lanes = FastDiv((uint32_t)lanes);
+  g.side = groups / lanes;
+  const int most = g.side > kMostTokens ? g.side : kMostTokens / g.side * g.side;
+  g.strip = (int)(few < g.side ? g.side : few < most ? few / g.side * g.side : most);
+  const size_t smem = (size_t)g.strip * a.n * sizeof(float2);
+  auto kern = rotary_kernel<T, V, HALF>;
   if (!kernel_ready(reinterpret_cast<const void*>(kern), (int)smem, nullptr)) return EVOATTN_ERR_CUDA;
-  kern<<<(unsigned)((a.tokens + strip - 1) / strip), kThreads, smem, st>>>(a, (int)strip);
+  launch_dependent(kern, dim3((unsigned)((a.tokens + g.strip - 1) / g.strip)), kThreads, smem, st, a, g);
   return cudaGetLastError() == cudaSuccess ? EVOATTN_OK : EVOATTN_ERR_CUDA;
 }
 
@@ -162,7 +218,8 @@ extern "C" int evoattn_rotary(const evoattn_rotary_params* p, void* cuda_stream)
   cudaStream_t st = reinterpret_cast<cudaStream_t>(cuda_stream);
   return with_dtype(p->dtype, [&](auto t) {
     using T = decltype(t);
-    if (wide) return launch<T, 16 / (int)sizeof(T)>(a, st);
-    return launch<T, 1>(a, st);
+    constexpr int V = 16 / (int)sizeof(T);
+    if (wide) return a.half ? launch<T, V, true>(a, st) : launch<T, V, false>(a, st);
+    return a.half ? launch<T, 1, true>(a, st) : launch<T, 1, false>(a, st);
   });
 }
