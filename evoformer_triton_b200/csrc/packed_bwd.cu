@@ -27,6 +27,11 @@ using namespace ptx;
 constexpr int BT = kTileRows;
 constexpr int kThreads = 384, kServiceRegs = 56, kComputeRegs = 224;
 
+#ifndef EMUB
+#define EMUB 4
+#endif
+__device__ __forceinline__ constexpr bool on_fma(int pair) { return pair * EMUB / 16 != (pair + 1) * EMUB / 16; }
+
 template <int DP>
 struct Tiles {
   static constexpr int kPanels = DP / 64, kPanel = BT * 128, kTile = kPanels * kPanel;
@@ -36,8 +41,11 @@ struct DkvCfg : Tiles<DP> {
   using Tiles<DP>::kTile;
   static constexpr int kStages = DP == 128 ? 2 : 3;
   static constexpr int offK = 0, offV = kTile, offQ = 2 * kTile, offD = offQ + kStages * kTile, offStats = offD + kStages * kTile;
-  static constexpr int offBars = offStats + kStages * 2 * BT * 4, kBars = 4 + 6 * kStages + 5;
-  static constexpr size_t bytes = offBars + kBars * 8 + 64 + 1024;
+  static constexpr int offOut = offStats + kStages * 2 * BT * 4, offBars = offOut + 8 * kStageBytes, kBars = 4 + 6 * kStages + 5 + 4;
+  // What aligning the tiles to 1024 bytes may take: less than that would leave no room at DP = 128, where the kernel checks that
+  // it is enough (the dynamic shared memory of a kernel without static shared memory starts on such a boundary here).
+  static constexpr int kSlack = DP == 128 ? 512 : 1024;
+  static constexpr size_t bytes = offBars + kBars * 8 + 64 + kSlack;
   static_assert(bytes <= 232448, "shared memory of one CTA");
   static constexpr int colS = 0, colP = BT, colDV = 2 * BT, colDK = colDV + DP;
   static_assert(colDK + DP <= 512, "tensor memory");
@@ -47,7 +55,7 @@ struct DqCfg : Tiles<DP> {
   using Tiles<DP>::kTile;
   static constexpr int kK = 3, kV = 2;
   static constexpr int offQ = 0, offD = kTile, offK = 2 * kTile, offV = offK + kK * kTile;
-  static constexpr int offBars = offV + kV * kTile, kBars = 2 + 3 * (kK + kV) + 5;
+  static constexpr int offBars = offV + kV * kTile, kBars = 2 + 3 * (kK + kV) + 5 + 4;
   static constexpr size_t bytes = offBars + kBars * 8 + 64 + 1024;
   static_assert(bytes <= 232448, "shared memory of one CTA");
   static constexpr int colS = 0, colP = 2 * BT, colDQ = 3 * BT;
@@ -140,11 +148,16 @@ __device__ __forceinline__ void store_rows(uint32_t t_src, T* out, int d0, int D
 template <class T, int DP>
 __global__ void __launch_bounds__(kThreads, 1)
 packed_dkv_sm100_kernel(const PackedArgs a, const PackedPlan plan, const FastDiv heads, const __grid_constant__ CUtensorMap tmQ,
-                        const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmD) {
+                        const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmD,
+                        const __grid_constant__ CUtensorMap tmDK, const __grid_constant__ CUtensorMap tmDV) {
   using C = DkvCfg<DP>;
   constexpr int NS = C::kStages;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  if (static_cast<int>(smem - smem_raw) > C::kSlack) {  // the same for every thread of every CTA
+    if (threadIdx.x == 0 && a.status) atomicCAS(a.status, 0, DEV_TIMEOUT_SYNC);
+    return;
+  }
   const uint32_t smem_s = smem_u32(smem);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::offBars);
   const uint32_t b0 = smem_u32(bars);
@@ -155,7 +168,7 @@ packed_dkv_sm100_kernel(const PackedArgs a, const PackedPlan plan, const FastDiv
   auto d_in = [&](uint32_t s) { return b0 + 8 * (4 + 3 * NS + s); };       // the same for dO
   auto d_full = [&](uint32_t s) { return b0 + 8 * (4 + 4 * NS + s); };
   auto d_empty = [&](uint32_t s) { return b0 + 8 * (4 + 5 * NS + s); };
-  const uint32_t s_full = b0 + 8 * (4 + 6 * NS), p_full = s_full + 8, dp_full = s_full + 16, ds_full = s_full + 24, out_full = s_full + 32;
+  const uint32_t s_full = b0 + 8 * (4 + 6 * NS), p_full = s_full + 8, dp_full = s_full + 16, ds_full = s_full + 24, out_full = s_full + 32, sched = s_full + 40;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + C::kBars);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + C::kBars + 1);
   const uint32_t abort_s = smem_u32(const_cast<int*>(abort_flag));
@@ -163,7 +176,7 @@ packed_dkv_sm100_kernel(const PackedArgs a, const PackedPlan plan, const FastDiv
   const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
 
   if (tid == 0) {
-    for (int i = 0; i < C::kBars; ++i) mbar_init_s(b0 + 8 * i, b0 + 8 * i == p_full || b0 + 8 * i == ds_full ? 8 : 1);
+    for (int i = 0; i < C::kBars; ++i) mbar_init_s(b0 + 8 * i, b0 + 8 * i == p_full || b0 + 8 * i == ds_full ? 8 : b0 + 8 * i >= sched + 16 ? 11 : 1);
     fence_mbar_init();
     prefetch_tmap(&tmQ); prefetch_tmap(&tmK); prefetch_tmap(&tmV); prefetch_tmap(&tmD);
   }
@@ -179,12 +192,12 @@ packed_dkv_sm100_kernel(const PackedArgs a, const PackedPlan plan, const FastDiv
   tc_fence_after();
   const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
   const bool failed = *abort_flag != 0;
-  const int n_items = failed ? 0 : __ldcg(plan.counts + 1) * (int)heads.d;
+  Schedule todo{sched, sched + 16, abort_s + 4, abort_s, plan.counts + 5, failed ? 0 : __ldcg(plan.counts + 1) * (int)heads.d};
 
   // The steps of a CTA, one after another over its items: head g of the group, query tile i, `left` of the item from here on.
   struct Step {
     PackedTile t;
-    int hk, turn, g, i, end, left;
+    int hk, g, i, end, left;
     __device__ __forceinline__ bool first() const { return left == t.steps; }
     __device__ __forceinline__ bool last() const { return left == 1; }
     __device__ __forceinline__ int real() const { return t.n - i * BT; }
@@ -202,8 +215,8 @@ packed_dkv_sm100_kernel(const PackedArgs a, const PackedPlan plan, const FastDiv
     s.g = s.t.tiles ? s.t.begin / s.t.tiles : 0;
     s.i = s.end - s.t.tiles + s.t.begin - s.g * s.t.tiles;
   };
-  auto begin = [&](Step& s) {  // the first step of the next item that has any, from s.turn on
-    for (int idx; (idx = item_of(s.turn)) < n_items; ++s.turn) {
+  auto begin = [&](Step& s, int idx) {  // the first step of that item, or of the next one that has any
+    for (; !todo.over(idx); idx = warp == 0 ? todo.take() : todo.next()) {
       item(idx, s);
       if (s.left > 0) return true;
     }
@@ -211,16 +224,13 @@ packed_dkv_sm100_kernel(const PackedArgs a, const PackedPlan plan, const FastDiv
   };
   auto advance = [&](Step& s) {
     s.next();
-    if (s.left > 0) return true;
-    ++s.turn;
-    return begin(s);
+    return s.left > 0 || begin(s, warp == 0 ? todo.take() : todo.next());
   };
 
   if (warp < 4) {
     setmaxnreg_dec<kServiceRegs>();
     Step s;
-    s.turn = 0;
-    bool more = begin(s);
+    bool more = begin(s, todo.first());
     uint32_t st = 0, par = 0;
     auto next = [&] { if (++st == NS) { st = 0; par ^= 1; } };
     if (warp == 0) {
@@ -365,7 +375,7 @@ packed_dkv_sm100_kernel(const PackedArgs a, const PackedPlan plan, const FastDiv
     const float kInf = __int_as_float(0x7f800000);
     uint32_t n = 0, kv = 0, st = 0, par = 0;
 #pragma unroll 1
-    for (int turn = 0, idx; (idx = item_of(turn)) < n_items; ++turn) {
+    for (int idx = todo.first(); !todo.over(idx); idx = todo.next()) {
       Step s;
       item(idx, s);
 #pragma unroll 1
@@ -373,32 +383,51 @@ packed_dkv_sm100_kernel(const PackedArgs a, const PackedPlan plan, const FastDiv
         // queries of this half before `lo` do not see the key
         const int lo = a.causal ? s.t.shift + row - s.i * BT - 64 * w : 0;
         const bool cut = __any_sync(0xffffffffu, lo > 0);
+        const int hidden = __shfl_sync(0xffffffffu, lo, 0) >> 5;  // pieces of 32 queries that do not see any key of the warp
         const uint32_t stats = smem_s + C::offStats + st * (2 * BT * 4) + 64 * w * 4;
         mbar_wait_s(q_full(st), par, abort_s, DEV_TIMEOUT_SYNC);
         mbar_wait_s(s_full, n & 1, abort_s, DEV_TIMEOUT_MMA);
         tc_fence_after();
         F2 p[32];
         auto exps = [&](auto with_mask) {
+          constexpr bool kMask = decltype(with_mask)::value;
           uint32_t sr[2][32];
-          tmem_ld32(tS, sr[0]);
+          if (!kMask) tmem_ld32(tS, sr[0]);
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
-            tmem_wait_ld();
-            if (k == 0) tmem_ld32(tS + 32, sr[1]);
             uint32_t pk[16];
+            if (kMask && k < hidden) {
+#pragma unroll
+              for (int e = 0; e < 16; ++e) {
+                p[16 * k + e] = f2_make(0.f, 0.f);
+                pk[e] = 0u;
+              }
+              tmem_st16(tS + 16 * k, pk);
+              continue;
+            }
+            if (kMask) tmem_ld32(tS + 32 * k, sr[k]);
+            tmem_wait_ld();
+            if (!kMask && k == 0) tmem_ld32(tS + 32, sr[1]);
 #pragma unroll
             for (int e = 0; e < 32; e += 4) {
               const float4 nl = lds_v4f(stats + (32 * k + e) * 4);
               const F2 nl2[2] = {f2_make(nl.x, nl.y), f2_make(nl.z, nl.w)};
 #pragma unroll
               for (int u = 0; u < 2; ++u) {
-                float x0, x1;
-                f2_get(f2_fma(f2_from_bits(sr[k][e + 2 * u], sr[k][e + 2 * u + 1]), c2, nl2[u]), x0, x1);
-                if constexpr (decltype(with_mask)::value) {
-                  x0 = 32 * k + e + 2 * u >= lo ? x0 : -kInf;
-                  x1 = 32 * k + e + 2 * u + 1 >= lo ? x1 : -kInf;
+                const F2 x = f2_fma(f2_from_bits(sr[k][e + 2 * u], sr[k][e + 2 * u + 1]), c2, nl2[u]);
+                float p0, p1;
+                if (!kMask && on_fma(e / 2 + u)) {
+                  exp2_fma<T, false>(x, p0, p1);
+                } else {
+                  float x0, x1;
+                  f2_get(x, x0, x1);
+                  if constexpr (kMask) {
+                    x0 = 32 * k + e + 2 * u >= lo ? x0 : -kInf;
+                    x1 = 32 * k + e + 2 * u + 1 >= lo ? x1 : -kInf;
+                  }
+                  p0 = ex2(x0);
+                  p1 = ex2(x1);
                 }
-                const float p0 = ex2(x0), p1 = ex2(x1);
                 p[16 * k + e / 2 + u] = f2_make(p0, p1);
                 pk[e / 2 + u] = Pack2<T>::pack(p0, p1);
               }
@@ -443,8 +472,11 @@ packed_dkv_sm100_kernel(const PackedArgs a, const PackedPlan plan, const FastDiv
       }
       const uint32_t src = t_lane + (w == 0 ? C::colDV : C::colDK);
       if (s.t.parts == 1) {
-        const long long at = ((long long)(s.t.row + row) * a.Hk + s.hk) * a.D;
-        store_rows<T, DP>(src, static_cast<T*>(w == 0 ? a.dv : a.dk) + at, 0, a.D, w == 0 ? 1.f : a.scale, row < s.t.rows, any);
+        const int first = (warp & 3) * 32;  // row of the warp's first lane
+        const int at = s.t.row + first;
+        store_rows_staged<T, DP>(smem_s + C::offOut + (warp - 4) * kStageBytes, src, w == 0 ? &tmDV : &tmDK, at, s.hk,
+                                 static_cast<T*>(w == 0 ? a.dv : a.dk) + ((long long)at * a.Hk + s.hk) * a.D, (long long)a.Hk * a.D, s.t.rows - first, a.D,
+                                 w == 0 ? 1.f : a.scale, any);
       } else {
         float4* out = reinterpret_cast<float4*>(plan.sums) + (((long long)s.t.slot * a.Hk + s.hk) * 2 + w) * (DP / 4 * BT) + row;
 #pragma unroll
@@ -459,6 +491,7 @@ packed_dkv_sm100_kernel(const PackedArgs a, const PackedPlan plan, const FastDiv
       }
       tc_fence_before();  // (the next item's first MMAs into them follow a later arrival)
     }
+    stores_done();
   }
 
   end_of_cta(abort_flag, a.status);
@@ -485,7 +518,7 @@ packed_dq_sm100_kernel(const PackedArgs a, const PackedPlan plan, const FastDiv 
   auto v_in = [&](uint32_t s) { return b0 + 8 * (2 + 3 * NK + s); };
   auto v_full = [&](uint32_t s) { return b0 + 8 * (2 + 3 * NK + NV + s); };
   auto v_empty = [&](uint32_t s) { return b0 + 8 * (2 + 3 * NK + 2 * NV + s); };
-  const uint32_t s_full = b0 + 8 * (2 + 3 * (NK + NV)), dp_full = s_full + 16, ds_full = s_full + 24, out_full = s_full + 32;  // (s_full: two)
+  const uint32_t s_full = b0 + 8 * (2 + 3 * (NK + NV)), dp_full = s_full + 16, ds_full = s_full + 24, out_full = s_full + 32, sched = s_full + 40;  // (s_full: two)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + C::kBars);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + C::kBars + 1);
   const uint32_t abort_s = smem_u32(const_cast<int*>(abort_flag));
@@ -493,7 +526,7 @@ packed_dq_sm100_kernel(const PackedArgs a, const PackedPlan plan, const FastDiv 
   const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
 
   if (tid == 0) {
-    for (int i = 0; i < C::kBars; ++i) mbar_init_s(b0 + 8 * i, b0 + 8 * i == ds_full ? 8 : 1);
+    for (int i = 0; i < C::kBars; ++i) mbar_init_s(b0 + 8 * i, b0 + 8 * i == ds_full ? 8 : b0 + 8 * i >= sched + 16 ? 11 : 1);
     fence_mbar_init();
     prefetch_tmap(&tmQ); prefetch_tmap(&tmK); prefetch_tmap(&tmV); prefetch_tmap(&tmD);
   }
@@ -511,7 +544,7 @@ packed_dq_sm100_kernel(const PackedArgs a, const PackedPlan plan, const FastDiv 
   tc_fence_after();
   const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
   const bool failed = *abort_flag != 0;
-  const int n_items = failed || !a.dq ? 0 : __ldcg(plan.counts) * (int)heads.d;
+  Schedule todo{sched, sched + 16, abort_s + 4, abort_s, plan.counts + 4, failed || !a.dq ? 0 : __ldcg(plan.counts) * (int)heads.d};
   auto item = [&](int idx, int& h) {
     const int tile = (int)heads.div((uint32_t)idx);
     h = idx - tile * (int)heads.d;
@@ -527,7 +560,7 @@ packed_dq_sm100_kernel(const PackedArgs a, const PackedPlan plan, const FastDiv 
       // =============================== TMA producer ===============================
       uint32_t n = 0;
 #pragma unroll 1
-      for (int turn = 0, idx; (idx = item_of(turn)) < n_items; ++turn) {
+      for (int idx = todo.first(); !todo.over(idx); idx = todo.take()) {
         int h;
         const PackedTile t = item(idx, h);
         if (t.tiles == 0) continue;
@@ -569,7 +602,7 @@ packed_dq_sm100_kernel(const PackedArgs a, const PackedPlan plan, const FastDiv 
       uint32_t n = 0, n_item = 0, sn = 0;  // steps, items, scores
       uint32_t cs = 0;                     // K stage of the step whose dQ is next
 #pragma unroll 1
-      for (int turn = 0, idx; (idx = item_of(turn)) < n_items; ++turn) {
+      for (int idx = todo.first(); !todo.over(idx); idx = todo.next()) {
         int h;
         const PackedTile t = item(idx, h);
         if (t.tiles == 0) continue;
@@ -617,7 +650,7 @@ packed_dq_sm100_kernel(const PackedArgs a, const PackedPlan plan, const FastDiv 
       // =============================== K (warp 2) and V (warp 3): what lies behind the end; rows of no sequence ===============================
       if (warp == 3 && !failed && a.dq) clear_outside(a.offsets, a.wide, a.B, a.Tq, a.dq, a.H * a.D / 8, lane);
 #pragma unroll 1
-      for (int turn = 0, idx; (idx = item_of(turn)) < n_items; ++turn) {
+      for (int idx = todo.first(); !todo.over(idx); idx = todo.next()) {
         int h;
         const PackedTile t = item(idx, h);
 #pragma unroll 1
@@ -650,7 +683,7 @@ packed_dq_sm100_kernel(const PackedArgs a, const PackedPlan plan, const FastDiv 
     const float kInf = __int_as_float(0x7f800000);
     uint32_t n = 0, n_item = 0;
 #pragma unroll 1
-    for (int turn = 0, idx; (idx = item_of(turn)) < n_items; ++turn) {
+    for (int idx = todo.first(); !todo.over(idx); idx = todo.next()) {
       int h;
       const PackedTile t = item(idx, h);
       const bool valid = row < t.rows;
@@ -677,13 +710,21 @@ packed_dq_sm100_kernel(const PackedArgs a, const PackedPlan plan, const FastDiv 
             if (k == 0) tmem_ld32(tS + 32, sr[1]);
 #pragma unroll
             for (int e = 0; e < 32; e += 2) {
-              float x0, x1;
-              f2_get(f2_fma(f2_from_bits(sr[k][e], sr[k][e + 1]), c2, nl2), x0, x1);
-              if constexpr (decltype(with_mask)::value) {
-                x0 = 32 * k + e <= lim ? x0 : -kInf;
-                x1 = 32 * k + e + 1 <= lim ? x1 : -kInf;
+              const F2 v = f2_fma(f2_from_bits(sr[k][e], sr[k][e + 1]), c2, nl2);
+              float p0, p1;
+              if (!decltype(with_mask)::value && on_fma(e / 2)) {
+                exp2_fma<T, false>(v, p0, p1);
+              } else {
+                float x0, x1;
+                f2_get(v, x0, x1);
+                if constexpr (decltype(with_mask)::value) {
+                  x0 = 32 * k + e <= lim ? x0 : -kInf;
+                  x1 = 32 * k + e + 1 <= lim ? x1 : -kInf;
+                }
+                p0 = ex2(x0);
+                p1 = ex2(x1);
               }
-              p[16 * k + e / 2] = f2_make(ex2(x0), ex2(x1));
+              p[16 * k + e / 2] = f2_make(p0, p1);
             }
           }
         };
@@ -769,10 +810,13 @@ int launch(const PackedArgs& a, const PackedPlan& plan, cudaStream_t st, int* la
   if (sms <= 0) return EVOATTN_ERR_CUDA;
   if (a.dk) {
     auto kern = packed_dkv_sm100_kernel<T, DP>;
+    CUtensorMap tdk, tdv;
+    const long long sk[2] = {(long long)a.Hk * a.D, a.D};
+    if (!make_packed_map(&tdk, a.dk, sk, a.Tk, a.Hk, a.D, 32) || !make_packed_map(&tdv, a.dv, sk, a.Tk, a.Hk, a.D, 32)) return EVOATTN_ERR_CUDA;
     const int rc = prepare(kern, DkvCfg<DP>::bytes);
     if (rc) return rc;
     const long long most = (key_tiles(a) + most_slots(a, sms)) * a.Hk;
-    launch_dependent(kern, dim3((unsigned)(most < sms ? most : sms)), kThreads, DkvCfg<DP>::bytes, st, a, plan, FastDiv((uint32_t)a.Hk), tq, tk, tv, td);
+    launch_dependent(kern, dim3((unsigned)(most < sms ? most : sms)), kThreads, DkvCfg<DP>::bytes, st, a, plan, FastDiv((uint32_t)a.Hk), tq, tk, tv, td, tdk, tdv);
     *launches += 1;
   }
   // (also where no dQ is wanted, if there may be parts of dK and dV to join)

@@ -15,10 +15,10 @@
 // warpgroup are issued by one thread in the order P V of tile n, S of tile n - 1, so that S lands when O is complete up
 // to tile n and may be rescaled.
 //
-// m is not the maximum up to this tile but a reference that the exponentials of the tile are taken against straight from
-// the scores, without looking for their maximum: any m gives the same o as long as nothing overflows.  It is the first
-// tile's maximum; if a tile's sum shows that some p may be too large, the tile's maximum is taken, O and l follow
-// it, and the tile is done again (P is kept in registers until then).
+// m is not the maximum but a reference that the exponentials of a tile are taken against straight from the scores, without
+// looking for their maximum: any m gives the same o as long as nothing leaves the range of P's type.  It is 0 to begin with; if
+// a tile's sum shows that some p may be too large, or a row's first sum that all of them are too small, the tile's maximum
+// is taken, O and l follow it, and the tile is done again (P is kept in registers until then).
 #include "packed_sm100.cuh"
 
 namespace evo {
@@ -29,25 +29,24 @@ using namespace ptx;
 constexpr int BM = kTileRows, BN = kTileRows;
 constexpr int kThreads = 384, kServiceRegs = 56, kSoftmaxRegs = 224;
 
-// kMaxSum: sum of a tile's exponentials up to which they serve (fp16 ends at 2^16; bf16 and the fp32 sums hold any); kRise:
-// rise of a tile's maximum, in powers of two, up to which the sum of its 128 cannot be more.
+// kMaxSum: sum of a tile's exponentials up to which they serve (fp16 ends at 2^16; bf16 and the fp32 sums hold any); kMinSum:
+// the least first sum of a row (fp16 has steps of 2^-24: against a sum of 2^-4 that is what rounding P costs at 2^-10
+// of it); kRise: rise of a tile's maximum, in powers of two, up to which the sum of its 128 cannot be more.
 template <class T> struct Lag;
-template <> struct Lag<__half> { static constexpr float kMaxSum = 32768.f, kRise = 8.f; };
-template <> struct Lag<__nv_bfloat16> { static constexpr float kMaxSum = 4294967296.f, kRise = 25.f; };
+template <> struct Lag<__half> { static constexpr float kMaxSum = 32768.f, kMinSum = 0.0625f, kRise = 8.f; };
+template <> struct Lag<__nv_bfloat16> { static constexpr float kMaxSum = 4294967296.f, kMinSum = 0x1p-40f, kRise = 25.f; };
 
-#ifndef EMU
-#define EMU 4
-#endif
-// Which pairs of 16 go to the FMA pipes.
-__device__ __forceinline__ constexpr bool on_fma(int pair) { return pair * EMU / 16 != (pair + 1) * EMU / 16; }
+// Which pairs of values go to the FMA pipes: four of sixteen.  Forward of [16384] causal, 16 heads, us, with none, two, four,
+// six and eight: D = 128 (4 key heads) 923, 876, 852, 913, 973; D = 64 818, 759, 712, 737, 811.
+__device__ __forceinline__ constexpr bool on_fma(int pair) { return pair % 4 == 3; }
 
 template <int DP>
 struct FwdCfg {
   static constexpr int kPanels = DP / 64;             // of 64 values: 128 bytes a row, swizzled
   static constexpr int kPanel = BM * 128, kTile = kPanels * kPanel;
-  static constexpr int kStages = DP == 128 ? 5 : 8;   // K and V tiles in the order of their use
-  static constexpr int offQ = 0, offKV = 2 * kTile, offBars = offKV + kStages * kTile;
-  static constexpr int kBars = 2 * kStages + 2 + 6;
+  static constexpr int kStages = DP == 128 ? 4 : 8;   // K and V tiles in the order of their use
+  static constexpr int offQ = 0, offKV = 2 * kTile, offOut = offKV + kStages * kTile, offBars = offOut + 8 * kStageBytes;
+  static constexpr int kBars = 2 * kStages + 2 + 6 + 4;
   static constexpr size_t bytes = offBars + kBars * 8 + 64 + 1024;
   static_assert(bytes <= 232448, "shared memory of one CTA");
   static constexpr int colO = 2 * BN;                 // S of both warpgroups, then O of both
@@ -57,7 +56,7 @@ struct FwdCfg {
 template <class T, int DP, bool PAIR>  // PAIR: two query tiles of one head, else one tile of two heads
 __global__ void __launch_bounds__(kThreads, 1)
 packed_fwd_sm100_kernel(const PackedArgs a, const PackedPlan plan, const FastDiv units, const __grid_constant__ CUtensorMap tmQ,
-                        const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV) {
+                        const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmO) {
   using C = FwdCfg<DP>;
   constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
   constexpr int NS = C::kStages;
@@ -72,6 +71,7 @@ packed_fwd_sm100_kernel(const PackedArgs a, const PackedPlan plan, const FastDiv
   auto s_full = [&](int w) { return q_full + 8 * (2 + w); };             // S of a tile (and O up to the tile before)
   auto p_full = [&](int w) { return q_full + 8 * (4 + w); };             // P of a tile is in tensor memory
   auto o_full = [&](int w) { return q_full + 8 * (6 + w); };             // O of an item
+  const uint32_t sched = q_full + 8 * 8;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + C::kBars);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + C::kBars + 1);
   const uint32_t abort_s = smem_u32(const_cast<int*>(abort_flag));
@@ -83,6 +83,7 @@ packed_fwd_sm100_kernel(const PackedArgs a, const PackedPlan plan, const FastDiv
     mbar_init_s(q_full, 1);
     mbar_init_s(q_empty, 1);
     for (int w = 0; w < 2; ++w) { mbar_init_s(s_full(w), 1); mbar_init_s(p_full(w), 4); mbar_init_s(o_full(w), 1); }
+    for (int i = 0; i < 2; ++i) { mbar_init_s(sched + 8 * i, 1); mbar_init_s(sched + 16 + 8 * i, 9); }
     fence_mbar_init();
     prefetch_tmap(&tmQ); prefetch_tmap(&tmK); prefetch_tmap(&tmV);
   }
@@ -99,7 +100,7 @@ packed_fwd_sm100_kernel(const PackedArgs a, const PackedPlan plan, const FastDiv
   tc_fence_after();
   const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
   const bool failed = *abort_flag != 0;
-  const int n_items = failed ? 0 : __ldcg(plan.counts) * (int)units.d;
+  Schedule todo{sched, sched + 16, abort_s + 4, abort_s, plan.counts + 4, failed ? 0 : __ldcg(plan.counts) * (int)units.d};
 
   // An item: its tile and first head, and of warpgroup w the valid rows, the last key of row 0 and the tiles of keys.
   struct Item {
@@ -135,7 +136,7 @@ packed_fwd_sm100_kernel(const PackedArgs a, const PackedPlan plan, const FastDiv
         if (++st == NS) { st = 0; par ^= 1; }
       };
 #pragma unroll 1
-      for (int turn = 0, idx; (idx = item_of(turn)) < n_items; ++turn) {
+      for (int idx = todo.first(); !todo.over(idx); idx = todo.take()) {
         const Item it = item_at(idx);
         if (it.t.tiles == 0) continue;
         const int hk = it.h / a.G;
@@ -176,7 +177,7 @@ packed_fwd_sm100_kernel(const PackedArgs a, const PackedPlan plan, const FastDiv
         mma_commit_if_s(el, s_full(w));
       };
 #pragma unroll 1
-      for (int turn = 0, idx; (idx = item_of(turn)) < n_items; ++turn) {
+      for (int idx = todo.first(); !todo.over(idx); idx = todo.next()) {
         const Item it = item_at(idx);
         const int tiles = it.t.tiles, tw[2] = {tiles_of(it, 0), tiles_of(it, 1)};
         if (tiles == 0) continue;
@@ -253,59 +254,66 @@ packed_fwd_sm100_kernel(const PackedArgs a, const PackedPlan plan, const FastDiv
     const float kInf = __int_as_float(0x7f800000);
     uint32_t g = 0, n = 0;  // tiles, items with any
 #pragma unroll 1
-    for (int turn = 0, idx; (idx = item_of(turn)) < n_items; ++turn) {
+    for (int idx = todo.first(); !todo.over(idx); idx = todo.next()) {
       const Item it = item_at(idx);
       const int rows = rows_of(it, w), tiles = tiles_of(it, w);
       const bool valid = row < rows;
       // the last key that this row sees, and the first one that some row of the warp does not
       const int last = a.causal ? min(it.t.n - 1, it.t.shift + (PAIR ? w * BM : 0) + row) : it.t.n - 1;
-      const int warp_last = __shfl_sync(0xffffffffu, last, 0);
-      float m = valid ? -kInf : 0.f, l = 0.f;
-      bool alive = !valid;
+      const int warp_last = __shfl_sync(0xffffffffu, last, 0), warp_most = __shfl_sync(0xffffffffu, last, 31);
+      float m = 0.f, l = 0.f;
+      bool steep = false;
 #pragma unroll 1
       for (int t = tiles - 1; t >= 0; --t, ++g) {
         mbar_wait_s(s_full(w), g & 1, abort_s, DEV_TIMEOUT_MMA);
         tc_fence_after();
         const int lim = last - t * BN;  // columns beyond are not seen
         const bool cut = warp_last - t * BN < BN - 1;
+        const int pieces = (warp_most - t * BN + 16) >> 4;  // of 16 keys, those that some row sees
         uint32_t pk[BN / 2];
         float lsum = 0.f;
-        bool go = !__any_sync(0xffffffffu, !alive), settled = false;
+        bool go = !__any_sync(0xffffffffu, steep), settled = false;
 #pragma unroll 1
         for (;;) {
           bool bad = true;
           if (go) {
-            const float nm = m == -kInf ? 0.f : -m;
-            const F2 nm2 = f2_make(nm, nm);
+            const F2 nm2 = f2_make(-m, -m);
             F2 ls[4];
 #pragma unroll
             for (int u = 0; u < 4; ++u) ls[u] = f2_make(0.f, 0.f);
             auto exps = [&](auto with_mask) {
-              uint32_t sr[2][32];
-              tmem_ld32(tS, sr[0]);
+              constexpr bool kMask = decltype(with_mask)::value;
+              uint32_t sr[2][16];
+              if (!kMask) tmem_ld16(tS, sr[0]);
 #pragma unroll
-              for (int k = 0; k < 4; ++k) {
+              for (int k = 0; k < 8; ++k) {
+                if (kMask && k >= pieces) {
+#pragma unroll
+                  for (int e = 0; e < 8; ++e) pk[8 * k + e] = 0u;
+                  continue;
+                }
+                if (kMask) tmem_ld16(tS + 16 * k, sr[k & 1]);
                 tmem_wait_ld();
-                if (k < 3) tmem_ld32(tS + 32 * (k + 1), sr[(k + 1) & 1]);
+                if (!kMask && k < 7) tmem_ld16(tS + 16 * (k + 1), sr[(k + 1) & 1]);
                 const uint32_t* s = sr[k & 1];
 #pragma unroll
-                for (int e = 0; e < 32; e += 2) {
+                for (int e = 0; e < 16; e += 2) {
                   const F2 x = f2_fma(f2_from_bits(s[e], s[e + 1]), c2, nm2);
                   float p0, p1;
-                  if (!decltype(with_mask)::value && on_fma(e / 2)) {
+                  if (!kMask && on_fma(e / 2)) {
                     exp2_fma<T, true>(x, p0, p1);
                   } else {
                     float x0, x1;
                     f2_get(x, x0, x1);
-                    if constexpr (decltype(with_mask)::value) {
-                      x0 = 32 * k + e <= lim ? x0 : -kInf;
-                      x1 = 32 * k + e + 1 <= lim ? x1 : -kInf;
+                    if constexpr (kMask) {
+                      x0 = 16 * k + e <= lim ? x0 : -kInf;
+                      x1 = 16 * k + e + 1 <= lim ? x1 : -kInf;
                     }
                     p0 = ex2(x0);
                     p1 = ex2(x1);
                   }
                   ls[(e / 2) & 3] = f2_add(ls[(e / 2) & 3], f2_make(p0, p1));
-                  pk[16 * k + e / 2] = Pack2<T>::pack(p0, p1);
+                  pk[8 * k + e / 2] = Pack2<T>::pack(p0, p1);
                 }
               }
             };
@@ -315,7 +323,7 @@ packed_fwd_sm100_kernel(const PackedArgs a, const PackedPlan plan, const FastDiv
 #pragma unroll
             for (int u = 0; u < 4; ++u) f2_get(ls[u], s8[2 * u], s8[2 * u + 1]);
             lsum = ((s8[0] + s8[1]) + (s8[2] + s8[3])) + ((s8[4] + s8[5]) + (s8[6] + s8[7]));
-            bad = __any_sync(0xffffffffu, valid && !(lsum <= Lag<T>::kMaxSum));
+            bad = __any_sync(0xffffffffu, valid && !(lsum <= Lag<T>::kMaxSum && (l > 0.f || lim < 0 || lsum >= Lag<T>::kMinSum)));
           }
           if (__builtin_expect(!bad || settled, 1)) break;
           // The tile's own maximum, and the reference follows it.
@@ -339,9 +347,10 @@ packed_fwd_sm100_kernel(const PackedArgs a, const PackedPlan plan, const FastDiv
             }
           }
           const float m_old = m;
-          if (valid) m = fmaxf(m, mx * c);
-          if (t < tiles - 1 && __any_sync(0xffffffffu, m > m_old)) {
-            const float alpha = m > m_old ? ex2(m_old - m) : 1.f;
+          const bool fresh = l == 0.f;  // (nothing of the row is in O yet)
+          if (valid && mx != -kInf) m = fresh ? mx * c : fmaxf(m, mx * c);
+          if (t < tiles - 1 && __any_sync(0xffffffffu, !fresh && m > m_old)) {
+            const float alpha = !fresh && m > m_old ? ex2(m_old - m) : 1.f;
             l *= alpha;
 #pragma unroll 1
             for (int d0 = 0; d0 < DP; d0 += 16) {
@@ -354,7 +363,7 @@ packed_fwd_sm100_kernel(const PackedArgs a, const PackedPlan plan, const FastDiv
             }
           }
           // (scores that rise from tile to tile: the next one's maximum is taken first, and its exponentials once)
-          alive = !valid || (m != -kInf && !(t < tiles - 1 && m > m_old + Lag<T>::kRise));
+          steep = valid && !fresh && m > m_old + Lag<T>::kRise;
           go = settled = true;
         }
         l += lsum;
@@ -373,30 +382,14 @@ packed_fwd_sm100_kernel(const PackedArgs a, const PackedPlan plan, const FastDiv
         ++n;
         tc_fence_after();
       }
-      T* out = static_cast<T*>(a.o) + (out_row * a.H + h) * a.D;
-      const bool any = tiles > 0 && m != -kInf;
-      const float inv = any ? 1.f / l : 0.f;
-#pragma unroll
-      for (int d0 = 0; d0 < DP; d0 += 32) {
-        uint32_t o[32];
-        if (tiles > 0) {
-          tmem_ld32(tO + d0, o);
-          tmem_wait_ld();
-        }
-#pragma unroll
-        for (int e = 0; e < 32; e += 8) {
-          if (valid && d0 + e < a.D) {
-            uint32_t p[4];
-#pragma unroll
-            for (int u = 0; u < 4; ++u)
-              p[u] = any ? Pack2<T>::pack(__uint_as_float(o[e + 2 * u]) * inv, __uint_as_float(o[e + 2 * u + 1]) * inv) : 0u;
-            *reinterpret_cast<uint4*>(out + d0 + e) = make_uint4(p[0], p[1], p[2], p[3]);
-          }
-        }
-      }
+      const bool any = l > 0.f;
+      const int first = (warp & 3) * 32;  // row of the warp's first lane
+      store_rows_staged<T, DP>(smem_s + C::offOut + (warp - 4) * kStageBytes, tO, &tmO, (int)(out_row - lane), h, static_cast<T*>(a.o) + ((out_row - lane) * a.H + h) * a.D,
+                               (long long)a.H * a.D, rows - first, a.D, any ? 1.f / l : 0.f, tiles > 0);
       if (valid && a.lse) a.lse[(long long)h * a.lse_ld + out_row] = any ? m + log2f(l) : -kInf;
       tc_fence_before();  // (the next item's first P V, which overwrites O, follows a later arrival)
     }
+    stores_done();
   }
 
   end_of_cta(abort_flag, a.status);
@@ -410,8 +403,10 @@ template <class T, int DP, bool PAIR>
 int launch(const PackedArgs& a, void* ws, cudaStream_t st, int* launches) {
   using C = FwdCfg<DP>;
   constexpr int unit = PAIR ? 2 * BM : BM;
-  CUtensorMap tq, tk, tv;
-  if (!make_packed_map(&tq, a.q, a.sq, a.Tq, a.H, a.D) || !make_packed_map(&tk, a.k, a.sk, a.Tk, a.Hk, a.D) || !make_packed_map(&tv, a.v, a.sv, a.Tk, a.Hk, a.D))
+  CUtensorMap tq, tk, tv, to;
+  const long long so[2] = {(long long)a.H * a.D, a.D};
+  if (!make_packed_map(&tq, a.q, a.sq, a.Tq, a.H, a.D) || !make_packed_map(&tk, a.k, a.sk, a.Tk, a.Hk, a.D) || !make_packed_map(&tv, a.v, a.sv, a.Tk, a.Hk, a.D) ||
+      !make_packed_map(&to, a.o, so, a.Tq, a.H, a.D, 32))
     return EVOATTN_ERR_CUDA;
   const int sms = sm_count();
   if (sms <= 0) return EVOATTN_ERR_CUDA;
@@ -425,7 +420,7 @@ int launch(const PackedArgs& a, void* ws, cudaStream_t st, int* launches) {
   if (rc) return rc;
   const int heads = PAIR ? a.H : a.H / 2;
   const long long most = query_units(a, unit) * heads;
-  launch_dependent(kern, dim3((unsigned)(most < sms ? most : sms)), kThreads, C::bytes, st, a, plan, FastDiv((uint32_t)heads), tq, tk, tv);
+  launch_dependent(kern, dim3((unsigned)(most < sms ? most : sms)), kThreads, C::bytes, st, a, plan, FastDiv((uint32_t)heads), tq, tk, tv, to);
   *launches += 1;
   return cudaGetLastError() == cudaSuccess ? EVOATTN_OK : EVOATTN_ERR_CUDA;
 }

@@ -103,7 +103,10 @@ __device__ __forceinline__ void make_list(const PackedArgs& a, const PackedPlan&
     s.first[kEach * threadIdx.x + i] = before;
     before += x[i];
   }
-  if (threadIdx.x == 0) plan.counts[queries ? 0 : 1] = all;
+  if (threadIdx.x == 0) {
+    plan.counts[queries ? 0 : 1] = all;
+    plan.counts[queries ? 4 : 5] = 0;
+  }
   __syncthreads();
   tiles.each(a, queries, unit, [&](PackedTile t) {
     const int steps = t.steps, parts = cut(t), each = (steps + parts - 1) / parts;

@@ -29,7 +29,7 @@ struct PackedJoin {
 
 // Where lists lie in a workspace: 256 bytes with their lengths, the tiles, the key tiles whose parts are to be joined and the parts.
 struct PackedPlan {
-  int* counts;               // [0] query units, [1] key tiles and parts, [2] joins
+  int* counts;               // [0] query units, [1] key tiles and parts, [2] joins; [4], [5] items that have been taken of the two lists
   PackedTile *queries, *keys;
   PackedJoin* joins;
   float* sums;               // [slot][Hk][dV, dK][DP / 4][128 rows][4]
@@ -130,15 +130,102 @@ __device__ __forceinline__ void exp2_fma(ptx::F2 x, float& p0, float& p1) {
   p1 = __uint_as_float(__float_as_uint(p1) + (__float_as_uint(t1) << 23));
 }
 
+// DP columns of an accumulator, times f, as 16-bit values to the rows of a warp: lane i has row i, of which the first `rows`
+// are stored, at out + i ld and, as the map has it, at (row0, head); zeros where `any` is not set.  By way of 4 KB of
+// shared memory a warp, 64 columns at a time, which leave by one TMA store where all 32 rows are the sequence's (what is
+// behind it belongs to the next one).  An SM takes more than a microsecond to get rid of a 128 x 128 tile: as plain stores
+// that is waited for at the end of every item (2.0 us from the lanes, 1.6 by way of shared memory).
+constexpr int kStageBytes = 32 * 128;
+template <class T, int DP>
+__device__ __forceinline__ void store_rows_staged(uint32_t stage_s, uint32_t t_src, const CUtensorMap* map, int row0, int head, T* out, long long ld, int rows, int D,
+                                                  float f, bool any) {
+  using namespace ptx;
+  const int lane = threadIdx.x & 31;
+  const bool whole = rows >= 32;
+#pragma unroll 1
+  for (int c0 = 0; c0 < DP; c0 += 32) {
+    const int half = (c0 >> 5) & 1;
+    uint32_t r[32];
+    if (any) {
+      tmem_ld32(t_src + c0, r);
+      tmem_wait_ld();
+    }
+    if (half == 0) {
+      if (lane == 0) tma_wait_group_read0();
+      __syncwarp();  // (what the stage held before has been read)
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      uint32_t p[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) p[u] = any ? Pack2<T>::pack(__uint_as_float(r[8 * i + 2 * u]) * f, __uint_as_float(r[8 * i + 2 * u + 1]) * f) : 0u;
+      sts_v4(stage_s + lane * 128 + (((4 * half + i) ^ (lane & 7)) << 4), p[0], p[1], p[2], p[3]);
+    }
+    if (half == 0) continue;
+    if (whole) {
+      fence_async_shared();
+      __syncwarp();
+      if (lane == 0) {
+        tma_store_3d_s(map, stage_s, c0 - 32, row0, head);
+        tma_commit_group();
+      }
+      continue;
+    }
+    __syncwarp();
+    const int c = lane & 7, d = c0 - 32 + 8 * c;
+#pragma unroll 1
+    for (int i = lane >> 3; i < rows; i += 4)
+      if (d < D) *reinterpret_cast<uint4*>(out + i * ld + d) = lds_v4(stage_s + i * 128 + ((c ^ (i & 7)) << 4));
+    __syncwarp();
+  }
+}
+// What the stores of a warp still read or write, at the end of a kernel.
+__device__ __forceinline__ void stores_done() {
+  if ((threadIdx.x & 31) == 0) ptx::tma_wait_group0();
+  __syncwarp();
+}
+
 __device__ __forceinline__ PackedTile load_tile(const PackedTile* p) {
   const uint4* x = reinterpret_cast<const uint4*>(p);
   const uint4 u = __ldcg(x), v = __ldcg(x + 1), w = __ldcg(x + 2);
   return PackedTile{(int)u.x, (int)u.y, (int)u.z, (int)u.w, (int)v.x, (int)v.y, (int)v.z, (int)v.w, (int)w.x, (int)w.y, {0, 0}};
 }
-// The items of a CTA in turns that go back and forth over the CTAs, so that the last one to get a long item is the first
-// to get a short one.
-__device__ __forceinline__ int item_of(int turn) {
-  return turn * (int)gridDim.x + (turn & 1 ? (int)gridDim.x - 1 - (int)blockIdx.x : (int)blockIdx.x);
-}
+// Which item a CTA works on next: the first is its own, the others it takes from a counter, the most work first as the list
+// has them.  The warp that loads takes one when it has asked for all tiles of the item before (no sooner: who has the
+// longest item should not have the next as well), and hands it to the other warps by way of two words of shared memory.
+struct Schedule {
+  uint32_t full, empty, words;  // shared addresses: two barriers each (empty: of all other warps that work on items), two words
+  uint32_t abort_s;
+  int* counter;
+  int n_items;
+  uint32_t n = 0;
+  __device__ __forceinline__ int first() const { return (int)blockIdx.x; }
+  __device__ __forceinline__ bool over(int idx) const { return idx >= n_items; }
+  __device__ __forceinline__ int take() {  // the warp that loads
+    int idx = 0;
+    if ((threadIdx.x & 31) == 0) idx = (int)gridDim.x + atomicAdd(counter, 1);
+    idx = __shfl_sync(0xffffffffu, idx, 0);
+    const uint32_t at = n & 1;
+    ptx::mbar_wait_s(empty + 8 * at, ((n >> 1) & 1) ^ 1, abort_s, DEV_TIMEOUT_SYNC);
+    if ((threadIdx.x & 31) == 0) {
+      ptx::sts_u32(words + 4 * at, (uint32_t)idx);
+      ptx::mbar_arrive_s(full + 8 * at);
+    }
+    __syncwarp();
+    ++n;
+    return stopped() ? n_items : idx;
+  }
+  __device__ __forceinline__ int next() {  // the others
+    const uint32_t at = n & 1;
+    ptx::mbar_wait_s(full + 8 * at, (n >> 1) & 1, abort_s, DEV_TIMEOUT_SYNC);
+    const int idx = (int)ptx::lds_u32(words + 4 * at);
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) ptx::mbar_arrive_s(empty + 8 * at);
+    ++n;
+    return stopped() ? n_items : idx;
+  }
+  // (a wait that gave up hands on no item)
+  __device__ __forceinline__ bool stopped() const { return __any_sync(0xffffffffu, ptx::lds_u32(abort_s) != 0); }
+};
 
 }  // namespace evo

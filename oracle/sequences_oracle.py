@@ -41,7 +41,8 @@ def attention(q, k, v, spans, causal, scale=None, d=None):
     G = H // Hk
     small = t != torch.float32
     u = torch.finfo(t).eps / 2 if small else 0.0
-    # P and dS below the smallest normal fp16: half of the smallest step
+    # P and dS below the smallest normal fp16: half of the smallest step.  In the forward P is not yet divided by its row's sum,
+    # of which a kernel makes sure that it is at least 2^-4.
     least = 2.0 ** -25 if t == torch.float16 else 0.0
     zeros = lambda x: torch.zeros(x.shape, dtype=torch.float64, device=x.device)  # noqa: E731
     out, eout = zeros(q), zeros(q)
@@ -68,7 +69,7 @@ def attention(q, k, v, spans, causal, scale=None, d=None):
             o = p @ V
             # P rounded, its sum of either the rounded or the unrounded values; the product's sum
             ebig = p @ V.abs()
-            eo = (2 * u + 2 * ep + nk * E) * ebig + least * V.abs().sum(0) + least * nk * ebig
+            eo = (2 * u + 2 * ep + nk * E) * ebig + 16 * least * (V.abs().sum(0) + nk * ebig)
             out[i0:i0 + nq, h] = o
             eout[i0:i0 + nq, h] = eo + rounding(t, o.abs() + eo)
             if d is None:
