@@ -815,12 +815,12 @@ int launch(const PackedArgs& a, const PackedPlan& plan, cudaStream_t st, int* la
     if (!make_packed_map(&tdk, a.dk, sk, a.Tk, a.Hk, a.D, 32) || !make_packed_map(&tdv, a.dv, sk, a.Tk, a.Hk, a.D, 32)) return EVOATTN_ERR_CUDA;
     const int rc = prepare(kern, DkvCfg<DP>::bytes);
     if (rc) return rc;
-    const long long most = (key_tiles(a) + most_slots(a, sms)) * a.Hk;
+    const long long most = (key_tiles(a) + key_slots(a, sms)) * a.Hk;
     launch_dependent(kern, dim3((unsigned)(most < sms ? most : sms)), kThreads, DkvCfg<DP>::bytes, st, a, plan, FastDiv((uint32_t)a.Hk), tq, tk, tv, td, tdk, tdv);
     *launches += 1;
   }
   // (also where no dQ is wanted, if there may be parts of dK and dV to join)
-  if (a.dq || most_slots(a, sms) > 0) {
+  if (a.dq || key_slots(a, sms) > 0) {
     auto kern = packed_dq_sm100_kernel<T, DP>;
     const int rc = prepare(kern, DqCfg<DP>::bytes);
     if (rc) return rc;

@@ -46,7 +46,7 @@ struct FwdCfg {
   static constexpr int kPanel = BM * 128, kTile = kPanels * kPanel;
   static constexpr int kStages = DP == 128 ? 4 : 8;   // K and V tiles in the order of their use
   static constexpr int offQ = 0, offKV = 2 * kTile, offOut = offKV + kStages * kTile, offBars = offOut + 8 * kStageBytes;
-  static constexpr int kBars = 2 * kStages + 2 + 6 + 4;
+  static constexpr int kBars = 2 * kStages + 2 + 6 + 4 + 2;
   static constexpr size_t bytes = offBars + kBars * 8 + 64 + 1024;
   static_assert(bytes <= 232448, "shared memory of one CTA");
   static constexpr int colO = 2 * BN;                 // S of both warpgroups, then O of both
@@ -62,6 +62,7 @@ packed_fwd_sm100_kernel(const PackedArgs a, const PackedPlan plan, const FastDiv
   constexpr int NS = C::kStages;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  __shared__ volatile int arrived[2];
   const uint32_t smem_s = smem_u32(smem);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::offBars);
   const uint32_t bars_s = smem_u32(bars);
@@ -72,6 +73,7 @@ packed_fwd_sm100_kernel(const PackedArgs a, const PackedPlan plan, const FastDiv
   auto p_full = [&](int w) { return q_full + 8 * (4 + w); };             // P of a tile is in tensor memory
   auto o_full = [&](int w) { return q_full + 8 * (6 + w); };             // O of an item
   const uint32_t sched = q_full + 8 * 8;
+  auto together = [&](int w) { return q_full + 8 * (12 + w); };          // the warps of a warpgroup (where parts are joined)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + C::kBars);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + C::kBars + 1);
   const uint32_t abort_s = smem_u32(const_cast<int*>(abort_flag));
@@ -82,7 +84,7 @@ packed_fwd_sm100_kernel(const PackedArgs a, const PackedPlan plan, const FastDiv
     for (int i = 0; i < NS; ++i) { mbar_init_s(t_full(i), 1); mbar_init_s(t_empty(i), 1); }
     mbar_init_s(q_full, 1);
     mbar_init_s(q_empty, 1);
-    for (int w = 0; w < 2; ++w) { mbar_init_s(s_full(w), 1); mbar_init_s(p_full(w), 4); mbar_init_s(o_full(w), 1); }
+    for (int w = 0; w < 2; ++w) { mbar_init_s(s_full(w), 1); mbar_init_s(p_full(w), 4); mbar_init_s(o_full(w), 1); mbar_init_s(together(w), 4); }
     for (int i = 0; i < 2; ++i) { mbar_init_s(sched + 8 * i, 1); mbar_init_s(sched + 16 + 8 * i, 9); }
     fence_mbar_init();
     prefetch_tmap(&tmQ); prefetch_tmap(&tmK); prefetch_tmap(&tmV);
@@ -115,9 +117,12 @@ packed_fwd_sm100_kernel(const PackedArgs a, const PackedPlan plan, const FastDiv
     return it;
   };
   auto rows_of = [&](const Item& it, int w) { return PAIR ? max(0, min(BM, it.t.rows - w * BM)) : it.t.rows; };
-  auto tiles_of = [&](const Item& it, int w) {
-    if (!PAIR || w == 1 || it.t.rows <= BM) return PAIR && w == 1 && it.t.rows <= BM ? 0 : it.t.tiles;
-    return a.causal ? max(0, min(it.t.tiles, (min(it.t.n, it.t.shift + BM) + BN - 1) / BN)) : it.t.tiles;
+  // (key tiles [begin, this) are those of the item that it works on)
+  auto end_of = [&](const Item& it, int w) {
+    const int end = it.t.begin + it.t.steps;
+    if (!PAIR || rows_of(it, 1) == 0) return PAIR && w == 1 ? it.t.begin : end;
+    if (w == 1 || !a.causal) return end;
+    return max(it.t.begin, min(end, (min(it.t.n, it.t.shift + BM) + BN - 1) / BN));
   };
 
   if (warp < 4) {
@@ -138,8 +143,8 @@ packed_fwd_sm100_kernel(const PackedArgs a, const PackedPlan plan, const FastDiv
 #pragma unroll 1
       for (int idx = todo.first(); !todo.over(idx); idx = todo.take()) {
         const Item it = item_at(idx);
-        if (it.t.tiles == 0) continue;
-        const int hk = it.h / a.G;
+        if (it.t.steps == 0) continue;
+        const int hk = it.h / a.G, first = it.t.begin, end = first + it.t.steps;
         mbar_wait_s(q_empty, (n & 1) ^ 1, abort_s, DEV_TIMEOUT_SYNC);
         ++n;
         if (elect_one()) {
@@ -151,11 +156,11 @@ packed_fwd_sm100_kernel(const PackedArgs a, const PackedPlan plan, const FastDiv
               tma_load_3d_s(smem_s + C::offQ + w * C::kTile + p * C::kPanel, &tmQ, q_full, 64 * p, it.t.row + (PAIR ? w * BM : 0), it.h + (PAIR ? 0 : w));
         }
         __syncwarp();
-        load(&tmK, it.t.other + (it.t.tiles - 1) * BN, hk);
+        load(&tmK, it.t.other + (end - 1) * BN, hk);
 #pragma unroll 1
-        for (int t = it.t.tiles - 1; t >= 0; --t) {
+        for (int t = end - 1; t >= first; --t) {
           load(&tmV, it.t.other + t * BN, hk);
-          if (t > 0) load(&tmK, it.t.other + (t - 1) * BN, hk);
+          if (t > first) load(&tmK, it.t.other + (t - 1) * BN, hk);
         }
       }
     } else if (warp == 1) {
@@ -179,21 +184,21 @@ packed_fwd_sm100_kernel(const PackedArgs a, const PackedPlan plan, const FastDiv
 #pragma unroll 1
       for (int idx = todo.first(); !todo.over(idx); idx = todo.next()) {
         const Item it = item_at(idx);
-        const int tiles = it.t.tiles, tw[2] = {tiles_of(it, 0), tiles_of(it, 1)};
-        if (tiles == 0) continue;
+        const int first = it.t.begin, end = first + it.t.steps, tw[2] = {end_of(it, 0), end_of(it, 1)};
+        if (it.t.steps == 0) continue;
         mbar_wait_s(q_full, n & 1, abort_s, DEV_TIMEOUT_TMA);
         ++n;
         mbar_wait_s(t_full(st), par, abort_s, DEV_TIMEOUT_TMA);
         tc_fence_after();
 #pragma unroll
         for (int w = 0; w < 2; ++w)
-          if (tw[w] == tiles) scores(w, st);
+          if (tw[w] == end) scores(w, st);
         uint32_t el = elect_one();
         mma_commit_if_s(el, t_empty(st));
-        if (tiles == 1) mma_commit_if_s(el, q_empty);
+        if (it.t.steps == 1) mma_commit_if_s(el, q_empty);
         next();
 #pragma unroll 1
-        for (int t = tiles - 1; t >= 0; --t) {
+        for (int t = end - 1; t >= first; --t) {
           const uint32_t vs = st, vpar = par;
           next();
           const uint32_t ks = st, kpar = par;
@@ -208,7 +213,7 @@ packed_fwd_sm100_kernel(const PackedArgs a, const PackedPlan plan, const FastDiv
             fence_async_shared();
             __syncwarp();
           }
-          if (t > 0) mbar_wait_s(t_full(ks), kpar, abort_s, DEV_TIMEOUT_TMA);
+          if (t > first) mbar_wait_s(t_full(ks), kpar, abort_s, DEV_TIMEOUT_TMA);
           const uint32_t va = (kv + vs * (C::kTile >> 4)) | kLoMN;
 #pragma unroll
           for (int w = 0; w < 2; ++w) {
@@ -220,16 +225,16 @@ packed_fwd_sm100_kernel(const PackedArgs a, const PackedPlan plan, const FastDiv
 #pragma unroll
               for (int kk = 0; kk < BN / 16; ++kk)  // 16 keys: 8 packed columns of P, 16 rows of V
                 mma_ts_e(el, tmem + C::colO + w * DP, tmem + w * BN + 8 * kk, pack_desc(va + kk * 128, kHi), kIdescO, (kk > 0 || t < tw[w] - 1) ? 1u : 0u);
-              if (t == 0) mma_commit_if_s(el, o_full(w));
+              if (t == first) mma_commit_if_s(el, o_full(w));
             }
-            if (t > 0 && t - 1 < tw[w]) scores(w, ks);
+            if (t > first && t - 1 < tw[w]) scores(w, ks);
           }
           el = elect_one();
           mma_commit_if_s(el, t_empty(vs));
-          if (t > 0) {
+          if (t > first) {
             mma_commit_if_s(el, t_empty(ks));
             next();
-            if (t == 1) mma_commit_if_s(el, q_empty);
+            if (t == first + 1) mma_commit_if_s(el, q_empty);
           }
         }
       }
@@ -252,11 +257,16 @@ packed_fwd_sm100_kernel(const PackedArgs a, const PackedPlan plan, const FastDiv
     const float c = a.scale * kLog2e;
     const F2 c2 = f2_make(c, c);
     const float kInf = __int_as_float(0x7f800000);
-    uint32_t g = 0, n = 0;  // tiles, items with any
+    uint32_t g = 0, n = 0, met = 0;  // tiles, items with any, meetings of the warpgroup
+    auto meet = [&] {
+      __syncwarp();
+      if (lane == 0) mbar_arrive_s(together(w));
+      mbar_wait_s(together(w), met++ & 1, abort_s, DEV_TIMEOUT_SYNC);
+    };
 #pragma unroll 1
     for (int idx = todo.first(); !todo.over(idx); idx = todo.next()) {
       const Item it = item_at(idx);
-      const int rows = rows_of(it, w), tiles = tiles_of(it, w);
+      const int rows = rows_of(it, w), first_tile = it.t.begin, end = end_of(it, w);
       const bool valid = row < rows;
       // the last key that this row sees, and the first one that some row of the warp does not
       const int last = a.causal ? min(it.t.n - 1, it.t.shift + (PAIR ? w * BM : 0) + row) : it.t.n - 1;
@@ -264,7 +274,7 @@ packed_fwd_sm100_kernel(const PackedArgs a, const PackedPlan plan, const FastDiv
       float m = 0.f, l = 0.f;
       bool steep = false;
 #pragma unroll 1
-      for (int t = tiles - 1; t >= 0; --t, ++g) {
+      for (int t = end - 1; t >= first_tile; --t, ++g) {
         mbar_wait_s(s_full(w), g & 1, abort_s, DEV_TIMEOUT_MMA);
         tc_fence_after();
         const int lim = last - t * BN;  // columns beyond are not seen
@@ -349,7 +359,7 @@ packed_fwd_sm100_kernel(const PackedArgs a, const PackedPlan plan, const FastDiv
           const float m_old = m;
           const bool fresh = l == 0.f;  // (nothing of the row is in O yet)
           if (valid && mx != -kInf) m = fresh ? mx * c : fmaxf(m, mx * c);
-          if (t < tiles - 1 && __any_sync(0xffffffffu, !fresh && m > m_old)) {
+          if (t < end - 1 && __any_sync(0xffffffffu, !fresh && m > m_old)) {
             const float alpha = !fresh && m > m_old ? ex2(m_old - m) : 1.f;
             l *= alpha;
 #pragma unroll 1
@@ -377,15 +387,76 @@ packed_fwd_sm100_kernel(const PackedArgs a, const PackedPlan plan, const FastDiv
       if (rows == 0) continue;
       const int h = it.h + (PAIR ? 0 : w);
       const long long out_row = it.t.row + (PAIR ? w * BM : 0) + row;
-      if (tiles > 0) {
+      bool some = end > first_tile;  // there is something in O
+      if (some) {
         mbar_wait_s(o_full(w), n & 1, abort_s, DEV_TIMEOUT_MMA);
         ++n;
         tc_fence_after();
       }
+      if (it.t.parts > 1) {
+        // A part leaves O, m and l; the last part of a tile to arrive adds them up, in their order, back into tensor memory.
+        const int u = PAIR ? it.h : it.h / 2;
+        auto place = [&](int slot) { return ((long long)slot * units.d + u) * 2 + w; };
+        const long long at = place(it.t.slot);
+        float4* to = reinterpret_cast<float4*>(plan.sums) + at * (DP / 4 * BM) + row;
+#pragma unroll 1
+        for (int d = 0; some && d < DP; d += 32) {
+          uint32_t r[32];
+          tmem_ld32(tO + d, r);
+          tmem_wait_ld();
+#pragma unroll
+          for (int e = 0; e < 32; e += 4) to[(d + e) / 4 * BM] = make_float4(__uint_as_float(r[e]), __uint_as_float(r[e + 1]), __uint_as_float(r[e + 2]), __uint_as_float(r[e + 3]));
+        }
+        plan.ml[at * BM + row] = make_float2(m, some ? l : 0.f);
+        __threadfence();
+        meet();
+        if (row == 0) arrived[w] = atomicAdd(plan.arrived + place(it.t.slot - it.t.part), 1);
+        meet();
+        if (arrived[w] != it.t.parts - 1) {
+          tc_fence_before();
+          continue;
+        }
+        __threadfence();
+        some = true;
+        m = -kInf;
+        l = 0.f;
+        const int slot0 = it.t.slot - it.t.part;
+#pragma unroll 1
+        for (int p = 0; p < it.t.parts; ++p) {
+          const float2 x = __ldcg(plan.ml + place(slot0 + p) * BM + row);
+          if (x.y > 0.f) m = fmaxf(m, x.x);
+        }
+        if (m == -kInf) m = 0.f;
+#pragma unroll 1
+        for (int d = 0; d < DP; d += 16) {
+          float acc[16] = {};
+          l = 0.f;
+#pragma unroll 1
+          for (int p = 0; p < it.t.parts; ++p) {
+            const float2 x = __ldcg(plan.ml + place(slot0 + p) * BM + row);
+            const float f = x.y > 0.f ? ex2(x.x - m) : 0.f;
+            const float4* from = reinterpret_cast<const float4*>(plan.sums) + place(slot0 + p) * (DP / 4 * BM) + d / 4 * BM + row;
+            l = fmaf(x.y, f, l);
+            if (f > 0.f) {  // (a part that this row sees nothing of may have left nothing)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const float4 v = __ldcg(from + e * BM);
+                acc[4 * e] = fmaf(v.x, f, acc[4 * e]); acc[4 * e + 1] = fmaf(v.y, f, acc[4 * e + 1]);
+                acc[4 * e + 2] = fmaf(v.z, f, acc[4 * e + 2]); acc[4 * e + 3] = fmaf(v.w, f, acc[4 * e + 3]);
+              }
+            }
+          }
+          uint32_t r[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) r[e] = __float_as_uint(acc[e]);
+          tmem_st16(tO + d, r);
+        }
+        tmem_wait_st();
+      }
       const bool any = l > 0.f;
       const int first = (warp & 3) * 32;  // row of the warp's first lane
       store_rows_staged<T, DP>(smem_s + C::offOut + (warp - 4) * kStageBytes, tO, &tmO, (int)(out_row - lane), h, static_cast<T*>(a.o) + ((out_row - lane) * a.H + h) * a.D,
-                               (long long)a.H * a.D, rows - first, a.D, any ? 1.f / l : 0.f, tiles > 0);
+                               (long long)a.H * a.D, rows - first, a.D, any ? 1.f / l : 0.f, some);
       if (valid && a.lse) a.lse[(long long)h * a.lse_ld + out_row] = any ? m + log2f(l) : -kInf;
       tc_fence_before();  // (the next item's first P V, which overwrites O, follows a later arrival)
     }
@@ -398,6 +469,7 @@ packed_fwd_sm100_kernel(const PackedArgs a, const PackedPlan plan, const FastDiv
 
 // Two heads of a group where there are pairs of them, else two query tiles of one head.
 bool head_pairs(const PackedArgs& a) { return a.G % 2 == 0; }
+PackedCut query_cut(const PackedArgs& a, bool pair) { return PackedCut{100, 10, pair ? a.H : a.H / 2}; }
 
 template <class T, int DP, bool PAIR>
 int launch(const PackedArgs& a, void* ws, cudaStream_t st, int* launches) {
@@ -415,11 +487,12 @@ int launch(const PackedArgs& a, void* ws, cudaStream_t st, int* launches) {
   if (!kernel_ready(reinterpret_cast<const void*>(kern), (int)C::bytes, &regs)) return EVOATTN_ERR_CUDA;
   // (setmaxnreg.inc would wait for registers that the launch does not have)
   if (kThreads * regs < 256 * kSoftmaxRegs + 128 * kServiceRegs) return EVOATTN_ERR_UNSUPPORTED;
-  const PackedPlan plan = place_plan(ws, plan_bytes(a, true, unit, false, sms));
-  const int rc = launch_packed_prepare(std::is_same<T, __nv_bfloat16>::value ? EVOATTN_BF16 : EVOATTN_FP16, a, plan, true, unit, false, false, st, launches);
+  const PackedCut cut = query_cut(a, PAIR);
+  const PackedPlan plan = place_plan(ws, plan_bytes(a, true, unit, false, sms, cut));
+  const int rc = launch_packed_prepare(std::is_same<T, __nv_bfloat16>::value ? EVOATTN_BF16 : EVOATTN_FP16, a, plan, true, unit, false, false, st, launches, cut);
   if (rc) return rc;
   const int heads = PAIR ? a.H : a.H / 2;
-  const long long most = query_units(a, unit) * heads;
+  const long long most = (query_units(a, unit) + query_slots(a, unit, sms, cut)) * heads;
   launch_dependent(kern, dim3((unsigned)(most < sms ? most : sms)), kThreads, C::bytes, st, a, plan, FastDiv((uint32_t)heads), tq, tk, tv, to);
   *launches += 1;
   return cudaGetLastError() == cudaSuccess ? EVOATTN_OK : EVOATTN_ERR_CUDA;
@@ -439,7 +512,7 @@ bool sm100_packed_supported(int dtype, const PackedArgs& a) {
   if (reinterpret_cast<uintptr_t>(a.o) & 15) return false;
   return packed_map_ok(a.q, a.sq, a.Tq, a.H) && packed_map_ok(a.k, a.sk, a.Tk, a.Hk) && packed_map_ok(a.v, a.sv, a.Tk, a.Hk);
 }
-size_t sm100_packed_fwd_workspace_bytes(const PackedArgs& a) { return plan_bytes(a, true, head_pairs(a) ? BM : 2 * BM, false, sm_count()).all(); }
+size_t sm100_packed_fwd_workspace_bytes(const PackedArgs& a) { return plan_bytes(a, true, head_pairs(a) ? BM : 2 * BM, false, sm_count(), query_cut(a, !head_pairs(a))).all(); }
 int launch_sm100_packed_fwd(int dtype, const PackedArgs& a, void* ws, cudaStream_t st, int* launches) {
   if (dtype == EVOATTN_BF16) return launch_d<__nv_bfloat16>(a, ws, st, launches);
   return launch_d<__half>(a, ws, st, launches);

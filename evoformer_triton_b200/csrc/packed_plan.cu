@@ -55,25 +55,29 @@ struct Tiles {
   }
 };
 
-// A list by a counting sort, most work first, so that what a persistent grid ends with is short.  Key tiles whose steps are
-// more than `share` times those of an SM are cut into parts, which leave fp32 sums to be joined: a group of
-// heads or a long sequence makes single tiles that would outlast everything else.
-__device__ __forceinline__ void make_list(const PackedArgs& a, const PackedPlan& plan, bool queries, int unit, int sms, Sums& s) {
+// A list by a counting sort, most work first, so that what a persistent grid ends with is short.  Tiles with more steps than a
+// share of those of an SM are cut into parts, which leave fp32 sums to be joined: a group of heads or a long
+// sequence makes single tiles that would outlast everything else.
+__device__ __forceinline__ void make_list(const PackedArgs& a, const PackedPlan& plan, bool queries, int unit, int sms, const PackedCut& c, Sums& s) {
   const Tiles tiles(a);
   PackedTile* out = queries ? plan.queries : plan.keys;
   for (int i = threadIdx.x; i < kClasses; i += kThreads) s.first[i] = 0;
+  if (queries)
+    for (int i = threadIdx.x; i < plan.n_arrived; i += kThreads) plan.arrived[i] = 0;
   if (threadIdx.x == 0) { s.steps = 0; s.slots = 0; s.joins = 0; }
   __syncthreads();
-  int longest = kLongest;
-  if (!queries) {
+  int longest = 0x7fffffff;
+  if (c.heads) {
     long long sum = 0;
-    tiles.each(a, false, unit, [&](const PackedTile& t) { sum += t.steps; });
-    if (sum) atomicAdd(reinterpret_cast<unsigned long long*>(&s.steps), (unsigned long long)sum);
+    tiles.each(a, queries, unit, [&](const PackedTile& t) { sum += t.steps; });
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if ((threadIdx.x & 31) == 0 && sum) atomicAdd(reinterpret_cast<unsigned long long*>(&s.steps), (unsigned long long)sum);
     __syncthreads();
-    longest = part_steps(s.steps * a.Hk, sms);
+    longest = part_steps(s.steps, sms, c);
   }
   auto place = [](int steps) { return kClasses - 1 - min(steps, kClasses - 1); };
-  auto cut = [&](const PackedTile& t) { return t.steps > longest ? (t.steps + longest - 1) / longest : 1; };
+  auto cut = [&](const PackedTile& t) { return t.steps - longest > longest / 2 ? (t.steps + longest / 2) / longest : 1; };
   tiles.each(a, queries, unit, [&](const PackedTile& t) {
     const int parts = cut(t);
     atomicAdd(&s.first[place((t.steps + parts - 1) / parts)], parts);
@@ -109,16 +113,17 @@ __device__ __forceinline__ void make_list(const PackedArgs& a, const PackedPlan&
   }
   __syncthreads();
   tiles.each(a, queries, unit, [&](PackedTile t) {
-    const int steps = t.steps, parts = cut(t), each = (steps + parts - 1) / parts;
+    const int steps = t.steps, parts = cut(t);
     if (parts > 1) {
       t.slot = atomicAdd(&s.slots, parts);
-      plan.joins[atomicAdd(&s.joins, 1)] = PackedJoin{t.row, t.rows, t.slot, parts};
+      if (!queries) plan.joins[atomicAdd(&s.joins, 1)] = PackedJoin{t.row, t.rows, t.slot, parts};
     }
-    const int at = atomicAdd(&s.first[place(each)], parts);
+    const int at = atomicAdd(&s.first[place((steps + parts - 1) / parts)], parts);
     t.parts = parts;
     for (int p = 0; p < parts; ++p) {
-      t.begin = p * each;
-      t.steps = min(each, steps - t.begin);
+      t.part = p;
+      t.begin = (int)((long long)steps * p / parts);
+      t.steps = (int)((long long)steps * (p + 1) / parts) - t.begin;
       out[at + p] = t;
       ++t.slot;
     }
@@ -183,14 +188,14 @@ __device__ __forceinline__ void row_sums(const PackedArgs& a, long long block, l
 // Block 0 makes the list of queries, block 1 (or 0) that of keys, the others the row sums.
 template <class T, bool VEC>
 __global__ void __launch_bounds__(kThreads) packed_prepare_kernel(const PackedArgs a, const PackedPlan plan, const int queries, const int unit, const int keys,
-                                                                  const int sms, const int lanes, const FastDiv heads) {
+                                                                  const int sms, const PackedCut qcut, const PackedCut kcut, const int lanes, const FastDiv heads) {
   __shared__ Sums s;
   ptx::grid_dependency_wait();
   ptx::grid_launch_dependents();
   const int lists = queries + keys;
   if ((int)blockIdx.x < lists) {
     const bool q = queries && blockIdx.x == 0;
-    make_list(a, plan, q, q ? unit : kTileRows, sms, s);
+    make_list(a, plan, q, q ? unit : kTileRows, sms, q ? qcut : kcut, s);
   } else {
     row_sums<T, VEC>(a, blockIdx.x - lists, gridDim.x - lists, lanes, heads);
   }
@@ -198,7 +203,8 @@ __global__ void __launch_bounds__(kThreads) packed_prepare_kernel(const PackedAr
 
 }  // namespace
 
-int launch_packed_prepare(int dtype, const PackedArgs& a, const PackedPlan& plan, bool queries, int unit, bool keys, bool delta, cudaStream_t st, int* launches) {
+int launch_packed_prepare(int dtype, const PackedArgs& a, const PackedPlan& plan, bool queries, int unit, bool keys, bool delta, cudaStream_t st, int* launches,
+                          const PackedCut& qcut) {
   const int sms = sm_count();
   if (sms <= 0) return EVOATTN_ERR_CUDA;
   return with_dtype(dtype, [&](auto t) {
@@ -210,7 +216,7 @@ int launch_packed_prepare(int dtype, const PackedArgs& a, const PackedPlan& plan
     const long long rows = ((long long)a.Tq * a.H + kThreads / lanes * 4 - 1) / (kThreads / lanes * 4);
     const int blocks = (queries ? 1 : 0) + (keys ? 1 : 0) + (delta ? (int)(rows < sms * 4LL ? rows : sms * 4LL) : 0);
     launch_dependent(vec ? packed_prepare_kernel<T, true> : packed_prepare_kernel<T, false>, dim3((unsigned)blocks), kThreads, 0, st, a, plan, (int)queries, unit, (int)keys,
-                     sms, lanes, FastDiv((uint32_t)a.H));
+                     sms, qcut, key_cut(a), lanes, FastDiv((uint32_t)a.H));
     *launches += 1;
     return cudaGetLastError() == cudaSuccess ? EVOATTN_OK : EVOATTN_ERR_CUDA;
   });

@@ -19,8 +19,8 @@ struct PackedTile {
                     // key j is seen by the queries from j + shift on
   int tiles;        // tiles of 128 rows of the other tensor that it meets: the first ones of the keys; the last ones of the queries
   int begin, steps; // of the steps of a key tile (the tiles of the group's heads, one after another) this part's
-  int parts, slot;  // parts of the tile, and where this one leaves its sums
-  int pad[2];
+  int parts, part;  // parts of the tile, and which this is
+  int slot, pad;    // where it leaves its sums (those of part 0 lie `part` slots before)
 };
 static_assert(sizeof(PackedTile) == 48, "three 16-byte loads");
 struct PackedJoin {
@@ -32,44 +32,60 @@ struct PackedPlan {
   int* counts;               // [0] query units, [1] key tiles and parts, [2] joins; [4], [5] items that have been taken of the two lists
   PackedTile *queries, *keys;
   PackedJoin* joins;
-  float* sums;               // [slot][Hk][dV, dK][DP / 4][128 rows][4]
+  float* sums;               // key tiles: [slot][Hk][dV, dK][DP / 4][128 rows][4]; query units: [slot][units of heads][2 tiles][DP / 4][128][4]
+  float2* ml;                // [slot][units of heads][2 tiles][128 rows]: reference and sum
+  int *arrived, n_arrived;   // [slot][units of heads][2 tiles]: parts that are through, of the tile whose first part has that slot
 };
-// Steps of a part: half of what an SM has to do, and no fewer than kShortest, which is what a part costs by itself.
-constexpr int kShortest = 4, kLongest = 0x7fffffff;
-__host__ __device__ inline int part_steps(long long steps, int sms) {
-  const long long n = (steps + 2 * sms - 1) / (2 * sms);
-  return n < kShortest ? kShortest : n > kLongest ? kLongest : (int)n;
+// What a list cuts: tiles of one and a half times as many steps and more as `part` hundredths of what an SM has to do, and as
+// `least`; `heads` is how many of each there are on the list.
+struct PackedCut {
+  int part, least, heads;
+};
+// Steps of a part: a share of what an SM has to do, and no fewer than what a part costs by itself.
+__host__ __device__ inline int part_steps(long long steps, int sms, const PackedCut& c) {
+  const long long n = (steps * c.heads * c.part + 100LL * sms - 1) / (100LL * sms);
+  return n < c.least ? c.least : n > 0x7fffffff ? 0x7fffffff : (int)n;
 }
+inline PackedCut key_cut(const PackedArgs& a) { return PackedCut{50, 4, a.Hk}; }
 inline long long query_units(const PackedArgs& a, int unit) { return a.Tq / unit + a.B; }
 inline long long key_tiles(const PackedArgs& a) { return a.Tk / kTileRows + a.B; }
-// A tile of more than n = part_steps() steps makes fewer than 2 steps / n parts, and all steps are at most 2 sms n: so all
-// heads' slots are fewer than 4 sms, and no more than kShortest allows.  The same bounds what parts add to the list.
-inline long long most_slots(const PackedArgs& a, int sms) {
-  const long long steps = (a.Tq / kTileRows + 1LL) * a.G, each = (steps + kShortest - 1) / kShortest, all = key_tiles(a) * each, most = (4LL * sms + a.Hk - 1) / a.Hk;
+// A tile of 3 n / 2 steps or more, n = part_steps(), makes at most steps / n + 1 / 2 < 2 steps / n parts, and all heads' steps are at most
+// 100 sms n / part: so all heads' slots are fewer than 200 sms / part, and no more than `least` allows.  The same bounds what
+// parts add to the list.
+inline long long most_slots(long long tiles, long long steps, int sms, const PackedCut& c) {
+  const long long each = (steps + c.least - 1) / c.least, all = tiles * each, most = (200LL * sms / c.part + c.heads - 1) / c.heads;
   return each < 2 ? 0 : all < most ? all : most;
 }
+inline long long key_slots(const PackedArgs& a, int sms) { return most_slots(key_tiles(a), (a.Tq / kTileRows + 1LL) * a.G, sms, key_cut(a)); }
+inline long long query_slots(const PackedArgs& a, int unit, int sms, const PackedCut& c) { return most_slots(query_units(a, unit), a.Tk / kTileRows + 1LL, sms, c); }
 inline size_t round256(size_t n) { return (n + 255) / 256 * 256; }
 struct PlanBytes {
-  size_t queries, keys, joins, sums;
-  size_t all() const { return 256 + queries + keys + joins + sums; }
+  size_t queries, keys, joins, sums, ml, arrived;
+  size_t all() const { return 256 + queries + keys + joins + sums + ml + arrived; }
 };
-inline PlanBytes plan_bytes(const PackedArgs& a, bool queries, int unit, bool keys, int sms) {
-  const long long slots = keys ? most_slots(a, sms) : 0;
-  const int dp = a.D <= 64 ? 64 : 128;
-  return PlanBytes{queries ? round256(query_units(a, unit) * sizeof(PackedTile)) : 0, keys ? round256((key_tiles(a) + slots) * sizeof(PackedTile)) : 0,
-                   round256(slots * sizeof(PackedJoin)), round256((size_t)slots * a.Hk * 2 * kTileRows * dp * sizeof(float))};
+// qcut.heads = 0: the query units are not cut.
+inline PlanBytes plan_bytes(const PackedArgs& a, bool queries, int unit, bool keys, int sms, const PackedCut& qcut = PackedCut{100, 1, 0}) {
+  const long long ks = keys ? key_slots(a, sms) : 0, qs = queries && qcut.heads ? query_slots(a, unit, sms, qcut) : 0;
+  const size_t tile = (size_t)kTileRows * (a.D <= 64 ? 64 : 128) * sizeof(float), tiles = (size_t)qs * qcut.heads * 2;
+  return PlanBytes{queries ? round256((query_units(a, unit) + qs) * sizeof(PackedTile)) : 0, keys ? round256((key_tiles(a) + ks) * sizeof(PackedTile)) : 0,
+                   round256(ks * sizeof(PackedJoin)), round256(tile * (ks * a.Hk * 2 + tiles)), round256(tiles * kTileRows * sizeof(float2)), round256(tiles * sizeof(int))};
 }
 inline PackedPlan place_plan(void* ws, const PlanBytes& n) {
   unsigned char* p = static_cast<unsigned char*>(ws);
-  PackedPlan plan{reinterpret_cast<int*>(p), nullptr, nullptr, nullptr, nullptr};
+  PackedPlan plan{};
+  plan.counts = reinterpret_cast<int*>(p);
   plan.queries = reinterpret_cast<PackedTile*>(p += 256);
   plan.keys = reinterpret_cast<PackedTile*>(p += n.queries);
   plan.joins = reinterpret_cast<PackedJoin*>(p += n.keys);
-  plan.sums = reinterpret_cast<float*>(p + n.joins);
+  plan.sums = reinterpret_cast<float*>(p += n.joins);
+  plan.ml = reinterpret_cast<float2*>(p += n.sums);
+  plan.arrived = reinterpret_cast<int*>(p + n.ml);
+  plan.n_arrived = (int)(n.arrived / sizeof(int));
   return plan;
 }
 // Writes the lists, those with the most work first, and the row sums of dO * O, in one launch (packed_plan.cu).
-int launch_packed_prepare(int dtype, const PackedArgs& a, const PackedPlan& plan, bool queries, int unit, bool keys, bool delta, cudaStream_t st, int* launches);
+int launch_packed_prepare(int dtype, const PackedArgs& a, const PackedPlan& plan, bool queries, int unit, bool keys, bool delta, cudaStream_t st, int* launches,
+                          const PackedCut& qcut = PackedCut{100, 1, 0});
 
 // [T][heads][D] rows of 16 bits as a 3-D map (D, T, heads) with boxes of 64 values (128 bytes, swizzled) by `rows`;
 // values beyond D and rows beyond T read as zero.
@@ -188,7 +204,7 @@ __device__ __forceinline__ void stores_done() {
 __device__ __forceinline__ PackedTile load_tile(const PackedTile* p) {
   const uint4* x = reinterpret_cast<const uint4*>(p);
   const uint4 u = __ldcg(x), v = __ldcg(x + 1), w = __ldcg(x + 2);
-  return PackedTile{(int)u.x, (int)u.y, (int)u.z, (int)u.w, (int)v.x, (int)v.y, (int)v.z, (int)v.w, (int)w.x, (int)w.y, {0, 0}};
+  return PackedTile{(int)u.x, (int)u.y, (int)u.z, (int)u.w, (int)v.x, (int)v.y, (int)v.z, (int)v.w, (int)w.x, (int)w.y, (int)w.z, 0};
 }
 // Which item a CTA works on next: the first is its own, the others it takes from a counter, the most work first as the list
 // has them.  The warp that loads takes one when it has asked for all tiles of the item before (no sooner: who has the

@@ -108,6 +108,15 @@ def test_a_few_tokens_each_and_one_long(dtype):
     _check(*_qkv(sum(nq), sum(nk), 8, 2, 128, dtype), nq, nk, train=False)
 
 
+@pytest.mark.parametrize("dtype", [BF, HF], ids=IDS.get)
+@pytest.mark.parametrize("nq,nk", [([300], [9000]), ([129, 40, 7], [5000, 40, 6100]), ([256], [4000]), ([1000], None), ([2500], None)], ids=str)
+def test_long_rows_of_tiles_are_cut(nq, nk, dtype):
+    """Few queries against many keys, and few heads: parts of a tile that are joined, in both directions."""
+    for H, Hk, D in ((2, 1, 64), (1, 1, 128), (3, 1, 128), (6, 1, 96)):
+        for causal in (True, False):
+            _check(*_qkv(sum(nq), sum(nk or nq), H, Hk, D, dtype), nq, nk, causal)
+
+
 def test_thousands_of_tokens():
     """More sequences than a launch of the kernel for few rows takes; empty ones, sequences without keys, rows of none."""
     import evoformer_triton_b200 as evo
