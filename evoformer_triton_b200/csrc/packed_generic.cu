@@ -12,6 +12,8 @@
 // order in which blocks run.
 #include <math.h>
 
+#include <type_traits>
+
 #include "packed.cuh"
 
 namespace evo {
@@ -20,30 +22,54 @@ namespace {
 constexpr int kThreads = 256;
 constexpr float kLog2e = 1.4426950408889634f;
 
-template <int DP>
+// TILE is 64, or 32 where that makes more blocks than an SM's worth of work each (and above D = 128, where four tiles of 64
+// rows would not fit).
+template <int DP, int TILE_>
 struct GenericCfg {
-  static constexpr int TILE = DP > 128 ? 32 : 64;  // (four tiles of 64 x 256 floats would not fit)
+  static constexpr int TILE = TILE_;
   static constexpr int NR = TILE / 16, NC = DP / 64, LD = DP + 4, LP = TILE + 4;
   static constexpr size_t bytes(int tiles, int scores) { return sizeof(float) * ((size_t)tiles * TILE * LD + (size_t)scores * TILE * LP + 2 * TILE); }
 };
 
-// Rows [0, n) of a tile into shared memory as floats, zeros beyond n and D.
-template <class T, int DP>
-__device__ __forceinline__ void load_rows(float* dst, const void* src, long long stride, int n, int D) {
-  constexpr int TILE = GenericCfg<DP>::TILE, LD = GenericCfg<DP>::LD;
-  const T* p = static_cast<const T*>(src);
-  for (int i = threadIdx.x; i < TILE * DP; i += kThreads) {
-    const int r = i / DP, d = i % DP;
-    dst[r * LD + d] = r < n && d < D ? to_float(p[r * stride + d]) : 0.f;
+// Rows [0, n) of a tile on their way to shared memory as floats, zeros beyond n and D: get() asks for all of them at once (one
+// at a time they took 9 of a tile's 11 us), put() stores them.  VEC: 16 bytes at a time.
+template <class T, int DP, int TILE, bool VEC>
+struct Rows {
+  static constexpr int LD = GenericCfg<DP, TILE>::LD, V = VEC ? kPer16<T> : 1, PER = DP / V, N = TILE * PER / kThreads;
+  using Raw = typename std::conditional<VEC, uint4, T>::type;
+  Raw raw[N];
+  __device__ __forceinline__ void get(const void* src, long long stride, int n, int D) {
+    const T* p = static_cast<const T*>(src);
+#pragma unroll
+    for (int u = 0; u < N; ++u) {
+      const int i = threadIdx.x + u * kThreads, r = i / PER, d = i % PER * V;
+      raw[u] = Raw{};
+      if (r < n && d < D) raw[u] = *reinterpret_cast<const Raw*>(p + r * stride + d);
+    }
   }
-}
+  __device__ __forceinline__ void put(float* dst) const {
+#pragma unroll
+    for (int u = 0; u < N; ++u) {
+      const int i = threadIdx.x + u * kThreads;
+      float* to = dst + i / PER * LD + i % PER * V;
+      if constexpr (VEC) {
+        float f[V];
+        unpack16<T>(raw[u], f);
+#pragma unroll
+        for (int e = 0; e < V; e += 4) *reinterpret_cast<float4*>(to + e) = make_float4(f[e], f[e + 1], f[e + 2], f[e + 3]);
+      } else {
+        *to = to_float(raw[u]);
+      }
+    }
+  }
+};
 __device__ __forceinline__ float4 ld4(const float* p) { return *reinterpret_cast<const float4*>(p); }
 __device__ __forceinline__ float dot4(float4 a, float4 b, float s) { return fmaf(a.x, b.x, fmaf(a.y, b.y, fmaf(a.z, b.z, fmaf(a.w, b.w, s)))); }
 
 // s[r][c] = row (ty + 16 r) of x times row (tx + 16 c) of y.
-template <int DP>
-__device__ __forceinline__ void products(const float* x, const float* y, int ty, int tx, float (&s)[GenericCfg<DP>::NR][GenericCfg<DP>::NR]) {
-  constexpr int NR = GenericCfg<DP>::NR, LD = GenericCfg<DP>::LD;
+template <class C, int DP>
+__device__ __forceinline__ void products(const float* x, const float* y, int ty, int tx, float (&s)[C::NR][C::NR]) {
+  constexpr int NR = C::NR, LD = C::LD;
 #pragma unroll
   for (int r = 0; r < NR; ++r)
 #pragma unroll
@@ -61,22 +87,25 @@ __device__ __forceinline__ void products(const float* x, const float* y, int ty,
       for (int c = 0; c < NR; ++c) s[r][c] = dot4(u[r], w[c], s[r][c]);
   }
 }
-// acc[r][.] += sum_j p(row ty + 16 r, j) * y[j][4 tx + 64 c ..]; p as [row][j] (ROWS) or [j][row].
-template <int DP, bool ROWS>
-__device__ __forceinline__ void accumulate(const float* p, const float* y, int ty, int tx, float4 (&acc)[GenericCfg<DP>::NR][GenericCfg<DP>::NC]) {
-  using C = GenericCfg<DP>;
-#pragma unroll 4
-  for (int j = 0; j < C::TILE; ++j) {
-    float w[C::NR];
+// acc[r][.] += sum_j p[ty + 16 r][j] * y[j][4 tx + 64 c ..].
+template <class C>
+__device__ __forceinline__ void accumulate(const float* p, const float* y, int ty, int tx, float4 (&acc)[C::NR][C::NC]) {
+#pragma unroll 2
+  for (int j = 0; j < C::TILE; j += 4) {
+    float4 w[C::NR];
 #pragma unroll
-    for (int r = 0; r < C::NR; ++r) w[r] = ROWS ? p[(ty + 16 * r) * C::LP + j] : p[j * C::LP + ty + 16 * r];
+    for (int r = 0; r < C::NR; ++r) w[r] = ld4(p + (ty + 16 * r) * C::LP + j);
 #pragma unroll
-    for (int c = 0; c < C::NC; ++c) {
-      const float4 v = ld4(y + j * C::LD + 4 * tx + 64 * c);
+    for (int e = 0; e < 4; ++e) {
 #pragma unroll
-      for (int r = 0; r < C::NR; ++r) {
-        acc[r][c].x = fmaf(w[r], v.x, acc[r][c].x); acc[r][c].y = fmaf(w[r], v.y, acc[r][c].y);
-        acc[r][c].z = fmaf(w[r], v.z, acc[r][c].z); acc[r][c].w = fmaf(w[r], v.w, acc[r][c].w);
+      for (int c = 0; c < C::NC; ++c) {
+        const float4 v = ld4(y + (j + e) * C::LD + 4 * tx + 64 * c);
+#pragma unroll
+        for (int r = 0; r < C::NR; ++r) {
+          const float f = e == 0 ? w[r].x : e == 1 ? w[r].y : e == 2 ? w[r].z : w[r].w;
+          acc[r][c].x = fmaf(f, v.x, acc[r][c].x); acc[r][c].y = fmaf(f, v.y, acc[r][c].y);
+          acc[r][c].z = fmaf(f, v.z, acc[r][c].z); acc[r][c].w = fmaf(f, v.w, acc[r][c].w);
+        }
       }
     }
   }
@@ -99,10 +128,10 @@ __device__ __forceinline__ float sum16(float v) {
   return v;
 }
 
-template <class T, int DP>
+template <class T, int DP, int TILE, bool VEC>
 __global__ void __launch_bounds__(kThreads) packed_generic_fwd_kernel(const PackedArgs a) {
-  using C = GenericCfg<DP>;
-  constexpr int TILE = C::TILE, NR = C::NR, NC = C::NC;
+  using C = GenericCfg<DP, TILE>;
+  constexpr int NR = C::NR, NC = C::NC;
   extern __shared__ __align__(16) float sm[];
   float *sQ = sm, *sK = sQ + TILE * C::LD, *sV = sK + TILE * C::LD, *sP = sV + TILE * C::LD;
   __shared__ int place[34];
@@ -114,7 +143,15 @@ __global__ void __launch_bounds__(kThreads) packed_generic_fwd_kernel(const Pack
   const Span qs = query_span(a, at.seq), ks = key_span(a, at.seq);
   const int i0 = at.tile * TILE, rows = min(TILE, qs.n - i0), shift = ks.n - qs.n, hk = h / a.G;
   const int seen = keys_seen(a, qs.n, ks.n, i0, TILE);
-  load_rows<T, DP>(sQ, static_cast<const T*>(a.q) + (long long)(qs.begin + i0) * a.sq[0] + (long long)h * a.sq[1], a.sq[0], rows, a.D);
+  Rows<T, DP, TILE, VEC> x, y;
+  x.get(static_cast<const T*>(a.q) + (long long)(qs.begin + i0) * a.sq[0] + (long long)h * a.sq[1], a.sq[0], rows, a.D);
+  x.put(sQ);
+  auto fetch = [&](int j0) {
+    const long long row = ks.begin + j0;
+    x.get(static_cast<const T*>(a.k) + row * a.sk[0] + (long long)hk * a.sk[1], a.sk[0], ks.n - j0, a.D);
+    y.get(static_cast<const T*>(a.v) + row * a.sv[0] + (long long)hk * a.sv[1], a.sv[0], ks.n - j0, a.D);
+  };
+  if (seen > 0) fetch(0);
   const float c = a.scale * kLog2e;
   float m[NR], l[NR];
   float4 acc[NR][NC];
@@ -127,12 +164,12 @@ __global__ void __launch_bounds__(kThreads) packed_generic_fwd_kernel(const Pack
   }
   for (int j0 = 0; j0 < seen; j0 += TILE) {
     __syncthreads();
-    const long long row = ks.begin + j0;
-    load_rows<T, DP>(sK, static_cast<const T*>(a.k) + row * a.sk[0] + (long long)hk * a.sk[1], a.sk[0], ks.n - j0, a.D);
-    load_rows<T, DP>(sV, static_cast<const T*>(a.v) + row * a.sv[0] + (long long)hk * a.sv[1], a.sv[0], ks.n - j0, a.D);
+    x.put(sK);
+    y.put(sV);
     __syncthreads();
+    if (j0 + TILE < seen) fetch(j0 + TILE);  // (the next tile's rows are on their way under this one's arithmetic)
     float s[NR][NR];
-    products<DP>(sQ, sK, ty, tx, s);
+    products<C, DP>(sQ, sK, ty, tx, s);
 #pragma unroll
     for (int r = 0; r < NR; ++r) {
       const int last = a.causal ? min(ks.n - 1, i0 + ty + 16 * r + shift) : ks.n - 1;  // the last key of this row
@@ -158,7 +195,7 @@ __global__ void __launch_bounds__(kThreads) packed_generic_fwd_kernel(const Pack
       for (int k = 0; k < NC; ++k) { acc[r][k].x *= alpha; acc[r][k].y *= alpha; acc[r][k].z *= alpha; acc[r][k].w *= alpha; }
     }
     __syncthreads();
-    accumulate<DP, true>(sP, sV, ty, tx, acc);
+    accumulate<C>(sP, sV, ty, tx, acc);
   }
 #pragma unroll
   for (int r = 0; r < NR; ++r) {
@@ -188,18 +225,18 @@ __device__ __forceinline__ void p_and_ds(const PackedArgs& a, float (&s)[NR][NR]
     }
   }
 }
-template <int DP>
+template <int TILE>
 __device__ __forceinline__ void load_statistics(const PackedArgs& a, float* lse, float* delta, int h, int row, int rows) {
-  for (int i = threadIdx.x; i < GenericCfg<DP>::TILE; i += kThreads) {
+  for (int i = threadIdx.x; i < TILE; i += kThreads) {
     lse[i] = i < rows ? a.lse[(long long)h * a.lse_ld + row + i] : 0.f;
     delta[i] = i < rows ? a.delta[(long long)h * a.lse_ld + row + i] : 0.f;
   }
 }
 
-template <class T, int DP>
+template <class T, int DP, int TILE, bool VEC>
 __global__ void __launch_bounds__(kThreads) packed_generic_dq_kernel(const PackedArgs a) {
-  using C = GenericCfg<DP>;
-  constexpr int TILE = C::TILE, NR = C::NR, NC = C::NC;
+  using C = GenericCfg<DP, TILE>;
+  constexpr int NR = C::NR, NC = C::NC;
   extern __shared__ __align__(16) float sm[];
   float *sQ = sm, *sO = sQ + TILE * C::LD, *sK = sO + TILE * C::LD, *sV = sK + TILE * C::LD, *sS = sV + TILE * C::LD;
   float *lse = sS + TILE * C::LP, *delta = lse + TILE;
@@ -211,9 +248,18 @@ __global__ void __launch_bounds__(kThreads) packed_generic_dq_kernel(const Packe
   const Span qs = query_span(a, at.seq), ks = key_span(a, at.seq);
   const int i0 = at.tile * TILE, rows = min(TILE, qs.n - i0), hk = h / a.G, seen = keys_seen(a, qs.n, ks.n, i0, TILE);
   const long long row = qs.begin + i0;
-  load_rows<T, DP>(sQ, static_cast<const T*>(a.q) + row * a.sq[0] + (long long)h * a.sq[1], a.sq[0], rows, a.D);
-  load_rows<T, DP>(sO, static_cast<const T*>(a.d_o) + row * a.sdo[0] + (long long)h * a.sdo[1], a.sdo[0], rows, a.D);
-  load_statistics<DP>(a, lse, delta, h, (int)row, rows);
+  Rows<T, DP, TILE, VEC> x, y;
+  x.get(static_cast<const T*>(a.q) + row * a.sq[0] + (long long)h * a.sq[1], a.sq[0], rows, a.D);
+  y.get(static_cast<const T*>(a.d_o) + row * a.sdo[0] + (long long)h * a.sdo[1], a.sdo[0], rows, a.D);
+  x.put(sQ);
+  y.put(sO);
+  auto fetch = [&](int j0) {
+    const long long key = ks.begin + j0;
+    x.get(static_cast<const T*>(a.k) + key * a.sk[0] + (long long)hk * a.sk[1], a.sk[0], ks.n - j0, a.D);
+    y.get(static_cast<const T*>(a.v) + key * a.sv[0] + (long long)hk * a.sv[1], a.sv[0], ks.n - j0, a.D);
+  };
+  if (seen > 0) fetch(0);
+  load_statistics<TILE>(a, lse, delta, h, (int)row, rows);
   float4 acc[NR][NC];
 #pragma unroll
   for (int r = 0; r < NR; ++r)
@@ -221,20 +267,20 @@ __global__ void __launch_bounds__(kThreads) packed_generic_dq_kernel(const Packe
     for (int k = 0; k < NC; ++k) acc[r][k] = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int j0 = 0; j0 < seen; j0 += TILE) {
     __syncthreads();
-    const long long key = ks.begin + j0;
-    load_rows<T, DP>(sK, static_cast<const T*>(a.k) + key * a.sk[0] + (long long)hk * a.sk[1], a.sk[0], ks.n - j0, a.D);
-    load_rows<T, DP>(sV, static_cast<const T*>(a.v) + key * a.sv[0] + (long long)hk * a.sv[1], a.sv[0], ks.n - j0, a.D);
+    x.put(sK);
+    y.put(sV);
     __syncthreads();
+    if (j0 + TILE < seen) fetch(j0 + TILE);
     float s[NR][NR], dp[NR][NR];
-    products<DP>(sQ, sK, ty, tx, s);
-    products<DP>(sO, sV, ty, tx, dp);
+    products<C, DP>(sQ, sK, ty, tx, s);
+    products<C, DP>(sO, sV, ty, tx, dp);
     p_and_ds(a, s, dp, lse, delta, i0, j0, qs.n, ks.n, ty, tx);
 #pragma unroll
     for (int r = 0; r < NR; ++r)
 #pragma unroll
       for (int k = 0; k < NR; ++k) sS[(ty + 16 * r) * C::LP + tx + 16 * k] = dp[r][k];
     __syncthreads();
-    accumulate<DP, true>(sS, sK, ty, tx, acc);
+    accumulate<C>(sS, sK, ty, tx, acc);
   }
 #pragma unroll
   for (int r = 0; r < NR; ++r) {
@@ -245,10 +291,10 @@ __global__ void __launch_bounds__(kThreads) packed_generic_dq_kernel(const Packe
   }
 }
 
-template <class T, int DP>
+template <class T, int DP, int TILE, bool VEC>
 __global__ void __launch_bounds__(kThreads) packed_generic_dkv_kernel(const PackedArgs a) {
-  using C = GenericCfg<DP>;
-  constexpr int TILE = C::TILE, NR = C::NR, NC = C::NC;
+  using C = GenericCfg<DP, TILE>;
+  constexpr int NR = C::NR, NC = C::NC;
   extern __shared__ __align__(16) float sm[];
   float *sQ = sm, *sO = sQ + TILE * C::LD, *sK = sO + TILE * C::LD, *sV = sK + TILE * C::LD, *sP = sV + TILE * C::LD, *sS = sP + TILE * C::LP;
   float *lse = sS + TILE * C::LP, *delta = lse + TILE;
@@ -264,8 +310,11 @@ __global__ void __launch_bounds__(kThreads) packed_generic_dkv_kernel(const Pack
   const Span qs = query_span(a, at.seq), ks = key_span(a, at.seq);
   const int j0 = at.tile * TILE, keys = min(TILE, ks.n - j0);
   const long long key = ks.begin + j0;
-  load_rows<T, DP>(sK, static_cast<const T*>(a.k) + key * a.sk[0] + (long long)hk * a.sk[1], a.sk[0], keys, a.D);
-  load_rows<T, DP>(sV, static_cast<const T*>(a.v) + key * a.sv[0] + (long long)hk * a.sv[1], a.sv[0], keys, a.D);
+  Rows<T, DP, TILE, VEC> x, y;
+  x.get(static_cast<const T*>(a.k) + key * a.sk[0] + (long long)hk * a.sk[1], a.sk[0], keys, a.D);
+  y.get(static_cast<const T*>(a.v) + key * a.sv[0] + (long long)hk * a.sv[1], a.sv[0], keys, a.D);
+  x.put(sK);
+  y.put(sV);
   float4 dk[NR][NC], dv[NR][NC];
 #pragma unroll
   for (int r = 0; r < NR; ++r)
@@ -273,30 +322,40 @@ __global__ void __launch_bounds__(kThreads) packed_generic_dkv_kernel(const Pack
     for (int k = 0; k < NC; ++k) dk[r][k] = dv[r][k] = make_float4(0.f, 0.f, 0.f, 0.f);
   // the first query that sees a key of this tile
   const int first = a.causal ? max(0, j0 - (ks.n - qs.n)) : 0;
+  const int i_first = first / TILE * TILE;
+  auto fetch = [&](int h, int i0) {
+    const long long row = qs.begin + i0;
+    const int rows = min(TILE, qs.n - i0);
+    x.get(static_cast<const T*>(a.q) + row * a.sq[0] + (long long)h * a.sq[1], a.sq[0], rows, a.D);
+    y.get(static_cast<const T*>(a.d_o) + row * a.sdo[0] + (long long)h * a.sdo[1], a.sdo[0], rows, a.D);
+  };
+  if (i_first < qs.n) fetch(hk * a.G, i_first);
   for (int g = 0; g < a.G; ++g) {
     const int h = hk * a.G + g;
-    for (int i0 = first / TILE * TILE; i0 < qs.n; i0 += TILE) {
+    for (int i0 = i_first; i0 < qs.n; i0 += TILE) {
       __syncthreads();
       const long long row = qs.begin + i0;
       const int rows = min(TILE, qs.n - i0);
-      load_rows<T, DP>(sQ, static_cast<const T*>(a.q) + row * a.sq[0] + (long long)h * a.sq[1], a.sq[0], rows, a.D);
-      load_rows<T, DP>(sO, static_cast<const T*>(a.d_o) + row * a.sdo[0] + (long long)h * a.sdo[1], a.sdo[0], rows, a.D);
-      load_statistics<DP>(a, lse, delta, h, (int)row, rows);
+      x.put(sQ);
+      y.put(sO);
+      load_statistics<TILE>(a, lse, delta, h, (int)row, rows);
       __syncthreads();
+      if (i0 + TILE < qs.n) fetch(h, i0 + TILE);
+      else if (g + 1 < a.G) fetch(h + 1, i_first);
       float s[NR][NR], dp[NR][NR];
-      products<DP>(sQ, sK, ty, tx, s);
-      products<DP>(sO, sV, ty, tx, dp);
+      products<C, DP>(sQ, sK, ty, tx, s);
+      products<C, DP>(sO, sV, ty, tx, dp);
       p_and_ds(a, s, dp, lse, delta, i0, j0, qs.n, ks.n, ty, tx);
 #pragma unroll
       for (int r = 0; r < NR; ++r)
 #pragma unroll
         for (int k = 0; k < NR; ++k) {
-          sP[(ty + 16 * r) * C::LP + tx + 16 * k] = s[r][k];
-          sS[(ty + 16 * r) * C::LP + tx + 16 * k] = dp[r][k];
+          sP[(tx + 16 * k) * C::LP + ty + 16 * r] = s[r][k];  // (by keys)
+          sS[(tx + 16 * k) * C::LP + ty + 16 * r] = dp[r][k];
         }
       __syncthreads();
-      accumulate<DP, false>(sP, sO, ty, tx, dv);
-      accumulate<DP, false>(sS, sQ, ty, tx, dk);
+      accumulate<C>(sP, sO, ty, tx, dv);
+      accumulate<C>(sS, sQ, ty, tx, dk);
     }
   }
 #pragma unroll
@@ -318,33 +377,41 @@ int run(K kern, const PackedArgs& a, long long rows, int tile, int heads, size_t
   *launches += 1;
   return cudaGetLastError() == cudaSuccess ? EVOATTN_OK : EVOATTN_ERR_CUDA;
 }
-template <class T, int DP>
-int fwd(const PackedArgs& a, cudaStream_t st, int* launches) {
-  using C = GenericCfg<DP>;
-  return run(packed_generic_fwd_kernel<T, DP>, a, a.Tq, C::TILE, a.H, C::bytes(3, 1), st, launches);
-}
-template <class T, int DP>
-int bwd(const PackedArgs& a, cudaStream_t st, int* launches) {
-  using C = GenericCfg<DP>;
+template <class T, int DP, int TILE, bool VEC>
+int both(bool back, const PackedArgs& a, cudaStream_t st, int* launches) {
+  using C = GenericCfg<DP, TILE>;
+  if (!back) return run(packed_generic_fwd_kernel<T, DP, TILE, VEC>, a, a.Tq, TILE, a.H, C::bytes(3, 1), st, launches);
   if (a.dk) {
-    const int rc = run(packed_generic_dkv_kernel<T, DP>, a, a.Tk, C::TILE, a.Hk, C::bytes(4, 2), st, launches);
+    const int rc = run(packed_generic_dkv_kernel<T, DP, TILE, VEC>, a, a.Tk, TILE, a.Hk, C::bytes(4, 2), st, launches);
     if (rc) return rc;
   }
-  return a.dq ? run(packed_generic_dq_kernel<T, DP>, a, a.Tq, C::TILE, a.H, C::bytes(4, 1), st, launches) : EVOATTN_OK;
+  return a.dq ? run(packed_generic_dq_kernel<T, DP, TILE, VEC>, a, a.Tq, TILE, a.H, C::bytes(4, 1), st, launches) : EVOATTN_OK;
+}
+template <class T>
+bool vectors(const PackedArgs& a, bool bwd) {
+  constexpr int V = kPer16<T>;
+  const auto ok = [](const void* p, const long long* st) { return ((uintptr_t)p & 15) == 0 && st[0] % V == 0 && st[1] % V == 0; };
+  return a.D % V == 0 && ok(a.q, a.sq) && ok(a.k, a.sk) && ok(a.v, a.sv) && (!bwd || ok(a.d_o, a.sdo));
+}
+template <class T, int DP>
+int launch(bool back, const PackedArgs& a, cudaStream_t st, int* launches) {
+  const bool vec = vectors<T>(a, back);
+  if constexpr (DP <= 128) {
+    const long long blocks = (a.Tq / 64 + a.B) * (long long)(back ? a.Hk : a.H);
+    if (blocks > 3LL * sm_count()) return vec ? both<T, DP, 64, true>(back, a, st, launches) : both<T, DP, 64, false>(back, a, st, launches);
+  }
+  return vec ? both<T, DP, 32, true>(back, a, st, launches) : both<T, DP, 32, false>(back, a, st, launches);
+}
+int launch_any(int dtype, bool back, const PackedArgs& a, cudaStream_t st, int* launches) {
+  return with_dtype(dtype, [&](auto t) {
+    using T = decltype(t);
+    return a.D <= 64 ? launch<T, 64>(back, a, st, launches) : a.D <= 128 ? launch<T, 128>(back, a, st, launches) : launch<T, 256>(back, a, st, launches);
+  });
 }
 
 }  // namespace
 
-int launch_packed_generic_fwd(int dtype, const PackedArgs& a, cudaStream_t st, int* launches) {
-  return with_dtype(dtype, [&](auto t) {
-    using T = decltype(t);
-    return a.D <= 64 ? fwd<T, 64>(a, st, launches) : a.D <= 128 ? fwd<T, 128>(a, st, launches) : fwd<T, 256>(a, st, launches);
-  });
-}
-int launch_packed_generic_bwd(int dtype, const PackedArgs& a, cudaStream_t st, int* launches) {
-  return with_dtype(dtype, [&](auto t) {
-    using T = decltype(t);
-    return a.D <= 64 ? bwd<T, 64>(a, st, launches) : a.D <= 128 ? bwd<T, 128>(a, st, launches) : bwd<T, 256>(a, st, launches);
-  });
-}
+int launch_packed_generic_fwd(int dtype, const PackedArgs& a, cudaStream_t st, int* launches) { return launch_any(dtype, false, a, st, launches); }
+int launch_packed_generic_bwd(int dtype, const PackedArgs& a, cudaStream_t st, int* launches) { return launch_any(dtype, true, a, st, launches); }
+
 }  // namespace evo

@@ -8,7 +8,10 @@ namespace {
 constexpr int kThreads = 512;
 constexpr int kClasses = 2048;  // by work; what has more is of one class
 
+constexpr int kKept = 1024;
+
 struct Sums {
+  int4 spans[kKept];
   int first[kClasses];
   int warps[kThreads / 32 + 1];
   long long steps;
@@ -16,18 +19,28 @@ struct Sums {
 };
 
 // The tiles of all sequences, a warp per sequence and its lanes over the tiles; called several times, so the spans of the
-// first sequence (with 16 or fewer the only one) stay in registers.
+// first kKept sequences are kept in shared memory.
 struct Tiles {
-  Span q, k;
-  __device__ __forceinline__ Tiles(const PackedArgs& a) {
-    const int b = threadIdx.x >> 5;
-    if (b < a.B) { q = query_span(a, b); k = key_span(a, b); }
+  const int4* kept;
+  __device__ __forceinline__ Tiles(const PackedArgs& a, int4* keep) : kept(keep) {
+    for (int b = threadIdx.x; b < a.B && b < kKept; b += kThreads) {
+      const Span q = query_span(a, b), k = key_span(a, b);
+      keep[b] = make_int4(q.begin, q.n, k.begin, k.n);
+    }
+    __syncthreads();
   }
   template <class F>
   __device__ __forceinline__ void each(const PackedArgs& a, bool queries, int unit, F&& f) const {
     for (int b = threadIdx.x >> 5; b < a.B; b += kThreads / 32) {
-      const bool mine = b < kThreads / 32;
-      const Span qs = mine ? q : query_span(a, b), ks = mine ? k : key_span(a, b);
+      Span qs, ks;
+      if (b < kKept) {
+        const int4 x = kept[b];
+        qs = Span{x.x, x.y};
+        ks = Span{x.z, x.w};
+      } else {
+        qs = query_span(a, b);
+        ks = key_span(a, b);
+      }
       const int n = !queries ? ks.n : qs.n > a.few_tokens ? qs.n : 0;
       for (int x = (threadIdx.x & 31) * unit; x < n; x += 32 * unit) {
         PackedTile t{};
@@ -59,7 +72,7 @@ struct Tiles {
 // share of those of an SM are cut into parts, which leave fp32 sums to be joined: a group of heads or a long
 // sequence makes single tiles that would outlast everything else.
 __device__ __forceinline__ void make_list(const PackedArgs& a, const PackedPlan& plan, bool queries, int unit, int sms, const PackedCut& c, Sums& s) {
-  const Tiles tiles(a);
+  const Tiles tiles(a, s.spans);
   PackedTile* out = queries ? plan.queries : plan.keys;
   for (int i = threadIdx.x; i < kClasses; i += kThreads) s.first[i] = 0;
   if (queries)
