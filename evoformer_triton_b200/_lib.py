@@ -129,7 +129,7 @@ class PackedParams(C.Structure):
         ("Tq", C.c_int64), ("Tk", C.c_int64),
         ("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p),
         ("q_stride", C.c_int64 * 2), ("k_stride", C.c_int64 * 2), ("v_stride", C.c_int64 * 2),
-        ("offsets", C.c_void_p), ("key_offsets", C.c_void_p), ("o", C.c_void_p), ("lse", C.c_void_p), ("status", C.c_void_p),
+        ("offsets", C.c_void_p), ("key_offsets", C.c_void_p), ("o", C.c_void_p), ("lse", C.c_void_p), ("o_rest", C.c_void_p), ("status", C.c_void_p),
         ("d_o", C.c_void_p), ("do_stride", C.c_int64 * 2), ("dq", C.c_void_p), ("dk", C.c_void_p), ("dv", C.c_void_p),
         ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
     ]

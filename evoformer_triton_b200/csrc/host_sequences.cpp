@@ -146,7 +146,7 @@ struct PackedPlan {
   double scale;
 };
 struct PackedCall {
-  Tensor q, k, v, offsets, keys, o, lse;
+  Tensor q, k, v, offsets, keys, o, lse, rest;
   evoattn_packed_params p{};
   PackedCall(const Tensor& q_in, const Tensor& k_in, const Tensor& v_in, const Tensor& off, const Tensor& key_off, const PackedPlan& plan)
       : q(mapped(q_in)), k(mapped(k_in)), v(mapped(v_in)), offsets(off), keys(key_off) {
@@ -182,6 +182,7 @@ struct PackedCall {
     if (keep_lse) {
       lse = at::empty({p.H, p.Tq}, q.options().dtype(at::kFloat));
       p.lse = lse.data_ptr<float>();
+      if (p.dtype != EVOATTN_FP32) rest = at::empty(q.sizes(), q.options()), p.o_rest = rest.data_ptr();
     }
     const Tensor ws = scratch(evoattn_packed_fwd_workspace_bytes(&p));
     check(evoattn_packed_fwd(&p, stream()), "evoattn_packed_fwd");
@@ -195,7 +196,7 @@ struct Packed : public torch::autograd::Function<Packed> {
     const c10::cuda::CUDAGuard guard(q.device());
     PackedCall c(q, k, v, offsets, keys ? *keys : Tensor(), {causal, scale});
     c.run(true);
-    ctx->save_for_backward({c.q, c.k, c.v, c.offsets, c.keys, c.o, c.lse});
+    ctx->save_for_backward({c.q, c.k, c.v, c.offsets, c.keys, c.o, c.lse, c.rest});
     ctx->saved_data["causal"] = causal;
     ctx->saved_data["scale"] = scale;
     return c.o;
@@ -215,6 +216,7 @@ struct Packed : public torch::autograd::Function<Packed> {
       const Tensor d = mapped(grads[0].scalar_type() == c.q.scalar_type() ? grads[0] : grads[0].to(c.q.scalar_type()));
       p.o = s[5].data_ptr();
       p.lse = s[6].data_ptr<float>();
+      p.o_rest = s[7].defined() ? s[7].data_ptr() : nullptr;
       p.d_o = d.data_ptr();
       PackedCall::strides(d, p.do_stride);
       const Tensor ws = c.scratch(evoattn_packed_bwd_workspace_bytes(&p));

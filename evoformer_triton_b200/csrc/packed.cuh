@@ -12,6 +12,7 @@ namespace evo {
 struct PackedArgs {
   const void *q, *k, *v;
   void* o;             // [Tq,H,D] dense; backward: in
+  void* o_rest;        // what rounding left of o, or null
   float* lse;          // [H][lse_ld]: log2 of a row's sum of exp2(score * scale * log2 e); -inf: no key
   const void *d_o;     // backward
   void *dq, *dk, *dv;  // dense, as q, k, v

@@ -23,7 +23,7 @@ int validate(const evoattn_packed_params* p, bool bwd) {
 
 PackedArgs arguments(const evoattn_packed_params* p) {
   PackedArgs a{};
-  a.q = p->q; a.k = p->k; a.v = p->v; a.o = p->o; a.lse = p->lse;
+  a.q = p->q; a.k = p->k; a.v = p->v; a.o = p->o; a.o_rest = p->o_rest; a.lse = p->lse;
   a.d_o = p->d_o; a.dq = p->dq; a.dk = p->dk; a.dv = p->dv;
   for (int i = 0; i < 2; ++i) a.sq[i] = p->q_stride[i], a.sk[i] = p->k_stride[i], a.sv[i] = p->v_stride[i], a.sdo[i] = p->do_stride[i];
   a.offsets = p->offsets;

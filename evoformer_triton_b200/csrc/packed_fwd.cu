@@ -18,7 +18,9 @@
 // m is not the maximum but a reference that the exponentials of a tile are taken against straight from the scores, without
 // looking for their maximum: any m gives the same o as long as nothing leaves the range of P's type.  It is 0 to begin with; if
 // a tile's sum shows that some p may be too large, or a row's first sum that all of them are too small, the tile's maximum
-// is taken, O and l follow it, and the tile is done again (P is kept in registers until then).
+// is taken, O and l follow it, and the tile is done again (P is kept in registers until then).  O is divided by the sum of the
+// P that it was made of, rounded (with that of the unrounded values it was off by 0.0023 instead of 0.0021 of its norm, where
+// its own rounding makes 0.0016); the log-sum-exp is that of the unrounded ones.
 #include "packed_sm100.cuh"
 
 namespace evo {
@@ -53,10 +55,10 @@ struct FwdCfg {
   static_assert(colO + 2 * DP <= 512, "tensor memory");
 };
 
-template <class T, int DP, bool PAIR>  // PAIR: two query tiles of one head, else one tile of two heads
+template <class T, int DP, bool PAIR, bool LSE>  // PAIR: two query tiles of one head, else one tile of two heads; LSE: for a backward pass
 __global__ void __launch_bounds__(kThreads, 1)
 packed_fwd_sm100_kernel(const PackedArgs a, const PackedPlan plan, const FastDiv units, const __grid_constant__ CUtensorMap tmQ,
-                        const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmO) {
+                        const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmO, const __grid_constant__ CUtensorMap tmR) {
   using C = FwdCfg<DP>;
   constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
   constexpr int NS = C::kStages;
@@ -271,7 +273,7 @@ packed_fwd_sm100_kernel(const PackedArgs a, const PackedPlan plan, const FastDiv
       // the last key that this row sees, and the first one that some row of the warp does not
       const int last = a.causal ? min(it.t.n - 1, it.t.shift + (PAIR ? w * BM : 0) + row) : it.t.n - 1;
       const int warp_last = __shfl_sync(0xffffffffu, last, 0), warp_most = __shfl_sync(0xffffffffu, last, 31);
-      float m = 0.f, l = 0.f;
+      float m = 0.f, l = 0.f, lu = 0.f;  // l of P as rounded, lu of P as it is
       bool steep = false;
 #pragma unroll 1
       for (int t = end - 1; t >= first_tile; --t, ++g) {
@@ -281,16 +283,16 @@ packed_fwd_sm100_kernel(const PackedArgs a, const PackedPlan plan, const FastDiv
         const bool cut = warp_last - t * BN < BN - 1;
         const int pieces = (warp_most - t * BN + 16) >> 4;  // of 16 keys, those that some row sees
         uint32_t pk[BN / 2];
-        float lsum = 0.f;
+        float lsum = 0.f, lsum_u = 0.f;
         bool go = !__any_sync(0xffffffffu, steep), settled = false;
 #pragma unroll 1
         for (;;) {
           bool bad = true;
           if (go) {
             const F2 nm2 = f2_make(-m, -m);
-            F2 ls[4];
+            F2 ls[4], lsu[4];
 #pragma unroll
-            for (int u = 0; u < 4; ++u) ls[u] = f2_make(0.f, 0.f);
+            for (int u = 0; u < 4; ++u) ls[u] = lsu[u] = f2_make(0.f, 0.f);
             auto exps = [&](auto with_mask) {
               constexpr bool kMask = decltype(with_mask)::value;
               uint32_t sr[2][16];
@@ -322,17 +324,23 @@ packed_fwd_sm100_kernel(const PackedArgs a, const PackedPlan plan, const FastDiv
                     p0 = ex2(x0);
                     p1 = ex2(x1);
                   }
+                  if constexpr (LSE) lsu[(e / 2) & 3] = f2_add(lsu[(e / 2) & 3], f2_make(p0, p1));
+                  const uint32_t both = Pack2<T>::pack(p0, p1);
+                  pk[8 * k + e / 2] = both;
+                  unpack2<T>(both, p0, p1);
                   ls[(e / 2) & 3] = f2_add(ls[(e / 2) & 3], f2_make(p0, p1));
-                  pk[8 * k + e / 2] = Pack2<T>::pack(p0, p1);
                 }
               }
             };
             if (cut) exps(std::true_type{});
             else exps(std::false_type{});
-            float s8[8];
-#pragma unroll
-            for (int u = 0; u < 4; ++u) f2_get(ls[u], s8[2 * u], s8[2 * u + 1]);
-            lsum = ((s8[0] + s8[1]) + (s8[2] + s8[3])) + ((s8[4] + s8[5]) + (s8[6] + s8[7]));
+            auto total = [](const F2 (&x)[4]) {
+              float s0, s1;
+              f2_get(f2_add(f2_add(x[0], x[1]), f2_add(x[2], x[3])), s0, s1);
+              return s0 + s1;
+            };
+            lsum = total(ls);
+            if constexpr (LSE) lsum_u = total(lsu);
             bad = __any_sync(0xffffffffu, valid && !(lsum <= Lag<T>::kMaxSum && (l > 0.f || lim < 0 || lsum >= Lag<T>::kMinSum)));
           }
           if (__builtin_expect(!bad || settled, 1)) break;
@@ -362,6 +370,7 @@ packed_fwd_sm100_kernel(const PackedArgs a, const PackedPlan plan, const FastDiv
           if (t < end - 1 && __any_sync(0xffffffffu, !fresh && m > m_old)) {
             const float alpha = !fresh && m > m_old ? ex2(m_old - m) : 1.f;
             l *= alpha;
+            lu *= alpha;
 #pragma unroll 1
             for (int d0 = 0; d0 < DP; d0 += 16) {
               uint32_t o[16];
@@ -377,6 +386,7 @@ packed_fwd_sm100_kernel(const PackedArgs a, const PackedPlan plan, const FastDiv
           go = settled = true;
         }
         l += lsum;
+        lu += lsum_u;
         tmem_st32(tS, *reinterpret_cast<uint32_t(*)[32]>(&pk[0]));
         tmem_st32(tS + 32, *reinterpret_cast<uint32_t(*)[32]>(&pk[32]));
         tmem_wait_st();
@@ -407,7 +417,7 @@ packed_fwd_sm100_kernel(const PackedArgs a, const PackedPlan plan, const FastDiv
 #pragma unroll
           for (int e = 0; e < 32; e += 4) to[(d + e) / 4 * BM] = make_float4(__uint_as_float(r[e]), __uint_as_float(r[e + 1]), __uint_as_float(r[e + 2]), __uint_as_float(r[e + 3]));
         }
-        plan.ml[at * BM + row] = make_float2(m, some ? l : 0.f);
+        plan.ml[at * BM + row] = make_float4(m, some ? l : 0.f, lu, 0.f);
         __threadfence();
         meet();
         if (row == 0) arrived[w] = atomicAdd(plan.arrived + place(it.t.slot - it.t.part), 1);
@@ -423,20 +433,21 @@ packed_fwd_sm100_kernel(const PackedArgs a, const PackedPlan plan, const FastDiv
         const int slot0 = it.t.slot - it.t.part;
 #pragma unroll 1
         for (int p = 0; p < it.t.parts; ++p) {
-          const float2 x = __ldcg(plan.ml + place(slot0 + p) * BM + row);
+          const float4 x = __ldcg(plan.ml + place(slot0 + p) * BM + row);
           if (x.y > 0.f) m = fmaxf(m, x.x);
         }
         if (m == -kInf) m = 0.f;
 #pragma unroll 1
         for (int d = 0; d < DP; d += 16) {
           float acc[16] = {};
-          l = 0.f;
+          l = lu = 0.f;
 #pragma unroll 1
           for (int p = 0; p < it.t.parts; ++p) {
-            const float2 x = __ldcg(plan.ml + place(slot0 + p) * BM + row);
+            const float4 x = __ldcg(plan.ml + place(slot0 + p) * BM + row);
             const float f = x.y > 0.f ? ex2(x.x - m) : 0.f;
             const float4* from = reinterpret_cast<const float4*>(plan.sums) + place(slot0 + p) * (DP / 4 * BM) + d / 4 * BM + row;
             l = fmaf(x.y, f, l);
+            lu = fmaf(x.z, f, lu);
             if (f > 0.f) {  // (a part that this row sees nothing of may have left nothing)
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
@@ -457,7 +468,12 @@ packed_fwd_sm100_kernel(const PackedArgs a, const PackedPlan plan, const FastDiv
       const int first = (warp & 3) * 32;  // row of the warp's first lane
       store_rows_staged<T, DP>(smem_s + C::offOut + (warp - 4) * kStageBytes, tO, &tmO, (int)(out_row - lane), h, static_cast<T*>(a.o) + ((out_row - lane) * a.H + h) * a.D,
                                (long long)a.H * a.D, rows - first, a.D, any ? 1.f / l : 0.f, some);
-      if (valid && a.lse) a.lse[(long long)h * a.lse_ld + out_row] = any ? m + log2f(l) : -kInf;
+      if constexpr (LSE) {
+        if (a.o_rest)
+          store_rows_staged<T, DP, true>(smem_s + C::offOut + (warp - 4) * kStageBytes, tO, &tmR, (int)(out_row - lane), h,
+                                         static_cast<T*>(a.o_rest) + ((out_row - lane) * a.H + h) * a.D, (long long)a.H * a.D, rows - first, a.D, any ? 1.f / l : 0.f, some);
+        if (valid) a.lse[(long long)h * a.lse_ld + out_row] = any ? m + log2f(lu) : -kInf;
+      }
       tc_fence_before();  // (the next item's first P V, which overwrites O, follows a later arrival)
     }
     stores_done();
@@ -471,18 +487,18 @@ packed_fwd_sm100_kernel(const PackedArgs a, const PackedPlan plan, const FastDiv
 bool head_pairs(const PackedArgs& a) { return a.G % 2 == 0; }
 PackedCut query_cut(const PackedArgs& a, bool pair) { return PackedCut{100, 10, pair ? a.H : a.H / 2}; }
 
-template <class T, int DP, bool PAIR>
+template <class T, int DP, bool PAIR, bool LSE>
 int launch(const PackedArgs& a, void* ws, cudaStream_t st, int* launches) {
   using C = FwdCfg<DP>;
   constexpr int unit = PAIR ? 2 * BM : BM;
-  CUtensorMap tq, tk, tv, to;
+  CUtensorMap tq, tk, tv, to, tr;
   const long long so[2] = {(long long)a.H * a.D, a.D};
   if (!make_packed_map(&tq, a.q, a.sq, a.Tq, a.H, a.D) || !make_packed_map(&tk, a.k, a.sk, a.Tk, a.Hk, a.D) || !make_packed_map(&tv, a.v, a.sv, a.Tk, a.Hk, a.D) ||
-      !make_packed_map(&to, a.o, so, a.Tq, a.H, a.D, 32))
+      !make_packed_map(&to, a.o, so, a.Tq, a.H, a.D, 32) || !make_packed_map(&tr, a.o_rest ? a.o_rest : a.o, so, a.Tq, a.H, a.D, 32))
     return EVOATTN_ERR_CUDA;
   const int sms = sm_count();
   if (sms <= 0) return EVOATTN_ERR_CUDA;
-  auto kern = packed_fwd_sm100_kernel<T, DP, PAIR>;
+  auto kern = packed_fwd_sm100_kernel<T, DP, PAIR, LSE>;
   int regs = 0;
   if (!kernel_ready(reinterpret_cast<const void*>(kern), (int)C::bytes, &regs)) return EVOATTN_ERR_CUDA;
   // (setmaxnreg.inc would wait for registers that the launch does not have)
@@ -493,14 +509,14 @@ int launch(const PackedArgs& a, void* ws, cudaStream_t st, int* launches) {
   if (rc) return rc;
   const int heads = PAIR ? a.H : a.H / 2;
   const long long most = (query_units(a, unit) + query_slots(a, unit, sms, cut)) * heads;
-  launch_dependent(kern, dim3((unsigned)(most < sms ? most : sms)), kThreads, C::bytes, st, a, plan, FastDiv((uint32_t)heads), tq, tk, tv, to);
+  launch_dependent(kern, dim3((unsigned)(most < sms ? most : sms)), kThreads, C::bytes, st, a, plan, FastDiv((uint32_t)heads), tq, tk, tv, to, tr);
   *launches += 1;
   return cudaGetLastError() == cudaSuccess ? EVOATTN_OK : EVOATTN_ERR_CUDA;
 }
-template <class T>
+template <class T, int DP>
 int launch_d(const PackedArgs& a, void* ws, cudaStream_t st, int* launches) {
-  if (a.D <= 64) return head_pairs(a) ? launch<T, 64, false>(a, ws, st, launches) : launch<T, 64, true>(a, ws, st, launches);
-  return head_pairs(a) ? launch<T, 128, false>(a, ws, st, launches) : launch<T, 128, true>(a, ws, st, launches);
+  if (a.lse) return head_pairs(a) ? launch<T, DP, false, true>(a, ws, st, launches) : launch<T, DP, true, true>(a, ws, st, launches);
+  return head_pairs(a) ? launch<T, DP, false, false>(a, ws, st, launches) : launch<T, DP, true, false>(a, ws, st, launches);
 }
 
 }  // namespace
@@ -509,13 +525,13 @@ bool sm100_packed_supported(int dtype, const PackedArgs& a) {
   if (dtype == EVOATTN_FP32 || a.D % 8 || a.D > 128 || !(a.scale > 0.f)) return false;
   // (numbers of items fit 31 bits)
   if ((a.Tq / kTileRows + a.B) * (long long)a.H >= 1LL << 31 || (a.Tk / kTileRows + a.B) * (long long)a.Hk >= 1LL << 31) return false;
-  if (reinterpret_cast<uintptr_t>(a.o) & 15) return false;
+  if ((reinterpret_cast<uintptr_t>(a.o) | reinterpret_cast<uintptr_t>(a.o_rest)) & 15) return false;
   return packed_map_ok(a.q, a.sq, a.Tq, a.H) && packed_map_ok(a.k, a.sk, a.Tk, a.Hk) && packed_map_ok(a.v, a.sv, a.Tk, a.Hk);
 }
 size_t sm100_packed_fwd_workspace_bytes(const PackedArgs& a) { return plan_bytes(a, true, head_pairs(a) ? BM : 2 * BM, false, sm_count(), query_cut(a, !head_pairs(a))).all(); }
 int launch_sm100_packed_fwd(int dtype, const PackedArgs& a, void* ws, cudaStream_t st, int* launches) {
-  if (dtype == EVOATTN_BF16) return launch_d<__nv_bfloat16>(a, ws, st, launches);
-  return launch_d<__half>(a, ws, st, launches);
+  if (dtype == EVOATTN_BF16) return a.D <= 64 ? launch_d<__nv_bfloat16, 64>(a, ws, st, launches) : launch_d<__nv_bfloat16, 128>(a, ws, st, launches);
+  return a.D <= 64 ? launch_d<__half, 64>(a, ws, st, launches) : launch_d<__half, 128>(a, ws, st, launches);
 }
 
 }  // namespace evo

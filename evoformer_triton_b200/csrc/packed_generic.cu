@@ -205,6 +205,13 @@ __global__ void __launch_bounds__(kThreads) packed_generic_fwd_kernel(const Pack
     T* out = o + ((long long)(qs.begin + i0 + i) * a.H + h) * a.D;
 #pragma unroll
     for (int k = 0; k < NC; ++k) store_row(out, tx, k, acc[r][k], m[r] == -INFINITY ? 0.f : inv, a.D);
+    if (a.o_rest) {
+      T* rest = static_cast<T*>(a.o_rest) + (out - o);
+      const float by = m[r] == -INFINITY ? 0.f : inv;
+      auto left = [&](float v) { return v * by - to_float(from_float<T>(v * by)); };
+#pragma unroll
+      for (int k = 0; k < NC; ++k) store_row(rest, tx, k, make_float4(left(acc[r][k].x), left(acc[r][k].y), left(acc[r][k].z), left(acc[r][k].w)), 1.f, a.D);
+    }
     if (tx == 0 && a.lse) a.lse[(long long)h * a.lse_ld + qs.begin + i0 + i] = m[r] == -INFINITY ? -INFINITY : m[r] + log2f(l[r]);
   }
 }

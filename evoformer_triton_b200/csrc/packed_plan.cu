@@ -152,6 +152,7 @@ __device__ __forceinline__ void row_sums(const PackedArgs& a, long long block, l
   const long long items = (long long)a.Tq * a.H;
   const T* o = static_cast<const T*>(a.o);
   const T* d_o = static_cast<const T*>(a.d_o);
+  const T* rest = static_cast<const T*>(a.o_rest);
   constexpr int V = VEC ? kPer16<T> : 1, U = 4;
   for (long long i0 = block * teams * U + team; i0 < items; i0 += blocks * teams * U) {
     float s[U] = {};
@@ -167,18 +168,22 @@ __device__ __forceinline__ void row_sums(const PackedArgs& a, long long block, l
     }
     for (int x = lane * V; x < a.D; x += lanes * V) {
       if constexpr (VEC) {
-        uint4 w[U], z[U];
+        uint4 w[U], y[U], z[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
           const long long i = min(i0 + (long long)u * teams, items - 1);
           w[u] = *reinterpret_cast<const uint4*>(o + i * a.D + x);
           z[u] = *reinterpret_cast<const uint4*>(d[u] + x);
+          y[u] = rest ? *reinterpret_cast<const uint4*>(rest + i * a.D + x) : make_uint4(0, 0, 0, 0);
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-          float f[V], g[V];
+          float f[V], h[V], g[V];
           unpack16<T>(w[u], f);
+          unpack16<T>(y[u], h);
           unpack16<T>(z[u], g);
+#pragma unroll
+          for (int e = 0; e < V; ++e) f[e] += h[e];
 #pragma unroll
           for (int e = 0; e < V; ++e) s[u] = fmaf(f[e], g[e], s[u]);
         }
@@ -186,7 +191,7 @@ __device__ __forceinline__ void row_sums(const PackedArgs& a, long long block, l
 #pragma unroll
         for (int u = 0; u < U; ++u) {
           const long long i = min(i0 + (long long)u * teams, items - 1);
-          s[u] = fmaf(to_float(o[i * a.D + x]), to_float(d[u][x]), s[u]);
+          s[u] = fmaf(to_float(o[i * a.D + x]) + (rest ? to_float(rest[i * a.D + x]) : 0.f), to_float(d[u][x]), s[u]);
         }
       }
     }
@@ -223,7 +228,7 @@ int launch_packed_prepare(int dtype, const PackedArgs& a, const PackedPlan& plan
   return with_dtype(dtype, [&](auto t) {
     using T = decltype(t);
     constexpr int V = kPer16<T>;
-    const bool vec = delta && a.D % V == 0 && ((reinterpret_cast<uintptr_t>(a.o) | reinterpret_cast<uintptr_t>(a.d_o)) & 15) == 0 && a.sdo[0] % V == 0 && a.sdo[1] % V == 0;
+    const bool vec = delta && a.D % V == 0 && ((reinterpret_cast<uintptr_t>(a.o) | reinterpret_cast<uintptr_t>(a.o_rest) | reinterpret_cast<uintptr_t>(a.d_o)) & 15) == 0 && a.sdo[0] % V == 0 && a.sdo[1] % V == 0;
     int lanes = 1;
     while (lanes < 32 && lanes * (vec ? V : 1) < a.D) lanes *= 2;
     const long long rows = ((long long)a.Tq * a.H + kThreads / lanes * 4 - 1) / (kThreads / lanes * 4);

@@ -33,7 +33,7 @@ struct PackedPlan {
   PackedTile *queries, *keys;
   PackedJoin* joins;
   float* sums;               // key tiles: [slot][Hk][dV, dK][DP / 4][128 rows][4]; query units: [slot][units of heads][2 tiles][DP / 4][128][4]
-  float2* ml;                // [slot][units of heads][2 tiles][128 rows]: reference and sum
+  float4* ml;                // [slot][units of heads][2 tiles][128 rows]: reference, sum of P as rounded, and as it is
   int *arrived, n_arrived;   // [slot][units of heads][2 tiles]: parts that are through, of the tile whose first part has that slot
 };
 // What a list cuts: tiles of one and a half times as many steps and more as `part` hundredths of what an SM has to do, and as
@@ -68,7 +68,7 @@ inline PlanBytes plan_bytes(const PackedArgs& a, bool queries, int unit, bool ke
   const long long ks = keys ? key_slots(a, sms) : 0, qs = queries && qcut.heads ? query_slots(a, unit, sms, qcut) : 0;
   const size_t tile = (size_t)kTileRows * (a.D <= 64 ? 64 : 128) * sizeof(float), tiles = (size_t)qs * qcut.heads * 2;
   return PlanBytes{queries ? round256((query_units(a, unit) + qs) * sizeof(PackedTile)) : 0, keys ? round256((key_tiles(a) + ks) * sizeof(PackedTile)) : 0,
-                   round256(ks * sizeof(PackedJoin)), round256(tile * (ks * a.Hk * 2 + tiles)), round256(tiles * kTileRows * sizeof(float2)), round256(tiles * sizeof(int))};
+                   round256(ks * sizeof(PackedJoin)), round256(tile * (ks * a.Hk * 2 + tiles)), round256(tiles * kTileRows * sizeof(float4)), round256(tiles * sizeof(int))};
 }
 inline PackedPlan place_plan(void* ws, const PlanBytes& n) {
   unsigned char* p = static_cast<unsigned char*>(ws);
@@ -78,7 +78,7 @@ inline PackedPlan place_plan(void* ws, const PlanBytes& n) {
   plan.keys = reinterpret_cast<PackedTile*>(p += n.queries);
   plan.joins = reinterpret_cast<PackedJoin*>(p += n.keys);
   plan.sums = reinterpret_cast<float*>(p += n.joins);
-  plan.ml = reinterpret_cast<float2*>(p += n.sums);
+  plan.ml = reinterpret_cast<float4*>(p += n.sums);
   plan.arrived = reinterpret_cast<int*>(p + n.ml);
   plan.n_arrived = (int)(n.arrived / sizeof(int));
   return plan;
@@ -152,7 +152,8 @@ __device__ __forceinline__ void exp2_fma(ptx::F2 x, float& p0, float& p1) {
 // behind it belongs to the next one).  An SM takes more than a microsecond to get rid of a 128 x 128 tile: as plain stores
 // that is waited for at the end of every item (2.0 us from the lanes, 1.6 by way of shared memory).
 constexpr int kStageBytes = 32 * 128;
-template <class T, int DP>
+// REST: what rounding leaves of them instead.
+template <class T, int DP, bool REST = false>
 __device__ __forceinline__ void store_rows_staged(uint32_t stage_s, uint32_t t_src, const CUtensorMap* map, int row0, int head, T* out, long long ld, int rows, int D,
                                                   float f, bool any) {
   using namespace ptx;
@@ -174,7 +175,16 @@ __device__ __forceinline__ void store_rows_staged(uint32_t stage_s, uint32_t t_s
     for (int i = 0; i < 4; ++i) {
       uint32_t p[4];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) p[u] = any ? Pack2<T>::pack(__uint_as_float(r[8 * i + 2 * u]) * f, __uint_as_float(r[8 * i + 2 * u + 1]) * f) : 0u;
+      for (int u = 0; u < 4; ++u) {
+        const float x0 = __uint_as_float(r[8 * i + 2 * u]) * f, x1 = __uint_as_float(r[8 * i + 2 * u + 1]) * f;
+        p[u] = Pack2<T>::pack(x0, x1);
+        if constexpr (REST) {
+          float y0, y1;
+          unpack2<T>(p[u], y0, y1);
+          p[u] = Pack2<T>::pack(x0 - y0, x1 - y1);
+        }
+        if (!any) p[u] = 0u;
+      }
       sts_v4(stage_s + lane * 128 + (((4 * half + i) ^ (lane & 7)) << 4), p[0], p[1], p[2], p[3]);
     }
     if (half == 0) continue;
