@@ -842,7 +842,7 @@ size_t sm100_packed_bwd_workspace_bytes(const PackedArgs& a) { return delta_byte
 int launch_sm100_packed_bwd(int dtype, const PackedArgs& args, void* ws, cudaStream_t st, int* launches) {
   PackedArgs a = args;
   a.delta = static_cast<float*>(ws);
-  const PackedPlan plan = place_plan(static_cast<unsigned char*>(ws) + delta_bytes(a), plan_bytes(a, true, BT, true, sm_count()));
+  const PackedPlan plan = place_plan(a, BT, static_cast<unsigned char*>(ws) + delta_bytes(a), plan_bytes(a, true, BT, true, sm_count()));
   const int rc = launch_packed_prepare(dtype, a, plan, true, BT, true, true, st, launches);
   if (rc) return rc;
   if (dtype == EVOATTN_BF16) return a.D <= 64 ? launch<__nv_bfloat16, 64>(a, plan, st, launches) : launch<__nv_bfloat16, 128>(a, plan, st, launches);

@@ -15,7 +15,7 @@ struct Sums {
   int first[kClasses];
   int warps[kThreads / 32 + 1];
   long long steps;
-  int slots, joins;
+  int slots, joins, tiles;
 };
 
 // The tiles of all sequences, a warp per sequence and its lanes over the tiles; called several times, so the spans of the
@@ -77,18 +77,33 @@ __device__ __forceinline__ void make_list(const PackedArgs& a, const PackedPlan&
   for (int i = threadIdx.x; i < kClasses; i += kThreads) s.first[i] = 0;
   if (queries)
     for (int i = threadIdx.x; i < plan.n_arrived; i += kThreads) plan.arrived[i] = 0;
-  if (threadIdx.x == 0) { s.steps = 0; s.slots = 0; s.joins = 0; }
+  if (threadIdx.x == 0) { s.steps = 0; s.slots = 0; s.joins = 0; s.tiles = 0; }
   __syncthreads();
-  int longest = 0x7fffffff;
-  if (c.heads) {
-    long long sum = 0;
-    tiles.each(a, queries, unit, [&](const PackedTile& t) { sum += t.steps; });
+  long long work = 0;
+  int n = 0;
+  tiles.each(a, queries, unit, [&](const PackedTile& t) {
+    work += t.steps;
+    ++n;
+  });
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if ((threadIdx.x & 31) == 0 && sum) atomicAdd(reinterpret_cast<unsigned long long*>(&s.steps), (unsigned long long)sum);
-    __syncthreads();
-    longest = part_steps(s.steps, sms, c);
+  for (int o = 16; o > 0; o >>= 1) {
+    work += __shfl_xor_sync(0xffffffffu, work, o);
+    n += __shfl_xor_sync(0xffffffffu, n, o);
   }
+  if ((threadIdx.x & 31) == 0 && n) {
+    atomicAdd(reinterpret_cast<unsigned long long*>(&s.steps), (unsigned long long)work);
+    atomicAdd(&s.tiles, n);
+  }
+  __syncthreads();
+  // (offsets that do not ascend may make sequences that overlap, and more tiles than there is room for: none are listed)
+  if (s.tiles > (queries ? plan.most_queries : plan.most_keys)) {
+    if (threadIdx.x == 0) {
+      plan.counts[queries ? 0 : 1] = plan.counts[queries ? 4 : 5] = 0;
+      if (!queries) plan.counts[2] = 0;
+    }
+    return;
+  }
+  const int longest = c.heads ? part_steps(s.steps, sms, c) : 0x7fffffff;
   auto place = [](int steps) { return kClasses - 1 - min(steps, kClasses - 1); };
   auto cut = [&](const PackedTile& t) { return t.steps - longest > longest / 2 ? (t.steps + longest / 2) / longest : 1; };
   tiles.each(a, queries, unit, [&](const PackedTile& t) {

@@ -31,6 +31,7 @@ struct PackedJoin {
 struct PackedPlan {
   int* counts;               // [0] query units, [1] key tiles and parts, [2] joins; [4], [5] items that have been taken of the two lists
   PackedTile *queries, *keys;
+  int most_queries, most_keys;  // tiles that the lists have room for before any is cut: those of sequences that do not overlap
   PackedJoin* joins;
   float* sums;               // key tiles: [slot][Hk][dV, dK][DP / 4][128 rows][4]; query units: [slot][units of heads][2 tiles][DP / 4][128][4]
   float4* ml;                // [slot][units of heads][2 tiles][128 rows]: reference, sum of P as rounded, and as it is
@@ -70,10 +71,12 @@ inline PlanBytes plan_bytes(const PackedArgs& a, bool queries, int unit, bool ke
   return PlanBytes{queries ? round256((query_units(a, unit) + qs) * sizeof(PackedTile)) : 0, keys ? round256((key_tiles(a) + ks) * sizeof(PackedTile)) : 0,
                    round256(ks * sizeof(PackedJoin)), round256(tile * (ks * a.Hk * 2 + tiles)), round256(tiles * kTileRows * sizeof(float4)), round256(tiles * sizeof(int))};
 }
-inline PackedPlan place_plan(void* ws, const PlanBytes& n) {
+inline PackedPlan place_plan(const PackedArgs& a, int unit, void* ws, const PlanBytes& n) {
   unsigned char* p = static_cast<unsigned char*>(ws);
   PackedPlan plan{};
   plan.counts = reinterpret_cast<int*>(p);
+  plan.most_queries = (int)query_units(a, unit);
+  plan.most_keys = (int)key_tiles(a);
   plan.queries = reinterpret_cast<PackedTile*>(p += 256);
   plan.keys = reinterpret_cast<PackedTile*>(p += n.queries);
   plan.joins = reinterpret_cast<PackedJoin*>(p += n.keys);

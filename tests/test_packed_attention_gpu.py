@@ -395,10 +395,12 @@ def test_offsets_that_make_no_sense_touch_nothing():
     """Descending, negative and far offsets: rows outside the tensors are not touched, and the next call is right."""
     import evoformer_triton_b200 as evo
     q, k, v = (t.requires_grad_() for t in _qkv(200, 200, 4, 2, 64, BF))
-    for bad in ([0, 10 ** 12, 200], [-5, 50, 10 ** 6], [150, 20, 90], [300, 400, 500], [-2 ** 60, 2 ** 60, 0]):
+    for bad in ([0, 10 ** 12, 200], [-5, 50, 10 ** 6], [150, 20, 90], [300, 400, 500], [-2 ** 60, 2 ** 60, 0], [0, 200] * 40, [200, 0] * 300):
         out = evo.packed_attention(q, k, v, torch.tensor(bad, device=DEV))
         torch.autograd.grad(out.sum(), (q, k, v))
-        evo.packed_attention(q[:2].detach(), k.detach(), v.detach(), torch.tensor([0, 1, 2], device=DEV), torch.tensor(bad, device=DEV))
+        few = torch.arange(len(bad), device=DEV).clamp(max=2)
+        evo.packed_attention(q[:2].detach(), k.detach(), v.detach(), few, torch.tensor(bad, device=DEV))
+        evo.packed_attention(q.detach(), k.detach(), v.detach(), torch.tensor(bad, device=DEV), torch.tensor(bad, device=DEV))
     torch.cuda.synchronize()
     evo.check_device_status()
     _check(q, k, v, [60, 140])
