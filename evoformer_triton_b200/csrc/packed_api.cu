@@ -44,18 +44,20 @@ bool tensor_cores(const evoattn_packed_params* p, const PackedArgs& a, bool bwd)
 // queries are few altogether go there as a whole (the worst is that all queries are one sequence's: 64 units then),
 // which saves the launches for the tiles.
 struct Forward {
-  bool generic;
-  size_t few, tiles;
-  size_t bytes() const { return few + tiles; }
+  bool generic, few, tiles;
+  size_t few_bytes, tile_bytes;
+  size_t bytes() const { return few_bytes + tile_bytes; }
 };
 int few_tokens(const PackedArgs& a) { return a.G > 16 ? 2 : 32 / a.G; }
 Forward forward_plan(const evoattn_packed_params* p, const PackedArgs& a) {
-  Forward f{!tensor_cores(p, a, false), 0, 0};
+  Forward f{!tensor_cores(p, a, false), false, false, 0, 0};
   if (f.generic) return f;
   const bool own_keys = p->key_offsets && !p->lse;
   const bool all_few = own_keys && a.Tq <= (long long)few_tokens(a) * a.B && (long long)a.Tq * a.G <= 1024;
-  if (own_keys && (a.B > 1 || all_few)) f.few = (packed_few_workspace_bytes(a) + 255) / 256 * 256;
-  if (!all_few) f.tiles = sm100_packed_fwd_workspace_bytes(a);
+  f.few = own_keys && (a.B > 1 || all_few);
+  f.tiles = !all_few;
+  if (f.few) f.few_bytes = (packed_few_workspace_bytes(a) + 255) / 256 * 256;
+  if (f.tiles) f.tile_bytes = sm100_packed_fwd_workspace_bytes(a);
   return f;
 }
 int check_workspace(const evoattn_packed_params* p, size_t need) {
@@ -94,7 +96,7 @@ int evoattn_packed_fwd(const evoattn_packed_params* p, void* cuda_stream) {
       a.few_tokens = f.tiles ? few_tokens(a) : a.Tq;
       rc = launch_packed_few(p->dtype, a, !f.tiles, p->workspace, st, &launches);
     }
-    if (!rc && f.tiles) rc = launch_sm100_packed_fwd(p->dtype, a, static_cast<unsigned char*>(p->workspace) + f.few, st, &launches);
+    if (!rc && f.tiles) rc = launch_sm100_packed_fwd(p->dtype, a, static_cast<unsigned char*>(p->workspace) + f.few_bytes, st, &launches);
   }
   note_call(f.generic ? EVOATTN_PATH_GENERIC : EVOATTN_PATH_TCGEN05, launches);
   return rc;

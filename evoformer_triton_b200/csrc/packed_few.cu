@@ -529,6 +529,11 @@ int ctas_an_sm(const PackedArgs& a, int B) {
   return need + 1024 <= 114 * 1024 ? 2 : 1;
 }
 int padded(const PackedArgs& a) { return a.D <= 64 ? 64 : 128; }
+// Few keys leave nothing to join, wherever they lie.
+bool may_split(const PackedArgs& a, int ctas) {
+  const int nh = heads_of(a, ctas), block = a.D <= 64 ? block_of<64>(nh) : block_of<128>(nh);
+  return (a.Tk + block - 1LL) / block > kShort;
+}
 
 template <class T, int DP>
 int launch(const PackedArgs& args, bool clear, void* ws, cudaStream_t st, int* launches) {
@@ -551,9 +556,7 @@ int launch(const PackedArgs& args, bool clear, void* ws, cudaStream_t st, int* l
     if (!kernel_ready(reinterpret_cast<const void*>(kern), (int)smem, nullptr)) return EVOATTN_ERR_CUDA;
     launch_dependent(kern, dim3((unsigned)ctas), kThreads, smem, st, a, parts, clear && b0 == 0 ? args.B : 0, nh, tk, tv);
     *launches += 1;
-    // (few keys leave nothing to join, wherever they lie)
-    const int block = block_of<DP>(nh);
-    if ((args.Tk + block - 1LL) / block > kShort) {
+    if (may_split(a, ctas)) {
       const size_t jsmem = (size_t)(a.B + 1) * 28 + 16;
       if (!kernel_ready(reinterpret_cast<const void*>(join), (int)jsmem, nullptr)) return EVOATTN_ERR_CUDA;
       const long long rows = (long long)args.Tq * a.H;
@@ -568,7 +571,8 @@ int launch(const PackedArgs& args, bool clear, void* ws, cudaStream_t st, int* l
 
 size_t packed_few_workspace_bytes(const PackedArgs& a) {
   const int sms = sm_count();
-  return (size_t)(sms > 0 ? sms : 1) * 2 * 2 * kWarps * kRows * ((size_t)padded(a) * 4 + 8);
+  if (sms <= 0 || !may_split(a, sms * ctas_an_sm(a, a.B < kFewMaxSequences ? a.B : kFewMaxSequences))) return 0;
+  return (size_t)sms * 2 * 2 * kWarps * kRows * ((size_t)padded(a) * 4 + 8);
 }
 int launch_packed_few(int dtype, const PackedArgs& a, bool clear, void* ws, cudaStream_t st, int* launches) {
   if (dtype == EVOATTN_BF16) return a.D <= 64 ? launch<__nv_bfloat16, 64>(a, clear, ws, st, launches) : launch<__nv_bfloat16, 128>(a, clear, ws, st, launches);

@@ -241,7 +241,7 @@ __device__ __forceinline__ void load_statistics(const PackedArgs& a, float* lse,
 }
 
 template <class T, int DP, int TILE, bool VEC>
-__global__ void __launch_bounds__(kThreads) packed_generic_dq_kernel(const PackedArgs a) {
+__global__ void __launch_bounds__(kThreads) packed_generic_dq_kernel(const PackedArgs a, const int follows) {
   using C = GenericCfg<DP, TILE>;
   constexpr int NR = C::NR, NC = C::NC;
   extern __shared__ __align__(16) float sm[];
@@ -251,7 +251,10 @@ __global__ void __launch_bounds__(kThreads) packed_generic_dq_kernel(const Packe
   const int h = blockIdx.y, tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
   if (h == 0) zero_outside(a.offsets, a.wide, a.B, a.Tq, a.dq, (long long)a.H * a.D * sizeof(T), blockIdx.x, gridDim.x);
   const Place at = locate(a.B, blockIdx.x, TILE, place, [&](int b) { return query_span(a, b).n; });
-  if (at.seq < 0) return;
+  if (at.seq < 0) {
+    if (follows) ptx::grid_dependency_wait();
+    return;
+  }
   const Span qs = query_span(a, at.seq), ks = key_span(a, at.seq);
   const int i0 = at.tile * TILE, rows = min(TILE, qs.n - i0), hk = h / a.G, seen = keys_seen(a, qs.n, ks.n, i0, TILE);
   const long long row = qs.begin + i0;
@@ -296,6 +299,7 @@ __global__ void __launch_bounds__(kThreads) packed_generic_dq_kernel(const Packe
 #pragma unroll
     for (int k = 0; k < NC; ++k) store_row(out, tx, k, acc[r][k], a.scale, a.D);
   }
+  if (follows) ptx::grid_dependency_wait();
 }
 
 template <class T, int DP, int TILE, bool VEC>
@@ -306,6 +310,7 @@ __global__ void __launch_bounds__(kThreads) packed_generic_dkv_kernel(const Pack
   float *sQ = sm, *sO = sQ + TILE * C::LD, *sK = sO + TILE * C::LD, *sV = sK + TILE * C::LD, *sP = sV + TILE * C::LD, *sS = sP + TILE * C::LP;
   float *lse = sS + TILE * C::LP, *delta = lse + TILE;
   __shared__ int place[34];
+  ptx::grid_launch_dependents();
   const int hk = blockIdx.y, tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
   const long long row_bytes = (long long)a.Hk * a.D * sizeof(T);
   if (hk == 0) {
@@ -377,22 +382,26 @@ __global__ void __launch_bounds__(kThreads) packed_generic_dkv_kernel(const Pack
   }
 }
 
-template <class K>
-int run(K kern, const PackedArgs& a, long long rows, int tile, int heads, size_t smem, cudaStream_t st, int* launches) {
+template <class K, class... X>
+int run(K kern, const PackedArgs& a, long long rows, int tile, int heads, size_t smem, cudaStream_t st, int* launches, bool early, X... x) {
   if (!kernel_ready(reinterpret_cast<const void*>(kern), (int)smem, nullptr)) return EVOATTN_ERR_CUDA;
-  kern<<<dim3((unsigned)(rows / tile + a.B), (unsigned)heads), kThreads, smem, st>>>(a);
+  const dim3 grid((unsigned)(rows / tile + a.B), (unsigned)heads);
+  if (early) launch_dependent(kern, grid, kThreads, smem, st, a, x...);
+  else kern<<<grid, kThreads, smem, st>>>(a, x...);
   *launches += 1;
   return cudaGetLastError() == cudaSuccess ? EVOATTN_OK : EVOATTN_ERR_CUDA;
 }
 template <class T, int DP, int TILE, bool VEC>
 int both(bool back, const PackedArgs& a, cudaStream_t st, int* launches) {
   using C = GenericCfg<DP, TILE>;
-  if (!back) return run(packed_generic_fwd_kernel<T, DP, TILE, VEC>, a, a.Tq, TILE, a.H, C::bytes(3, 1), st, launches);
+  if (!back) return run(packed_generic_fwd_kernel<T, DP, TILE, VEC>, a, a.Tq, TILE, a.H, C::bytes(3, 1), st, launches, false);
   if (a.dk) {
-    const int rc = run(packed_generic_dkv_kernel<T, DP, TILE, VEC>, a, a.Tk, TILE, a.Hk, C::bytes(4, 2), st, launches);
+    const int rc = run(packed_generic_dkv_kernel<T, DP, TILE, VEC>, a, a.Tk, TILE, a.Hk, C::bytes(4, 2), st, launches, false);
     if (rc) return rc;
   }
-  return a.dq ? run(packed_generic_dq_kernel<T, DP, TILE, VEC>, a, a.Tq, TILE, a.H, C::bytes(4, 1), st, launches) : EVOATTN_OK;
+  // (dQ needs nothing of the kernel before it, which began when the statistics were complete: it runs beside it, and waits for
+  // it at its end)
+  return a.dq ? run(packed_generic_dq_kernel<T, DP, TILE, VEC>, a, a.Tq, TILE, a.H, C::bytes(4, 1), st, launches, a.dk != nullptr, (int)(a.dk != nullptr)) : EVOATTN_OK;
 }
 template <class T>
 bool vectors(const PackedArgs& a, bool bwd) {
