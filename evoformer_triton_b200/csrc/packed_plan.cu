@@ -6,7 +6,7 @@ namespace evo {
 namespace {
 
 constexpr int kThreads = 512;
-constexpr int kClasses = 2048;  // by work; what has more is of one class
+constexpr int kClasses = kThreads;  // by work, in steps that are as wide as the longest tile makes them
 
 constexpr int kKept = 1024;
 
@@ -15,7 +15,8 @@ struct Sums {
   int first[kClasses];
   int warps[kThreads / 32 + 1];
   long long steps;
-  int slots, joins, tiles;
+  long long tiles;
+  int slots, joins, most;
 };
 
 // The tiles of all sequences, a warp per sequence and its lanes over the tiles; called several times, so the spans of the
@@ -77,14 +78,16 @@ __device__ __forceinline__ void make_list(const PackedArgs& a, const PackedPlan&
   for (int i = threadIdx.x; i < kClasses; i += kThreads) s.first[i] = 0;
   if (queries)
     for (int i = threadIdx.x; i < plan.n_arrived; i += kThreads) plan.arrived[i] = 0;
-  if (threadIdx.x == 0) { s.steps = 0; s.slots = 0; s.joins = 0; s.tiles = 0; }
+  if (threadIdx.x == 0) { s.steps = 0; s.slots = 0; s.joins = 0; s.tiles = 0; s.most = 0; }
   __syncthreads();
-  long long work = 0;
-  int n = 0;
+  long long work = 0, n = 0;
+  int most = 0;
   tiles.each(a, queries, unit, [&](const PackedTile& t) {
     work += t.steps;
+    most = max(most, t.steps);
     ++n;
   });
+  most = __reduce_max_sync(0xffffffffu, most);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     work += __shfl_xor_sync(0xffffffffu, work, o);
@@ -92,7 +95,8 @@ __device__ __forceinline__ void make_list(const PackedArgs& a, const PackedPlan&
   }
   if ((threadIdx.x & 31) == 0 && n) {
     atomicAdd(reinterpret_cast<unsigned long long*>(&s.steps), (unsigned long long)work);
-    atomicAdd(&s.tiles, n);
+    atomicAdd(reinterpret_cast<unsigned long long*>(&s.tiles), (unsigned long long)n);
+    atomicMax(&s.most, most);
   }
   __syncthreads();
   // (offsets that do not ascend may make sequences that overlap, and more tiles than there is room for: none are listed)
@@ -104,19 +108,17 @@ __device__ __forceinline__ void make_list(const PackedArgs& a, const PackedPlan&
     return;
   }
   const int longest = c.heads ? part_steps(s.steps, sms, c) : 0x7fffffff;
-  auto place = [](int steps) { return kClasses - 1 - min(steps, kClasses - 1); };
+  // (parts are of up to one and a half times `longest`; 9 bits for 512 classes)
+  const int shift = max(0, 32 - __clz((int)min((long long)s.most, longest + longest / 2LL)) - 9);
+  auto place = [&](int steps) { return kClasses - 1 - min(steps >> shift, kClasses - 1); };
   auto cut = [&](const PackedTile& t) { return t.steps - longest > longest / 2 ? (t.steps + longest / 2) / longest : 1; };
   tiles.each(a, queries, unit, [&](const PackedTile& t) {
     const int parts = cut(t);
     atomicAdd(&s.first[place((t.steps + parts - 1) / parts)], parts);
   });
   __syncthreads();
-  // exclusive sums of the classes, four a thread
-  constexpr int kEach = kClasses / kThreads;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int x[kEach], own = 0;
-#pragma unroll
-  for (int i = 0; i < kEach; ++i) own += x[i] = s.first[kEach * threadIdx.x + i];
+  // exclusive sums of the classes, one a thread
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, own = s.first[threadIdx.x];
   int sum = own;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -126,15 +128,12 @@ __device__ __forceinline__ void make_list(const PackedArgs& a, const PackedPlan&
   if (lane == 31) s.warps[warp] = sum;
   __syncthreads();
   int before = sum - own, all = 0;
+#pragma unroll
   for (int w = 0; w < kThreads / 32; ++w) {
     if (w < warp) before += s.warps[w];
     all += s.warps[w];
   }
-#pragma unroll
-  for (int i = 0; i < kEach; ++i) {
-    s.first[kEach * threadIdx.x + i] = before;
-    before += x[i];
-  }
+  s.first[threadIdx.x] = before;
   if (threadIdx.x == 0) {
     plan.counts[queries ? 0 : 1] = all;
     plan.counts[queries ? 4 : 5] = 0;
@@ -160,7 +159,7 @@ __device__ __forceinline__ void make_list(const PackedArgs& a, const PackedPlan&
   if (threadIdx.x == 0 && !queries) plan.counts[2] = s.joins;
 }
 
-// delta: VEC values of 16 bytes at a time, `lanes` lanes a row (a power of two), four rows of a lane on their way.
+// delta: VEC values of 16 bytes at a time, `lanes` lanes a row (a power of two), two rows of a lane on their way.
 template <class T, bool VEC>
 __device__ __forceinline__ void row_sums(const PackedArgs& a, long long block, long long blocks, int lanes, const FastDiv& heads) {
   const int team = threadIdx.x / lanes, lane = threadIdx.x % lanes, teams = kThreads / lanes;
@@ -168,7 +167,7 @@ __device__ __forceinline__ void row_sums(const PackedArgs& a, long long block, l
   const T* o = static_cast<const T*>(a.o);
   const T* d_o = static_cast<const T*>(a.d_o);
   const T* rest = static_cast<const T*>(a.o_rest);
-  constexpr int V = VEC ? kPer16<T> : 1, U = 4;
+  constexpr int V = VEC ? kPer16<T> : 1, U = 2;
   for (long long i0 = block * teams * U + team; i0 < items; i0 += blocks * teams * U) {
     float s[U] = {};
     long long to[U];
@@ -220,7 +219,7 @@ __device__ __forceinline__ void row_sums(const PackedArgs& a, long long block, l
 
 // Block 0 makes the list of queries, block 1 (or 0) that of keys, the others the row sums.
 template <class T, bool VEC>
-__global__ void __launch_bounds__(kThreads) packed_prepare_kernel(const PackedArgs a, const PackedPlan plan, const int queries, const int unit, const int keys,
+__global__ void __launch_bounds__(kThreads, 2) packed_prepare_kernel(const PackedArgs a, const PackedPlan plan, const int queries, const int unit, const int keys,
                                                                   const int sms, const PackedCut qcut, const PackedCut kcut, const int lanes, const FastDiv heads) {
   __shared__ Sums s;
   ptx::grid_dependency_wait();
@@ -246,8 +245,8 @@ int launch_packed_prepare(int dtype, const PackedArgs& a, const PackedPlan& plan
     const bool vec = delta && a.D % V == 0 && ((reinterpret_cast<uintptr_t>(a.o) | reinterpret_cast<uintptr_t>(a.o_rest) | reinterpret_cast<uintptr_t>(a.d_o)) & 15) == 0 && a.sdo[0] % V == 0 && a.sdo[1] % V == 0;
     int lanes = 1;
     while (lanes < 32 && lanes * (vec ? V : 1) < a.D) lanes *= 2;
-    const long long rows = ((long long)a.Tq * a.H + kThreads / lanes * 4 - 1) / (kThreads / lanes * 4);
-    const int blocks = (queries ? 1 : 0) + (keys ? 1 : 0) + (delta ? (int)(rows < sms * 4LL ? rows : sms * 4LL) : 0);
+    const long long rows = ((long long)a.Tq * a.H + kThreads / lanes * 2 - 1) / (kThreads / lanes * 2);
+    const int blocks = (queries ? 1 : 0) + (keys ? 1 : 0) + (delta ? (int)(rows < sms * 8LL ? rows : sms * 8LL) : 0);
     launch_dependent(vec ? packed_prepare_kernel<T, true> : packed_prepare_kernel<T, false>, dim3((unsigned)blocks), kThreads, 0, st, a, plan, (int)queries, unit, (int)keys,
                      sms, qcut, key_cut(a), lanes, FastDiv((uint32_t)a.H));
     *launches += 1;
