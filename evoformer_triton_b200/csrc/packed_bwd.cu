@@ -14,6 +14,15 @@
 // land before the MMAs do and clear what lies behind the end of the sequence in it (0 times infinity is not 0), warps 4
 // to 11 compute: a thread has one row of the 128 x 128 scores and half of its columns, P in registers from S to dS.
 //
+// Items are handed out as in the forward.  A key tile of long sequences or many heads is cut into parts, whose fp32 sums
+// the second kernel adds up, in their order, before it ends ([5 sequences of up to 1 499, 12 heads of 96 over 2]: dK and dV
+// 124 us whole, 38 in parts).  The second kernel begins as CTAs of the first leave, and waits for it only at its end.
+//
+// Bound by the tensor cores and the shared memory that feeds them: a step of the first kernel (four products of 128 x 128 x
+// DP) needs 1.1 us of either and takes 1.75, one of the second 0.8 and 1.35.  [8192] causal, 16 heads of 128: 403 and 321 us, 1.36
+// and 1.28 PFLOP/s of the products that are formed, 950 TFLOP/s of the five that a gradient cannot do without.  With 16 compute warps
+// instead of 8 (a quarter of a row each) 442 and 322.
+//
 // dK, dV: tensor memory holds S^T, dP^T (128 columns each), dV and dK (DP each).  P^T goes back over S^T and dS^T over dP^T,
 // as the A operands of dV += P^T dO and dK += dS^T Q.  The MMAs go in the order dV(n), S(n + 1), dK(n), dP(n + 1): while the
 // exponentials of a step run, its dP^T and the products of the step before are on the tensor cores.
@@ -27,10 +36,9 @@ using namespace ptx;
 constexpr int BT = kTileRows;
 constexpr int kThreads = 384, kServiceRegs = 56, kComputeRegs = 224;
 
-#ifndef EMUB
-#define EMUB 4
-#endif
-__device__ __forceinline__ constexpr bool on_fma(int pair) { return pair * EMUB / 16 != (pair + 1) * EMUB / 16; }
+// Which pairs of values go to the FMA pipes: four of sixteen.  Both kernels at D = 64, [8192] causal, 16 heads, us, with none,
+// two, four and six: 583, 594, 561, 571; at D = 128 all alike.
+__device__ __forceinline__ constexpr bool on_fma(int pair) { return pair % 4 == 3; }
 
 template <int DP>
 struct Tiles {

@@ -8,7 +8,9 @@
 // query.  The two tiles are those of two heads that read the same keys (an even number of heads a group), or two
 // neighbouring ones of one head: one load of K and V serves both, and while one warpgroup's MMAs run, the other has the
 // exponentials.  Keys in tiles of 128, the last first: those are the ones that a mask cuts, and the others take a loop
-// without it.
+// without it.  Items (a unit of tiles, a head or two) go out most work first from a counter; with long rows of key tiles and
+// few items, an item is a part of a row, and the last part to arrive adds them up in their order (the same bits in
+// every run): [512 512 300 77] queries against up to 6 001 keys, 16 heads of 64, 99 us whole, 59 in parts.
 //
 // S = Q K^T lands in tensor memory (128 columns a warpgroup); P goes back over it in 16 bits, from where it is the A
 // operand of P V; O accumulates next to it (DP columns): with DP = 128 that is all of tensor memory.  The MMAs of a
@@ -20,7 +22,12 @@
 // a tile's sum shows that some p may be too large, or a row's first sum that all of them are too small, the tile's maximum
 // is taken, O and l follow it, and the tile is done again (P is kept in registers until then).  O is divided by the sum of the
 // P that it was made of, rounded (with that of the unrounded values it was off by 0.0023 instead of 0.0021 of its norm, where
-// its own rounding makes 0.0016); the log-sum-exp is that of the unrounded ones.
+// its own rounding makes 0.0016, and a forward took 4 % less); the log-sum-exp is that of the unrounded ones.
+//
+// Bound at D = 128 by the chain of a warpgroup's tile: 0.7 us of softmax, 0.27 us each for P V and S, and three hand-overs;
+// 1.9 us for a tile of each, of which the tensor cores work 1.1 and shared memory feeds them without a pause (S reads
+// both operands there).  [16384] causal, 16 heads of 128 over 4: 894 us, 1.23 PFLOP/s; under the power cap, calls back to
+// back, 1 055.  At D = 64 by the issue slots and units of the exponentials: 16 heads 740 us.  An item costs some 3 us besides.
 #include "packed_sm100.cuh"
 
 namespace evo {

@@ -9,7 +9,10 @@
 // and as many rows of every product.  Keys and queries of a thread are 16 apart, so that its rows of DP + 4 floats lie in
 // other banks than its neighbours'.  The backward is two kernels, one that walks the queries of a key tile (all heads of
 // the group in turn) and one that walks the keys of a query tile: the scores are formed twice, and no sum depends on the
-// order in which blocks run.
+// order in which blocks run; they run beside one another where there is room.
+//
+// Bound by FMA issue and shared-memory loads, where it is large (fp32, [8192] causal, 8 heads of 64: 2.6 ms forward, 26 TFLOP/s),
+// and by the latency of a block's tiles, 2.5 us each, where it is small ([437 300 129], 4 heads of 64: 112 us forward and backward).
 #include <math.h>
 
 #include <type_traits>
