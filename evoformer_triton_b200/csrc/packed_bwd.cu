@@ -131,6 +131,16 @@ __device__ __forceinline__ void clear_outside(const void* offsets, int wide, int
   }
 }
 
+// The same for keys that no query sees: the tiles [begin, begin + n) of a list.
+__device__ __forceinline__ void clear_tiles(const PackedTile* list, int begin, int n, void* dst, int row16, int lane) {
+#pragma unroll 1
+  for (int i = blockIdx.x; i < n; i += gridDim.x) {
+    const PackedTile t = load_tile(list + begin + i);
+    uint4* p = static_cast<uint4*>(dst) + (long long)t.row * row16;
+    for (int x = lane; x < t.rows * row16; x += 32) p[x] = make_uint4(0, 0, 0, 0);
+  }
+}
+
 // COLS columns of an accumulator, times f, to a row of 16-bit values; zeros where `any` is not set.
 template <class T, int COLS>
 __device__ __forceinline__ void store_rows(uint32_t t_src, T* out, int d0, int D, float f, bool valid, bool any) {
@@ -200,7 +210,8 @@ packed_dkv_sm100_kernel(const PackedArgs a, const PackedPlan plan, const FastDiv
   tc_fence_after();
   const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
   const bool failed = *abort_flag != 0;
-  Schedule todo{sched, sched + 16, abort_s + 4, abort_s, plan.counts + 5, failed ? 0 : __ldcg(plan.counts + 1) * (int)heads.d};
+  const int tiles = failed ? 0 : __ldcg(plan.counts + 1);
+  Schedule todo{sched, sched + 16, abort_s + 4, abort_s, plan.counts + 5, tiles * (int)heads.d};
 
   // The steps of a CTA, one after another over its items: head g of the group, query tile i, `left` of the item from here on.
   struct Step {
@@ -223,12 +234,12 @@ packed_dkv_sm100_kernel(const PackedArgs a, const PackedPlan plan, const FastDiv
     s.g = s.t.tiles ? s.t.begin / s.t.tiles : 0;
     s.i = s.end - s.t.tiles + s.t.begin - s.g * s.t.tiles;
   };
-  auto begin = [&](Step& s, int idx) {  // the first step of that item, or of the next one that has any
-    for (; !todo.over(idx); idx = warp == 0 ? todo.take() : todo.next()) {
-      item(idx, s);
-      if (s.left > 0) return true;
-    }
-    return false;
+  // The first step of that item.  Every item has one: the MMAs are a step ahead, and what they asked for behind an item without
+  // steps would wait for the warps that compute, and these for the MMAs' word that the item before is done.
+  auto begin = [&](Step& s, int idx) {
+    if (todo.over(idx)) return false;
+    item(idx, s);
+    return true;
   };
   auto advance = [&](Step& s) {
     s.next();
@@ -361,6 +372,9 @@ packed_dkv_sm100_kernel(const PackedArgs a, const PackedPlan plan, const FastDiv
       if (!failed) {
         clear_outside(a.key_offsets, a.wide, a.B, a.Tk, a.dk, a.Hk * a.D / 8, lane);
         clear_outside(a.key_offsets, a.wide, a.B, a.Tk, a.dv, a.Hk * a.D / 8, lane);
+        const int unseen = __ldcg(plan.counts + 3);
+        clear_tiles(plan.keys, tiles, unseen, a.dk, a.Hk * a.D / 8, lane);
+        clear_tiles(plan.keys, tiles, unseen, a.dv, a.Hk * a.D / 8, lane);
       }
 #pragma unroll 1
       while (more) {
@@ -472,19 +486,16 @@ packed_dkv_sm100_kernel(const PackedArgs a, const PackedPlan plan, const FastDiv
         if (lane == 0) mbar_arrive_s(ds_full);
         if (++st == NS) { st = 0; par ^= 1; }
       }
-      const bool any = s.t.steps > 0;
-      if (any) {
-        mbar_wait_s(out_full, kv & 1, abort_s, DEV_TIMEOUT_MMA);
-        ++kv;
-        tc_fence_after();
-      }
+      mbar_wait_s(out_full, kv & 1, abort_s, DEV_TIMEOUT_MMA);
+      ++kv;
+      tc_fence_after();
       const uint32_t src = t_lane + (w == 0 ? C::colDV : C::colDK);
       if (s.t.parts == 1) {
         const int first = (warp & 3) * 32;  // row of the warp's first lane
         const int at = s.t.row + first;
         store_rows_staged<T, DP>(smem_s + C::offOut + (warp - 4) * kStageBytes, src, w == 0 ? &tmDV : &tmDK, at, s.hk,
                                  static_cast<T*>(w == 0 ? a.dv : a.dk) + ((long long)at * a.Hk + s.hk) * a.D, (long long)a.Hk * a.D, s.t.rows - first, a.D,
-                                 w == 0 ? 1.f : a.scale, any);
+                                 w == 0 ? 1.f : a.scale, true);
       } else {
         float4* out = reinterpret_cast<float4*>(plan.sums) + (((long long)s.t.slot * a.Hk + s.hk) * 2 + w) * (DP / 4 * BT) + row;
 #pragma unroll

@@ -103,14 +103,14 @@ __device__ __forceinline__ void make_list(const PackedArgs& a, const PackedPlan&
   if (s.tiles > (queries ? plan.most_queries : plan.most_keys)) {
     if (threadIdx.x == 0) {
       plan.counts[queries ? 0 : 1] = plan.counts[queries ? 4 : 5] = 0;
-      if (!queries) plan.counts[2] = 0;
+      if (!queries) plan.counts[2] = plan.counts[3] = 0;
     }
     return;
   }
   const int longest = c.heads ? part_steps(s.steps, sms, c) : 0x7fffffff;
   // (parts are of up to one and a half times `longest`; 9 bits for 512 classes)
   const int shift = max(0, 32 - __clz((int)min((long long)s.most, longest + longest / 2LL)) - 9);
-  auto place = [&](int steps) { return kClasses - 1 - min(steps >> shift, kClasses - 1); };
+  auto place = [&](int steps) { return steps == 0 ? kClasses - 1 : kClasses - 2 - min(steps >> shift, kClasses - 2); };
   auto cut = [&](const PackedTile& t) { return t.steps - longest > longest / 2 ? (t.steps + longest / 2) / longest : 1; };
   tiles.each(a, queries, unit, [&](const PackedTile& t) {
     const int parts = cut(t);
@@ -134,8 +134,9 @@ __device__ __forceinline__ void make_list(const PackedArgs& a, const PackedPlan&
     all += s.warps[w];
   }
   s.first[threadIdx.x] = before;
-  if (threadIdx.x == 0) {
-    plan.counts[queries ? 0 : 1] = all;
+  if (threadIdx.x == kClasses - 1) {  // (its class: tiles without a step)
+    plan.counts[queries ? 0 : 1] = queries ? all : before;
+    if (!queries) plan.counts[3] = own;
     plan.counts[queries ? 4 : 5] = 0;
   }
   __syncthreads();

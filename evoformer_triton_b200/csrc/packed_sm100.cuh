@@ -29,7 +29,8 @@ struct PackedJoin {
 
 // Where lists lie in a workspace: 256 bytes with their lengths, the tiles, the key tiles whose parts are to be joined and the parts.
 struct PackedPlan {
-  int* counts;               // [0] query units, [1] key tiles and parts, [2] joins; [4], [5] items that have been taken of the two lists
+  int* counts;               // [0] query units, [1] key tiles and parts that have steps, [2] joins, [3] key tiles that no query sees, behind those;
+                             // [4], [5] items that have been taken of the two lists
   PackedTile *queries, *keys;
   int most_queries, most_keys;  // tiles that the lists have room for before any is cut: those of sequences that do not overlap
   PackedJoin* joins;
@@ -115,7 +116,7 @@ int launch_packed_few(int dtype, const PackedArgs& a, bool clear, void* workspac
 // 2^x of two values on the FMA pipes, for a part of the exponentials of a tile: the special-function units make 16 a cycle
 // and SM, which is as long as the tile's MMAs take (head dimension 128) or twice that (64).  x = n + f with n whole (by
 // adding and taking off 1.5 2^23) and |f| <= 1/2; 2^f by a polynomial whose largest relative error is the smallest there
-// is for its degree (fitted by exchange): 7.5e-5 of degree 3, 2.6e-6 of degree 4, a twenty-fifth and a hundredth of half a step of bf16 and fp16;
+// is for its degree (fitted by exchange): 7.5e-5 of degree 3, 2.6e-6 of degree 4, a fiftieth and a two-hundredth of half a step of bf16 and fp16;
 // n is added to the exponent's bits.  Exponents below -126 count as that; with BOTH those above 126 too.
 template <class T, bool BOTH>
 __device__ __forceinline__ void exp2_fma(ptx::F2 x, float& p0, float& p1) {

@@ -93,6 +93,15 @@ def test_many_sequences(D, dtype):
 
 
 @pytest.mark.parametrize("dtype", [BF, HF, F32], ids=IDS.get)
+@pytest.mark.parametrize("D", [64, 128])
+def test_many_tiles_of_keys_that_no_query_sees(D, dtype):
+    """Far more of them than there are SMs, behind and between tiles with queries: their rows of dK and dV are zero."""
+    nq, nk = [130, 0, 300] + [0] * 200 + [5], [260, 700, 1] + [130] * 200 + [140]
+    _check(*_qkv(sum(nq) + 6, sum(nk) + 6, 8, 4, D, dtype), nq, nk, before=3)
+    _check(*_qkv(sum(nq), sum(nk), 8, 4, D, dtype), nq, nk, causal=False)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF, F32], ids=IDS.get)
 @pytest.mark.parametrize("nk", [1, 15, 16, 17, 64, 65, 500, 5000])
 @pytest.mark.parametrize("H,Hk,D", [(8, 8, 64), (32, 8, 128), (12, 2, 96), (40, 2, 32), (4, 1, 256), (3, 1, 20)])
 def test_single_tokens(H, Hk, D, nk, dtype):
