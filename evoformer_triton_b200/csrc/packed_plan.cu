@@ -164,12 +164,15 @@ __device__ __forceinline__ void make_list(const PackedArgs& a, const PackedPlan&
 template <class T, bool VEC>
 __device__ __forceinline__ void row_sums(const PackedArgs& a, long long block, long long blocks, int lanes, const FastDiv& heads) {
   const int team = threadIdx.x / lanes, lane = threadIdx.x % lanes, teams = kThreads / lanes;
+  const int ahead = (threadIdx.x & 31) / lanes;  // teams of the warp before this one
   const long long items = (long long)a.Tq * a.H;
   const T* o = static_cast<const T*>(a.o);
   const T* d_o = static_cast<const T*>(a.d_o);
   const T* rest = static_cast<const T*>(a.o_rest);
   constexpr int V = VEC ? kPer16<T> : 1, U = 2;
-  for (long long i0 = block * teams * U + team; i0 < items; i0 += blocks * teams * U) {
+  // (the teams of a warp meet in shuffles: as long as the first of them has a row, all go on, the others with a row that
+  // is there and nothing to store)
+  for (long long i0 = block * teams * U + team; i0 - ahead < items; i0 += blocks * teams * U) {
     float s[U] = {};
     long long to[U];
     const T* d[U];
