@@ -11,7 +11,10 @@
 // Bound by reading K and V once.  A CTA is four warps, each with its own ring of tiles of 16 keys (D <= 64: 32), filled by
 // TMA by the warp itself, and its own running maximum, sum and O.  Where there are four key heads or more, a warp has
 // one each and all four read the same keys, which lie side by side in memory; else two or four warps share the keys of a
-// head and meet at the end of a unit.  Products of 16 rows are warp-level MMAs: tcgen05 would work on 128.
+// head and meet at the end of a unit.  Products of 16 rows are warp-level MMAs: tcgen05 would work on 128.  P enters its
+// product in two pieces of the type, itself rounded and what that left: a second MMA a tile, which costs nothing beside the
+// loads (86.4 us for the case below, 87.7 with one piece), and results are off by their own rounding only (bf16, of the norm: 0.0016
+// for one token, 0.0022 with one piece).
 //
 // 32 sequences of 1 to 8 191 keys, 32 heads of 128 over 8: 89 us, the 465 MB at 5.2 TB/s (118 with units weighed by
 // their keys alone, one head a CTA and exchanges in every tile); even ones of 4 096 keys 98 us, 5.5 TB/s; 16 heads of 64, 16
@@ -168,7 +171,7 @@ __device__ __forceinline__ void ldmatrix4_t(uint32_t (&r)[4], uint32_t at) {
 }
 
 template <class T, int DP>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, 2)
 packed_few_kernel(const PackedArgs a, const Parts parts, const int clear, const int nh, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV) {
   using C = FewCfg<DP>;
   constexpr int NS = C::kStages, kKeys = C::kKeys;
@@ -349,7 +352,7 @@ packed_few_kernel(const PackedArgs a, const Parts parts, const int clear, const 
           m[e] = up;
         }
       }
-      uint32_t pa[kKeys / 16][4];
+      uint32_t pa[kKeys / 16][4], pl[kKeys / 16][4];  // P rounded, and what rounding left
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const float nm = m[e] == -INFINITY ? 0.f : m[e];
@@ -359,7 +362,11 @@ packed_few_kernel(const PackedArgs a, const Parts parts, const int clear, const 
 #pragma unroll
         for (int f = 0; f < kKeys / 4; f += 2) {
           l[e] += p[f] + p[f + 1];
-          pa[f / 4][(f / 2 & 1) * 2 + e] = Pack2<T>::pack(p[f], p[f + 1]);
+          const int at = (f / 2 & 1) * 2 + e;
+          float r0, r1;
+          pa[f / 4][at] = Pack2<T>::pack(p[f], p[f + 1]);
+          unpack2<T>(pa[f / 4][at], r0, r1);
+          pl[f / 4][at] = Pack2<T>::pack(p[f] - r0, p[f + 1] - r1);
         }
       }
 #pragma unroll
@@ -371,6 +378,8 @@ packed_few_kernel(const PackedArgs a, const Parts parts, const int clear, const 
           ldmatrix4_t(b, vt + (i >> 2) * C::kPanel + r * 128 + ((ch ^ (r & 7)) << 4));
           mma16816<T>(o[2 * i], pa[n], b[0], b[1]);
           mma16816<T>(o[2 * i + 1], pa[n], b[2], b[3]);
+          mma16816<T>(o[2 * i], pl[n], b[0], b[1]);
+          mma16816<T>(o[2 * i + 1], pl[n], b[2], b[3]);
         }
       }
       __syncwarp();  // (every lane has read the tile)
