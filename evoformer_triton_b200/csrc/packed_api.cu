@@ -122,7 +122,8 @@ int evoattn_packed_bwd(const evoattn_packed_params* p, void* cuda_stream) {
     rc = launch_sm100_packed_bwd(p->dtype, a, p->workspace, st, &launches);
   } else {
     a.delta = static_cast<float*>(p->workspace);
-    rc = launch_packed_prepare(p->dtype, a, PackedPlan{}, false, 0, false, true, st, &launches);
+    PackedPlan none{};
+    rc = launch_packed_prepare(p->dtype, a, none, false, 0, false, true, st, &launches);
     if (!rc) rc = launch_packed_generic_bwd(p->dtype, a, st, &launches);
   }
   note_call(fast ? EVOATTN_PATH_TCGEN05 : EVOATTN_PATH_GENERIC, launches);

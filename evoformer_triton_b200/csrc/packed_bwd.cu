@@ -121,6 +121,50 @@ __device__ __forceinline__ void scores_gradient(const uint32_t (&d)[32], const F
   }
 }
 
+// fp16 ends at 2^16 and has steps of 2^-24 below 2^-14: dS = P (dP - delta) of a long row or a small dO would lose its bits, or all of
+// it, although the sums that it enters are ordinary numbers, and that of a large dO v would overflow.  So dS is formed times 2^e, which
+// its products carry to the end.  |dS_ij| <= |dO_i| (|V_j| + |o_i|) <= 2 sqrt(D) max |dO_id| max |V_j|; e takes that bound to 2^15 at most.  It is
+// in the exponent of P, for nothing; P itself enters dV times 2^14.  One power for a call, from maxima that the row sums leave: forward and
+// backward of [3088 in 5], 12 heads of 96 over 2, 117 -> 121 us, [8192] of 16 heads of 128 over 4, 1 117 -> 1 145.  bf16 has the exponents of fp32.
+template <class T>
+struct Lift {
+  static constexpr bool kAny = std::is_same<T, __half>::value;
+  static constexpr float kDv = kAny ? 0x1p-14f : 1.f;  // of dV
+  float e = 0.f;     // in the exponent of P
+  float p = 1.f;     // of that P where it enters dV
+  float back = 1.f;  // of dK and dQ
+};
+__device__ __forceinline__ float exp2_whole(int e) { return __int_as_float((e + 127) << 23); }
+// The words begin as zeros; every thread of a CTA brings its share of the maxima to them.
+__device__ __forceinline__ void bring_norms(const PackedPlan& plan, uint32_t* words) {
+  uint32_t m0 = 0, m1 = 0;
+  for (int i = threadIdx.x; i < plan.n_norms; i += kThreads) {
+    const uint2 x = __ldcg(reinterpret_cast<const uint2*>(plan.norms + i));
+    m0 = max(m0, x.x);
+    m1 = max(m1, x.y);
+  }
+  m0 = __reduce_max_sync(0xffffffffu, m0);
+  m1 = __reduce_max_sync(0xffffffffu, m1);
+  if ((threadIdx.x & 31) == 0) {
+    atomicMax(words, m0);
+    atomicMax(words + 1, m1);
+  }
+}
+template <class T>
+__device__ __forceinline__ Lift<T> lift_of(const uint32_t* words, int D) {
+  Lift<T> l;
+  if constexpr (Lift<T>::kAny) {
+    const float x = __uint_as_float(words[0]);
+    const uint32_t b = __float_as_uint(x * x * __uint_as_float(words[1]) * (float)D);  // below 2^(k + 1)
+    const int k = (int)(b >> 23) - 127;
+    const int e = b == 0 ? 0 : 14 - ((k + 2) >> 1);  // (its root below 2^ceil((k + 1) / 2))
+    l.e = (float)e;
+    l.p = exp2_whole(14 - e);
+    l.back = exp2_whole(-e);
+  }
+  return l;
+}
+
 // Rows of no sequence in a dense tensor of 16-bit values, by a warp.
 __device__ __forceinline__ void clear_outside(const void* offsets, int wide, int B, int rows, void* dst, int row16, int lane) {
   const Span all = clamped(packed_offset(offsets, wide, 0), packed_offset(offsets, wide, B), rows);
@@ -190,26 +234,31 @@ packed_dkv_sm100_kernel(const PackedArgs a, const PackedPlan plan, const FastDiv
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + C::kBars);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + C::kBars + 1);
   const uint32_t abort_s = smem_u32(const_cast<int*>(abort_flag));
+  uint32_t* norm_words = reinterpret_cast<uint32_t*>(bars + C::kBars + 3);
   const int tid = threadIdx.x, lane = tid & 31;
   const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
 
   if (tid == 0) {
     for (int i = 0; i < C::kBars; ++i) mbar_init_s(b0 + 8 * i, b0 + 8 * i == p_full || b0 + 8 * i == ds_full ? 8 : b0 + 8 * i >= sched + 16 ? 11 : 1);
     fence_mbar_init();
+    if constexpr (Lift<T>::kAny) norm_words[0] = norm_words[1] = 0u;
     prefetch_tmap(&tmQ); prefetch_tmap(&tmK); prefetch_tmap(&tmV); prefetch_tmap(&tmD);
   }
   if (warp == 0) {
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
   }
+  if constexpr (Lift<T>::kAny) __syncthreads();
   grid_dependency_wait();
   grid_launch_dependents();
   if (tid == 0) *abort_flag = (a.status && *reinterpret_cast<volatile int*>(a.status) != 0) ? 1 : 0;
+  if constexpr (Lift<T>::kAny) bring_norms(plan, norm_words);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
   const bool failed = *abort_flag != 0;
+  const Lift<T> lift = lift_of<T>(norm_words, a.D);
   const int tiles = failed ? 0 : __ldcg(plan.counts + 1);
   Schedule todo{sched, sched + 16, abort_s + 4, abort_s, plan.counts + 5, tiles * (int)heads.d};
 
@@ -346,11 +395,11 @@ packed_dkv_sm100_kernel(const PackedArgs a, const PackedPlan plan, const FastDiv
       while (more) {
         const int h = s.hk * a.G + s.g, real = s.real();
         const long long at = (long long)h * a.lse_ld + s.t.other + s.i * BT;
-        float nl[4], nd[4];  // (rows behind the end: 2^0 of queries and gradients that are zero)
+        float nl[4], nd[4];  // (rows behind the end: 2^e of queries and gradients that are zero)
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
           const int r = lane + 32 * u;
-          nl[u] = r < real ? -__ldcg(a.lse + at + r) : 0.f;
+          nl[u] = (r < real ? -__ldcg(a.lse + at + r) : 0.f) + lift.e;
           nd[u] = r < real ? -__ldcg(a.delta + at + r) : 0.f;
         }
         mbar_wait_s(q_empty(st), par ^ 1, abort_s, DEV_TIMEOUT_SYNC);
@@ -451,6 +500,7 @@ packed_dkv_sm100_kernel(const PackedArgs a, const PackedPlan plan, const FastDiv
                   p1 = ex2(x1);
                 }
                 p[16 * k + e / 2 + u] = f2_make(p0, p1);
+                if constexpr (Lift<T>::kAny) f2_get(f2_mul(f2_make(p0, p1), f2_make(lift.p, lift.p)), p0, p1);
                 pk[e / 2 + u] = Pack2<T>::pack(p0, p1);
               }
             }
@@ -495,7 +545,7 @@ packed_dkv_sm100_kernel(const PackedArgs a, const PackedPlan plan, const FastDiv
         const int at = s.t.row + first;
         store_rows_staged<T, DP>(smem_s + C::offOut + (warp - 4) * kStageBytes, src, w == 0 ? &tmDV : &tmDK, at, s.hk,
                                  static_cast<T*>(w == 0 ? a.dv : a.dk) + ((long long)at * a.Hk + s.hk) * a.D, (long long)a.Hk * a.D, s.t.rows - first, a.D,
-                                 w == 0 ? 1.f : a.scale, true);
+                                 w == 0 ? Lift<T>::kDv : a.scale * lift.back, true);
       } else {
         float4* out = reinterpret_cast<float4*>(plan.sums) + (((long long)s.t.slot * a.Hk + s.hk) * 2 + w) * (DP / 4 * BT) + row;
 #pragma unroll
@@ -541,28 +591,33 @@ packed_dq_sm100_kernel(const PackedArgs a, const PackedPlan plan, const FastDiv 
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + C::kBars);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + C::kBars + 1);
   const uint32_t abort_s = smem_u32(const_cast<int*>(abort_flag));
+  uint32_t* norm_words = reinterpret_cast<uint32_t*>(bars + C::kBars + 3);
   const int tid = threadIdx.x, lane = tid & 31;
   const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
 
   if (tid == 0) {
     for (int i = 0; i < C::kBars; ++i) mbar_init_s(b0 + 8 * i, b0 + 8 * i == ds_full ? 8 : b0 + 8 * i >= sched + 16 ? 11 : 1);
     fence_mbar_init();
+    if constexpr (Lift<T>::kAny) norm_words[0] = norm_words[1] = 0u;
     prefetch_tmap(&tmQ); prefetch_tmap(&tmK); prefetch_tmap(&tmV); prefetch_tmap(&tmD);
   }
   if (warp == 0) {
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
   }
+  if constexpr (Lift<T>::kAny) __syncthreads();
   // Behind the kernel for dK and dV this one begins as its CTAs leave: it reads nothing of theirs before the end, and what it
   // reads was complete before they began.
   if (!follows) grid_dependency_wait();
   grid_launch_dependents();
   if (tid == 0) *abort_flag = (a.status && *reinterpret_cast<volatile int*>(a.status) != 0) ? 1 : 0;
+  if constexpr (Lift<T>::kAny) bring_norms(plan, norm_words);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
   const bool failed = *abort_flag != 0;
+  const Lift<T> lift = lift_of<T>(norm_words, a.D);
   Schedule todo{sched, sched + 16, abort_s + 4, abort_s, plan.counts + 4, failed || !a.dq ? 0 : __ldcg(plan.counts) * (int)heads.d};
   auto item = [&](int idx, int& h) {
     const int tile = (int)heads.div((uint32_t)idx);
@@ -709,7 +764,7 @@ packed_dq_sm100_kernel(const PackedArgs a, const PackedPlan plan, const FastDiv 
       const long long at = (long long)h * a.lse_ld + t.row + row;
       float nl = valid ? -__ldcg(a.lse + at) : 0.f;
       const float nd = valid ? -__ldcg(a.delta + at) : 0.f;
-      if (nl == kInf) nl = 0.f;  // (a row without a key: the mask hides all of it)
+      nl = nl == kInf ? 0.f : nl + lift.e;  // (a row without a key: the mask hides all of it)
       const F2 nl2 = f2_make(nl, nl), nd2 = f2_make(nd, nd);
       const int last = (a.causal ? min(t.n - 1, t.shift + row) : t.n - 1) - 64 * w;
       const int warp_last = __shfl_sync(0xffffffffu, last, 0);
@@ -774,7 +829,7 @@ packed_dq_sm100_kernel(const PackedArgs a, const PackedPlan plan, const FastDiv 
         ++n_item;
         tc_fence_after();
       }
-      store_rows<T, DP / 2>(t_lane + C::colDQ + w * (DP / 2), static_cast<T*>(a.dq) + ((long long)(t.row + row) * a.H + h) * a.D, w * (DP / 2), a.D, a.scale, valid, any);
+      store_rows<T, DP / 2>(t_lane + C::colDQ + w * (DP / 2), static_cast<T*>(a.dq) + ((long long)(t.row + row) * a.H + h) * a.D, w * (DP / 2), a.D, a.scale * lift.back, valid, any);
       tc_fence_before();  // (the next item's first dQ follows a later arrival)
     }
     if (follows) {
@@ -798,7 +853,7 @@ packed_dq_sm100_kernel(const PackedArgs a, const PackedPlan plan, const FastDiv 
           f[4] += v.x; f[5] += v.y; f[6] += v.z; f[7] += v.w;
           in += (long long)a.Hk * 2 * (DP / 4 * BT);
         }
-        const float by = is_dk ? a.scale : 1.f;
+        const float by = is_dk ? a.scale * lift.back : Lift<T>::kDv;
         uint32_t o[4];
 #pragma unroll
         for (int u = 0; u < 4; ++u) o[u] = Pack2<T>::pack(f[2 * u] * by, f[2 * u + 1] * by);
@@ -861,7 +916,7 @@ size_t sm100_packed_bwd_workspace_bytes(const PackedArgs& a) { return delta_byte
 int launch_sm100_packed_bwd(int dtype, const PackedArgs& args, void* ws, cudaStream_t st, int* launches) {
   PackedArgs a = args;
   a.delta = static_cast<float*>(ws);
-  const PackedPlan plan = place_plan(a, BT, static_cast<unsigned char*>(ws) + delta_bytes(a), plan_bytes(a, true, BT, true, sm_count()));
+  PackedPlan plan = place_plan(a, BT, static_cast<unsigned char*>(ws) + delta_bytes(a), plan_bytes(a, true, BT, true, sm_count()));
   const int rc = launch_packed_prepare(dtype, a, plan, true, BT, true, true, st, launches);
   if (rc) return rc;
   if (dtype == EVOATTN_BF16) return a.D <= 64 ? launch<__nv_bfloat16, 64>(a, plan, st, launches) : launch<__nv_bfloat16, 128>(a, plan, st, launches);

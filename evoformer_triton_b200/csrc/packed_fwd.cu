@@ -511,7 +511,7 @@ int launch(const PackedArgs& a, void* ws, cudaStream_t st, int* launches) {
   // (setmaxnreg.inc would wait for registers that the launch does not have)
   if (kThreads * regs < 256 * kSoftmaxRegs + 128 * kServiceRegs) return EVOATTN_ERR_UNSUPPORTED;
   const PackedCut cut = query_cut(a, PAIR);
-  const PackedPlan plan = place_plan(a, unit, ws, plan_bytes(a, true, unit, false, sms, cut));
+  PackedPlan plan = place_plan(a, unit, ws, plan_bytes(a, true, unit, false, sms, cut));
   const int rc = launch_packed_prepare(std::is_same<T, __nv_bfloat16>::value ? EVOATTN_BF16 : EVOATTN_FP16, a, plan, true, unit, false, false, st, launches, cut);
   if (rc) return rc;
   const int heads = PAIR ? a.H : a.H / 2;

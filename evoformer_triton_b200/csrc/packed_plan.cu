@@ -160,9 +160,11 @@ __device__ __forceinline__ void make_list(const PackedArgs& a, const PackedPlan&
   if (threadIdx.x == 0 && !queries) plan.counts[2] = s.joins;
 }
 
-// delta: VEC values of 16 bytes at a time, `lanes` lanes a row (a power of two), two rows of a lane on their way.
-template <class T, bool VEC>
-__device__ __forceinline__ void row_sums(const PackedArgs& a, long long block, long long blocks, int lanes, const FastDiv& heads) {
+// delta: VEC values of 16 bytes at a time, `lanes` lanes a row (a power of two), two rows of a lane on their way.  NORMS: the largest
+// value of dO among queries that see a key and |V_j|^2 of keys of a sequence as well (those that are not finite have no say: theirs
+// are the only rows that they reach).
+template <class T, bool VEC, bool NORMS>
+__device__ __forceinline__ void row_sums(const PackedArgs& a, const PackedPlan& plan, long long block, long long blocks, int lanes, const FastDiv& heads) {
   const int team = threadIdx.x / lanes, lane = threadIdx.x % lanes, teams = kThreads / lanes;
   const int ahead = (threadIdx.x & 31) / lanes;  // teams of the warp before this one
   const long long items = (long long)a.Tq * a.H;
@@ -170,11 +172,23 @@ __device__ __forceinline__ void row_sums(const PackedArgs& a, long long block, l
   const T* d_o = static_cast<const T*>(a.d_o);
   const T* rest = static_cast<const T*>(a.o_rest);
   constexpr int V = VEC ? kPer16<T> : 1, U = 2;
+  const Span queries = NORMS ? clamped(packed_offset(a.offsets, a.wide, 0), packed_offset(a.offsets, a.wide, a.B), a.Tq) : Span{0, 0};
+  const Span keys = NORMS ? clamped(packed_offset(a.key_offsets, a.wide, 0), packed_offset(a.key_offsets, a.wide, a.B), a.Tk) : Span{0, 0};
+  __half2 most_do{};
+  float most_v = 0.f;
+  // (|x|, and NaN, which a maximum passes over, for what is not finite)
+  auto finite = [](uint32_t w) {
+    const __half2 x = __habs2(*reinterpret_cast<const __half2*>(&w));
+    return __hfma2(x, __half2{}, x);
+  };
+  auto larger = [](float a, float b) { return b > a && b < INFINITY ? b : a; };
   // (the teams of a warp meet in shuffles: as long as the first of them has a row, all go on, the others with a row that
   // is there and nothing to store)
   for (long long i0 = block * teams * U + team; i0 - ahead < items; i0 += blocks * teams * U) {
     float s[U] = {};
+    __half2 top[U] = {};
     long long to[U];
+    bool counts[U] = {};
     const T* d[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -183,6 +197,7 @@ __device__ __forceinline__ void row_sums(const PackedArgs& a, long long block, l
       const int h = i < items ? (int)(i - t * a.H) : 0;
       d[u] = d_o + t * a.sdo[0] + (long long)h * a.sdo[1];
       to[u] = (long long)h * a.lse_ld + t;
+      if constexpr (NORMS) counts[u] = i < items && t >= queries.begin && t - queries.begin < queries.n && a.lse[to[u]] != -INFINITY;
     }
     for (int x = lane * V; x < a.D; x += lanes * V) {
       if constexpr (VEC) {
@@ -204,12 +219,19 @@ __device__ __forceinline__ void row_sums(const PackedArgs& a, long long block, l
           for (int e = 0; e < V; ++e) f[e] += h[e];
 #pragma unroll
           for (int e = 0; e < V; ++e) s[u] = fmaf(f[e], g[e], s[u]);
+          if constexpr (NORMS) {
+            const uint32_t words[4] = {z[u].x, z[u].y, z[u].z, z[u].w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) top[u] = __hmax2(top[u], finite(words[e]));
+          }
         }
       } else {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
           const long long i = min(i0 + (long long)u * teams, items - 1);
-          s[u] = fmaf(to_float(o[i * a.D + x]) + (rest ? to_float(rest[i * a.D + x]) : 0.f), to_float(d[u][x]), s[u]);
+          const float g = to_float(d[u][x]);
+          s[u] = fmaf(to_float(o[i * a.D + x]) + (rest ? to_float(rest[i * a.D + x]) : 0.f), g, s[u]);
+          if constexpr (NORMS) top[u] = __hmax2(top[u], finite(__half_as_ushort(d[u][x])));
         }
       }
     }
@@ -217,12 +239,60 @@ __device__ __forceinline__ void row_sums(const PackedArgs& a, long long block, l
     for (int u = 0; u < U; ++u) {
       for (int m = lanes / 2; m > 0; m >>= 1) s[u] += __shfl_xor_sync(0xffffffffu, s[u], m);
       if (lane == 0 && i0 + (long long)u * teams < items) a.delta[to[u]] = s[u];
+      if constexpr (NORMS)
+        if (counts[u]) most_do = __hmax2(most_do, top[u]);
+    }
+  }
+  if constexpr (NORMS) {
+    const long long key_items = (long long)keys.n * a.Hk;
+    const T* v = static_cast<const T*>(a.v);
+    // (the last blocks first: there may be some without rows of dO)
+    for (long long i0 = (blocks - 1 - block) * teams * U + team; i0 - ahead < key_items; i0 += blocks * teams * U) {
+      float sq[U] = {};
+      const T* from[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const long long i = min(i0 + (long long)u * teams, key_items - 1), t = i / a.Hk;
+        from[u] = v + (keys.begin + t) * a.sv[0] + (i - t * a.Hk) * a.sv[1];
+      }
+      for (int x = lane * V; x < a.D; x += lanes * V) {
+        if constexpr (VEC) {
+          uint4 w[U];
+#pragma unroll
+          for (int u = 0; u < U; ++u) w[u] = *reinterpret_cast<const uint4*>(from[u] + x);
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            float f[V];
+            unpack16<T>(w[u], f);
+#pragma unroll
+            for (int e = 0; e < V; ++e) sq[u] = fmaf(f[e], f[e], sq[u]);
+          }
+        } else {
+#pragma unroll
+          for (int u = 0; u < U; ++u) sq[u] = fmaf(to_float(from[u][x]), to_float(from[u][x]), sq[u]);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        for (int m = lanes / 2; m > 0; m >>= 1) sq[u] += __shfl_xor_sync(0xffffffffu, sq[u], m);
+        most_v = larger(most_v, sq[u]);
+      }
+    }
+    __shared__ uint32_t both[2][kThreads / 32];
+    const float of_do = fmaxf(__low2float(most_do), __high2float(most_do));
+    const uint32_t m0 = __reduce_max_sync(0xffffffffu, __float_as_uint(of_do)), m1 = __reduce_max_sync(0xffffffffu, __float_as_uint(most_v));
+    if ((threadIdx.x & 31) == 0) { both[0][threadIdx.x >> 5] = m0; both[1][threadIdx.x >> 5] = m1; }
+    __syncthreads();
+    if (threadIdx.x < 32) {
+      const uint32_t x = threadIdx.x < kThreads / 32 ? both[0][threadIdx.x] : 0, y = threadIdx.x < kThreads / 32 ? both[1][threadIdx.x] : 0;
+      const float2 most = make_float2(__uint_as_float(__reduce_max_sync(0xffffffffu, x)), __uint_as_float(__reduce_max_sync(0xffffffffu, y)));
+      if (threadIdx.x == 0) plan.norms[block] = most;
     }
   }
 }
 
 // Block 0 makes the list of queries, block 1 (or 0) that of keys, the others the row sums.
-template <class T, bool VEC>
+template <class T, bool VEC, bool NORMS>
 __global__ void __launch_bounds__(kThreads, 2) packed_prepare_kernel(const PackedArgs a, const PackedPlan plan, const int queries, const int unit, const int keys,
                                                                   const int sms, const PackedCut qcut, const PackedCut kcut, const int lanes, const FastDiv heads) {
   __shared__ Sums s;
@@ -233,25 +303,32 @@ __global__ void __launch_bounds__(kThreads, 2) packed_prepare_kernel(const Packe
     const bool q = queries && blockIdx.x == 0;
     make_list(a, plan, q, q ? unit : kTileRows, sms, q ? qcut : kcut, s);
   } else {
-    row_sums<T, VEC>(a, blockIdx.x - lists, gridDim.x - lists, lanes, heads);
+    row_sums<T, VEC, NORMS>(a, plan, blockIdx.x - lists, gridDim.x - lists, lanes, heads);
   }
 }
 
 }  // namespace
 
-int launch_packed_prepare(int dtype, const PackedArgs& a, const PackedPlan& plan, bool queries, int unit, bool keys, bool delta, cudaStream_t st, int* launches,
+int launch_packed_prepare(int dtype, const PackedArgs& a, PackedPlan& plan, bool queries, int unit, bool keys, bool delta, cudaStream_t st, int* launches,
                           const PackedCut& qcut) {
   const int sms = sm_count();
   if (sms <= 0) return EVOATTN_ERR_CUDA;
   return with_dtype(dtype, [&](auto t) {
     using T = decltype(t);
     constexpr int V = kPer16<T>;
-    const bool vec = delta && a.D % V == 0 && ((reinterpret_cast<uintptr_t>(a.o) | reinterpret_cast<uintptr_t>(a.o_rest) | reinterpret_cast<uintptr_t>(a.d_o)) & 15) == 0 && a.sdo[0] % V == 0 && a.sdo[1] % V == 0;
+    const bool norms = std::is_same<T, __half>::value && delta && keys;
+    bool vec = delta && a.D % V == 0 && ((reinterpret_cast<uintptr_t>(a.o) | reinterpret_cast<uintptr_t>(a.o_rest) | reinterpret_cast<uintptr_t>(a.d_o)) & 15) == 0 && a.sdo[0] % V == 0 && a.sdo[1] % V == 0;
+    if (norms) vec = vec && (reinterpret_cast<uintptr_t>(a.v) & 15) == 0 && a.sv[0] % V == 0 && a.sv[1] % V == 0;
     int lanes = 1;
     while (lanes < 32 && lanes * (vec ? V : 1) < a.D) lanes *= 2;
-    const long long rows = ((long long)a.Tq * a.H + kThreads / lanes * 2 - 1) / (kThreads / lanes * 2);
-    const int blocks = (queries ? 1 : 0) + (keys ? 1 : 0) + (delta ? (int)(rows < sms * 8LL ? rows : sms * 8LL) : 0);
-    launch_dependent(vec ? packed_prepare_kernel<T, true> : packed_prepare_kernel<T, false>, dim3((unsigned)blocks), kThreads, 0, st, a, plan, (int)queries, unit, (int)keys,
+    const long long each = kThreads / lanes * 2, most = (long long)sms * kSumBlocks;
+    const long long rows = ((long long)a.Tq * a.H + each - 1) / each + (norms ? ((long long)a.Tk * a.Hk + each - 1) / each : 0);
+    const int sums = delta ? (int)(rows < most ? rows : most) : 0, blocks = (queries ? 1 : 0) + (keys ? 1 : 0) + sums;
+    plan.n_norms = norms ? sums : 0;
+    auto kern = vec ? packed_prepare_kernel<T, true, false> : packed_prepare_kernel<T, false, false>;
+    if constexpr (std::is_same<T, __half>::value)
+      if (norms) kern = vec ? packed_prepare_kernel<T, true, true> : packed_prepare_kernel<T, false, true>;
+    launch_dependent(kern, dim3((unsigned)blocks), kThreads, 0, st, a, plan, (int)queries, unit, (int)keys,
                      sms, qcut, key_cut(a), lanes, FastDiv((uint32_t)a.H));
     *launches += 1;
     return cudaGetLastError() == cudaSuccess ? EVOATTN_OK : EVOATTN_ERR_CUDA;

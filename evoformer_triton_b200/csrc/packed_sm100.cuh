@@ -37,7 +37,10 @@ struct PackedPlan {
   float* sums;               // key tiles: [slot][Hk][dV, dK][DP / 4][128 rows][4]; query units: [slot][units of heads][2 tiles][DP / 4][128][4]
   float4* ml;                // [slot][units of heads][2 tiles][128 rows]: reference, sum of P as rounded, and as it is
   int *arrived, n_arrived;   // [slot][units of heads][2 tiles]: parts that are through, of the tile whose first part has that slot
+  float2* norms;             // fp16 backward: the largest value of dO and |V_j|^2 that a block of the row sums has met
+  int n_norms;
 };
+constexpr int kSumBlocks = 8;  // of the row sums an SM, at most
 // What a list cuts: tiles of one and a half times as many steps and more as `part` hundredths of what an SM has to do, and as
 // `least`; `heads` is how many of each there are on the list.
 struct PackedCut {
@@ -62,15 +65,16 @@ inline long long key_slots(const PackedArgs& a, int sms) { return most_slots(key
 inline long long query_slots(const PackedArgs& a, int unit, int sms, const PackedCut& c) { return most_slots(query_units(a, unit), a.Tk / kTileRows + 1LL, sms, c); }
 inline size_t round256(size_t n) { return (n + 255) / 256 * 256; }
 struct PlanBytes {
-  size_t queries, keys, joins, sums, ml, arrived;
-  size_t all() const { return 256 + queries + keys + joins + sums + ml + arrived; }
+  size_t queries, keys, joins, sums, ml, arrived, norms;
+  size_t all() const { return 256 + queries + keys + joins + sums + ml + arrived + norms; }
 };
 // qcut.heads = 0: the query units are not cut.
 inline PlanBytes plan_bytes(const PackedArgs& a, bool queries, int unit, bool keys, int sms, const PackedCut& qcut = PackedCut{100, 1, 0}) {
   const long long ks = keys ? key_slots(a, sms) : 0, qs = queries && qcut.heads ? query_slots(a, unit, sms, qcut) : 0;
   const size_t tile = (size_t)kTileRows * (a.D <= 64 ? 64 : 128) * sizeof(float), tiles = (size_t)qs * qcut.heads * 2;
   return PlanBytes{queries ? round256((query_units(a, unit) + qs) * sizeof(PackedTile)) : 0, keys ? round256((key_tiles(a) + ks) * sizeof(PackedTile)) : 0,
-                   round256(ks * sizeof(PackedJoin)), round256(tile * (ks * a.Hk * 2 + tiles)), round256(tiles * kTileRows * sizeof(float4)), round256(tiles * sizeof(int))};
+                   round256(ks * sizeof(PackedJoin)), round256(tile * (ks * a.Hk * 2 + tiles)), round256(tiles * kTileRows * sizeof(float4)), round256(tiles * sizeof(int)),
+                   keys ? round256((size_t)sms * kSumBlocks * sizeof(float2)) : 0};
 }
 inline PackedPlan place_plan(const PackedArgs& a, int unit, void* ws, const PlanBytes& n) {
   unsigned char* p = static_cast<unsigned char*>(ws);
@@ -83,12 +87,14 @@ inline PackedPlan place_plan(const PackedArgs& a, int unit, void* ws, const Plan
   plan.joins = reinterpret_cast<PackedJoin*>(p += n.keys);
   plan.sums = reinterpret_cast<float*>(p += n.joins);
   plan.ml = reinterpret_cast<float4*>(p += n.sums);
-  plan.arrived = reinterpret_cast<int*>(p + n.ml);
+  plan.arrived = reinterpret_cast<int*>(p += n.ml);
+  plan.norms = reinterpret_cast<float2*>(p + n.arrived);
   plan.n_arrived = (int)(n.arrived / sizeof(int));
   return plan;
 }
-// Writes the lists, those with the most work first, and the row sums of dO * O, in one launch (packed_plan.cu).
-int launch_packed_prepare(int dtype, const PackedArgs& a, const PackedPlan& plan, bool queries, int unit, bool keys, bool delta, cudaStream_t st, int* launches,
+// Writes the lists, those with the most work first, and the row sums of dO * O (with both lists and fp16 the norms too, whose number
+// it sets), in one launch (packed_plan.cu).
+int launch_packed_prepare(int dtype, const PackedArgs& a, PackedPlan& plan, bool queries, int unit, bool keys, bool delta, cudaStream_t st, int* launches,
                           const PackedCut& qcut = PackedCut{100, 1, 0});
 
 // [T][heads][D] rows of 16 bits as a 3-D map (D, T, heads) with boxes of 64 values (128 bytes, swizzled) by `rows`;

@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from oracle import sequences_oracle as oc
-from test_packed_attention_gpu import BF, DEV, F32, HF, IDS, _check, _qkv, _spans, _sums
+from test_packed_attention_gpu import BF, DEV, F32, HF, IDS, _check, _draw, _qkv, _spans, _sums
 
 pytestmark = pytest.mark.gpu
 
@@ -32,3 +32,70 @@ def test_tokens_lose_only_the_rounding_of_their_results(nk, H, Hk, D, dtype):
     # the second piece rounded (fp16: by half of its smallest step too, against a sum of one or more)
     bound = bound + u * u * big + (max(nk) * 2.0 ** -25 * v.abs().max().double() if dtype == HF else 0.0)
     oc.check("o", out, (value, bound + oc.rounding(dtype, value.abs() + bound)))
+
+
+HALF_LENGTHS = [[1500], [700, 37, 900]]
+
+
+def _half_gradients(q, k, v, d, lengths, causal):
+    import evoformer_triton_b200 as evo
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    return torch.autograd.grad(evo.packed_attention(*leaves, torch.tensor(_sums(lengths), device=DEV), causal=causal), leaves, d)
+
+
+@pytest.mark.parametrize("causal", [True, False], ids=["causal", "both"])
+@pytest.mark.parametrize("lengths", HALF_LENGTHS, ids=str)
+@pytest.mark.parametrize("H,Hk,D", [(4, 2, 64), (2, 1, 96), (2, 2, 128)])
+def test_fp16_gradients_of_a_gradient_of_any_size(H, Hk, D, lengths, causal):
+    """A gradient times a power of two makes gradients times that power but for the rounding of the results: dS neither
+    loses its bits at the lower end of fp16 nor passes its upper end.  Roundings are even over a step: half a step over the root
+    of three each, which is 0.58 of it; the rest is for the few dS that round to the other side."""
+    q, k, v = _qkv(sum(lengths), sum(lengths), H, Hk, D, HF)
+    d = (_draw(q.shape, F32, 5) * 64).round() / 64  # (multiples of 2^-6, which fp16 holds exactly times 2^-18 as well)
+    base = _half_gradients(q, k, v, d.to(HF), lengths, causal)
+    for power in (-18, -12, -8, 5, 12):
+        got = _half_gradients(q, k, v, (d * 2.0 ** power).to(HF), lengths, causal)
+        for name, g, b in zip(("dq", "dk", "dv"), got, base):
+            want = b.double() * 2.0 ** power
+            off = torch.where(want.abs() < 65000, g.double() - want, 0.0)
+            steps = float(oc.rounding(HF, b.double()).norm()) * 2.0 ** power + float(oc.rounding(HF, want).norm())
+            assert float(off.norm()) <= 0.65 * steps, (name, power, float(off.norm()) / steps)
+            assert torch.equal(torch.isfinite(g), torch.isfinite(want.to(HF))) or power == 12
+
+
+@pytest.mark.parametrize("std", [1.0, 1e-3, 1e-4, 3000.0])
+@pytest.mark.parametrize("H,Hk,D", [(4, 1, 64), (2, 1, 96)])
+def test_fp16_gradients_by_their_norm(H, Hk, D, std):
+    """Of far rows too: what rounding the results makes (half a step over the root of three, 0.58 of it), and half a step more for
+    those of P and dS, which are as independent."""
+    T = 1600
+    q, k, v = _qkv(T, T, H, Hk, D, HF)
+    d = _draw(q.shape, HF, 5, std)
+    want = oc.attention(q, k, v, [(0, T, 0, T)], True, d=d)[1:]
+    for name, g, (w, _) in zip(("dq", "dk", "dv"), _half_gradients(q, k, v, d, [T], True), want):
+        for rows in (slice(0, 400), slice(400, 1000), slice(1000, T)):
+            x = w[rows]
+            assert float((g[rows].double() - x).norm()) <= 0.65 * float(oc.rounding(HF, x).norm()) + torch.finfo(HF).eps / 2 * float(x.norm()), (name, rows)
+
+
+@pytest.mark.parametrize("bad", [float("inf"), float("nan"), 6e4])
+def test_fp16_gradients_beside_ones_of_another_size(bad):
+    """Sequences, and rows of none, whose gradients or values are huge or not finite say nothing about the others."""
+    lengths, D = [300, 200, 129], 64
+    T = sum(lengths) + 9
+    q, k, v = _qkv(T, T, 4, 2, D, HF)
+    d = _draw(q.shape, HF, 5)
+    for t in (q, k, v, d):
+        t[:4], t[-5:] = bad, float("nan")
+    d[4 + 300:4 + 500] = bad
+    spans = _spans(lengths, lengths, 4, 4)
+    import evoformer_triton_b200 as evo
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    got = torch.autograd.grad(evo.packed_attention(*leaves, torch.tensor(_sums(lengths, 4), device=DEV)), leaves, d)
+    clean = [torch.nan_to_num(t, 0.0, 0.0, 0.0) for t in (q, k, v, d)]
+    keep = torch.zeros(T, dtype=torch.bool, device=DEV)
+    keep[4:304] = keep[504:-5] = True
+    for name, g, (w, e) in zip(("dq", "dk", "dv"), got, oc.attention(*clean[:3], spans, True, d=clean[3])[1:]):
+        if bad < 1e5:
+            oc.check(name, g, (w, e))
+        oc.check(name, g[keep], (w[keep], e[keep]))
