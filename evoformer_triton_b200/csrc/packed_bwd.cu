@@ -75,13 +75,15 @@ __device__ __forceinline__ void load_tile_rows(uint32_t dst, const CUtensorMap* 
 #pragma unroll
   for (int p = 0; p < DP / 64; ++p) tma_load_3d_s(dst + p * Tiles<DP>::kPanel, map, bar, 64 * p, row, h);
 }
-// Zeros in the rows of a staged tile from `real` on, by a warp.
+// Zeros in the rows of a staged tile from `real` on, and in those before `blind`, by a warp.
 template <int DP>
-__device__ __forceinline__ void clear_rows(uint32_t tile_s, int real, int lane) {
-  if (real >= BT) return;
+__device__ __forceinline__ void clear_rows(uint32_t tile_s, int real, int lane, int blind = 0) {
+  if (real >= BT && blind <= 0) return;
 #pragma unroll 1
-  for (int p = 0; p < DP / 64; ++p)
+  for (int p = 0; p < DP / 64; ++p) {
     for (int x = real * 128 + lane * 16; x < Tiles<DP>::kPanel; x += 512) sts_v4(tile_s + p * Tiles<DP>::kPanel + x, 0, 0, 0, 0);
+    for (int x = lane * 16; x < min(blind, BT) * 128; x += 512) sts_v4(tile_s + p * Tiles<DP>::kPanel + x, 0, 0, 0, 0);
+  }
   fence_async_shared();
 }
 
@@ -185,9 +187,9 @@ __device__ __forceinline__ void clear_tiles(const PackedTile* list, int begin, i
   }
 }
 
-// COLS columns of an accumulator, times f, to a row of 16-bit values; zeros where `any` is not set.
+// COLS columns of an accumulator, times f, to a row of 16-bit values; zeros where `any` is not set, and in rows that are not `seen`.
 template <class T, int COLS>
-__device__ __forceinline__ void store_rows(uint32_t t_src, T* out, int d0, int D, float f, bool valid, bool any) {
+__device__ __forceinline__ void store_rows(uint32_t t_src, T* out, int d0, int D, float f, bool valid, bool any, bool seen) {
 #pragma unroll
   for (int c = 0; c < COLS; c += 32) {
     uint32_t r[32];
@@ -200,7 +202,7 @@ __device__ __forceinline__ void store_rows(uint32_t t_src, T* out, int d0, int D
       if (valid && d0 + c + e < D) {
         uint32_t p[4];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) p[u] = any ? Pack2<T>::pack(__uint_as_float(r[e + 2 * u]) * f, __uint_as_float(r[e + 2 * u + 1]) * f) : 0u;
+        for (int u = 0; u < 4; ++u) p[u] = any && seen ? Pack2<T>::pack(__uint_as_float(r[e + 2 * u]) * f, __uint_as_float(r[e + 2 * u + 1]) * f) : 0u;
         *reinterpret_cast<uint4*>(out + d0 + c + e) = make_uint4(p[0], p[1], p[2], p[3]);
       }
     }
@@ -269,6 +271,7 @@ packed_dkv_sm100_kernel(const PackedArgs a, const PackedPlan plan, const FastDiv
     __device__ __forceinline__ bool first() const { return left == t.steps; }
     __device__ __forceinline__ bool last() const { return left == 1; }
     __device__ __forceinline__ int real() const { return t.n - i * BT; }
+    __device__ __forceinline__ int blind() const { return t.blind - i * BT; }
     __device__ __forceinline__ void next() {
       --left;
       if (++i == end) { i = end - t.tiles; ++g; }
@@ -393,14 +396,15 @@ packed_dkv_sm100_kernel(const PackedArgs a, const PackedPlan plan, const FastDiv
       // =============================== Q: its end, and the statistics of its rows ===============================
 #pragma unroll 1
       while (more) {
-        const int h = s.hk * a.G + s.g, real = s.real();
+        const int h = s.hk * a.G + s.g, real = s.real(), blind = s.blind();
         const long long at = (long long)h * a.lse_ld + s.t.other + s.i * BT;
-        float nl[4], nd[4];  // (rows behind the end: 2^e of queries and gradients that are zero)
+        float nl[4], nd[4];  // (rows behind the end, or without a key: 2^e of queries and gradients that are zero)
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
           const int r = lane + 32 * u;
-          nl[u] = (r < real ? -__ldcg(a.lse + at + r) : 0.f) + lift.e;
-          nd[u] = r < real ? -__ldcg(a.delta + at + r) : 0.f;
+          const bool seen = r >= blind && r < real;
+          nl[u] = (seen ? -__ldcg(a.lse + at + r) : 0.f) + lift.e;
+          nd[u] = seen ? -__ldcg(a.delta + at + r) : 0.f;
         }
         mbar_wait_s(q_empty(st), par ^ 1, abort_s, DEV_TIMEOUT_SYNC);
         const uint32_t stats = smem_s + C::offStats + st * (2 * BT * 4);
@@ -410,7 +414,7 @@ packed_dkv_sm100_kernel(const PackedArgs a, const PackedPlan plan, const FastDiv
           sts_f32(stats + (BT + lane + 32 * u) * 4, nd[u]);
         }
         mbar_wait_s(q_in(st), par, abort_s, DEV_TIMEOUT_TMA);
-        clear_rows<DP>(smem_s + C::offQ + st * C::kTile, real, lane);
+        clear_rows<DP>(smem_s + C::offQ + st * C::kTile, real, lane, blind);
         __syncwarp();
         if (lane == 0) mbar_arrive_s(q_full(st));
         next();
@@ -428,7 +432,7 @@ packed_dkv_sm100_kernel(const PackedArgs a, const PackedPlan plan, const FastDiv
 #pragma unroll 1
       while (more) {
         mbar_wait_s(d_in(st), par, abort_s, DEV_TIMEOUT_TMA);
-        clear_rows<DP>(smem_s + C::offD + st * C::kTile, s.real(), lane);
+        clear_rows<DP>(smem_s + C::offD + st * C::kTile, s.real(), lane, s.blind());
         __syncwarp();
         if (lane == 0) mbar_arrive_s(d_full(st));
         next();
@@ -766,6 +770,7 @@ packed_dq_sm100_kernel(const PackedArgs a, const PackedPlan plan, const FastDiv 
       const float nd = valid ? -__ldcg(a.delta + at) : 0.f;
       nl = nl == kInf ? 0.f : nl + lift.e;  // (a row without a key: the mask hides all of it)
       const F2 nl2 = f2_make(nl, nl), nd2 = f2_make(nd, nd);
+      const bool seen = !a.causal || t.shift + row >= 0;  // (a query without a key: whatever q and dO hold there)
       const int last = (a.causal ? min(t.n - 1, t.shift + row) : t.n - 1) - 64 * w;
       const int warp_last = __shfl_sync(0xffffffffu, last, 0);
 #pragma unroll 1
@@ -829,7 +834,7 @@ packed_dq_sm100_kernel(const PackedArgs a, const PackedPlan plan, const FastDiv 
         ++n_item;
         tc_fence_after();
       }
-      store_rows<T, DP / 2>(t_lane + C::colDQ + w * (DP / 2), static_cast<T*>(a.dq) + ((long long)(t.row + row) * a.H + h) * a.D, w * (DP / 2), a.D, a.scale * lift.back, valid, any);
+      store_rows<T, DP / 2>(t_lane + C::colDQ + w * (DP / 2), static_cast<T*>(a.dq) + ((long long)(t.row + row) * a.H + h) * a.D, w * (DP / 2), a.D, a.scale * lift.back, valid, any, seen);
       tc_fence_before();  // (the next item's first dQ follows a later arrival)
     }
     if (follows) {

@@ -34,20 +34,20 @@ struct GenericCfg {
   static constexpr size_t bytes(int tiles, int scores) { return sizeof(float) * ((size_t)tiles * TILE * LD + (size_t)scores * TILE * LP + 2 * TILE); }
 };
 
-// Rows [0, n) of a tile on their way to shared memory as floats, zeros beyond n and D: get() asks for all of them at once (one
+// Rows [from, n) of a tile on their way to shared memory as floats, zeros before, beyond n and beyond D: get() asks for all of them at once (one
 // at a time they took 9 of a tile's 11 us), put() stores them.  VEC: 16 bytes at a time.
 template <class T, int DP, int TILE, bool VEC>
 struct Rows {
   static constexpr int LD = GenericCfg<DP, TILE>::LD, V = VEC ? kPer16<T> : 1, PER = DP / V, N = TILE * PER / kThreads;
   using Raw = typename std::conditional<VEC, uint4, T>::type;
   Raw raw[N];
-  __device__ __forceinline__ void get(const void* src, long long stride, int n, int D) {
+  __device__ __forceinline__ void get(const void* src, long long stride, int n, int D, int from = 0) {
     const T* p = static_cast<const T*>(src);
 #pragma unroll
     for (int u = 0; u < N; ++u) {
       const int i = threadIdx.x + u * kThreads, r = i / PER, d = i % PER * V;
       raw[u] = Raw{};
-      if (r < n && d < D) raw[u] = *reinterpret_cast<const Raw*>(p + r * stride + d);
+      if (r >= from && r < n && d < D) raw[u] = *reinterpret_cast<const Raw*>(p + r * stride + d);
     }
   }
   __device__ __forceinline__ void put(float* dst) const {
@@ -337,12 +337,12 @@ __global__ void __launch_bounds__(kThreads) packed_generic_dkv_kernel(const Pack
     for (int k = 0; k < NC; ++k) dk[r][k] = dv[r][k] = make_float4(0.f, 0.f, 0.f, 0.f);
   // the first query that sees a key of this tile
   const int first = a.causal ? max(0, j0 - (ks.n - qs.n)) : 0;
-  const int i_first = first / TILE * TILE;
+  const int i_first = first / TILE * TILE, blind = a.causal ? qs.n - ks.n : 0;  // (the queries before `blind` see no key: whatever they hold)
   auto fetch = [&](int h, int i0) {
     const long long row = qs.begin + i0;
     const int rows = min(TILE, qs.n - i0);
-    x.get(static_cast<const T*>(a.q) + row * a.sq[0] + (long long)h * a.sq[1], a.sq[0], rows, a.D);
-    y.get(static_cast<const T*>(a.d_o) + row * a.sdo[0] + (long long)h * a.sdo[1], a.sdo[0], rows, a.D);
+    x.get(static_cast<const T*>(a.q) + row * a.sq[0] + (long long)h * a.sq[1], a.sq[0], rows, a.D, blind - i0);
+    y.get(static_cast<const T*>(a.d_o) + row * a.sdo[0] + (long long)h * a.sdo[1], a.sdo[0], rows, a.D, blind - i0);
   };
   if (i_first < qs.n) fetch(hk * a.G, i_first);
   for (int g = 0; g < a.G; ++g) {

@@ -62,6 +62,7 @@ struct Tiles {
           const int first = a.causal ? max(0, t.shift) : 0;  // the first query that sees a key of the tile
           t.tiles = first < qs.n ? (qs.n + kTileRows - 1) / kTileRows - first / kTileRows : 0;
           t.steps = t.tiles * a.G;
+          t.blind = a.causal ? max(0, qs.n - ks.n) : 0;
         }
         f(t);
       }

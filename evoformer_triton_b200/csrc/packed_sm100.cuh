@@ -20,7 +20,8 @@ struct PackedTile {
   int tiles;        // tiles of 128 rows of the other tensor that it meets: the first ones of the keys; the last ones of the queries
   int begin, steps; // of the steps of a key tile (the tiles of the group's heads, one after another) this part's
   int parts, part;  // parts of the tile, and which this is
-  int slot, pad;    // where it leaves its sums (those of part 0 lie `part` slots before)
+  int slot;         // where it leaves its sums (those of part 0 lie `part` slots before)
+  int blind;        // of key tiles: queries at the start of the sequence that see no key at all
 };
 static_assert(sizeof(PackedTile) == 48, "three 16-byte loads");
 struct PackedJoin {
@@ -224,7 +225,7 @@ __device__ __forceinline__ void stores_done() {
 __device__ __forceinline__ PackedTile load_tile(const PackedTile* p) {
   const uint4* x = reinterpret_cast<const uint4*>(p);
   const uint4 u = __ldcg(x), v = __ldcg(x + 1), w = __ldcg(x + 2);
-  return PackedTile{(int)u.x, (int)u.y, (int)u.z, (int)u.w, (int)v.x, (int)v.y, (int)v.z, (int)v.w, (int)w.x, (int)w.y, (int)w.z, 0};
+  return PackedTile{(int)u.x, (int)u.y, (int)u.z, (int)u.w, (int)v.x, (int)v.y, (int)v.z, (int)v.w, (int)w.x, (int)w.y, (int)w.z, (int)w.w};
 }
 // Which item a CTA works on next: the first is its own, the others it takes from a counter, the most work first as the list
 // has them.  The warp that loads takes one when it has asked for all tiles of the item before (no sooner: who has the

@@ -99,3 +99,25 @@ def test_fp16_gradients_beside_ones_of_another_size(bad):
         if bad < 1e5:
             oc.check(name, g, (w, e))
         oc.check(name, g[keep], (w[keep], e[keep]))
+
+
+@pytest.mark.parametrize("dtype", [BF, HF, F32], ids=IDS.get)
+@pytest.mark.parametrize("H,Hk,D", [(4, 2, 64), (3, 1, 128), (2, 2, 20)])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_queries_without_a_key_may_hold_anything(bad, H, Hk, D, dtype):
+    """q and the gradient of queries that the mask leaves no key (more queries than keys, or no keys at all): zeros come back, and
+    nothing of them reaches the other rows."""
+    import evoformer_triton_b200 as evo
+    nq, nk = [300, 7, 129, 40, 260], [100, 0, 1, 40, 132]
+    q, k, v = _qkv(sum(nq), sum(nk), H, Hk, D, dtype)
+    d = _draw(q.shape, dtype, 5)
+    blind = torch.zeros(sum(nq), dtype=torch.bool, device=DEV)
+    for i, n, _, m in _spans(nq, nk):
+        blind[i:i + max(0, n - m)] = True
+    dirty = [torch.where(blind[:, None, None], bad, t) for t in (q, d)]
+    leaves = [t.detach().requires_grad_() for t in (dirty[0], k, v)]
+    out = evo.packed_attention(*leaves, torch.tensor(_sums(nq), device=DEV), torch.tensor(_sums(nk), device=DEV))
+    grads = torch.autograd.grad(out, leaves, dirty[1])
+    assert not out[blind].any() and not grads[0][blind].any()
+    for name, g, w in zip(("o", "dq", "dk", "dv"), (out, *grads), oc.attention(q, k, v, _spans(nq, nk), True, d=d)):
+        oc.check(name, g, w)
