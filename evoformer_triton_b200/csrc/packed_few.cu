@@ -400,7 +400,7 @@ packed_few_kernel(const PackedArgs a, const Parts parts, const int clear, const 
       if (!valid[e]) return;
       const int row = r0 + lane / 4 + 8 * e, i = row / a.G, h = hk * a.G + row - i * a.G, d0 = i0 * 8 + 2 * (lane & 3);
       if (whole) {
-        const float inv = l[e] > 0.f ? 1.f / l[e] : 0.f;
+        const float inv = l[e] != 0.f ? 1.f / l[e] : 0.f;
         T* out = static_cast<T*>(a.o) + ((long long)(qs.begin + i) * a.H + h) * a.D + d0;
 #pragma unroll
         for (int n = 0; n < N; ++n)
@@ -534,7 +534,7 @@ __global__ void __launch_bounds__(kThreads) packed_join_kernel(const PackedArgs 
       float v = 0.f;
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) v += sums[w][d];
-      static_cast<T*>(a.o)[((long long)t * a.H + h) * a.D + d] = from_float<T>(l > 0.f ? v / l : 0.f);
+      static_cast<T*>(a.o)[((long long)t * a.H + h) * a.D + d] = from_float<T>(l != 0.f ? v / l : 0.f);
     }
   }
 }

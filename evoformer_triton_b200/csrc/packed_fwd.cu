@@ -20,7 +20,8 @@
 // m is not the maximum but a reference that the exponentials of a tile are taken against straight from the scores, without
 // looking for their maximum: any m gives the same o as long as nothing leaves the range of P's type.  It is 0 to begin with; if
 // a tile's sum shows that some p may be too large, or a row's first sum that all of them are too small, the tile's maximum
-// is taken, O and l follow it, and the tile is done again (P is kept in registers until then).  O is divided by the sum of the
+// is taken, O and l follow it, and the tile is done again (P is kept in registers until then).  A score that is infinite or NaN
+// comes this way too, since its p is, and makes l, and with it the row, NaN.  O is divided by the sum of the
 // P that it was made of, rounded (with that of the unrounded values it was off by 0.0023 instead of 0.0021 of its norm, where
 // its own rounding makes 0.0016, and a forward took 4 % less); the log-sum-exp is that of the unrounded ones.
 //
@@ -364,16 +365,19 @@ packed_fwd_sm100_kernel(const PackedArgs a, const PackedPlan plan, const FastDiv
               if (cut) {
 #pragma unroll
                 for (int e = 0; e < 32; e += 2)
-                  mx = max3(mx, 32 * k + e <= lim ? __uint_as_float(s[e]) : -kInf, 32 * k + e + 1 <= lim ? __uint_as_float(s[e + 1]) : -kInf);
+                  mx = max3_nan(mx, 32 * k + e <= lim ? __uint_as_float(s[e]) : -kInf, 32 * k + e + 1 <= lim ? __uint_as_float(s[e + 1]) : -kInf);
               } else {
 #pragma unroll
-                for (int e = 0; e < 32; e += 2) mx = max3(mx, __uint_as_float(s[e]), __uint_as_float(s[e + 1]));
+                for (int e = 0; e < 32; e += 2) mx = max3_nan(mx, __uint_as_float(s[e]), __uint_as_float(s[e + 1]));
               }
             }
           }
           const float m_old = m;
+          mx *= c;
+          const bool odd = valid && !(mx < kInf);
+          if (odd) l = lu = __int_as_float(0x7fffffff);
           const bool fresh = l == 0.f;  // (nothing of the row is in O yet)
-          if (valid && mx != -kInf) m = fresh ? mx * c : fmaxf(m, mx * c);
+          if (valid && !odd && mx != -kInf) m = fresh ? mx : fmaxf(m, mx);
           if (t < end - 1 && __any_sync(0xffffffffu, !fresh && m > m_old)) {
             const float alpha = !fresh && m > m_old ? ex2(m_old - m) : 1.f;
             l *= alpha;
@@ -441,7 +445,7 @@ packed_fwd_sm100_kernel(const PackedArgs a, const PackedPlan plan, const FastDiv
 #pragma unroll 1
         for (int p = 0; p < it.t.parts; ++p) {
           const float4 x = __ldcg(plan.ml + place(slot0 + p) * BM + row);
-          if (x.y > 0.f) m = fmaxf(m, x.x);
+          if (x.y != 0.f) m = fmaxf(m, x.x);
         }
         if (m == -kInf) m = 0.f;
 #pragma unroll 1
@@ -451,7 +455,7 @@ packed_fwd_sm100_kernel(const PackedArgs a, const PackedPlan plan, const FastDiv
 #pragma unroll 1
           for (int p = 0; p < it.t.parts; ++p) {
             const float4 x = __ldcg(plan.ml + place(slot0 + p) * BM + row);
-            const float f = x.y > 0.f ? ex2(x.x - m) : 0.f;
+            const float f = x.y != 0.f ? ex2(x.x - m) : 0.f;
             const float4* from = reinterpret_cast<const float4*>(plan.sums) + place(slot0 + p) * (DP / 4 * BM) + d / 4 * BM + row;
             l = fmaf(x.y, f, l);
             lu = fmaf(x.z, f, lu);
@@ -471,7 +475,7 @@ packed_fwd_sm100_kernel(const PackedArgs a, const PackedPlan plan, const FastDiv
         }
         tmem_wait_st();
       }
-      const bool any = l > 0.f;
+      const bool any = l != 0.f;
       const int first = (warp & 3) * 32;  // row of the warp's first lane
       store_rows_staged<T, DP>(smem_s + C::offOut + (warp - 4) * kStageBytes, tO, &tmO, (int)(out_row - lane), h, static_cast<T*>(a.o) + ((out_row - lane) * a.H + h) * a.D,
                                (long long)a.H * a.D, rows - first, a.D, any ? 1.f / l : 0.f, some);

@@ -204,18 +204,17 @@ __global__ void __launch_bounds__(kThreads) packed_generic_fwd_kernel(const Pack
   for (int r = 0; r < NR; ++r) {
     const int i = ty + 16 * r;
     if (i >= rows) continue;
-    const float inv = l[r] > 0.f ? 1.f / l[r] : 0.f;
+    const float inv = l[r] != 0.f ? 1.f / l[r] : 0.f;  // (0: no key; NaN where a score is infinite or NaN)
     T* out = o + ((long long)(qs.begin + i0 + i) * a.H + h) * a.D;
 #pragma unroll
-    for (int k = 0; k < NC; ++k) store_row(out, tx, k, acc[r][k], m[r] == -INFINITY ? 0.f : inv, a.D);
+    for (int k = 0; k < NC; ++k) store_row(out, tx, k, acc[r][k], inv, a.D);
     if (a.o_rest) {
       T* rest = static_cast<T*>(a.o_rest) + (out - o);
-      const float by = m[r] == -INFINITY ? 0.f : inv;
-      auto left = [&](float v) { return v * by - to_float(from_float<T>(v * by)); };
+      auto left = [&](float v) { return v * inv - to_float(from_float<T>(v * inv)); };
 #pragma unroll
       for (int k = 0; k < NC; ++k) store_row(rest, tx, k, make_float4(left(acc[r][k].x), left(acc[r][k].y), left(acc[r][k].z), left(acc[r][k].w)), 1.f, a.D);
     }
-    if (tx == 0 && a.lse) a.lse[(long long)h * a.lse_ld + qs.begin + i0 + i] = m[r] == -INFINITY ? -INFINITY : m[r] + log2f(l[r]);
+    if (tx == 0 && a.lse) a.lse[(long long)h * a.lse_ld + qs.begin + i0 + i] = l[r] == 0.f ? -INFINITY : m[r] + log2f(l[r]);
   }
 }
 

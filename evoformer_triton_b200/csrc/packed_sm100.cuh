@@ -124,17 +124,18 @@ int launch_packed_few(int dtype, const PackedArgs& a, bool clear, void* workspac
 // and SM, which is as long as the tile's MMAs take (head dimension 128) or twice that (64).  x = n + f with n whole (by
 // adding and taking off 1.5 2^23) and |f| <= 1/2; 2^f by a polynomial whose largest relative error is the smallest there
 // is for its degree (fitted by exchange): 7.5e-5 of degree 3, 2.6e-6 of degree 4, a fiftieth and a two-hundredth of half a step of bf16 and fp16;
-// n is added to the exponent's bits.  Exponents below -126 count as that; with BOTH those above 126 too.
+// n is added to the exponent's bits.  Exponents below -126 count as that; with BOTH those above 126 too.  NaN makes the largest
+// number there is (the sum of its bits), which no 16-bit type holds and no sum of exponentials reaches.
 template <class T, bool BOTH>
 __device__ __forceinline__ void exp2_fma(ptx::F2 x, float& p0, float& p1) {
   using namespace ptx;
   float x0, x1;
   f2_get(x, x0, x1);
-  x0 = fmaxf(x0, -126.f);
-  x1 = fmaxf(x1, -126.f);
+  x0 = max_nan(x0, -126.f);
+  x1 = max_nan(x1, -126.f);
   if constexpr (BOTH) {
-    x0 = fminf(x0, 126.f);
-    x1 = fminf(x1, 126.f);
+    x0 = min_nan(x0, 126.f);
+    x1 = min_nan(x1, 126.f);
   }
   x = f2_make(x0, x1);
   const F2 t = f2_add(x, f2_make(12582912.f, 12582912.f));

@@ -365,6 +365,23 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return d;
 }
 
+// Maxima and minima that NaN survives.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float d;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
 // Move registers between the warps of a CTA (whole-warp instructions).  The requests of all
 // warps must sum to at most the launch-time pool, or `inc` blocks for ever.
 template <int N> __device__ __forceinline__ void setmaxnreg_inc() {

@@ -76,7 +76,8 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
 
     With ``causal``, query i of n sees the keys up to ``i + n_k - n``: the last query sees all, a single one is a new token
     against the keys so far.  A query that sees no key gets zeros (and gives no gradient), as do rows outside every sequence.
-    Values there, and in key rows outside the sequence, may be anything; within a sequence q, k and v have to be finite.
+    Values there, and in key rows outside the sequence, may be anything; within a sequence q, k and v have to be finite (where a
+    score is NaN or plus infinity, the queries that see it get what is not finite either).
 
     16-bit types: P enters its products rounded to the type, as in the package's other attention; statistics and sums are
     fp32.  Gradients: q, k, v (k and v not with ``[B, 2]`` ranges)."""

@@ -121,3 +121,33 @@ def test_queries_without_a_key_may_hold_anything(bad, H, Hk, D, dtype):
     assert not out[blind].any() and not grads[0][blind].any()
     for name, g, w in zip(("o", "dq", "dk", "dv"), (out, *grads), oc.attention(q, k, v, _spans(nq, nk), True, d=d)):
         oc.check(name, g, w)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF, F32], ids=IDS.get)
+@pytest.mark.parametrize("H,Hk,D", [(2, 1, 64), (3, 1, 128), (2, 1, 20)])
+@pytest.mark.parametrize("bad", ["nan", "inf", "overflow"])
+def test_scores_that_are_not_finite_show(bad, H, Hk, D, dtype):
+    """One key whose scores are NaN or plus infinity, at every place of eight and in a tile that no mask cuts: the rows that see it
+    are not finite, whichever kernel and however the keys are cut up, nor are their gradients; the others are."""
+    import evoformer_triton_b200 as evo
+    if bad == "overflow" and dtype == HF:
+        return  # (65 504 squared is a number)
+    for nq, nk in ((400, 400), (300, 9000)):
+        q, k, v = _qkv(nq, nk, H, Hk, D, dtype)
+        q[..., 0] = q[..., 0].abs() + 0.5
+        off, koff = torch.tensor([0, nq], device=DEV), torch.tensor([0, nk], device=DEV)
+        for place in range(8):
+            at = nk - nq + 40 + place
+            k2 = k.clone()
+            k2[at, :, 0] = {"nan": float("nan"), "inf": float("inf"), "overflow": 3e38}[bad]
+            q2 = q * 20 if bad == "overflow" else q
+            leaves = [t.detach().requires_grad_() for t in (q2, k2, v)]
+            out = evo.packed_attention(*leaves, off, koff)
+            (dq,) = torch.autograd.grad(out, leaves[:1], torch.ones_like(out))
+            with torch.no_grad():
+                infer = evo.packed_attention(q2, k2, v, off, koff)
+                tokens = evo.packed_attention(q2[-3:], k2, v, torch.arange(4, device=DEV), torch.tensor([[0, nk], [at, at + 1], [0, at]], device=DEV))
+            for t in (out, infer):
+                assert torch.isfinite(t[:40 + place]).all() and not torch.isfinite(t[40 + place:]).any(), place
+            assert not torch.isfinite(dq[40 + place:]).any(), place
+            assert not torch.isfinite(tokens[:2]).any() and torch.isfinite(tokens[2]).all(), place
