@@ -15,6 +15,7 @@ int validate(const evoattn_packed_params* p, bool bwd) {
   if (p->key_form != EVOATTN_PACKED_KEY_OFFSETS && p->key_form != EVOATTN_PACKED_KEY_RANGES) return EVOATTN_ERR_DTYPE;
   if (p->key_form == EVOATTN_PACKED_KEY_RANGES && !p->key_offsets) return EVOATTN_ERR_NULL;
   if (!(p->scale - p->scale == 0.f)) return EVOATTN_ERR_SHAPE;  // (NaN or infinite)
+  if (p->o_rest && !p->lse) return EVOATTN_ERR_NULL;  // (only the kernels for training leave it)
   if (!bwd) return EVOATTN_OK;
   if (!p->lse || !p->d_o || !p->dk != !p->dv) return EVOATTN_ERR_NULL;
   if (p->dk && p->key_form != EVOATTN_PACKED_KEY_OFFSETS) return EVOATTN_ERR_UNSUPPORTED;

@@ -419,7 +419,7 @@ typedef struct evoattn_packed_params {
   void* o;                /* [Tq][H][D], dense.  Forward: out; backward: in */
   float* lse;             /* [H][Tq]: log2 of the sum of exp2(scale log2(e) q k), -inf for a row without a key.  Forward: out,
                              or null; backward: in */
-  void* o_rest;           /* [Tq][H][D], dense, or null: what rounding left of o, in the same type.  Forward: out; backward: in, for
+  void* o_rest;           /* [Tq][H][D], dense, or null: what rounding left of o, in the same type.  Forward: out, with lse only; backward: in, for
                              the row sums of dO * O, whose error from o's rounding is as large as that of dS's */
   int32_t* status;        /* optional device word, as in evoattn_fwd_params */
   const void* d_o;        /* backward */
