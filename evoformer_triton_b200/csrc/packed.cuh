@@ -17,6 +17,7 @@ struct PackedArgs {
   const void *d_o;     // backward
   void *dq, *dk, *dv;  // dense, as q, k, v
   float* delta;        // [H][lse_ld]: the row sums of dO * O
+  const int* overlap;  // backward on CUDA cores: whether queries, and keys, of sequences overlap (then gradients are zeros)
   long long sq[2], sk[2], sv[2], sdo[2];  // element strides of (row, head)
   const void *offsets, *key_offsets;
   int B, H, Hk, D, G;  // G = H / Hk
@@ -95,9 +96,9 @@ __device__ __forceinline__ Place locate(int B, int t, int tile, int* sm, F&& cou
 }
 
 // Zeros in the rows of a dense tensor [rows][row_bytes] that belong to no sequence, those before the first and behind
-// the last, shared out over the blocks.
-__device__ __forceinline__ void zero_outside(const void* offsets, int wide, int B, int rows, void* dst, long long row_bytes, long long block, long long blocks) {
-  const Span all = clamped(packed_offset(offsets, wide, 0), packed_offset(offsets, wide, B), rows);
+// the last (or in all of them), shared out over the blocks.
+__device__ __forceinline__ void zero_outside(const void* offsets, int wide, int B, int rows, void* dst, long long row_bytes, long long block, long long blocks, bool overlap = false) {
+  const Span all = overlap ? Span{0, 0} : clamped(packed_offset(offsets, wide, 0), packed_offset(offsets, wide, B), rows);
   const long long outside = rows - all.n;
   for (long long i = block; i < outside; i += blocks) {
     const long long r = i < all.begin ? i : i + all.n;

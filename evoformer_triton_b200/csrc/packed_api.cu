@@ -106,7 +106,7 @@ int evoattn_packed_fwd(const evoattn_packed_params* p, void* cuda_stream) {
 size_t evoattn_packed_bwd_workspace_bytes(const evoattn_packed_params* p) {
   if (validate(p, true)) return 0;
   const PackedArgs a = arguments(p);
-  return tensor_cores(p, a, true) ? sm100_packed_bwd_workspace_bytes(a) : (size_t)p->H * p->Tq * sizeof(float);
+  return tensor_cores(p, a, true) ? sm100_packed_bwd_workspace_bytes(a) : 256 + (size_t)p->H * p->Tq * sizeof(float);
 }
 
 int evoattn_packed_bwd(const evoattn_packed_params* p, void* cuda_stream) {
@@ -122,9 +122,11 @@ int evoattn_packed_bwd(const evoattn_packed_params* p, void* cuda_stream) {
   if (fast) {
     rc = launch_sm100_packed_bwd(p->dtype, a, p->workspace, st, &launches);
   } else {
-    a.delta = static_cast<float*>(p->workspace);
-    PackedPlan none{};
-    rc = launch_packed_prepare(p->dtype, a, none, false, 0, false, true, st, &launches);
+    PackedPlan plan{};
+    plan.counts = static_cast<int*>(p->workspace);
+    a.overlap = plan.counts + 6;
+    a.delta = reinterpret_cast<float*>(static_cast<unsigned char*>(p->workspace) + 256);
+    rc = launch_packed_prepare(p->dtype, a, plan, false, 0, false, true, st, &launches);
     if (!rc) rc = launch_packed_generic_bwd(p->dtype, a, st, &launches);
   }
   note_call(fast ? EVOATTN_PATH_TCGEN05 : EVOATTN_PATH_GENERIC, launches);

@@ -167,9 +167,9 @@ __device__ __forceinline__ Lift<T> lift_of(const uint32_t* words, int D) {
   return l;
 }
 
-// Rows of no sequence in a dense tensor of 16-bit values, by a warp.
-__device__ __forceinline__ void clear_outside(const void* offsets, int wide, int B, int rows, void* dst, int row16, int lane) {
-  const Span all = clamped(packed_offset(offsets, wide, 0), packed_offset(offsets, wide, B), rows);
+// Rows of no sequence in a dense tensor of 16-bit values (all of them where sequences overlap), by a warp.
+__device__ __forceinline__ void clear_outside(const void* offsets, int wide, int B, int rows, void* dst, int row16, int lane, bool overlap) {
+  const Span all = overlap ? Span{0, 0} : clamped(packed_offset(offsets, wide, 0), packed_offset(offsets, wide, B), rows);
 #pragma unroll 1
   for (int i = blockIdx.x; i < rows - all.n; i += gridDim.x) {
     uint4* p = static_cast<uint4*>(dst) + (long long)(i < all.begin ? i : i + all.n) * row16;
@@ -261,7 +261,8 @@ packed_dkv_sm100_kernel(const PackedArgs a, const PackedPlan plan, const FastDiv
   const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
   const bool failed = *abort_flag != 0;
   const Lift<T> lift = lift_of<T>(norm_words, a.D);
-  const int tiles = failed ? 0 : __ldcg(plan.counts + 1);
+  const bool overlap = __ldcg(plan.counts + 6) || __ldcg(plan.counts + 7);
+  const int tiles = failed || overlap ? 0 : __ldcg(plan.counts + 1);
   Schedule todo{sched, sched + 16, abort_s + 4, abort_s, plan.counts + 5, tiles * (int)heads.d};
 
   // The steps of a CTA, one after another over its items: head g of the group, query tile i, `left` of the item from here on.
@@ -423,9 +424,9 @@ packed_dkv_sm100_kernel(const PackedArgs a, const PackedPlan plan, const FastDiv
     } else {
       // =============================== dO: its end; rows of no sequence ===============================
       if (!failed) {
-        clear_outside(a.key_offsets, a.wide, a.B, a.Tk, a.dk, a.Hk * a.D / 8, lane);
-        clear_outside(a.key_offsets, a.wide, a.B, a.Tk, a.dv, a.Hk * a.D / 8, lane);
-        const int unseen = __ldcg(plan.counts + 3);
+        clear_outside(a.key_offsets, a.wide, a.B, a.Tk, a.dk, a.Hk * a.D / 8, lane, overlap);
+        clear_outside(a.key_offsets, a.wide, a.B, a.Tk, a.dv, a.Hk * a.D / 8, lane, overlap);
+        const int unseen = overlap ? 0 : __ldcg(plan.counts + 3);
         clear_tiles(plan.keys, tiles, unseen, a.dk, a.Hk * a.D / 8, lane);
         clear_tiles(plan.keys, tiles, unseen, a.dv, a.Hk * a.D / 8, lane);
       }
@@ -726,7 +727,7 @@ packed_dq_sm100_kernel(const PackedArgs a, const PackedPlan plan, const FastDiv 
       }
     } else {
       // =============================== K (warp 2) and V (warp 3): what lies behind the end; rows of no sequence ===============================
-      if (warp == 3 && !failed && a.dq) clear_outside(a.offsets, a.wide, a.B, a.Tq, a.dq, a.H * a.D / 8, lane);
+      if (warp == 3 && !failed && a.dq) clear_outside(a.offsets, a.wide, a.B, a.Tq, a.dq, a.H * a.D / 8, lane, __ldcg(plan.counts + 6) != 0);
 #pragma unroll 1
       for (int idx = todo.first(); !todo.over(idx); idx = todo.next()) {
         int h;
@@ -840,7 +841,7 @@ packed_dq_sm100_kernel(const PackedArgs a, const PackedPlan plan, const FastDiv 
     if (follows) {
       // The parts of dK and dV, in order: 8 columns of a row a thread, neighbours have neighbouring rows.
       grid_dependency_wait();
-      const int joins = failed ? 0 : __ldcg(plan.counts + 2);
+      const int joins = failed || __ldcg(plan.counts + 6) || __ldcg(plan.counts + 7) ? 0 : __ldcg(plan.counts + 2);
       constexpr int kPieces = 2 * DP / 8;  // of (dV, dK)
       const int at = (warp - 4) * 32 + lane;
 #pragma unroll 1

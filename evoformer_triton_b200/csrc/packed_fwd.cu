@@ -250,7 +250,7 @@ packed_fwd_sm100_kernel(const PackedArgs a, const PackedPlan plan, const FastDiv
       }
     } else if (warp == 2 && !failed) {
       // =============================== rows of no sequence ===============================
-      const Span all = clamped(packed_offset(a.offsets, a.wide, 0), packed_offset(a.offsets, a.wide, a.B), a.Tq);
+      const Span all = __ldcg(plan.counts + 6) ? Span{0, 0} : clamped(packed_offset(a.offsets, a.wide, 0), packed_offset(a.offsets, a.wide, a.B), a.Tq);
       const int row16 = a.H * a.D / 8;
 #pragma unroll 1
       for (int i = blockIdx.x; i < a.Tq - all.n; i += gridDim.x) {

@@ -141,8 +141,15 @@ __global__ void __launch_bounds__(kThreads) packed_generic_fwd_kernel(const Pack
   const int h = blockIdx.y, tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
   T* o = static_cast<T*>(a.o);
   if (h == 0) zero_outside(a.offsets, a.wide, a.B, a.Tq, a.o, (long long)a.H * a.D * sizeof(T), blockIdx.x, gridDim.x);
-  const Place at = locate(a.B, blockIdx.x, TILE, place, [&](int b) { return query_span(a, b).n; });
+  auto count = [&](int b) { return query_span(a, b).n; };
+  const Place at = locate(a.B, blockIdx.x, TILE, place, count);
   if (at.seq < 0) return;
+  // Offsets that do not ascend may make sequences that overlap, and more tiles than there are blocks: then the last one zeroes the
+  // head's rows, so that nothing comes back as memory was.
+  if (blockIdx.x + 1 == gridDim.x && locate(a.B, (int)gridDim.x, TILE, place, count).seq >= 0) {
+    for (long long i = threadIdx.x; i < (long long)a.Tq * a.D; i += kThreads) o[(i / a.D * a.H + h) * a.D + i % a.D] = from_float<T>(0.f);
+    return;
+  }
   const Span qs = query_span(a, at.seq), ks = key_span(a, at.seq);
   const int i0 = at.tile * TILE, rows = min(TILE, qs.n - i0), shift = ks.n - qs.n, hk = h / a.G;
   const int seen = keys_seen(a, qs.n, ks.n, i0, TILE);
@@ -251,8 +258,9 @@ __global__ void __launch_bounds__(kThreads) packed_generic_dq_kernel(const Packe
   float *lse = sS + TILE * C::LP, *delta = lse + TILE;
   __shared__ int place[34];
   const int h = blockIdx.y, tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  if (h == 0) zero_outside(a.offsets, a.wide, a.B, a.Tq, a.dq, (long long)a.H * a.D * sizeof(T), blockIdx.x, gridDim.x);
-  const Place at = locate(a.B, blockIdx.x, TILE, place, [&](int b) { return query_span(a, b).n; });
+  const bool overlap = __ldcg(a.overlap) != 0;
+  if (h == 0) zero_outside(a.offsets, a.wide, a.B, a.Tq, a.dq, (long long)a.H * a.D * sizeof(T), blockIdx.x, gridDim.x, overlap);
+  const Place at = overlap ? Place{-1, 0} : locate(a.B, blockIdx.x, TILE, place, [&](int b) { return query_span(a, b).n; });
   if (at.seq < 0) {
     if (follows) ptx::grid_dependency_wait();
     return;
@@ -315,10 +323,12 @@ __global__ void __launch_bounds__(kThreads) packed_generic_dkv_kernel(const Pack
   ptx::grid_launch_dependents();
   const int hk = blockIdx.y, tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
   const long long row_bytes = (long long)a.Hk * a.D * sizeof(T);
+  const bool overlap = __ldcg(a.overlap) || __ldcg(a.overlap + 1);
   if (hk == 0) {
-    zero_outside(a.key_offsets, a.wide, a.B, a.Tk, a.dk, row_bytes, blockIdx.x, gridDim.x);
-    zero_outside(a.key_offsets, a.wide, a.B, a.Tk, a.dv, row_bytes, blockIdx.x, gridDim.x);
+    zero_outside(a.key_offsets, a.wide, a.B, a.Tk, a.dk, row_bytes, blockIdx.x, gridDim.x, overlap);
+    zero_outside(a.key_offsets, a.wide, a.B, a.Tk, a.dv, row_bytes, blockIdx.x, gridDim.x, overlap);
   }
+  if (overlap) return;
   const Place at = locate(a.B, blockIdx.x, TILE, place, [&](int b) { return key_span(a, b).n; });
   if (at.seq < 0) return;
   const Span qs = query_span(a, at.seq), ks = key_span(a, at.seq);

@@ -15,7 +15,7 @@ struct Sums {
   int first[kClasses];
   int warps[kThreads / 32 + 1];
   long long steps;
-  long long tiles;
+  long long rows;
   int slots, joins, most;
 };
 
@@ -79,14 +79,14 @@ __device__ __forceinline__ void make_list(const PackedArgs& a, const PackedPlan&
   for (int i = threadIdx.x; i < kClasses; i += kThreads) s.first[i] = 0;
   if (queries)
     for (int i = threadIdx.x; i < plan.n_arrived; i += kThreads) plan.arrived[i] = 0;
-  if (threadIdx.x == 0) { s.steps = 0; s.slots = 0; s.joins = 0; s.tiles = 0; s.most = 0; }
+  if (threadIdx.x == 0) { s.steps = 0; s.slots = 0; s.joins = 0; s.rows = 0; s.most = 0; }
   __syncthreads();
   long long work = 0, n = 0;
   int most = 0;
   tiles.each(a, queries, unit, [&](const PackedTile& t) {
     work += t.steps;
     most = max(most, t.steps);
-    ++n;
+    n += t.rows;
   });
   most = __reduce_max_sync(0xffffffffu, most);
 #pragma unroll
@@ -96,12 +96,15 @@ __device__ __forceinline__ void make_list(const PackedArgs& a, const PackedPlan&
   }
   if ((threadIdx.x & 31) == 0 && n) {
     atomicAdd(reinterpret_cast<unsigned long long*>(&s.steps), (unsigned long long)work);
-    atomicAdd(reinterpret_cast<unsigned long long*>(&s.tiles), (unsigned long long)n);
+    atomicAdd(reinterpret_cast<unsigned long long*>(&s.rows), (unsigned long long)n);
     atomicMax(&s.most, most);
   }
   __syncthreads();
-  // (offsets that do not ascend may make sequences that overlap, and more tiles than there is room for: none are listed)
-  if (s.tiles > (queries ? plan.most_queries : plan.most_keys)) {
+  // (offsets that do not ascend may make sequences that overlap, and more tiles than there is room for: none are listed.  Where rows
+  // are no more than there are, tiles are none but a sequence's last more than rows / unit)
+  const bool overlap = s.rows > (queries ? a.Tq : a.Tk);
+  if (threadIdx.x == 0) plan.counts[queries ? 6 : 7] = overlap;
+  if (overlap) {
     if (threadIdx.x == 0) {
       plan.counts[queries ? 0 : 1] = plan.counts[queries ? 4 : 5] = 0;
       if (!queries) plan.counts[2] = plan.counts[3] = 0;
@@ -159,6 +162,25 @@ __device__ __forceinline__ void make_list(const PackedArgs& a, const PackedPlan&
   });
   __syncthreads();
   if (threadIdx.x == 0 && !queries) plan.counts[2] = s.joins;
+}
+
+// Without lists (the kernels on CUDA cores look their tiles up): whether sequences overlap, by a block.
+__device__ __forceinline__ void find_overlap(const PackedArgs& a, const PackedPlan& plan) {
+  __shared__ unsigned long long rows[2];
+  if (threadIdx.x < 2) rows[threadIdx.x] = 0;
+  __syncthreads();
+  long long q = 0, k = 0;
+  for (int b = threadIdx.x; b < a.B; b += kThreads) {
+    q += query_span(a, b).n;
+    k += key_span(a, b).n;
+  }
+  atomicAdd(&rows[0], (unsigned long long)q);
+  atomicAdd(&rows[1], (unsigned long long)k);
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    plan.counts[6] = (long long)rows[0] > a.Tq;
+    plan.counts[7] = (long long)rows[1] > a.Tk;
+  }
 }
 
 // delta: VEC values of 16 bytes at a time, `lanes` lanes a row (a power of two), two rows of a lane on their way.  NORMS: the largest
@@ -292,15 +314,17 @@ __device__ __forceinline__ void row_sums(const PackedArgs& a, const PackedPlan& 
   }
 }
 
-// Block 0 makes the list of queries, block 1 (or 0) that of keys, the others the row sums.
+// Block 0 makes the list of queries, block 1 (or 0) that of keys, the others the row sums; without lists block 0 looks for overlaps.
 template <class T, bool VEC, bool NORMS>
 __global__ void __launch_bounds__(kThreads, 2) packed_prepare_kernel(const PackedArgs a, const PackedPlan plan, const int queries, const int unit, const int keys,
                                                                   const int sms, const PackedCut qcut, const PackedCut kcut, const int lanes, const FastDiv heads) {
   __shared__ Sums s;
   ptx::grid_dependency_wait();
   ptx::grid_launch_dependents();
-  const int lists = queries + keys;
-  if ((int)blockIdx.x < lists) {
+  const int lists = max(queries + keys, 1);
+  if (queries + keys == 0 && blockIdx.x == 0) {
+    find_overlap(a, plan);
+  } else if ((int)blockIdx.x < lists) {
     const bool q = queries && blockIdx.x == 0;
     make_list(a, plan, q, q ? unit : kTileRows, sms, q ? qcut : kcut, s);
   } else {
@@ -324,7 +348,7 @@ int launch_packed_prepare(int dtype, const PackedArgs& a, PackedPlan& plan, bool
     while (lanes < 32 && lanes * (vec ? V : 1) < a.D) lanes *= 2;
     const long long each = kThreads / lanes * 2, most = (long long)sms * kSumBlocks;
     const long long rows = ((long long)a.Tq * a.H + each - 1) / each + (norms ? ((long long)a.Tk * a.Hk + each - 1) / each : 0);
-    const int sums = delta ? (int)(rows < most ? rows : most) : 0, blocks = (queries ? 1 : 0) + (keys ? 1 : 0) + sums;
+    const int sums = delta ? (int)(rows < most ? rows : most) : 0, blocks = (queries && keys ? 2 : 1) + sums;
     plan.n_norms = norms ? sums : 0;
     auto kern = vec ? packed_prepare_kernel<T, true, false> : packed_prepare_kernel<T, false, false>;
     if constexpr (std::is_same<T, __half>::value)

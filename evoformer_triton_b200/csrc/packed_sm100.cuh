@@ -31,9 +31,9 @@ struct PackedJoin {
 // Where lists lie in a workspace: 256 bytes with their lengths, the tiles, the key tiles whose parts are to be joined and the parts.
 struct PackedPlan {
   int* counts;               // [0] query units, [1] key tiles and parts that have steps, [2] joins, [3] key tiles that no query sees, behind those;
-                             // [4], [5] items that have been taken of the two lists
+                             // [4], [5] items that have been taken of the two lists; [6], [7] whether queries, and keys, of sequences overlap:
+                             // then nothing is listed, and results are zeros
   PackedTile *queries, *keys;
-  int most_queries, most_keys;  // tiles that the lists have room for before any is cut: those of sequences that do not overlap
   PackedJoin* joins;
   float* sums;               // key tiles: [slot][Hk][dV, dK][DP / 4][128 rows][4]; query units: [slot][units of heads][2 tiles][DP / 4][128][4]
   float4* ml;                // [slot][units of heads][2 tiles][128 rows]: reference, sum of P as rounded, and as it is
@@ -81,8 +81,6 @@ inline PackedPlan place_plan(const PackedArgs& a, int unit, void* ws, const Plan
   unsigned char* p = static_cast<unsigned char*>(ws);
   PackedPlan plan{};
   plan.counts = reinterpret_cast<int*>(p);
-  plan.most_queries = (int)query_units(a, unit);
-  plan.most_keys = (int)key_tiles(a);
   plan.queries = reinterpret_cast<PackedTile*>(p += 256);
   plan.keys = reinterpret_cast<PackedTile*>(p += n.queries);
   plan.joins = reinterpret_cast<PackedJoin*>(p += n.keys);

@@ -395,7 +395,8 @@ int evoattn_rotary(const evoattn_rotary_params* p, void* cuda_stream);
  * h / (H / Hk).  A query that sees no key gets 0; so does every row of o, dq, dk and dv that belongs to no sequence.
  *
  * offsets (on the device) are read by the kernels: the queries of sequence b are rows offsets[b] to offsets[b+1].  Whatever
- * they hold, no row outside the tensors is touched; they have to ascend for the rows to be right.  A key range [B][2] (begin,
+ * they hold, no row outside the tensors is touched; they have to ascend for the rows to be right (of sequences that
+ * overlap, every row of o, dq, dk and dv is written, as zeros or as that of one of them).  A key range [B][2] (begin,
  * end) lets the keys of a sequence lie anywhere, as in the slots of a cache; it has no backward. */
 enum { EVOATTN_PACKED_KEY_OFFSETS = 0, EVOATTN_PACKED_KEY_RANGES = 1 };
 #define EVOATTN_PACKED_MAX_D 256
