@@ -77,8 +77,12 @@ inline bool wants_grad(std::initializer_list<const Maybe*> inputs) {
   return false;
 }
 inline const void* address(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
-inline Tensor dense(const Maybe& t) { return t ? t->contiguous() : Tensor(); }
-inline Tensor last_axis_dense(const Tensor& t) { return t.dim() == 0 || t.size(-1) <= 1 || t.stride(-1) == 1 ? t : t.contiguous(); }
+// Memory holds the values of a tensor but where it is a view that has yet to be negated, as the imaginary part of a conjugate is.
+inline Tensor dense(const Maybe& t) { return t ? t->resolve_neg().contiguous() : Tensor(); }
+inline Tensor last_axis_dense(const Tensor& t) {
+  const Tensor r = t.resolve_neg();
+  return r.dim() == 0 || r.size(-1) <= 1 || r.stride(-1) == 1 ? r : r.contiguous();
+}
 
 // The axes before the last one as three (or fewer) with strides; false where that takes more.
 inline bool three_axes(const Tensor& t, int64_t* n, int64_t* st) {

@@ -118,7 +118,7 @@ py::object rotary_embedding(const Tensor& q, const Maybe& k, const Tensor& posit
   if (frequencies.dim() != 1 || frequencies.size(0) < 1 || 2 * frequencies.size(0) > D) value_error("frequencies must have the shape [n] with 1 <= n <= D / 2");
   if (at::GradMode::is_enabled() && frequencies.requires_grad()) value_error("rotary_embedding has no gradient for the frequencies");
   if (!std::isfinite(amplitude) || !std::isfinite((float)amplitude)) value_error("amplitude must be a finite number");
-  const Tensor f = frequencies.contiguous();
+  const Tensor f = dense(frequencies);
   variable_list out;
   if (wants_grad({&qm, &k})) {
     out = Rotary::apply(q, k, positions, f, layout, amplitude);
