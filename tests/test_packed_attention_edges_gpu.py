@@ -171,3 +171,37 @@ def test_offsets_that_overlap_leave_no_memory_as_it_was(bad, dtype, D):
             assert torch.isfinite(t).all()
             assert not t.any() or D == 20 or dtype == F32
     _check(*_qkv(200, 200, 4, 2, D, dtype), [60, 140])
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_thousands_of_tokens_between_rows_of_no_sequence(D):
+    """More sequences than a launch of the kernel for few rows takes, and rows of none around them: every value, on each side of every
+    border between launches."""
+    g = torch.Generator().manual_seed(3)
+    nk = torch.randint(0, 70, (5000,), generator=g).tolist()
+    nq = [int(i % 7 != 3) for i in range(5000)]
+    out = _check(*_qkv(sum(nq) + 9, sum(nk) + 9, 2, 1, D, BF), nq, nk, before=4, train=False)
+    assert not out[:4].any() and not out[-5:].any()
+    nq[4990], nk[4990] = 40, 3000  # one for the other kernel
+    out = _check(*_qkv(sum(nq) + 9, sum(nk) + 9, 2, 1, D, BF), nq, nk, before=4, train=False)
+    assert not out[:4].any() and not out[-5:].any()
+
+
+@pytest.mark.parametrize("causal", [True, False], ids=["causal", "both"])
+def test_gradients_against_differences_of_the_fourth_order(causal):
+    """Slopes along a direction from four points, h and 2 h to either side.  What is left out is h^4 / 30 of a fifth derivative: those of a
+    softmax along scores that move by up to 3 are within 10^4 of the slope's terms, 10^-5 of them all told.  Results are off by
+    some 2^-21 of the largest, independently; of the four, weighted 8, 8, 1 and 1 over 12 h, that is 95 times as much, four deviations."""
+    import evoformer_triton_b200 as evo
+    off, h = torch.tensor([0, 40, 97], device=DEV), 1e-2
+    x = [t.requires_grad_() for t in _qkv(97, 97, 4, 2, 16, F32)]
+    d = _draw((97, 4, 16), F32, 5)
+    out = evo.packed_attention(*x, off, causal=causal)
+    grads = torch.autograd.grad(out, x, d)
+    for n, g in enumerate(grads):
+        step = _draw(x[n].shape, F32, 6 + n)
+        with torch.no_grad():
+            at = lambda h: (evo.packed_attention(*(t + h * step if m == n else t for m, t in enumerate(x)), off, causal=causal).double() * d).sum()  # noqa: E731
+            slope = (8 * (at(h) - at(-h)) - (at(2 * h) - at(-2 * h))) / (12 * h)
+        tol = 4 * 95 * 2.0 ** -21 * float(d.norm()) * float(out.detach().abs().max()) + 1e-5 * float((g.double() * step).abs().sum())
+        assert abs(float(slope - (g.double() * step).sum())) < tol
