@@ -127,7 +127,7 @@ __device__ __forceinline__ void scores_gradient(const uint32_t (&d)[32], const F
 // it, although the sums that it enters are ordinary numbers, and that of a large dO v would overflow.  So dS is formed times 2^e, which
 // its products carry to the end.  |dS_ij| <= |dO_i| (|V_j| + |o_i|) <= 2 sqrt(D) max |dO_id| max |V_j|; e takes that bound to 2^15 at most.  It is
 // in the exponent of P, for nothing; P itself enters dV times 2^14.  One power for a call, from maxima that the row sums leave: forward and
-// backward of [3088 in 5], 12 heads of 96 over 2, 117 -> 121 us, [8192] of 16 heads of 128 over 4, 1 117 -> 1 145.  bf16 has the exponents of fp32.
+// backward of [3088 in 5], 12 heads of 96 over 2, 117 -> 119 us, [8192] of 16 heads of 128 over 4, 1 117 -> 1 120.  bf16 has the exponents of fp32.
 template <class T>
 struct Lift {
   static constexpr bool kAny = std::is_same<T, __half>::value;

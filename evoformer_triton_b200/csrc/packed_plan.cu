@@ -187,7 +187,7 @@ __device__ __forceinline__ void find_overlap(const PackedArgs& a, const PackedPl
 // value of dO among queries that see a key and |V_j|^2 of keys of a sequence as well (those that are not finite have no say: theirs
 // are the only rows that they reach).
 template <class T, bool VEC, bool NORMS>
-__device__ __forceinline__ void row_sums(const PackedArgs& a, const PackedPlan& plan, long long block, long long blocks, int lanes, const FastDiv& heads) {
+__device__ __forceinline__ void row_sums(const PackedArgs& a, const PackedPlan& plan, long long block, long long blocks, int lanes, const FastDiv& heads, const FastDiv& key_heads) {
   const int team = threadIdx.x / lanes, lane = threadIdx.x % lanes, teams = kThreads / lanes;
   const int ahead = (threadIdx.x & 31) / lanes;  // teams of the warp before this one
   const long long items = (long long)a.Tq * a.H;
@@ -211,7 +211,8 @@ __device__ __forceinline__ void row_sums(const PackedArgs& a, const PackedPlan& 
     float s[U] = {};
     __half2 top[U] = {};
     long long to[U];
-    bool counts[U] = {};
+    float lse[U] = {};
+    bool in[U] = {};
     const T* d[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -220,7 +221,10 @@ __device__ __forceinline__ void row_sums(const PackedArgs& a, const PackedPlan& 
       const int h = i < items ? (int)(i - t * a.H) : 0;
       d[u] = d_o + t * a.sdo[0] + (long long)h * a.sdo[1];
       to[u] = (long long)h * a.lse_ld + t;
-      if constexpr (NORMS) counts[u] = i < items && t >= queries.begin && t - queries.begin < queries.n && a.lse[to[u]] != -INFINITY;
+      if constexpr (NORMS) {
+        lse[u] = a.lse[to[u]];  // (compared when the rows are there: a branch around it would keep them waiting)
+        in[u] = i < items && t >= queries.begin && t - queries.begin < queries.n;
+      }
     }
     for (int x = lane * V; x < a.D; x += lanes * V) {
       if constexpr (VEC) {
@@ -263,7 +267,7 @@ __device__ __forceinline__ void row_sums(const PackedArgs& a, const PackedPlan& 
       for (int m = lanes / 2; m > 0; m >>= 1) s[u] += __shfl_xor_sync(0xffffffffu, s[u], m);
       if (lane == 0 && i0 + (long long)u * teams < items) a.delta[to[u]] = s[u];
       if constexpr (NORMS)
-        if (counts[u]) most_do = __hmax2(most_do, top[u]);
+        if (in[u] && lse[u] != -INFINITY) most_do = __hmax2(most_do, top[u]);
     }
   }
   if constexpr (NORMS) {
@@ -275,7 +279,8 @@ __device__ __forceinline__ void row_sums(const PackedArgs& a, const PackedPlan& 
       const T* from[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const long long i = min(i0 + (long long)u * teams, key_items - 1), t = i / a.Hk;
+        const long long i = min(i0 + (long long)u * teams, key_items - 1);
+        const long long t = key_items <= 0x7fffffffLL ? (long long)key_heads.div((uint32_t)i) : i / a.Hk;
         from[u] = v + (keys.begin + t) * a.sv[0] + (i - t * a.Hk) * a.sv[1];
       }
       for (int x = lane * V; x < a.D; x += lanes * V) {
@@ -317,7 +322,7 @@ __device__ __forceinline__ void row_sums(const PackedArgs& a, const PackedPlan& 
 // Block 0 makes the list of queries, block 1 (or 0) that of keys, the others the row sums; without lists block 0 looks for overlaps.
 template <class T, bool VEC, bool NORMS>
 __global__ void __launch_bounds__(kThreads, 2) packed_prepare_kernel(const PackedArgs a, const PackedPlan plan, const int queries, const int unit, const int keys,
-                                                                  const int sms, const PackedCut qcut, const PackedCut kcut, const int lanes, const FastDiv heads) {
+                                                                  const int sms, const PackedCut qcut, const PackedCut kcut, const int lanes, const FastDiv heads, const FastDiv key_heads) {
   __shared__ Sums s;
   ptx::grid_dependency_wait();
   ptx::grid_launch_dependents();
@@ -328,7 +333,7 @@ __global__ void __launch_bounds__(kThreads, 2) packed_prepare_kernel(const Packe
     const bool q = queries && blockIdx.x == 0;
     make_list(a, plan, q, q ? unit : kTileRows, sms, q ? qcut : kcut, s);
   } else {
-    row_sums<T, VEC, NORMS>(a, plan, blockIdx.x - lists, gridDim.x - lists, lanes, heads);
+    row_sums<T, VEC, NORMS>(a, plan, blockIdx.x - lists, gridDim.x - lists, lanes, heads, key_heads);
   }
 }
 
@@ -346,7 +351,9 @@ int launch_packed_prepare(int dtype, const PackedArgs& a, PackedPlan& plan, bool
     if (norms) vec = vec && (reinterpret_cast<uintptr_t>(a.v) & 15) == 0 && a.sv[0] % V == 0 && a.sv[1] % V == 0;
     int lanes = 1;
     while (lanes < 32 && lanes * (vec ? V : 1) < a.D) lanes *= 2;
-    const long long each = kThreads / lanes * 2, most = (long long)sms * kSumBlocks;
+    // (with norms as many as are resident beside the lists' two: a block has three waits of its own then, 33 us with eight an SM and 27
+    // so for [8192], 16 heads of 128)
+    const long long each = kThreads / lanes * 2, most = norms ? 2LL * sms - 2 : (long long)sms * kSumBlocks;
     const long long rows = ((long long)a.Tq * a.H + each - 1) / each + (norms ? ((long long)a.Tk * a.Hk + each - 1) / each : 0);
     const int sums = delta ? (int)(rows < most ? rows : most) : 0, blocks = (queries && keys ? 2 : 1) + sums;
     plan.n_norms = norms ? sums : 0;
@@ -354,7 +361,7 @@ int launch_packed_prepare(int dtype, const PackedArgs& a, PackedPlan& plan, bool
     if constexpr (std::is_same<T, __half>::value)
       if (norms) kern = vec ? packed_prepare_kernel<T, true, true> : packed_prepare_kernel<T, false, true>;
     launch_dependent(kern, dim3((unsigned)blocks), kThreads, 0, st, a, plan, (int)queries, unit, (int)keys,
-                     sms, qcut, key_cut(a), lanes, FastDiv((uint32_t)a.H));
+                     sms, qcut, key_cut(a), lanes, FastDiv((uint32_t)a.H), FastDiv((uint32_t)a.Hk));
     *launches += 1;
     return cudaGetLastError() == cudaSuccess ? EVOATTN_OK : EVOATTN_ERR_CUDA;
   });

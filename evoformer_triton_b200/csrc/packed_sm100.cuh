@@ -75,7 +75,7 @@ inline PlanBytes plan_bytes(const PackedArgs& a, bool queries, int unit, bool ke
   const size_t tile = (size_t)kTileRows * (a.D <= 64 ? 64 : 128) * sizeof(float), tiles = (size_t)qs * qcut.heads * 2;
   return PlanBytes{queries ? round256((query_units(a, unit) + qs) * sizeof(PackedTile)) : 0, keys ? round256((key_tiles(a) + ks) * sizeof(PackedTile)) : 0,
                    round256(ks * sizeof(PackedJoin)), round256(tile * (ks * a.Hk * 2 + tiles)), round256(tiles * kTileRows * sizeof(float4)), round256(tiles * sizeof(int)),
-                   keys ? round256((size_t)sms * kSumBlocks * sizeof(float2)) : 0};
+                   keys ? round256((size_t)sms * 2 * sizeof(float2)) : 0};
 }
 inline PackedPlan place_plan(const PackedArgs& a, int unit, void* ws, const PlanBytes& n) {
   unsigned char* p = static_cast<unsigned char*>(ws);
