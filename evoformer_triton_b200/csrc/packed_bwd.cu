@@ -125,9 +125,10 @@ __device__ __forceinline__ void scores_gradient(const uint32_t (&d)[32], const F
 
 // fp16 ends at 2^16 and has steps of 2^-24 below 2^-14: dS = P (dP - delta) of a long row or a small dO would lose its bits, or all of
 // it, although the sums that it enters are ordinary numbers, and that of a large dO v would overflow.  So dS is formed times 2^e, which
-// its products carry to the end.  |dS_ij| <= |dO_i| (|V_j| + |o_i|) <= 2 sqrt(D) max |dO_id| max |V_j|; e takes that bound to 2^15 at most.  It is
-// in the exponent of P, for nothing; P itself enters dV times 2^14.  One power for a call, from maxima that the row sums leave: forward and
-// backward of [3088 in 5], 12 heads of 96 over 2, 117 -> 119 us, [8192] of 16 heads of 128 over 4, 1 117 -> 1 120.  bf16 has the exponents of fp32.
+// its products carry to the end.  dS_ij = P_ij sum_k P_ik dO_i (V_j - V_k) is P (1 - P) 2 |dO| |V| at most, half of the largest |dO| times
+// the largest |V|; e takes that to 2^15.5 at most (what is left is for the roundings of P, O and delta).  It is in the exponent of P, for
+// nothing; P itself enters dV times 2^14.  One power for a call, from maxima that the row sums leave: forward and backward of
+// [3088 in 5], 12 heads of 96 over 2, 117 -> 120 us, [8192] of 16 heads of 128 over 4, 1 117 -> 1 130.  bf16 has the exponents of fp32.
 template <class T>
 struct Lift {
   static constexpr bool kAny = std::is_same<T, __half>::value;
@@ -153,13 +154,12 @@ __device__ __forceinline__ void bring_norms(const PackedPlan& plan, uint32_t* wo
   }
 }
 template <class T>
-__device__ __forceinline__ Lift<T> lift_of(const uint32_t* words, int D) {
+__device__ __forceinline__ Lift<T> lift_of(const uint32_t* words) {
   Lift<T> l;
   if constexpr (Lift<T>::kAny) {
-    const float x = __uint_as_float(words[0]);
-    const uint32_t b = __float_as_uint(x * x * __uint_as_float(words[1]) * (float)D);  // below 2^(k + 1)
+    const uint32_t b = __float_as_uint(__uint_as_float(words[0]) * __uint_as_float(words[1]));  // |dO|^2 |V|^2 < 2^(k + 1)
     const int k = (int)(b >> 23) - 127;
-    const int e = b == 0 ? 0 : 14 - ((k + 2) >> 1);  // (its root below 2^ceil((k + 1) / 2))
+    const int e = b == 0 ? 0 : (32 - k) >> 1;  // (a quarter of 2^(k + 1) 4^e is 2^31 at most)
     l.e = (float)e;
     l.p = exp2_whole(14 - e);
     l.back = exp2_whole(-e);
@@ -260,7 +260,7 @@ packed_dkv_sm100_kernel(const PackedArgs a, const PackedPlan plan, const FastDiv
   tc_fence_after();
   const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
   const bool failed = *abort_flag != 0;
-  const Lift<T> lift = lift_of<T>(norm_words, a.D);
+  const Lift<T> lift = lift_of<T>(norm_words);
   const bool overlap = __ldcg(plan.counts + 6) || __ldcg(plan.counts + 7);
   const int tiles = failed || overlap ? 0 : __ldcg(plan.counts + 1);
   Schedule todo{sched, sched + 16, abort_s + 4, abort_s, plan.counts + 5, tiles * (int)heads.d};
@@ -622,7 +622,7 @@ packed_dq_sm100_kernel(const PackedArgs a, const PackedPlan plan, const FastDiv 
   tc_fence_after();
   const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
   const bool failed = *abort_flag != 0;
-  const Lift<T> lift = lift_of<T>(norm_words, a.D);
+  const Lift<T> lift = lift_of<T>(norm_words);
   Schedule todo{sched, sched + 16, abort_s + 4, abort_s, plan.counts + 4, failed || !a.dq ? 0 : __ldcg(plan.counts) * (int)heads.d};
   auto item = [&](int idx, int& h) {
     const int tile = (int)heads.div((uint32_t)idx);

@@ -184,8 +184,8 @@ __device__ __forceinline__ void find_overlap(const PackedArgs& a, const PackedPl
 }
 
 // delta: VEC values of 16 bytes at a time, `lanes` lanes a row (a power of two), two rows of a lane on their way.  NORMS: the largest
-// value of dO among queries that see a key and |V_j|^2 of keys of a sequence as well (those that are not finite have no say: theirs
-// are the only rows that they reach).
+// |dO_i|^2 of queries that see a key and |V_j|^2 of keys of a sequence as well (those that are not finite have no say: theirs are the
+// only rows that they reach).
 template <class T, bool VEC, bool NORMS>
 __device__ __forceinline__ void row_sums(const PackedArgs& a, const PackedPlan& plan, long long block, long long blocks, int lanes, const FastDiv& heads, const FastDiv& key_heads) {
   const int team = threadIdx.x / lanes, lane = threadIdx.x % lanes, teams = kThreads / lanes;
@@ -197,19 +197,12 @@ __device__ __forceinline__ void row_sums(const PackedArgs& a, const PackedPlan& 
   constexpr int V = VEC ? kPer16<T> : 1, U = 2;
   const Span queries = NORMS ? clamped(packed_offset(a.offsets, a.wide, 0), packed_offset(a.offsets, a.wide, a.B), a.Tq) : Span{0, 0};
   const Span keys = NORMS ? clamped(packed_offset(a.key_offsets, a.wide, 0), packed_offset(a.key_offsets, a.wide, a.B), a.Tk) : Span{0, 0};
-  __half2 most_do{};
-  float most_v = 0.f;
-  // (|x|, and NaN, which a maximum passes over, for what is not finite)
-  auto finite = [](uint32_t w) {
-    const __half2 x = __habs2(*reinterpret_cast<const __half2*>(&w));
-    return __hfma2(x, __half2{}, x);
-  };
+  float most_do = 0.f, most_v = 0.f;
   auto larger = [](float a, float b) { return b > a && b < INFINITY ? b : a; };
   // (the teams of a warp meet in shuffles: as long as the first of them has a row, all go on, the others with a row that
   // is there and nothing to store)
   for (long long i0 = block * teams * U + team; i0 - ahead < items; i0 += blocks * teams * U) {
-    float s[U] = {};
-    __half2 top[U] = {};
+    float s[U] = {}, sq[U] = {};
     long long to[U];
     float lse[U] = {};
     bool in[U] = {};
@@ -247,9 +240,8 @@ __device__ __forceinline__ void row_sums(const PackedArgs& a, const PackedPlan& 
 #pragma unroll
           for (int e = 0; e < V; ++e) s[u] = fmaf(f[e], g[e], s[u]);
           if constexpr (NORMS) {
-            const uint32_t words[4] = {z[u].x, z[u].y, z[u].z, z[u].w};
 #pragma unroll
-            for (int e = 0; e < 4; ++e) top[u] = __hmax2(top[u], finite(words[e]));
+            for (int e = 0; e < V; ++e) sq[u] = fmaf(g[e], g[e], sq[u]);
           }
         }
       } else {
@@ -258,7 +250,7 @@ __device__ __forceinline__ void row_sums(const PackedArgs& a, const PackedPlan& 
           const long long i = min(i0 + (long long)u * teams, items - 1);
           const float g = to_float(d[u][x]);
           s[u] = fmaf(to_float(o[i * a.D + x]) + (rest ? to_float(rest[i * a.D + x]) : 0.f), g, s[u]);
-          if constexpr (NORMS) top[u] = __hmax2(top[u], finite(__half_as_ushort(d[u][x])));
+          if constexpr (NORMS) sq[u] = fmaf(g, g, sq[u]);
         }
       }
     }
@@ -266,8 +258,10 @@ __device__ __forceinline__ void row_sums(const PackedArgs& a, const PackedPlan& 
     for (int u = 0; u < U; ++u) {
       for (int m = lanes / 2; m > 0; m >>= 1) s[u] += __shfl_xor_sync(0xffffffffu, s[u], m);
       if (lane == 0 && i0 + (long long)u * teams < items) a.delta[to[u]] = s[u];
-      if constexpr (NORMS)
-        if (in[u] && lse[u] != -INFINITY) most_do = __hmax2(most_do, top[u]);
+      if constexpr (NORMS) {
+        for (int m = lanes / 2; m > 0; m >>= 1) sq[u] += __shfl_xor_sync(0xffffffffu, sq[u], m);
+        if (in[u] && lse[u] != -INFINITY) most_do = larger(most_do, sq[u]);
+      }
     }
   }
   if constexpr (NORMS) {
@@ -307,8 +301,7 @@ __device__ __forceinline__ void row_sums(const PackedArgs& a, const PackedPlan& 
       }
     }
     __shared__ uint32_t both[2][kThreads / 32];
-    const float of_do = fmaxf(__low2float(most_do), __high2float(most_do));
-    const uint32_t m0 = __reduce_max_sync(0xffffffffu, __float_as_uint(of_do)), m1 = __reduce_max_sync(0xffffffffu, __float_as_uint(most_v));
+    const uint32_t m0 = __reduce_max_sync(0xffffffffu, __float_as_uint(most_do)), m1 = __reduce_max_sync(0xffffffffu, __float_as_uint(most_v));
     if ((threadIdx.x & 31) == 0) { both[0][threadIdx.x >> 5] = m0; both[1][threadIdx.x >> 5] = m1; }
     __syncthreads();
     if (threadIdx.x < 32) {

@@ -38,7 +38,7 @@ struct PackedPlan {
   float* sums;               // key tiles: [slot][Hk][dV, dK][DP / 4][128 rows][4]; query units: [slot][units of heads][2 tiles][DP / 4][128][4]
   float4* ml;                // [slot][units of heads][2 tiles][128 rows]: reference, sum of P as rounded, and as it is
   int *arrived, n_arrived;   // [slot][units of heads][2 tiles]: parts that are through, of the tile whose first part has that slot
-  float2* norms;             // fp16 backward: the largest value of dO and |V_j|^2 that a block of the row sums has met
+  float2* norms;             // fp16 backward: the largest |dO_i|^2 and |V_j|^2 that a block of the row sums has met
   int n_norms;
 };
 constexpr int kSumBlocks = 8;  // of the row sums an SM, at most

@@ -205,3 +205,29 @@ def test_gradients_against_differences_of_the_fourth_order(causal):
             slope = (8 * (at(h) - at(-h)) - (at(2 * h) - at(-2 * h))) / (12 * h)
         tol = 4 * 95 * 2.0 ** -21 * float(d.norm()) * float(out.detach().abs().max()) + 1e-5 * float((g.double() * step).abs().sum())
         assert abs(float(slope - (g.double() * step).sum())) < tol
+
+
+@pytest.mark.parametrize("size", [2.0 ** -20, 1.0, 180.0, 16000.0])
+@pytest.mark.parametrize("D", [64, 128])
+def test_fp16_gradients_of_the_largest_scores_gradient(D, size):
+    """Two keys of equal scores and opposite values, and a gradient along them: dS is half of |dO| |V|, as large as it can be.  The sums are
+    short, so dQ is dS times the keys' difference but for a rounding each of dS and dQ, and P and its sum: two steps."""
+    import evoformer_triton_b200 as evo
+    T = 130
+    u = torch.ones(D, device=DEV)
+    u[::2] = -1
+    k = torch.zeros(2 * T, 1, D, device=DEV)
+    k[::2, :, 0], k[1::2, :, 0] = 2.0 ** -12, -(2.0 ** -12)
+    v = torch.stack([u, -u]).repeat(T, 1)[:, None] * 4
+    q = torch.zeros(T, 1, D, device=DEV)  # (scores: zero)
+    d = (u * size).expand(T, 1, D)
+    leaves = [t.to(HF).requires_grad_() for t in (q, k, v)]
+    off = torch.arange(T + 1, device=DEV)
+    out = evo.packed_attention(*leaves, off, off * 2, causal=False, scale=1.0)
+    dq, dk, dv = torch.autograd.grad(out, leaves, d.to(HF))
+    ds = 0.25 * 2 * 4 * D * float(d.to(HF).abs()[0, 0, 0])  # P (1 - P) dO (V - V')
+    want = torch.zeros(T, 1, D, device=DEV, dtype=torch.float64)
+    want[..., 0] = ds * 2 * 2.0 ** -12
+    oc.check("dq", dq, (want, 2 * torch.finfo(HF).eps * want + oc.rounding(HF, want)))
+    assert not dk.any()
+    oc.check("dv", dv, (d.to(HF).double().repeat_interleave(2, 0) / 2, oc.rounding(HF, d.to(HF).double().repeat_interleave(2, 0))))
