@@ -11,7 +11,7 @@
 // group's heads costs nothing.
 //
 // Both: persistent CTAs of 12 warps.  Warp 0 loads tiles by TMA, warp 1 issues the MMAs, warps 2 and 3 see each tile
-// land before the MMAs do and clear what lies behind the end of the sequence in it (0 times infinity is not 0), warps 4
+// land before the MMAs do and clear what lies behind the end of the sequence in it, and queries that see no key (0 times infinity is not 0), warps 4
 // to 11 compute: a thread has one row of the 128 x 128 scores and half of its columns, P in registers from S to dS.
 //
 // Items are handed out as in the forward.  A key tile of long sequences or many heads is cut into parts, whose fp32 sums

@@ -13,10 +13,10 @@
 // one each and all four read the same keys, which lie side by side in memory; else two or four warps share the keys of a
 // head and meet at the end of a unit.  Products of 16 rows are warp-level MMAs: tcgen05 would work on 128.  P enters its
 // product in two pieces of the type, itself rounded and what that left: a second MMA a tile, which costs nothing beside the
-// loads (86.4 us for the case below, 87.7 with one piece), and results are off by their own rounding only (bf16, of the norm: 0.0016
+// loads (86.4 us for the case below, 87.7 with one, the same minute), and results are off by their own rounding only (bf16, of the norm: 0.0016
 // for one token, 0.0022 with one piece).
 //
-// 32 sequences of 1 to 8 191 keys, 32 heads of 128 over 8: 89 us, the 465 MB at 5.2 TB/s (118 with units weighed by
+// 32 sequences of 1 to 8 191 keys, 32 heads of 128 over 8: 86 us, the 465 MB at 5.4 TB/s (with one piece of P 89, 118 with units weighed by
 // their keys alone, one head a CTA and exchanges in every tile); even ones of 4 096 keys 98 us, 5.5 TB/s; 16 heads of 64, 16
 // key heads, 32 of 4 096: 98 us, 151 with one head a CTA (rows of 128 bytes, 2 KB apart).  Some 10 us of that are the start,
 // the end and the joining.
