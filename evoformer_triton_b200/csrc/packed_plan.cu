@@ -196,7 +196,6 @@ __device__ __forceinline__ void row_sums(const PackedArgs& a, const PackedPlan& 
   const T* rest = static_cast<const T*>(a.o_rest);
   constexpr int V = VEC ? kPer16<T> : 1, U = 2;
   const Span queries = NORMS ? clamped(packed_offset(a.offsets, a.wide, 0), packed_offset(a.offsets, a.wide, a.B), a.Tq) : Span{0, 0};
-  const Span keys = NORMS ? clamped(packed_offset(a.key_offsets, a.wide, 0), packed_offset(a.key_offsets, a.wide, a.B), a.Tk) : Span{0, 0};
   float most_do = 0.f, most_v = 0.f;
   auto larger = [](float a, float b) { return b > a && b < INFINITY ? b : a; };
   // (the teams of a warp meet in shuffles: as long as the first of them has a row, all go on, the others with a row that
@@ -265,39 +264,43 @@ __device__ __forceinline__ void row_sums(const PackedArgs& a, const PackedPlan& 
     }
   }
   if constexpr (NORMS) {
-    const long long key_items = (long long)keys.n * a.Hk;
     const T* v = static_cast<const T*>(a.v);
-    // (the last blocks first: there may be some without rows of dO)
-    for (long long i0 = (blocks - 1 - block) * teams * U + team; i0 - ahead < key_items; i0 += blocks * teams * U) {
-      float sq[U] = {};
-      const T* from[U];
+    // (keys of packed sequences lie one behind another, those in ranges anywhere: one after another, by all blocks)
+    for (int b = 0; b < (a.ranges ? a.B : 1); ++b) {
+      const Span keys = a.ranges ? key_span(a, b) : clamped(packed_offset(a.key_offsets, a.wide, 0), packed_offset(a.key_offsets, a.wide, a.B), a.Tk);
+      const long long key_items = (long long)keys.n * a.Hk;
+      // (the last blocks first: there may be some without rows of dO)
+      for (long long i0 = (blocks - 1 - block) * teams * U + team; i0 - ahead < key_items; i0 += blocks * teams * U) {
+        float sq[U] = {};
+        const T* from[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const long long i = min(i0 + (long long)u * teams, key_items - 1);
-        const long long t = key_items <= 0x7fffffffLL ? (long long)key_heads.div((uint32_t)i) : i / a.Hk;
-        from[u] = v + (keys.begin + t) * a.sv[0] + (i - t * a.Hk) * a.sv[1];
-      }
-      for (int x = lane * V; x < a.D; x += lanes * V) {
-        if constexpr (VEC) {
-          uint4 w[U];
-#pragma unroll
-          for (int u = 0; u < U; ++u) w[u] = *reinterpret_cast<const uint4*>(from[u] + x);
-#pragma unroll
-          for (int u = 0; u < U; ++u) {
-            float f[V];
-            unpack16<T>(w[u], f);
-#pragma unroll
-            for (int e = 0; e < V; ++e) sq[u] = fmaf(f[e], f[e], sq[u]);
-          }
-        } else {
-#pragma unroll
-          for (int u = 0; u < U; ++u) sq[u] = fmaf(to_float(from[u][x]), to_float(from[u][x]), sq[u]);
+        for (int u = 0; u < U; ++u) {
+          const long long i = min(i0 + (long long)u * teams, key_items - 1);
+          const long long t = key_items <= 0x7fffffffLL ? (long long)key_heads.div((uint32_t)i) : i / a.Hk;
+          from[u] = v + (keys.begin + t) * a.sv[0] + (i - t * a.Hk) * a.sv[1];
         }
-      }
+        for (int x = lane * V; x < a.D; x += lanes * V) {
+          if constexpr (VEC) {
+            uint4 w[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        for (int m = lanes / 2; m > 0; m >>= 1) sq[u] += __shfl_xor_sync(0xffffffffu, sq[u], m);
-        most_v = larger(most_v, sq[u]);
+            for (int u = 0; u < U; ++u) w[u] = *reinterpret_cast<const uint4*>(from[u] + x);
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+              float f[V];
+              unpack16<T>(w[u], f);
+#pragma unroll
+              for (int e = 0; e < V; ++e) sq[u] = fmaf(f[e], f[e], sq[u]);
+            }
+          } else {
+#pragma unroll
+            for (int u = 0; u < U; ++u) sq[u] = fmaf(to_float(from[u][x]), to_float(from[u][x]), sq[u]);
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          for (int m = lanes / 2; m > 0; m >>= 1) sq[u] += __shfl_xor_sync(0xffffffffu, sq[u], m);
+          most_v = larger(most_v, sq[u]);
+        }
       }
     }
     __shared__ uint32_t both[2][kThreads / 32];

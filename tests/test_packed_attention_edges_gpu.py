@@ -231,3 +231,27 @@ def test_fp16_gradients_of_the_largest_scores_gradient(D, size):
     oc.check("dq", dq, (want, 2 * torch.finfo(HF).eps * want + oc.rounding(HF, want)))
     assert not dk.any()
     oc.check("dv", dv, (d.to(HF).double().repeat_interleave(2, 0) / 2, oc.rounding(HF, d.to(HF).double().repeat_interleave(2, 0))))
+
+
+@pytest.mark.parametrize("B", [2, 3, 5])
+@pytest.mark.parametrize("power", [-18, 12])
+def test_fp16_gradients_of_queries_with_keys_in_ranges(power, B):
+    """The gradient of q alone, with keys that lie anywhere: rows of the cache that no range names have no say in the size of dS, those
+    of every range have."""
+    import evoformer_triton_b200 as evo
+    nq, D = [700, 40, 129, 1, 300][:B], 64
+    ranges = [(2500, 4000), (100, 400), (1000, 1130), (0, 50), (1500, 2300)][:B]
+    q, k, v = _qkv(sum(nq), 4100, 4, 2, D, HF)
+    used = torch.zeros(4100, dtype=torch.bool, device=DEV)
+    for a, b in ranges:
+        used[a:b] = True
+    k[~used], v[~used] = 6e4, -6e4
+    d = (_draw(q.shape, F32, 5) * 64).round() / 64 * 2.0 ** power
+    x = q.clone().requires_grad_()
+    out = evo.packed_attention(x, k, v, torch.tensor(_sums(nq), device=DEV), torch.tensor(ranges, device=DEV))
+    (dq,) = torch.autograd.grad(out, x, d.to(HF))
+    spans = [(i, n, a, b - a) for i, n, (a, b) in zip(_sums(nq), nq, ranges)]
+    want = oc.attention(q, k, v, spans, True, d=d.to(HF))[1][0]
+    for i, n, _, _ in spans:
+        w = want[i:i + n]
+        assert float((dq[i:i + n].double() - w).norm()) <= 0.65 * float(oc.rounding(HF, w).norm()) + torch.finfo(HF).eps / 2 * float(w.norm()), i
