@@ -79,6 +79,6 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
     Values there, and in key rows outside the sequence, may be anything; within a sequence q, k and v have to be finite (where a
     score is NaN or plus infinity, the queries that see it get what is not finite either).
 
-    16-bit types: P enters its products rounded to the type, as in the package's other attention; statistics and sums are
-    fp32.  Gradients: q, k, v (k and v not with ``[B, 2]`` ranges)."""
+    16-bit types: P enters its products rounded to the type, as in the package's other attention (in two pieces of it for a few
+    queries without a gradient); statistics and sums are fp32.  Gradients: q, k, v (k and v not with ``[B, 2]`` ranges)."""
     return _lib.host().packed_attention(q, k, v, offsets, key_offsets, causal, scale)
